@@ -102,10 +102,11 @@ def build_host():
 
 def build_oracle():
     """The C restatement always; the reference emulator (oracle/_ref) only
-    where I4D_REF_ROOT names a reference tree."""
+    where I4D_REF_ROOT names a reference tree that holds its source."""
     _run(["make", "-s", "-C", os.path.join(ROOT, "oracle"), "oracle"])
     ref_root = os.environ.get("I4D_REF_ROOT")
-    if ref_root and os.path.isdir(ref_root):
+    source = os.path.join("software_sim", "llama2_decoder_sw_emulator.cpp")
+    if ref_root and os.path.isfile(os.path.join(ref_root, source)):
         _run(["make", "-s", "-C", os.path.join(ROOT, "oracle"), "ref", "REF_ROOT=" + ref_root])
 
 
