@@ -16,7 +16,8 @@ import os
 
 import numpy as np
 
-from . import formats
+from . import formats, longctx
+from .longctx import KV8Cache, RopeTable, rope_frequencies  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libi4d.so")
@@ -37,6 +38,7 @@ EXPORTS = [
     "i4d_decode_greedy", "i4d_argmax", "i4d_sampler_init", "i4d_sample", "i4d_decode_sample",
     "i4d_pack_autoround_matrix", "i4d_pack_fp32_head", "i4d_prefill", "i4d_prefill_tokens", "i4d_eval_nll",
     "i4d_device_arch", "i4d_profile_gemv", "i4d_profile_attention", "i4d_kv_write_tokens",
+    *longctx.SIGNATURES,
 ]
 
 SAMPLER_HOST = 0      # decode_host.cpp:724-868
@@ -137,6 +139,7 @@ def load_library():
         "i4d_pack_autoround_matrix": [P, ctypes.c_int, ctypes.c_int, P, P, P],
         "i4d_pack_fp32_head": [P, P, P],
     }
+    sig.update(longctx.SIGNATURES)
     for name, args in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args
@@ -183,7 +186,7 @@ def device_arch(device=0):
         raise I4DError(st, "i4d_device_arch failed")
     return b.value, cc.value
 
-class Context:
+class Context(longctx.LongContextOps):
     """One decode context on one GPU (i4d_ctx).  With world > 1 it is rank
     `rank` of a bank-sharded group (i4d_create_shard): it holds the banks
     shard_banks(rank, world) and must be attached to its peers (attach_peers)
@@ -200,6 +203,7 @@ class Context:
         if st != OK:
             raise I4DError(st, "i4d_create failed (see stderr)")
         self._h = h
+        self.device = device
         self.num_layers = num_layers
         self.kv_capacity = kv_capacity
         self.rank, self.world = rank, world

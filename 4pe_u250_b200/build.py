@@ -80,13 +80,26 @@ def build_i4d():
         return out
     obj_dir = os.path.join(ROOT, "_build")
     os.makedirs(obj_dir, exist_ok=True)
-    cu_obj = os.path.join(obj_dir, "i4d.o")
     tab_obj = os.path.join(obj_dir, "expf_fix_table.o")
-    _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-fmad=false", "-Xptxas", "-v",
-          "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-          "-c", os.path.join(CSRC, "i4d.cu"), "-o", cu_obj])
+    headers = [s for s in srcs if not s.endswith(".cu")]
+    # The decode path rounds every product and sum by itself; the serving
+    # operators state their rounding order where it matters.
+    units = [("i4d.cu", ["-fmad=false"]), ("i4d_ops.cu", [])]
+    running, objs = [], []
+    for name, flags in units:
+        src = os.path.join(CSRC, name)
+        obj = os.path.join(obj_dir, name[:-3] + ".o")
+        objs.append(obj)
+        if _newer(obj, headers + [src]):
+            cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", *flags, "-Xptxas", "-v", "-Xcompiler", "-fPIC",
+                   "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", src, "-o", obj]
+            print("+", " ".join(cmd), flush=True)
+            running.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
     _run(["gcc", "-O1", "-fPIC", "-c", table, "-o", tab_obj])
-    _run([NVCC, *ARCH, "-shared", "-o", out, cu_obj, tab_obj])
+    _run([NVCC, *ARCH, "-shared", "-o", out, *objs, tab_obj])
     return out
 
 

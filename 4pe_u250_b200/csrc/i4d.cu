@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "i4d.h"
+#include "i4d_internal.h"
 #include "i4d_attention.cuh"
 #include "i4d_blocks.cuh"
 #include "i4d_linear.cuh"
@@ -124,6 +125,7 @@ struct i4d_ctx {
     float* d_logits = nullptr;
     unsigned* d_counters = nullptr;
     unsigned* d_err = nullptr;
+    unsigned* d_op_err = nullptr;  // error word of the long-context operators
     int* d_pos = nullptr;
     int* d_tok = nullptr;                    // greedy: input token id
     unsigned long long* d_argmax = nullptr;  // greedy: argmax key of the step's logits
@@ -570,6 +572,22 @@ bool all_loaded(const i4d_ctx* c) {
 
 }  // namespace
 
+namespace i4d_ops {
+
+OpContext op_context(const i4d_ctx* c) { return {c->device, c->num_sms, c->stream, c->d_op_err}; }
+
+i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    if (c) c->err = buf;
+    return st;
+}
+
+}  // namespace i4d_ops
+
 // ===================================================================== C ABI
 
 extern "C" {
@@ -592,7 +610,7 @@ void i4d_destroy(i4d_ctx* c) {
                    c->d_tok, c->d_argmax, c->d_sample_hist, c->d_sample_keys, c->d_sample_idx,
                    c->d_sample_state, c->d_sample_out, c->d_sample_v, c->d_sample_smax, c->d_pf_resid,
                    c->d_pf_recip, c->d_pf_q, c->d_pf_e, c->d_pf_part, c->d_pf_qrot, c->d_pf_coef, c->d_pf_pos,
-                   c->d_pf_ids, c->d_pf_tgt, c->d_pf_lg, c->d_pf_terms};
+                   c->d_pf_ids, c->d_pf_tgt, c->d_pf_lg, c->d_pf_terms, c->d_op_err};
     for (void* p : dev)
         if (p) cudaFree(p);
     void* host[] = {c->h_resid_in, c->h_resid_out, c->h_logits, c->h_pos, c->h_err, c->h_tok, c->h_argmax,
@@ -689,6 +707,9 @@ static i4d_status create_impl(const i4d_config* cfg, int rank, int world, i4d_ct
     CKC(cudaMemset(c->d_counters, 0, kCounterSlots * sizeof(unsigned)));
     CKC(cudaMalloc(&c->d_err, sizeof(unsigned)));
     CKC(cudaMemset(c->d_err, 0, sizeof(unsigned)));
+    CKC(cudaMalloc(&c->d_op_err, sizeof(unsigned)));
+    CKC(cudaMemset(c->d_op_err, 0, sizeof(unsigned)));
+    CKC(i4d_ops::ops_init());
     CKC(cudaMalloc(&c->d_pos, sizeof(int)));
     CKC(cudaMalloc(&c->d_tok, sizeof(int)));
     CKC(cudaMalloc(&c->d_argmax, sizeof(unsigned long long)));
@@ -1328,7 +1349,8 @@ i4d_status i4d_kv_write_tokens(i4d_ctx* c, int bank, int layer, int lh, int toke
 i4d_status i4d_sync(i4d_ctx* c) {
     if (!c) return I4D_ERR_ARG;
     CK(cudaSetDevice(c->device));
-    return finish(c);
+    const i4d_status st = finish(c);
+    return st == I4D_OK ? i4d_ops::ops_report(c) : st;
 }
 
 void* i4d_stream(i4d_ctx* c) { return c ? static_cast<void*>(c->stream) : nullptr; }

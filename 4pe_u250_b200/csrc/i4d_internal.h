@@ -1,0 +1,26 @@
+// i4d_internal.h -- what the operators' translation unit needs of a context.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "i4d.h"
+
+namespace i4d_ops {
+
+struct OpContext {
+    int device;
+    int num_sms;
+    cudaStream_t stream;
+    unsigned* err;  // device error word of the operators
+};
+
+// i4d.cu
+OpContext op_context(const i4d_ctx* c);
+i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) __attribute__((format(printf, 3, 4)));
+
+// i4d_ops.cu: shared-memory sizes of the operators' kernels, with the context's device current.
+cudaError_t ops_init();
+// The operators' error word since the last call, and zero in its place; the caller has waited for their stream.
+i4d_status ops_report(i4d_ctx* c);
+
+}  // namespace i4d_ops

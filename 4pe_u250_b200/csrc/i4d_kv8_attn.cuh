@@ -1,0 +1,573 @@
+// i4d_kv8_attn.cuh -- attention over the cache of 8-bit codes.
+//
+// k_kv8_attn: eight (or sixteen) query rows of one cache head against a chunk
+// of its tokens.  Codes go from memory to registers in 16-byte pieces and are
+// never staged: the order of the summation index of a matrix instruction is
+// free, so a thread's 16 contiguous codes of a token serve as its part of four
+// steps of K q, and a V^T tile takes the codes of the four tokens whose
+// probabilities the thread holds.  The products are transposed (tokens x rows,
+// then dims x rows), which wastes half as much of a 16 x 8 tile on few rows.
+//   scores   S^T [16 tokens x 8 rows] = K [16 x dim] Q^T     (m16n8k16, FP16 in, FP32 sums)
+//   output   O^T [16 dims x 8 rows]  += V^T [16 x 16 tokens] P^T
+// Every code is exact in FP16.  A query row is scaled by a power of two into
+// FP16's range, which is exact for BF16 and FP16 rows up to 2^-39 of the row's
+// largest value; FP32 rows are split in two FP16 parts (2^-22).  Probabilities
+// go to FP16 in one part (2^-12, below the rounding of a 16-bit output) or,
+// for FP32 outputs, in two.
+//
+// One pass over the tokens: M is a bound of the scores so far (in powers of
+// two), l the sum of 2^(x - M), R a bound of x + log2(v_scale): the values
+// that enter the second product are 2^(x - R) v_scale, so a block whose scale
+// is far above the others' costs the others no bits unless it outweighs them.
+// M and R are raised only when a score passes them by more than 2^6 (FP16
+// holds 2^15), so most tiles do without the reduction over lanes.
+// Bound: the codes of K and V, read once.
+#pragma once
+
+#include "i4d_kv8_cache.cuh"
+
+namespace i4d_ops {
+
+constexpr int kAttnThreads = 128;
+constexpr int kAttnWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 6.f;
+
+struct AttnDev {
+    Kv8Dev cache;
+    SeqArrays seq;
+    const void* q;
+    void* out;
+    float* lse;
+    float* weights;
+    int64_t q_tok, q_head, out_tok, out_head, weights_stride;
+    int heads, group, window, dtype, max_length;
+    float scale_log2;  // softmax scale * log2(e)
+    int row_tiles;     // tiles of a (sequence, cache head)
+    int splits, chunk; // token chunks of a tile
+    float* part;       // workspace: [tile][split][rows][dim + 4]: O, M, l, R
+    float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Codes 2 PAIR and 2 PAIR + 1 of a word as two halves (INT8 words come with
+// their top bits flipped: 1024 + 128 + code is exact in FP16).
+template <int CODE, int PAIR>
+__device__ __forceinline__ uint32_t halves(uint32_t w) {
+    if constexpr (CODE == I4D_CODE_INT8) {
+        const uint32_t m = __byte_perm(w, 0x64646464u, PAIR ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        uint32_t h;
+        const uint16_t p = static_cast<uint16_t>(PAIR ? w >> 16 : w);
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
+        return h;
+    }
+}
+
+template <int CODE>
+__device__ __forceinline__ uint32_t flip(uint32_t w) {
+    return CODE == I4D_CODE_INT8 ? w ^ 0x80808080u : w;
+}
+
+__device__ __forceinline__ void mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float load_q(const AttnDev& a, int64_t i) {
+    if (a.dtype == I4D_F32) return static_cast<const float*>(a.q)[i];
+    if (a.dtype == I4D_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[i]);
+    return __half2float(static_cast<const __half*>(a.q)[i]);
+}
+
+__device__ __forceinline__ void store_out(const AttnDev& a, int64_t i, float v) {
+    if (a.dtype == I4D_F32) static_cast<float*>(a.out)[i] = v;
+    else if (a.dtype == I4D_BF16) static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(a.out)[i] = __float2half_rn(v);
+}
+
+// The query rows of a tile as B operands: row `nt * 8 + lane / 4`, codes'
+// order of the summation index.  factor[nt][j]: what the score sums of row
+// nt * 8 + 2 (lane % 4) + j are multiplied by (besides the block's scale).
+template <int DT, int NT, bool HL>
+struct QTile {
+    static constexpr int KS = DT / 16;
+    uint32_t hi[NT][KS][2];
+    uint32_t lo[HL ? NT : 1][HL ? KS : 1][2];
+    float factor[NT][2];
+};
+
+template <int DT, int NT, bool HL>
+__device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h, int row0, QTile<DT, NT, HL>& q) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dim = a.cache.dim;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = row0 + nt * 8 + g;
+        const bool live = row < s.n * a.group;
+        const int64_t base = live ? (s.first + row / a.group) * a.q_tok + (h * a.group + row % a.group) * a.q_head : 0;
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < DT / 64; ++c) {
+            const int d0 = (t + 4 * c) * 16;
+            if (live && d0 < dim)
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(load_q(a, base + d0 + i)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        // 2^e with the row's largest value in [2^13, 2^14)
+        const int e = max(-115, min(126, 13 - ((__float_as_int(top) >> 23) - 127)));
+        const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
+#pragma unroll
+        for (int c = 0; c < DT / 64; ++c) {
+            const int d0 = (t + 4 * c) * 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = 0.f, y = 0.f;
+                if (live && d0 < dim) {
+                    x = load_q(a, base + d0 + 2 * i) * up;
+                    y = load_q(a, base + d0 + 2 * i + 1) * up;
+                }
+                const uint32_t w = pack_h2(x, y);
+                q.hi[nt][c * 4 + i / 2][i & 1] = w;
+                if constexpr (HL) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                    q.lo[nt][c * 4 + i / 2][i & 1] = pack_h2(x - f.x, y - f.y);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) q.factor[nt][j] = __shfl_sync(~0u, down, (2 * t + j) * 4) * a.scale_log2;
+    }
+}
+
+// K codes of 16 tokens: the thread's 16-byte pieces of tokens g and g + 8.
+template <int DT>
+struct KTile {
+    uint4 w[2][DT / 64];
+};
+
+template <int DT>
+__device__ __forceinline__ void load_ktile(const uint8_t* k, int dim, int n, KTile<DT>& kt) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < DT / 64; ++c) {
+            const int d0 = (t + 4 * c) * 16;
+            kt.w[r][c] = (g + 8 * r < n && d0 < dim) ? __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * r) * dim + d0)) : make_uint4(0, 0, 0, 0);
+        }
+}
+
+template <int DT, int CODE, int NT, bool HL>
+__device__ __forceinline__ void score_tile(const KTile<DT>& kt, const QTile<DT, NT, HL>& q, float s[NT][4]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DT / 64; ++c) {
+        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&kt.w[0][c]);
+        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&kt.w[1][c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = flip<CODE>(w0[i]), y = flip<CODE>(w1[i]);
+            const uint32_t f[4] = {halves<CODE, 0>(x), halves<CODE, 0>(y), halves<CODE, 1>(x), halves<CODE, 1>(y)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma(s[nt], f, q.hi[nt][c * 4 + i][0], q.hi[nt][c * 4 + i][1]);
+                if constexpr (HL) mma(s[nt], f, q.lo[nt][c * 4 + i][0], q.lo[nt][c * 4 + i][1]);
+            }
+        }
+    }
+}
+
+// V codes of 16 tokens: the thread's DT / 8 dims (from (lane / 4) * DT / 8) of
+// tokens 2t, 2t + 1, 2t + 8, 2t + 9.
+template <int DT>
+struct VTile {
+    uint32_t w[4][DT / 32];
+};
+
+template <int DT>
+__device__ __forceinline__ void load_vtile(const uint8_t* v, int dim, int n, VTile<DT>& vt) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int tok = 2 * t + (r & 1) + (r >> 1) * 8;
+        if constexpr (DT == 64) {
+            const bool live = tok < n && g * 8 < dim;
+            const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(v + tok * dim + g * 8)) : make_uint2(0, 0);
+            vt.w[r][0] = x.x;
+            vt.w[r][1] = x.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < DT / 128; ++c) {
+                const int d0 = g * (DT / 8) + c * 16;
+                const uint4 x = tok < n && d0 < dim ? __ldg(reinterpret_cast<const uint4*>(v + tok * dim + d0)) : make_uint4(0, 0, 0, 0);
+                vt.w[r][4 * c] = x.x;
+                vt.w[r][4 * c + 1] = x.y;
+                vt.w[r][4 * c + 2] = x.z;
+                vt.w[r][4 * c + 3] = x.w;
+            }
+        }
+    }
+}
+
+// acc[i]: dims (lane / 4) * DT / 8 + 2 i and + 1, rows 2t and 2t + 1 of each tile.
+template <int DT, int CODE, int NT, bool HL>
+__device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (&p)[NT][2], const uint32_t (&pl)[NT][2], float acc[DT / 16][NT][4]) {
+#pragma unroll
+    for (int w = 0; w < DT / 32; ++w) {
+        const uint32_t w0 = flip<CODE>(vt.w[0][w]), w1 = flip<CODE>(vt.w[1][w]), w2 = flip<CODE>(vt.w[2][w]), w3 = flip<CODE>(vt.w[3][w]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(w0, w1, half ? 0x7362 : 0x5140), y = __byte_perm(w2, w3, half ? 0x7362 : 0x5140);
+            const uint32_t f[4] = {halves<CODE, 0>(x), halves<CODE, 1>(x), halves<CODE, 0>(y), halves<CODE, 1>(y)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma(acc[2 * w + half][nt], f, p[nt][0], p[nt][1]);
+                if constexpr (HL) mma(acc[2 * w + half][nt], f, pl[nt][0], pl[nt][1]);
+            }
+        }
+    }
+}
+
+// First and one past the last token that a row at cache index pos sees.
+__device__ __forceinline__ int2 row_span(const AttnDev& a, int pos) {
+    return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, pos + 1);
+}
+
+template <int DT, int CODE, int NT, bool HL>
+__global__ void __launch_bounds__(kAttnThreads) k_kv8_attn(AttnDev a) {
+    constexpr int kRows = 8 * NT;
+    constexpr int kSub = DT == 256 ? 1 : 2;  // 16-token tiles a step
+    constexpr int kStep = 16 * kSub;
+    __shared__ float merge[kAttnWarps][kRows][DT + 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % a.splits;
+    const int64_t tile = blockIdx.x / a.splits;
+    const int rt = tile % a.row_tiles, h = tile / a.row_tiles % a.cache.heads;
+    const int b = tile / a.row_tiles / a.cache.heads;
+    const bool report = split == 0 && rt == 0 && h == 0 && threadIdx.x == 0;
+    Seq s = load_seq(a.seq, b, report);
+    if (s.len > a.max_length) {
+        if (report) atomicOr(a.seq.err, kBadSequence);
+        return;
+    }
+    const int row0 = rt * kRows;
+    if (row0 >= s.n * a.group) return;
+    const int first = s.len - s.n;  // cache index of row 0's query
+    const int last_row = min(row0 + kRows, s.n * a.group) - 1;
+    // tokens that any row of the tile sees, and that all of them see
+    const int2 lo_span = row_span(a, first + row0 / a.group), hi_span = row_span(a, first + last_row / a.group);
+    const int begin = max(lo_span.x, split * a.chunk), end = min(hi_span.y, (split + 1) * a.chunk);
+    const int all_from = hi_span.x, all_to = lo_span.y;
+    int2 span[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) span[nt][j] = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
+
+    float M[NT][2], R[NT][2], l[NT][2], to_r[NT][2], acc[DT / 16][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            M[nt][j] = R[nt][j] = -INFINITY;
+            l[nt][j] = to_r[nt][j] = 0.f;
+        }
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][nt][j] = 0.f;
+
+    if (begin < end) {
+        QTile<DT, NT, HL> q;
+        load_qtile<DT, NT, HL>(a, s, h, row0, q);
+        const int bs = a.cache.block_tokens, dim = a.cache.dim;
+        for (int tok = (begin & ~15) + warp * kStep; tok < end; tok += kAttnWarps * kStep) {
+            KTile<DT> kt[kSub];
+            VTile<DT> vt[kSub];
+            float ks[kSub], vs[kSub];
+            int live[kSub];  // tokens of the 16 that are there
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const int at = tok + 16 * u;
+                int id = -1;
+                if (at < end) id = load_block(a.seq, b, at / bs, lane == 0);
+                live[u] = id < 0 ? 0 : min(16, end - at);
+                ks[u] = vs[u] = 0.f;
+                const uint8_t *kp = nullptr, *vp = nullptr;
+                if (id >= 0) {
+                    const int64_t off = code_offset(a.cache, id, h) + static_cast<int64_t>(at % bs) * dim;
+                    kp = a.cache.codes[0] + off;
+                    vp = a.cache.codes[1] + off;
+                    ks[u] = __ldg(a.cache.scale[0] + static_cast<int64_t>(id) * a.cache.heads + h);
+                    vs[u] = __ldg(a.cache.scale[1] + static_cast<int64_t>(id) * a.cache.heads + h);
+                }
+                load_ktile<DT>(kp, dim, live[u], kt[u]);
+                load_vtile<DT>(vp, dim, live[u], vt[u]);
+            }
+            float x[kSub][NT][4];
+            float top[NT][2], rtop[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) top[nt][j] = rtop[nt][j] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const int at = tok + 16 * u;
+                score_tile<DT, CODE, NT, HL>(kt[u], q, x[u]);
+                const float lvs = __log2f(vs[u]);  // only a bound: its rounding cancels
+                const bool whole = live[u] == 16 && at >= all_from && at + 16 <= all_to;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = i & 1, n = g + (i >> 1) * 8;
+                        float y = x[u][nt][i] * (q.factor[nt][j] * ks[u]);
+                        if (!whole && !(n < live[u] && at + n >= span[nt][j].x && at + n < span[nt][j].y)) y = -INFINITY;
+                        x[u][nt][i] = y;
+                        top[nt][j] = fmaxf(top[nt][j], y);
+                        rtop[nt][j] = fmaxf(rtop[nt][j], y + lvs);
+                    }
+            }
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) raise |= top[nt][j] > M[nt][j] + kSlack || rtop[nt][j] > R[nt][j] + kSlack;
+            if (__any_sync(~0u, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float m = top[nt][j], r = rtop[nt][j];
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) {
+                            m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                            r = fmaxf(r, __shfl_xor_sync(~0u, r, o));
+                        }
+                        m = fmaxf(m, M[nt][j]);
+                        r = fmaxf(r, R[nt][j]);
+                        const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
+                        l[nt][j] *= fm;
+#pragma unroll
+                        for (int i = 0; i < DT / 16; ++i) {
+                            acc[i][nt][j] *= fr;
+                            acc[i][nt][j + 2] *= fr;
+                        }
+                        M[nt][j] = m;
+                        R[nt][j] = r;
+                        to_r[nt][j] = r == -INFINITY ? 0.f : ex2(m - r);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                uint32_t p[NT][2], pl[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = i & 1;
+                        const float e = ex2(x[u][nt][i] - (M[nt][j] == -INFINITY ? 0.f : M[nt][j]));
+                        l[nt][j] += e;
+                        w[i] = e * (to_r[nt][j] * vs[u]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
+                        p[nt][r] = transpose8(hi);
+                        pl[nt][r] = 0;
+                        if constexpr (HL) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
+                        }
+                    }
+                }
+                value_tile<DT, CODE, NT, HL>(vt[u], p, pl, acc);
+            }
+        }
+    }
+
+    // Join the four warps.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[nt][j] += __shfl_xor_sync(~0u, l[nt][j], o);
+            float* m = merge[warp][nt * 8 + 2 * t + j];
+#pragma unroll
+            for (int i = 0; i < DT / 16; ++i) {
+                m[g * (DT / 8) + 2 * i] = acc[i][nt][j];
+                m[g * (DT / 8) + 2 * i + 1] = acc[i][nt][j + 2];
+            }
+            if (g == 0) {
+                m[DT] = M[nt][j];
+                m[DT + 1] = l[nt][j];
+                m[DT + 2] = R[nt][j];
+            }
+        }
+    __syncthreads();
+    const int dim = a.cache.dim;
+    for (int i = threadIdx.x; i < kRows * DT; i += kAttnThreads) {
+        const int r = i / DT, d = i % DT, row = row0 + r;
+        if (row >= s.n * a.group || d >= dim) continue;
+        float m = -INFINITY, rr = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            m = fmaxf(m, merge[w][r][DT]);
+            rr = fmaxf(rr, merge[w][r][DT + 2]);
+        }
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            if (merge[w][r][DT] == -INFINITY) {  // the warp saw nothing of this row (its sums are 0, or NaN with the row's)
+                sum += merge[w][r][DT + 1];
+                o += merge[w][r][d];
+                continue;
+            }
+            sum += merge[w][r][DT + 1] * ex2(merge[w][r][DT] - m);
+            if (merge[w][r][DT + 2] != -INFINITY) o += merge[w][r][d] * ex2(merge[w][r][DT + 2] - rr);
+        }
+        if (a.splits == 1) {
+            const int64_t tok = s.first + row / a.group;
+            const int head = h * a.group + row % a.group;
+            const float back = rr == -INFINITY ? 0.f : ex2(rr - m);
+            store_out(a, tok * a.out_tok + head * a.out_head + d, sum == 0.f ? 0.f : o * back / sum);
+            if (d == 0) {
+                const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+                if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+                if (a.weights) a.lse2[tok * a.heads + head] = l2;
+            }
+        } else {
+            float* p = a.part + ((tile * a.splits + split) * kRows + r) * (dim + 4);
+            p[d] = o;
+            if (d == 0) {
+                p[dim] = m;
+                p[dim + 1] = sum;
+                p[dim + 2] = rr;
+            }
+        }
+    }
+}
+
+// Joins the chunks of a tile: one warp for a row.
+__global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_per_tile, int64_t rows_total) {
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kAttnWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, r = w % rows_per_tile;
+    const int64_t tile = w / rows_per_tile;
+    const int rt = tile % a.row_tiles, h = tile / a.row_tiles % a.cache.heads;
+    const int64_t b = tile / a.row_tiles / a.cache.heads;
+    if (w >= rows_total) return;
+    const Seq s = load_seq(a.seq, static_cast<int>(b), false);
+    const int row = rt * rows_per_tile + r;
+    if (s.len > a.max_length || row >= s.n * a.group) return;
+    const int2 sp = row_span(a, s.len - s.n + row / a.group);
+    // chunks that the row's tile looked at (a tile's first row may begin earlier; its chunk holds no token of this row then)
+    const int c0 = sp.x / a.chunk, c1 = (sp.y + a.chunk - 1) / a.chunk, dim = a.cache.dim;
+    const float* part = a.part + (tile * a.splits * rows_per_tile + r) * (dim + 4);
+    const int64_t step = static_cast<int64_t>(rows_per_tile) * (dim + 4);
+    float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+    for (int c = c0 + lane; c < c1; c += 32) {
+        m = fmaxf(m, part[c * step + dim]);
+        rr = fmaxf(rr, part[c * step + dim + 2]);
+    }
+    m = warp_max(m);
+    rr = warp_max(rr);
+    for (int c = c0 + lane; c < c1; c += 32) {
+        const float pm = part[c * step + dim];
+        sum += part[c * step + dim + 1] * (pm == -INFINITY ? 1.f : ex2(pm - m));
+    }
+    sum = warp_sum(sum);
+    const int64_t tok = s.first + row / a.group;
+    const int head = h * a.group + row % a.group;
+    const float back = rr == -INFINITY || sum == 0.f ? 0.f : ex2(rr - m) / sum;
+    for (int d = lane; d < dim; d += 32) {
+        float o = 0.f;
+        for (int c = c0; c < c1; ++c) {
+            const float pr = part[c * step + dim + 2];
+            o += part[c * step + d] * (pr == -INFINITY ? 1.f : ex2(pr - rr));
+        }
+        store_out(a, tok * a.out_tok + head * a.out_head + d, sum == 0.f ? 0.f : o * back);
+    }
+    if (lane == 0) {
+        const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+        if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+        if (a.weights) a.lse2[tok * a.heads + head] = l2;
+    }
+}
+
+// Probabilities summed over a head's rows for each token: the scores again,
+// 2^(x - lse2), a warp for 16 tokens, rows in order.
+template <int DT, int CODE, bool HL>
+__global__ void __launch_bounds__(kAttnThreads) k_kv8_weights(AttnDev a, int tiles) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % a.cache.heads, b = bh / a.cache.heads;
+    const Seq s = load_seq(a.seq, b, false);
+    const int at = (tile * kAttnWarps + (threadIdx.x >> 5)) * 16;
+    if (s.len > a.max_length || s.n == 0 || at >= s.len) return;
+    const int bs = a.cache.block_tokens, dim = a.cache.dim, first = s.len - s.n;
+    const int id = load_block(a.seq, b, at / bs, false);
+    if (id < 0) return;
+    const int live = min(16, s.len - at);
+    KTile<DT> kt;
+    load_ktile<DT>(a.cache.codes[0] + code_offset(a.cache, id, h) + static_cast<int64_t>(at % bs) * dim, dim, live, kt);
+    const float ks = __ldg(a.cache.scale[0] + static_cast<int64_t>(id) * a.cache.heads + h);
+    float sum[2] = {0.f, 0.f};
+    // rows whose query stands at or behind the first token and, with a window, not past the last one's
+    const int rows = s.n * a.group;
+    const int from = max(0, at - first) * a.group & ~7;
+    const int to = a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(rows), max(int64_t{0}, (static_cast<int64_t>(at) + 15 + a.window - first)) * a.group)) : rows;
+    for (int row0 = from; row0 < to; row0 += 8) {
+        QTile<DT, 1, HL> q;
+        load_qtile<DT, 1, HL>(a, s, h, row0, q);
+        float x[1][4];
+        score_tile<DT, CODE, 1, HL>(kt, q, x);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = row0 + 2 * t + j;
+            if (row >= rows) continue;
+            const float l2 = a.lse2[(s.first + row / a.group) * static_cast<int64_t>(a.heads) + h * a.group + row % a.group];
+            const int2 sp = row_span(a, first + row / a.group);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int n = at + g + 8 * r;
+                if (n < s.len && n >= sp.x && n < sp.y) sum[r] += ex2(fmaf(x[0][j + 2 * r], q.factor[0][j] * ks, -l2));
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
+        sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
+        const int n = at + g + 8 * r;
+        if (t == 0 && n < s.len) a.weights[(static_cast<int64_t>(b) * a.cache.heads + h) * a.weights_stride + n] += sum[r];
+    }
+}
+
+}  // namespace i4d_ops

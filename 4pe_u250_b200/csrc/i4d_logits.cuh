@@ -1,0 +1,173 @@
+// i4d_logits.cuh -- penalties, biases and masks on rows of logits.
+//
+// One cluster of CTAs for a row.  A CTA walks slices of the row: the counts of
+// the history's tokens that fall in the slice are gathered in shared memory
+// with integer atomics (their sum does not depend on the order), the biases
+// beside them, then each logit is read, changed and written once.  The row's
+// best index is joined over the cluster through distributed shared memory, so
+// nothing is kept in global memory between launches.
+// Bound: the logits in and out; for one row the chain of barriers.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "i4d_ops_common.cuh"
+
+namespace i4d_ops {
+
+constexpr int kLogitsThreads = 512;
+constexpr int kLogitsSlice = 8192;  // entries: 32 KB of counts and 32 KB of biases
+
+struct LogitsDev {
+    const void* in;
+    void* out;
+    int32_t* best;
+    const int32_t* history;
+    const int32_t* history_len;
+    const int32_t* prompt_len;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_ids;
+    const float* bias_values;
+    const int32_t* bias_len;
+    const uint32_t* mask;
+    int64_t stride, out_stride, history_stride, bias_stride, mask_stride;
+    int vocab;
+};
+
+// Greater value, greater key; of equal values the lower index.  0: none.
+__device__ __forceinline__ unsigned long long logit_key(float x, int index) {
+    if (!(x > -INFINITY)) return 0ull;  // NaN and -inf
+    const uint32_t u = __float_as_uint(x + 0.f);
+    const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return static_cast<unsigned long long>(k) << 32 | (0xffffffffu - index);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int V = 16 / sizeof(T);
+    int* counts = reinterpret_cast<int*>(smem);                  // bit 0: seen in the prompt, above: 2 * occurrences after it
+    float* bias = reinterpret_cast<float*>(counts + kLogitsSlice);
+    __shared__ unsigned long long keys[kLogitsThreads / 32];
+    __shared__ unsigned long long cta_key[16];
+    cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    if (a.best) cl.barrier_arrive();  // the wait stands before the first access to another CTA's memory
+    const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x;
+    const T* in = static_cast<const T*>(a.in) + row * a.stride;
+    T* out = static_cast<T*>(a.out) + row * a.out_stride;
+    const int32_t* hist = a.history ? a.history + row * a.history_stride : nullptr;
+    const int n_hist = hist ? static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.history_len + row), 0)), a.history_stride)) : 0;
+    const int n_prompt = hist && a.prompt_len ? __ldg(a.prompt_len + row) : 0;
+    const int n_bias = a.bias_ids ? static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.bias_len + row), 0)), a.bias_stride)) : 0;
+    const float rep = a.repetition ? __ldg(a.repetition + row) : 1.f;
+    const float freq = a.frequency ? __ldg(a.frequency + row) : 0.f;
+    const float pres = a.presence ? __ldg(a.presence + row) : 0.f;
+    const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    // Vector j holds entries [V j - skew, V j - skew + V): 16-byte aligned in
+    // the input, and in the output if its rows have the same alignment.
+    const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % V);
+    const bool aligned_out = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % V) == skew;
+    const int vecs = (a.vocab + skew + V - 1) / V;
+    const int per_cta = (vecs + ctas - 1) / ctas;
+    const int v_end = min(vecs, (rank + 1) * per_cta);
+    unsigned long long key = 0;
+    for (int v0 = rank * per_cta; v0 < v_end; v0 += kLogitsSlice / V) {
+        const int v1 = min(v_end, v0 + kLogitsSlice / V);
+        const int e0 = v0 * V - skew, span = (v1 - v0) * V;
+        __syncthreads();
+        if (n_hist)
+            for (int i = tid; i < span; i += kLogitsThreads) counts[i] = 0;
+        if (n_bias)
+            for (int i = tid; i < span; i += kLogitsThreads) bias[i] = 0.f;
+        __syncthreads();
+        for (int i = tid; i < n_hist; i += kLogitsThreads) {
+            const int id = __ldg(hist + i);
+            const unsigned at = static_cast<unsigned>(id) - static_cast<unsigned>(e0);
+            if (id >= 0 && id < a.vocab && id >= e0 && at < static_cast<unsigned>(span)) {
+                if (i < n_prompt) atomicOr(&counts[at], 1);
+                else atomicAdd(&counts[at], 2);
+            }
+        }
+        if (tid < 32) {  // one warp, so that the values of one id are added in their order
+            for (int i = 0; i < n_bias; i += 32) {
+                const bool live = i + tid < n_bias;
+                const int id = live ? __ldg(a.bias_ids + row * a.bias_stride + i + tid) : -1;
+                const float val = live ? __ldg(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
+                const bool mine = live && id >= 0 && id < a.vocab && id >= e0 && id - e0 < span;
+                const unsigned peers = __match_any_sync(~0u, mine ? id : -1 - tid);
+                const bool leader = __ffs(peers) - 1 == tid;
+                float sum = mine && leader ? bias[id - e0] : 0.f;
+                if (__any_sync(~0u, mine && !leader)) {
+                    for (int l = 0; l < 32; ++l) {
+                        const float v = __shfl_sync(~0u, val, l);
+                        if (peers >> l & 1) sum = __fadd_rn(sum, v);
+                    }
+                } else {
+                    sum = __fadd_rn(sum, val);
+                }
+                if (mine && leader) bias[id - e0] = sum;
+                __syncwarp();
+            }
+        }
+        __syncthreads();
+        for (int v = v0 + tid; v < v1; v += kLogitsThreads) {
+            const int e = v * V - skew;
+            const bool whole = e >= 0 && e + V <= a.vocab;
+            Vec<T, V> x;
+            if (whole) {
+                x = *reinterpret_cast<const Vec<T, V>*>(in + e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e + i >= 0 && e + i < a.vocab) x.v[i] = in[e + i];
+            }
+            uint32_t w0 = ~0u, w1 = ~0u;
+            if (mask) {
+                w0 = __ldg(mask + max(e, 0) / 32);
+                w1 = __ldg(mask + min(e + V - 1, a.vocab - 1) / 32);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int id = e + i;
+                if (id < 0 || id >= a.vocab) continue;
+                float y = to_f32(x.v[i]);
+                if (n_hist) {
+                    const int c = counts[id - e0], n = c >> 1;
+                    if (c) y = a.repetition ? (y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep)) : y;
+                    if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                }
+                if (n_bias) y = __fadd_rn(y, bias[id - e0]);
+                const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? w0 : w1;
+                if (!(w >> (id & 31) & 1)) y = -INFINITY;
+                x.v[i] = from_f32<T>(y);
+                key = max(key, logit_key(to_f32(x.v[i]), id));
+            }
+            if (whole && aligned_out) {
+                *reinterpret_cast<Vec<T, V>*>(out + e) = x;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e + i >= 0 && e + i < a.vocab) out[e + i] = x.v[i];
+            }
+        }
+    }
+    if (!a.best) return;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(~0u, key, o));
+    if ((tid & 31) == 0) keys[tid >> 5] = key;
+    __syncthreads();
+    cl.barrier_wait();
+    if (tid == 0) {
+        for (int w = 1; w < kLogitsThreads / 32; ++w) key = max(key, keys[w]);
+        *cl.map_shared_rank(&cta_key[rank], 0) = key;
+    }
+    cl.sync();
+    if (rank == 0 && tid == 0) {
+        for (int c = 0; c < ctas; ++c) key = max(key, cta_key[c]);
+        a.best[row] = key ? static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
+    }
+}
+
+}  // namespace i4d_ops

@@ -1,0 +1,656 @@
+// i4d_ops.cu -- host side of the long-context serving operators (see
+// include/i4d.h): checks of arguments, launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "i4d.h"
+#include "i4d_internal.h"
+#include "i4d_kv8_attn.cuh"
+#include "i4d_kv8_cache.cuh"
+#include "i4d_logits.cuh"
+#include "i4d_rope.cuh"
+
+using namespace i4d_ops;
+
+namespace {
+
+// The context's device for the length of a call; the caller's is put back.
+class DeviceScope {
+  public:
+    explicit DeviceScope(int device) {
+        err_ = cudaGetDevice(&before_);
+        if (err_ == cudaSuccess && before_ != device) {
+            err_ = cudaSetDevice(device);
+            changed_ = err_ == cudaSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (changed_) cudaSetDevice(before_);
+    }
+    cudaError_t error() const { return err_; }
+
+  private:
+    int before_ = 0;
+    bool changed_ = false;
+    cudaError_t err_;
+};
+
+#define OP_ARG(cond, ...)                                                \
+    do {                                                                 \
+        if (!(cond)) return op_fail(ctx, I4D_ERR_ARG, __VA_ARGS__);      \
+    } while (0)
+
+#define OP_CK(call)                                                                                  \
+    do {                                                                                             \
+        const cudaError_t e_ = (call);                                                               \
+        if (e_ != cudaSuccess) return op_fail(ctx, I4D_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_)); \
+    } while (0)
+
+int dtype_bytes(int t) { return t == I4D_F32 ? 4 : 2; }
+bool is_dtype(int t) { return t == I4D_F32 || t == I4D_BF16 || t == I4D_F16; }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+cudaStream_t stream_of(const OpContext& o, void* stream) {
+    return stream ? static_cast<cudaStream_t>(stream) : o.stream;
+}
+
+// Bytes [lo, hi) that `n` rows of `heads` heads touch.
+struct Span {
+    uintptr_t lo, hi;
+};
+Span span_of(const void* p, int64_t n, int64_t stride, int64_t heads, int64_t head_stride, int64_t inner, int bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (!p || n <= 0 || heads <= 0) return {at, at};
+    return {at, at + static_cast<uintptr_t>(((n - 1) * stride + (heads - 1) * head_stride + inner) * bytes)};
+}
+bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+i4d_status check_cache(i4d_ctx* ctx, const i4d_kv8& c) {
+    OP_ARG(c.k && c.v && c.k_scale && c.v_scale, "null cache buffer");
+    OP_ARG(c.blocks > 0 && c.heads > 0, "cache of %d blocks and %d heads", c.blocks, c.heads);
+    OP_ARG(c.block_tokens == 16 || c.block_tokens == 32 || c.block_tokens == 64 || c.block_tokens == 128,
+           "block_tokens %d (16, 32, 64 or 128)", c.block_tokens);
+    OP_ARG(c.dim > 0 && c.dim <= 256 && c.dim % 16 == 0, "dim %d (a multiple of 16 up to 256)", c.dim);
+    OP_ARG(c.code == I4D_CODE_INT8 || c.code == I4D_CODE_E4M3, "unknown code %d", c.code);
+    OP_ARG(aligned(c.k, 16) && aligned(c.v, 16), "cache codes need 16-byte alignment");
+    OP_ARG(aligned(c.k_scale, 4) && aligned(c.v_scale, 4), "cache scales need 4-byte alignment");
+    return I4D_OK;
+}
+
+Kv8Dev cache_dev(const i4d_kv8& c) {
+    Kv8Dev d = {};
+    d.codes[0] = static_cast<uint8_t*>(c.k);
+    d.codes[1] = static_cast<uint8_t*>(c.v);
+    d.scale[0] = c.k_scale;
+    d.scale[1] = c.v_scale;
+    d.heads = c.heads;
+    d.dim = c.dim;
+    d.block_tokens = c.block_tokens;
+    return d;
+}
+
+i4d_status check_batch(i4d_ctx* ctx, const int32_t* q_start, const int32_t* lengths, const int32_t* table,
+                       int64_t table_stride, int batch, int tokens, int max_q) {
+    OP_ARG(batch >= 0 && tokens >= 0 && max_q >= 0, "negative batch, tokens or max_q");
+    OP_ARG(batch == 0 || (q_start && lengths && table), "null q_start, lengths or block_table");
+    OP_ARG(aligned(q_start, 4) && aligned(lengths, 4) && aligned(table, 4), "index arrays need 4-byte alignment");
+    OP_ARG(table_stride >= 0, "negative table_stride");
+    return I4D_OK;
+}
+
+SeqArrays seq_arrays(const OpContext& o, const i4d_kv8& c, const int32_t* q_start, const int32_t* lengths,
+                     const int32_t* table, int64_t table_stride, int tokens, int max_q) {
+    SeqArrays s = {};
+    s.q_start = q_start;
+    s.lengths = lengths;
+    s.table = table;
+    s.table_stride = table_stride;
+    s.tokens = tokens;
+    s.max_q = max_q;
+    s.block_tokens = c.block_tokens;
+    s.blocks = c.blocks;
+    s.err = o.err;
+    return s;
+}
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+
+// ------------------------------------------------------------------ rope
+
+template <typename T, int V, bool IL>
+cudaError_t launch_rope(const RopeDev& d, int num_sms, cudaStream_t st) {
+    const int rot_items = (IL ? d.rot : d.rot / 2) / V;
+    const int items = (d.heads[0] + d.heads[1]) * (rot_items + (d.copy_tail ? (d.dim - d.rot) / V : 0));
+    // Few tokens: their heads are spread over CTAs, up to two waves of them.
+    const int most = (items + kRopeThreads - 1) / kRopeThreads;
+    const int groups = std::max(1, std::min(most, 2 * num_sms / d.tokens));
+    if (static_cast<int64_t>(d.tokens) * groups > kMaxGrid) return cudaErrorInvalidValue;
+    k_rope<T, V, IL><<<d.tokens * groups, kRopeThreads, 0, st>>>(d, groups);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_rope_t(const RopeDev& d, bool interleaved, bool wide, int num_sms, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    if (interleaved) return wide ? launch_rope<T, V, true>(d, num_sms, st) : launch_rope<T, 2, true>(d, num_sms, st);
+    return wide ? launch_rope<T, V, false>(d, num_sms, st) : launch_rope<T, 1, false>(d, num_sms, st);
+}
+
+// ---------------------------------------------------------------- append
+
+template <typename T, int V, int CODE>
+cudaError_t launch_append(const AppendDev& d, int64_t units, int64_t unit_items, cudaStream_t st) {
+    // A warp for the few values of a decode step, a CTA for a block of a prompt.
+    if (unit_items <= 64) {
+        k_kv8_append<T, V, CODE, 32><<<static_cast<unsigned>((units + 3) / 4), 128, 0, st>>>(d, static_cast<int>(units));
+    } else {
+        k_kv8_append<T, V, CODE, 256><<<static_cast<unsigned>(units), 256, 0, st>>>(d, static_cast<int>(units));
+    }
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_append_t(const AppendDev& d, int code, bool wide, int64_t units, int64_t items, cudaStream_t st) {
+    if (code == I4D_CODE_INT8)
+        return wide ? launch_append<T, 8, I4D_CODE_INT8>(d, units, items, st) : launch_append<T, 1, I4D_CODE_INT8>(d, units, items, st);
+    return wide ? launch_append<T, 8, I4D_CODE_E4M3>(d, units, items, st) : launch_append<T, 1, I4D_CODE_E4M3>(d, units, items, st);
+}
+
+// ------------------------------------------------------------- attention
+
+struct AttnPlan {
+    int dt, nt;  // padded dim, row tiles of eight a CTA
+    int row_tiles, splits, chunk;
+    int64_t tiles;
+    size_t part_bytes, lse2_bytes;
+};
+
+AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
+    AttnPlan p = {};
+    const i4d_kv8& c = a.cache;
+    const int64_t rows = static_cast<int64_t>(a.max_q) * (a.heads / c.heads);
+    p.dt = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    p.nt = rows > 8 && a.dtype != I4D_F32 && p.dt <= 128 ? 2 : 1;
+    p.row_tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.tiles = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
+    // Chunks: enough CTAs for four on every SM, none under 256 tokens.
+    const int64_t want = std::max<int64_t>(1, 4 * o.num_sms / std::max<int64_t>(1, p.tiles));
+    int64_t chunk = (a.max_length + want - 1) / want;
+    chunk = std::max<int64_t>(256, (chunk + 127) / 128 * 128);
+    p.chunk = static_cast<int>(chunk);
+    p.splits = static_cast<int>(std::max<int64_t>(1, (a.max_length + chunk - 1) / chunk));
+    if (p.splits > 1) p.part_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * (c.dim + 4) * sizeof(float);
+    if (a.weights) p.lse2_bytes = static_cast<size_t>(a.tokens) * a.heads * sizeof(float);
+    p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+    return p;
+}
+
+i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
+    OP_ARG(a, "null arguments");
+    i4d_status st = check_cache(ctx, a->cache);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st != I4D_OK) return st;
+    OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
+    OP_ARG(a->heads > 0 && a->heads % a->cache.heads == 0, "%d query heads over %d cache heads", a->heads, a->cache.heads);
+    OP_ARG(a->max_length >= 0 && a->max_length <= kMaxTokens, "max_length %d", a->max_length);
+    OP_ARG(a->window >= 0 && a->window <= kMaxTokens, "window %d", a->window);
+    OP_ARG(a->table_stride * a->cache.block_tokens >= a->max_length, "block_table rows of %lld blocks hold fewer than max_length %d tokens",
+           static_cast<long long>(a->table_stride), a->max_length);
+    OP_ARG(std::isfinite(a->scale), "scale is not finite");
+    OP_ARG(static_cast<int64_t>(a->max_q) * (a->heads / a->cache.heads) <= kMaxTokens, "too many rows");
+    return I4D_OK;
+}
+
+template <int DT, int CODE, int NT, bool HL>
+cudaError_t launch_attn(const AttnDev& d, int64_t grid, cudaStream_t st) {
+    k_kv8_attn<DT, CODE, NT, HL><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d);
+    return cudaGetLastError();
+}
+
+template <int DT, int CODE>
+cudaError_t launch_attn_d(const AttnDev& d, const AttnPlan& p, int64_t grid, cudaStream_t st) {
+    if (d.dtype == I4D_F32) return launch_attn<DT, CODE, 1, true>(d, grid, st);
+    if constexpr (DT <= 128) {
+        if (p.nt == 2) return launch_attn<DT, CODE, 2, false>(d, grid, st);
+    }
+    return launch_attn<DT, CODE, 1, false>(d, grid, st);
+}
+
+template <int CODE>
+cudaError_t launch_attn_c(const AttnDev& d, const AttnPlan& p, int64_t grid, cudaStream_t st) {
+    return p.dt == 64 ? launch_attn_d<64, CODE>(d, p, grid, st) : p.dt == 128 ? launch_attn_d<128, CODE>(d, p, grid, st) : launch_attn_d<256, CODE>(d, p, grid, st);
+}
+
+template <int DT, int CODE>
+cudaError_t launch_weights(const AttnDev& d, int tiles, int64_t grid, cudaStream_t st) {
+    if (d.dtype == I4D_F32) k_kv8_weights<DT, CODE, true><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d, tiles);
+    else k_kv8_weights<DT, CODE, false><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d, tiles);
+    return cudaGetLastError();
+}
+
+template <int CODE>
+cudaError_t launch_weights_c(const AttnDev& d, const AttnPlan& p, int tiles, int64_t grid, cudaStream_t st) {
+    return p.dt == 64 ? launch_weights<64, CODE>(d, tiles, grid, st) : p.dt == 128 ? launch_weights<128, CODE>(d, tiles, grid, st) : launch_weights<256, CODE>(d, tiles, grid, st);
+}
+
+// ----------------------------------------------------------------- evict
+
+size_t evict_workspace(const i4d_kv8_evict_args& a) {
+    const size_t old_blocks = (static_cast<size_t>(a.max_length) + a.cache.block_tokens - 1) / a.cache.block_tokens;
+    return static_cast<size_t>(a.batch) * a.cache.heads * 2 * old_blocks * sizeof(float);
+}
+
+i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
+    OP_ARG(a, "null arguments");
+    i4d_status st = check_cache(ctx, a->cache);
+    if (st != I4D_OK) return st;
+    OP_ARG(a->batch >= 0, "negative batch");
+    OP_ARG(a->max_length >= 0 && a->max_length <= kMaxTokens, "max_length %d", a->max_length);
+    OP_ARG(a->budget > 0 && a->recent >= 0 && a->recent <= a->budget, "budget %d, recent %d (0 <= recent <= budget, 0 < budget)", a->budget, a->recent);
+    OP_ARG(a->table_stride >= 0 && a->table_stride * a->cache.block_tokens >= a->max_length,
+           "block_table rows of %lld blocks hold fewer than max_length %d tokens", static_cast<long long>(a->table_stride), a->max_length);
+    OP_ARG(a->weights_stride >= a->max_length && a->weights_out_stride >= a->max_length, "weights' rows are shorter than max_length");
+    return I4D_OK;
+}
+
+}  // namespace
+
+namespace i4d_ops {
+
+cudaError_t ops_init() {
+    const int logits_smem = 2 * kLogitsSlice * 4;
+    cudaError_t e = cudaFuncSetAttribute(k_logits<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
+    return e;
+}
+
+i4d_status ops_report(i4d_ctx* ctx) {
+    const OpContext o = op_context(ctx);
+    unsigned e = 0;
+    OP_CK(cudaMemcpyAsync(&e, o.err, sizeof(e), cudaMemcpyDeviceToHost, o.stream));
+    OP_CK(cudaStreamSynchronize(o.stream));
+    if (!e) return I4D_OK;
+    OP_CK(cudaMemsetAsync(o.err, 0, sizeof(e), o.stream));
+    OP_CK(cudaStreamSynchronize(o.stream));
+    return op_fail(ctx, I4D_ERR_ARG, "an operator skipped tokens:%s%s", e & kBadSequence ? " q_start or lengths out of range;" : "",
+                   e & kBadBlock ? " block id outside the pool;" : "");
+}
+
+}  // namespace i4d_ops
+
+extern "C" {
+
+i4d_status i4d_rope_frequencies(int rot_dim, double base, int scaling, double factor, double original_length, double low,
+                                double high, uint64_t* turns_out) {
+    if (!turns_out || rot_dim < 2 || rot_dim > 256 || rot_dim % 2 || !(base > 1.0) || !std::isfinite(base)) return I4D_ERR_ARG;
+    if (scaling < I4D_ROPE_PLAIN || scaling > I4D_ROPE_PARTS) return I4D_ERR_ARG;
+    if (scaling != I4D_ROPE_PLAIN && !(factor >= 1.0 && std::isfinite(factor))) return I4D_ERR_ARG;
+    if (scaling == I4D_ROPE_BASE && rot_dim < 4) return I4D_ERR_ARG;
+    if (scaling == I4D_ROPE_PARTS && !(original_length > 0.0 && high > low && std::isfinite(high) && std::isfinite(low) && std::isfinite(original_length)))
+        return I4D_ERR_ARG;
+    const double two_pi = 6.283185307179586476925286766559;
+    if (scaling == I4D_ROPE_BASE) base *= std::pow(factor, rot_dim / (rot_dim - 2.0));
+    for (int i = 0; i < rot_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rot_dim);
+        if (scaling == I4D_ROPE_LINEAR) f /= factor;
+        if (scaling == I4D_ROPE_PARTS) {
+            const double g = std::min(1.0, std::max(0.0, (original_length * f / two_pi - low) / (high - low)));
+            f *= g + (1.0 - g) / factor;
+        }
+        turns_out[i] = static_cast<uint64_t>(f / two_pi * 18446744073709551616.0 + 0.5);  // f <= 1 radian: under 2^62
+    }
+    return I4D_OK;
+}
+
+i4d_status i4d_rope(i4d_ctx* ctx, const i4d_rope_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    OP_ARG(a, "null arguments");
+    OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
+    OP_ARG(a->tokens >= 0 && a->q_heads > 0 && a->k_heads >= 0, "tokens %d, q_heads %d, k_heads %d", a->tokens, a->q_heads, a->k_heads);
+    OP_ARG(a->dim > 0 && a->dim <= 4096, "dim %d (1 to 4096)", a->dim);
+    OP_ARG(a->rot_dim >= 2 && a->rot_dim % 2 == 0 && a->rot_dim <= a->dim && a->rot_dim <= 256, "rot_dim %d (even, up to dim %d and 256)", a->rot_dim, a->dim);
+    if (a->tokens == 0) return I4D_OK;
+    OP_ARG(a->q && a->q_out && a->positions && a->turns, "null buffer");
+    const bool has_k = a->k != nullptr && a->k_heads > 0;
+    OP_ARG(!has_k || a->k_out, "null k_out");
+    const int bytes = dtype_bytes(a->dtype);
+    RopeDev d = {};
+    const void* in[2] = {a->q, has_k ? a->k : nullptr};
+    void* out[2] = {a->q_out, has_k ? a->k_out : nullptr};
+    const int64_t in_s[2] = {a->q_stride, a->k_stride}, in_h[2] = {a->q_head_stride, a->k_head_stride};
+    const int64_t out_s[2] = {a->q_out_stride, a->k_out_stride}, out_h[2] = {a->q_out_head_stride, a->k_out_head_stride};
+    Span si[2], so[2];
+    const int vec = 16 / bytes;
+    bool wide = a->dim % vec == 0 && a->rot_dim % (a->interleaved ? vec : 2 * vec) == 0;
+    bool copy = false;
+    for (int i = 0; i < 2; ++i) {
+        const int heads = i ? (has_k ? a->k_heads : 0) : a->q_heads;
+        d.in[i] = in[i];
+        d.out[i] = out[i];
+        d.in_tok[i] = in_s[i];
+        d.in_head[i] = in_h[i];
+        d.out_tok[i] = out_s[i];
+        d.out_head[i] = out_h[i];
+        d.heads[i] = heads;
+        if (!heads) {
+            si[i] = so[i] = {0, 0};
+            continue;
+        }
+        OP_ARG(aligned(in[i], bytes) && aligned(out[i], bytes), "misaligned buffer");
+        OP_ARG(in_s[i] >= 0 && in_h[i] >= 0, "negative input stride");
+        // every output element has a place of its own
+        const bool head_inner = out_h[i] >= a->dim && out_s[i] >= (heads - 1) * out_h[i] + a->dim;
+        const bool token_inner = out_s[i] >= a->dim && out_h[i] >= (a->tokens - 1) * out_s[i] + a->dim;
+        OP_ARG(head_inner || token_inner || (heads == 1 && out_s[i] >= a->dim) || (a->tokens == 1 && out_h[i] >= a->dim), "output rows overlap");
+        si[i] = span_of(in[i], a->tokens, in_s[i], heads, in_h[i], a->dim, bytes);
+        so[i] = span_of(out[i], a->tokens, out_s[i], heads, out_h[i], a->dim, bytes);
+        wide = wide && aligned(in[i], 16) && aligned(out[i], 16) && in_s[i] % vec == 0 && in_h[i] % vec == 0 && out_s[i] % vec == 0 && out_h[i] % vec == 0;
+    }
+    for (int i = 0; i < 2; ++i) {
+        if (!d.heads[i]) continue;
+        const bool same = in[i] == out[i] && in_s[i] == out_s[i] && in_h[i] == out_h[i];
+        OP_ARG(same || !overlap(si[i], so[i]), "an output overlaps its input");
+        copy = copy || !same;
+    }
+    if (has_k) {
+        // q and k may be interleaved parts of one buffer; only plain overlap of different tensors is refused
+        OP_ARG(out[0] != out[1], "q_out is k_out");
+    }
+    d.positions = a->positions;
+    d.turns = a->turns;
+    d.tokens = a->tokens;
+    d.dim = a->dim;
+    d.rot = a->rot_dim;
+    d.inverse = a->inverse != 0;
+    d.copy_tail = copy && a->dim > a->rot_dim;
+    d.magnitude = a->magnitude;
+    const OpContext o = op_context(ctx);
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    const cudaStream_t st = stream_of(o, a->stream);
+    if (!wide && a->interleaved) OP_ARG((a->dim - a->rot_dim) % 2 == 0 || !d.copy_tail, "dim %d must be even", a->dim);
+    switch (a->dtype) {
+        case I4D_F32: OP_CK(launch_rope_t<float>(d, a->interleaved != 0, wide, o.num_sms, st)); break;
+        case I4D_BF16: OP_CK(launch_rope_t<__nv_bfloat16>(d, a->interleaved != 0, wide, o.num_sms, st)); break;
+        default: OP_CK(launch_rope_t<__half>(d, a->interleaved != 0, wide, o.num_sms, st)); break;
+    }
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    OP_ARG(a, "null arguments");
+    i4d_status st = check_cache(ctx, a->cache);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st != I4D_OK) return st;
+    OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
+    if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
+    OP_ARG(a->k && a->v, "null k or v");
+    const int bytes = dtype_bytes(a->dtype);
+    OP_ARG(aligned(a->k, bytes) && aligned(a->v, bytes), "misaligned k or v");
+    OP_ARG(a->k_stride >= 0 && a->k_head_stride >= 0 && a->v_stride >= 0 && a->v_head_stride >= 0, "negative stride");
+    const OpContext o = op_context(ctx);
+    AppendDev d = {};
+    d.cache = cache_dev(a->cache);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.in[0] = a->k;
+    d.in[1] = a->v;
+    d.tok[0] = a->k_stride;
+    d.tok[1] = a->v_stride;
+    d.head[0] = a->k_head_stride;
+    d.head[1] = a->v_head_stride;
+    const int bs = a->cache.block_tokens;
+    d.touched = (a->max_q + bs - 2) / bs + 1;
+    const int64_t units = static_cast<int64_t>(a->batch) * d.touched * a->cache.heads * 2;
+    OP_ARG(units <= kMaxGrid, "too many blocks in one call");
+    // 8 elements an access: two of 16 bytes for FP32, one for the others
+    const int vec = 16 / bytes;
+    const bool wide = aligned(a->k, 16) && aligned(a->v, 16) && a->k_stride % vec == 0 && a->k_head_stride % vec == 0 &&
+                      a->v_stride % vec == 0 && a->v_head_stride % vec == 0;
+    const int64_t items = static_cast<int64_t>(std::min(a->max_q, bs)) * a->cache.dim / 8;
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    const cudaStream_t s = stream_of(o, a->stream);
+    switch (a->dtype) {
+        case I4D_F32: OP_CK(launch_append_t<float>(d, a->cache.code, wide, units, items, s)); break;
+        case I4D_BF16: OP_CK(launch_append_t<__nv_bfloat16>(d, a->cache.code, wide, units, items, s)); break;
+        default: OP_CK(launch_append_t<__half>(d, a->cache.code, wide, units, items, s)); break;
+    }
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    OP_ARG(a, "null arguments");
+    i4d_status st = check_cache(ctx, a->cache);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st != I4D_OK) return st;
+    if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
+    OP_ARG(a->k_out && a->v_out && aligned(a->k_out, 16) && aligned(a->v_out, 16), "k_out and v_out need 16-byte alignment");
+    const OpContext o = op_context(ctx);
+    ReadDev d = {};
+    d.cache = cache_dev(a->cache);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.out[0] = static_cast<__nv_bfloat16*>(a->k_out);
+    d.out[1] = static_cast<__nv_bfloat16*>(a->v_out);
+    const int chunks = (a->max_q + kReadTokens - 1) / kReadTokens;
+    const int64_t grid = static_cast<int64_t>(a->batch) * chunks;
+    OP_ARG(grid <= kMaxGrid, "too many rows in one call");
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    const cudaStream_t s = stream_of(o, a->stream);
+    if (a->cache.code == I4D_CODE_INT8) k_kv8_read<I4D_CODE_INT8><<<static_cast<unsigned>(grid), 256, 0, s>>>(d, chunks);
+    else k_kv8_read<I4D_CODE_E4M3><<<static_cast<unsigned>(grid), 256, 0, s>>>(d, chunks);
+    OP_CK(cudaGetLastError());
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_attention_workspace(i4d_ctx* ctx, const i4d_kv8_attention_args* a, size_t* bytes_out) {
+    if (!ctx) return I4D_ERR_ARG;
+    const i4d_status st = check_attention(ctx, a);
+    if (st != I4D_OK) return st;
+    OP_ARG(bytes_out, "null bytes_out");
+    const AttnPlan p = attn_plan(op_context(ctx), *a);
+    *bytes_out = p.part_bytes + p.lse2_bytes;
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    const i4d_status st = check_attention(ctx, a);
+    if (st != I4D_OK) return st;
+    if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
+    OP_ARG(a->q && a->out, "null q or out");
+    const int bytes = dtype_bytes(a->dtype), dim = a->cache.dim;
+    OP_ARG(aligned(a->q, bytes) && aligned(a->out, bytes) && aligned(a->lse, 4) && aligned(a->weights, 4), "misaligned buffer");
+    OP_ARG(a->q_stride >= 0 && a->q_head_stride >= 0, "negative q stride");
+    const bool head_inner = a->out_head_stride >= dim && a->out_stride >= (a->heads - 1) * a->out_head_stride + dim;
+    const bool token_inner = a->out_stride >= dim && a->out_head_stride >= (a->tokens - 1) * a->out_stride + dim;
+    OP_ARG(head_inner || token_inner || (a->heads == 1 && a->out_stride >= dim) || (a->tokens == 1 && a->out_head_stride >= dim), "rows of out overlap");
+    OP_ARG(!overlap(span_of(a->q, a->tokens, a->q_stride, a->heads, a->q_head_stride, dim, bytes),
+                    span_of(a->out, a->tokens, a->out_stride, a->heads, a->out_head_stride, dim, bytes)), "out overlaps q");
+    OP_ARG(!a->weights || a->weights_stride >= a->max_length, "weights' rows are shorter than max_length");
+    const OpContext o = op_context(ctx);
+    const AttnPlan p = attn_plan(o, *a);
+    const size_t need = p.part_bytes + p.lse2_bytes;
+    OP_ARG(need == 0 || (a->workspace && aligned(a->workspace, 16)), "null or misaligned workspace (%zu bytes needed)", need);
+    if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
+    AttnDev d = {};
+    d.cache = cache_dev(a->cache);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.q = a->q;
+    d.out = a->out;
+    d.lse = a->lse;
+    d.weights = a->weights;
+    d.q_tok = a->q_stride;
+    d.q_head = a->q_head_stride;
+    d.out_tok = a->out_stride;
+    d.out_head = a->out_head_stride;
+    d.weights_stride = a->weights_stride;
+    d.heads = a->heads;
+    d.group = a->heads / a->cache.heads;
+    d.window = a->window;
+    d.dtype = a->dtype;
+    d.max_length = a->max_length;
+    d.scale_log2 = a->scale * kLog2e;
+    d.row_tiles = p.row_tiles;
+    d.splits = p.splits;
+    d.chunk = p.chunk;
+    d.part = static_cast<float*>(a->workspace);
+    d.lse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + p.part_bytes);
+    const int64_t grid = p.tiles * p.splits;
+    const int64_t joins = (p.tiles * 8 * p.nt + kAttnWarps - 1) / kAttnWarps;
+    const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
+    const int64_t wgrid = static_cast<int64_t>(a->batch) * a->cache.heads * wtiles;
+    OP_ARG(grid <= kMaxGrid && joins <= kMaxGrid && wgrid <= kMaxGrid, "too many rows in one call");
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    const cudaStream_t s = stream_of(o, a->stream);
+    const bool int8 = a->cache.code == I4D_CODE_INT8;
+    OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
+    if (p.splits > 1) {
+        k_kv8_join<<<static_cast<unsigned>(joins), kAttnThreads, 0, s>>>(d, 8 * p.nt, p.tiles * 8 * p.nt);
+        OP_CK(cudaGetLastError());
+    }
+    if (a->weights && wgrid > 0)
+        OP_CK(int8 ? launch_weights_c<I4D_CODE_INT8>(d, p, wtiles, wgrid, s) : launch_weights_c<I4D_CODE_E4M3>(d, p, wtiles, wgrid, s));
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_evict_workspace(i4d_ctx* ctx, const i4d_kv8_evict_args* a, size_t* bytes_out) {
+    if (!ctx) return I4D_ERR_ARG;
+    const i4d_status st = check_evict(ctx, a);
+    if (st != I4D_OK) return st;
+    OP_ARG(bytes_out, "null bytes_out");
+    *bytes_out = evict_workspace(*a);
+    return I4D_OK;
+}
+
+i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    const i4d_status st = check_evict(ctx, a);
+    if (st != I4D_OK) return st;
+    if (a->batch == 0) return I4D_OK;
+    OP_ARG(a->lengths && a->lengths_out && a->keep && a->block_table && a->weights && a->weights_out, "null buffer");
+    OP_ARG(aligned(a->lengths, 4) && aligned(a->lengths_out, 4) && aligned(a->keep, 4) && aligned(a->block_table, 4) &&
+               aligned(a->weights, 4) && aligned(a->weights_out, 4), "arrays need 4-byte alignment");
+    const int heads = a->cache.heads;
+    OP_ARG(!overlap(span_of(a->lengths, 1, 0, 1, 0, a->batch, 4), span_of(a->lengths_out, 1, 0, 1, 0, a->batch, 4)), "lengths_out overlaps lengths");
+    const Span win = span_of(a->weights, static_cast<int64_t>(a->batch) * heads, a->weights_stride, 1, 0, a->max_length, 4);
+    const Span wout = span_of(a->weights_out, static_cast<int64_t>(a->batch) * heads, a->weights_out_stride, 1, 0, a->max_length, 4);
+    OP_ARG((a->weights == a->weights_out && a->weights_stride == a->weights_out_stride) || !overlap(win, wout), "weights_out overlaps weights");
+    const size_t need = evict_workspace(*a);
+    OP_ARG(need == 0 || (a->workspace && aligned(a->workspace, 16)), "null or misaligned workspace (%zu bytes needed)", need);
+    if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
+    const OpContext o = op_context(ctx);
+    EvictDev d = {};
+    d.cache = cache_dev(a->cache);
+    d.seq = seq_arrays(o, a->cache, nullptr, a->lengths, a->block_table, a->table_stride, 0, 0);
+    d.weights = a->weights;
+    d.weights_out = a->weights_out;
+    d.weights_stride = a->weights_stride;
+    d.weights_out_stride = a->weights_out_stride;
+    d.lengths_out = a->lengths_out;
+    d.keep = a->keep;
+    d.old_scale = static_cast<float*>(a->workspace);
+    d.old_blocks = (a->max_length + a->cache.block_tokens - 1) / a->cache.block_tokens;
+    d.budget = a->budget;
+    d.recent = a->recent;
+    d.max_length = a->max_length;
+    const int slices = (a->cache.dim + 31) / 32;
+    const int64_t rows = static_cast<int64_t>(a->batch) * heads;
+    OP_ARG(rows * 2 * slices <= kMaxGrid, "too many sequences in one call");
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    const cudaStream_t s = stream_of(o, a->stream);
+    k_kv8_select<<<static_cast<unsigned>(rows), kSelectThreads, 0, s>>>(d);
+    OP_CK(cudaGetLastError());
+    if (a->max_length > a->budget) {
+        const unsigned grid = static_cast<unsigned>(rows * 2 * slices);
+        if (a->cache.code == I4D_CODE_INT8) k_kv8_move<I4D_CODE_INT8><<<grid, kMoveThreads, 0, s>>>(d, slices);
+        else k_kv8_move<I4D_CODE_E4M3><<<grid, kMoveThreads, 0, s>>>(d, slices);
+        OP_CK(cudaGetLastError());
+    }
+    return I4D_OK;
+}
+
+i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
+    if (!ctx) return I4D_ERR_ARG;
+    OP_ARG(a, "null arguments");
+    OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
+    OP_ARG(a->rows >= 0 && a->vocab > 0 && a->vocab <= kMaxTokens, "rows %d, vocab %d", a->rows, a->vocab);
+    if (a->rows == 0) return I4D_OK;
+    OP_ARG(a->logits && a->out, "null logits or out");
+    const int bytes = dtype_bytes(a->dtype);
+    OP_ARG(aligned(a->logits, bytes) && aligned(a->out, bytes), "misaligned logits or out");
+    OP_ARG(a->stride >= 0 && (a->rows == 1 || a->out_stride >= a->vocab), "stride %lld, out_stride %lld for %d entries",
+           static_cast<long long>(a->stride), static_cast<long long>(a->out_stride), a->vocab);
+    OP_ARG((a->logits == a->out && a->stride == a->out_stride) ||
+               !overlap(span_of(a->logits, a->rows, a->stride, 1, 0, a->vocab, bytes), span_of(a->out, a->rows, a->out_stride, 1, 0, a->vocab, bytes)),
+           "out overlaps logits");
+    OP_ARG(!a->history || (a->history_len && a->history_stride >= 0 && a->history_stride <= kMaxTokens), "history without history_len, or bad history_stride");
+    OP_ARG(a->history || !(a->repetition || a->frequency || a->presence || a->prompt_len), "penalties without a history");
+    OP_ARG(!a->bias_ids == !a->bias_values && !a->bias_ids == !a->bias_len, "bias_ids, bias_values and bias_len go together");
+    OP_ARG(!a->bias_ids || (a->bias_stride >= 0 && a->bias_stride <= kMaxTokens), "bad bias_stride");
+    OP_ARG(!a->mask || a->mask_stride >= 0, "negative mask_stride");
+    LogitsDev d = {};
+    d.in = a->logits;
+    d.out = a->out;
+    d.best = a->best;
+    d.history = a->history;
+    d.history_len = a->history_len;
+    d.prompt_len = a->prompt_len;
+    d.repetition = a->repetition;
+    d.frequency = a->frequency;
+    d.presence = a->presence;
+    d.bias_ids = a->bias_ids;
+    d.bias_values = a->bias_values;
+    d.bias_len = a->bias_len;
+    d.mask = a->mask;
+    d.stride = a->stride;
+    d.out_stride = a->out_stride;
+    d.history_stride = a->history_stride;
+    d.bias_stride = a->bias_stride;
+    d.mask_stride = a->mask_stride;
+    d.vocab = a->vocab;
+    // CTAs of a row: slices of at least 2048 entries, eight at most (the
+    // portable cluster size), fewer where the rows fill the GPU by themselves.
+    const OpContext o = op_context(ctx);
+    int ctas = 1;
+    while (ctas < 8 && a->vocab / (2 * ctas) >= 2048 && static_cast<int64_t>(a->rows) * ctas < 4 * o.num_sms) ctas *= 2;
+    OP_ARG(static_cast<int64_t>(a->rows) * ctas <= kMaxGrid, "too many rows in one call");
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a->rows * ctas));
+    cfg.blockDim = dim3(kLogitsThreads);
+    cfg.dynamicSmemBytes = 2 * kLogitsSlice * 4;
+    cfg.stream = stream_of(o, a->stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    switch (a->dtype) {
+        case I4D_F32: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<float>, d, ctas)); break;
+        case I4D_BF16: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<__nv_bfloat16>, d, ctas)); break;
+        default: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<__half>, d, ctas)); break;
+    }
+    return I4D_OK;
+}
+
+i4d_status i4d_ops_check(i4d_ctx* ctx, void* stream) {
+    if (!ctx) return I4D_ERR_ARG;
+    const OpContext o = op_context(ctx);
+    DeviceScope scope(o.device);
+    OP_CK(scope.error());
+    OP_CK(cudaStreamSynchronize(stream_of(o, stream)));
+    return ops_report(ctx);
+}
+
+}  // extern "C"

@@ -1,0 +1,178 @@
+// i4d_ops_common.cuh -- helpers of the long-context serving operators.
+//
+// Unlike the decode path these translation units are compiled with
+// multiply-add contraction; where a rounding order is part of an operator's
+// definition it is written with explicit intrinsics.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "i4d.h"
+
+namespace i4d_ops {
+
+// Bits of the operators' device error word.
+constexpr unsigned kBadSequence = 1u;  // q_start or lengths outside what the call's arguments allow
+constexpr unsigned kBadBlock = 2u;     // a block id outside the pool
+
+constexpr int kMaxTokens = 1 << 30;  // of one sequence, so that a block's end is an int
+
+template <int DT>
+struct ElemOf;
+template <>
+struct ElemOf<I4D_F32> { using T = float; };
+template <>
+struct ElemOf<I4D_BF16> { using T = __nv_bfloat16; };
+template <>
+struct ElemOf<I4D_F16> { using T = __half; };
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// N elements by 16-byte accesses (N * sizeof(T) a multiple of 16, aligned).
+template <typename T, int N>
+struct alignas(16) Vec {
+    T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+    Vec<T, N> r;
+    if constexpr (N * sizeof(T) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(N * sizeof(T) / 16); ++i)
+            reinterpret_cast<uint4*>(&r)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = p[i];
+    }
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& r) {
+    if constexpr (N * sizeof(T) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(N * sizeof(T) / 16); ++i)
+            reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&r)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = r.v[i];
+    }
+}
+
+// The arrays that say where the tokens of a batch are.
+struct SeqArrays {
+    const int32_t* q_start;
+    const int32_t* lengths;
+    const int32_t* table;
+    int64_t table_stride;
+    int tokens, max_q, block_tokens, blocks;
+    unsigned* err;
+};
+
+struct Seq {
+    int first, n, len;  // first row, rows, tokens in the cache
+};
+
+// A sequence whose arrays contradict the call's bounds is skipped (n = 0).
+__device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) {
+    const int q0 = __ldg(a.q_start + b), q1 = __ldg(a.q_start + b + 1), len = __ldg(a.lengths + b);
+    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.tokens && q1 - q0 <= a.max_q && len >= q1 - q0 &&
+                    len <= a.table_stride * a.block_tokens && len <= kMaxTokens;
+    if (!ok && report) atomicOr(a.err, kBadSequence);
+    return {q0, ok ? q1 - q0 : 0, ok ? len : 0};
+}
+
+// Block id of a table entry, or -1 for one outside the pool.
+__device__ __forceinline__ int load_block(const SeqArrays& a, int b, int j, bool report) {
+    const int id = __ldg(a.table + static_cast<int64_t>(b) * a.table_stride + j);
+    if (static_cast<unsigned>(id) < static_cast<unsigned>(a.blocks)) return id;
+    if (report) atomicOr(a.err, kBadBlock);
+    return -1;
+}
+
+// ------------------------------------------------------------- 8-bit codes
+
+// Least power of two s >= 2^-126 with amax <= 127 s (INT8) or 448 s (E4M3):
+// amax = f 2^e with f in [1, 2), 127 = 1.984375 * 2^6, 448 = 1.75 * 2^8.
+__device__ __forceinline__ float power_scale(float amax, int code) {
+    const int bits = __float_as_int(amax);
+    const int e = (bits >> 23) - 127, frac = bits & 0x7fffff;
+    int es = code == I4D_CODE_INT8 ? e - 6 + (frac > 0x7e0000) : e - 8 + (frac > 0x600000);
+    es = max(es, -126);
+    return __int_as_float((es + 127) << 23);
+}
+
+// Four codes of y (already divided by the scale): NaN 0, beyond the range the
+// largest code, else the nearest with ties to even.
+template <int CODE>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    a = a == a ? a : 0.f;
+    b = b == b ? b : 0.f;
+    c = c == c ? c : 0.f;
+    d = d == d ? d : 0.f;
+    if constexpr (CODE == I4D_CODE_INT8) {
+        const int ia = __float2int_rn(fminf(fmaxf(a, -127.f), 127.f)), ib = __float2int_rn(fminf(fmaxf(b, -127.f), 127.f));
+        const int ic = __float2int_rn(fminf(fmaxf(c, -127.f), 127.f)), id = __float2int_rn(fminf(fmaxf(d, -127.f), 127.f));
+        return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+    } else {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+        return lo | static_cast<uint32_t>(hi) << 16;
+    }
+}
+
+// The four code values of a word.
+template <int CODE>
+__device__ __forceinline__ void decode4(uint32_t w, float out[4]) {
+    if constexpr (CODE == I4D_CODE_INT8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t h;
+            const uint16_t p = static_cast<uint16_t>(w >> (16 * i));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
+            const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
+            out[2 * i] = f.x;
+            out[2 * i + 1] = f.y;
+        }
+    }
+}
+
+template <int CODE>
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+    float f[4];
+    decode4<CODE>(w, f);
+    return encode4<CODE>(__fmul_rn(f[0], ratio), __fmul_rn(f[1], ratio), __fmul_rn(f[2], ratio), __fmul_rn(f[3], ratio));
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+    return x;
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
+
+}  // namespace i4d_ops

@@ -396,6 +396,219 @@ i4d_status i4d_profile_gemv(i4d_ctx* ctx, int mode, int reps, float* ms_per_gemv
 i4d_status i4d_profile_attention(i4d_ctx* ctx, int layer, uint32_t position, const int32_t* qkv_dev, int fill,
                                  int reps, float* ms_per_step);
 
+/* ---- Long-context serving operators ----
+ * Rotary positions beyond the fixed-point table, a paged KV cache of 8-bit
+ * codes with a scale for each block of tokens and head, attention over it,
+ * eviction from it, and a logits processor ahead of the sampler.  They serve
+ * models and batches other than the built-in one (any head count, several
+ * sequences), next to i4d_attention and i4d_sample; no reference counterpart
+ * (the FPGA design has one sequence, a fixed cache and a fixed RoPE table).
+ *
+ * Every pointer in the argument structs is a device pointer on the context's
+ * device, owned by the caller; strides count elements.  The calls only
+ * enqueue work on `stream` (a cudaStream_t; NULL: the context's stream; pass
+ * cudaStreamLegacy for the legacy default stream), allocate nothing and can be
+ * captured into a graph.  A workspace must not be in use by another call at
+ * the same time: calls on different streams, and graphs that may run at the
+ * same time, need one each.  Arguments that the host can see wrong return
+ * I4D_ERR_ARG and enqueue nothing.  Wrong values in device arrays (a block id
+ * outside the pool, a length beyond the table) never lead to an access out of
+ * bounds: the tokens concerned are skipped and the call's device error bit is
+ * set, which i4d_ops_check reports.
+ *
+ * Sequences.  q_start[0..batch] are the first rows of each sequence in the
+ * packed token arrays (q_start[batch] <= tokens; rows behind it are left as
+ * they are).  lengths[b] counts the tokens of sequence b in the cache, its
+ * new ones included: row i of the n rows of sequence b stands at cache index
+ * lengths[b] - n + i.  max_q bounds every n, max_length every length.  Token
+ * t of sequence b lies in block block_table[b * table_stride + t /
+ * block_tokens]; the blocks that a call writes must differ from each other. */
+#define I4D_F32 0
+#define I4D_BF16 1
+#define I4D_F16 2
+#define I4D_CODE_INT8 0
+#define I4D_CODE_E4M3 1
+
+#define I4D_ROPE_PLAIN 0  /* f_i = base^(-2i/rot_dim) radians per position */
+#define I4D_ROPE_LINEAR 1 /* f_i / factor */
+#define I4D_ROPE_BASE 2   /* base * factor^(rot_dim/(rot_dim-2)) in place of base */
+#define I4D_ROPE_PARTS 3  /* f_i (g + (1-g)/factor), g = clamp((original_length f_i/2pi - low)/(high - low), 0, 1) */
+
+/* Fills turns_out[rot_dim / 2] (host memory) with the frequencies as turns
+ * per position in units of 2^-64: position * turns modulo 2^64 is the angle's
+ * fraction of a turn to within 2^-33 turns at any 32-bit position. */
+i4d_status i4d_rope_frequencies(int rot_dim, double base, int scaling, double factor, double original_length,
+                                double low, double high, uint64_t* turns_out);
+
+/* Rotary positions of q [tokens][q_heads][dim] and k [tokens][k_heads][dim]
+ * (k may be NULL): with (c, s) = magnitude * (cos, sin) of the angle of
+ * positions[t] and turns[i], pair (a, b) becomes (a c - b s, b c + a s); pair
+ * i of a head is elements (2i, 2i+1) (interleaved) or (i, i + rot_dim/2).
+ * Elements from rot_dim on are copied.  inverse != 0 rotates back (the
+ * transpose).  q_out may be q with the same strides (in place); otherwise
+ * outputs must not overlap inputs.  Rotated in FP32, rounded once. */
+typedef struct i4d_rope_args {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const int32_t* positions; /* [tokens], negative ones allowed */
+    const uint64_t* turns;    /* device copy of i4d_rope_frequencies' table */
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride;
+    int64_t q_out_stride, q_out_head_stride, k_out_stride, k_out_head_stride;
+    int tokens, q_heads, k_heads, dim, rot_dim;
+    int interleaved, inverse, dtype;
+    float magnitude;
+    void* stream;
+} i4d_rope_args;
+i4d_status i4d_rope(i4d_ctx* ctx, const i4d_rope_args* args);
+
+/* The cache: codes [blocks][heads][block_tokens][dim] (16-byte aligned) and
+ * scales [blocks][heads]; a value is code * scale.  block_tokens 16, 32, 64 or
+ * 128; dim a multiple of 16 up to 256. */
+typedef struct i4d_kv8 {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int blocks, heads, block_tokens, dim, code;
+} i4d_kv8;
+
+/* Writes the rows k, v [tokens][heads][dim] of every sequence into the cache.
+ * A block's scale becomes the least power of two s >= 2^-126 with
+ * amax <= 127 s (INT8) or 448 s (E4M3) over the new values of its head, and
+ * not less than its former scale if the block holds earlier tokens of the
+ * sequence, whose codes are then rewritten as round(code * old / s).  New
+ * codes are round(x / s), ties to even; NaN is stored as 0 and infinities as
+ * the largest code, and neither counts for amax.  Bytes of the block behind
+ * the sequence's last token are left as they are. */
+typedef struct i4d_kv8_append_args {
+    i4d_kv8 cache;
+    const void* k;
+    const void* v;
+    int64_t k_stride, k_head_stride, v_stride, v_head_stride;
+    const int32_t* q_start;
+    const int32_t* lengths;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int batch, tokens, max_q, dtype;
+    void* stream;
+} i4d_kv8_append_args;
+i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* args);
+
+/* Reads rows back as BF16 values, k_out and v_out [tokens][heads][dim]
+ * contiguous and 16-byte aligned: row i of the n rows of sequence b is the
+ * token at cache index lengths[b] - n + i (what i4d_kv8_append with the same
+ * arrays wrote; exact for scales that are powers of two). */
+typedef struct i4d_kv8_read_args {
+    i4d_kv8 cache;
+    void* k_out;
+    void* v_out;
+    const int32_t* q_start;
+    const int32_t* lengths;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int batch, tokens, max_q;
+    void* stream;
+} i4d_kv8_read_args;
+i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* args);
+
+/* Attention of q [tokens][heads][dim] over the cache; heads is a multiple of
+ * the cache's heads, query head h reads cache head h / (heads / cache heads).
+ * A row at cache index p sees the tokens j <= p and, with window > 0,
+ * j > p - window.  out (q's type) = softmax(scale q.k) v; lse [tokens][heads]
+ * FP32 (may be NULL) the logarithm of the softmax sum.  A row that sees
+ * nothing gives zeros and -inf.  weights (may be NULL): FP32
+ * [batch][cache heads][weights_stride], to whose first max_length entries of
+ * a head the probabilities are added that the call's rows of that head gave
+ * each token (what i4d_kv8_evict reads); the order of the sum is fixed.
+ * out must not overlap q.  workspace: i4d_kv8_attention_workspace bytes,
+ * 16-byte aligned (NULL where that is 0); nothing in it is kept. */
+typedef struct i4d_kv8_attention_args {
+    i4d_kv8 cache;
+    const void* q;
+    void* out;
+    float* lse;
+    float* weights;
+    int64_t q_stride, q_head_stride, out_stride, out_head_stride, weights_stride;
+    const int32_t* q_start;
+    const int32_t* lengths;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int batch, tokens, heads, max_q, max_length, window, dtype;
+    float scale;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} i4d_kv8_attention_args;
+i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* args);
+i4d_status i4d_kv8_attention_workspace(i4d_ctx* ctx, const i4d_kv8_attention_args* args, size_t* bytes_out);
+
+/* Brings every sequence that is longer than `budget` back to budget tokens,
+ * for each cache head on its own: its last `recent` tokens stay, and of the
+ * others the budget - recent of greatest weight (ties: the lower index; NaN
+ * counts as the least).  The kept tokens move up in their order within the
+ * sequence's own blocks, so the blocks behind the new length are free.  A
+ * block's scale becomes the greatest of the scales its tokens had, codes
+ * round(code * had / greatest).  keep [batch][cache heads][budget] receives
+ * the kept cache indices in order (-1 behind a shorter sequence's length),
+ * lengths_out [batch] the new lengths, weights_out the kept tokens' weights
+ * with zeros up to the old length; weights_out may be weights itself (same
+ * stride).  lengths_out must not overlap lengths.  Each sequence's blocks
+ * must be its own.  Shorter sequences keep their tokens and weights. */
+typedef struct i4d_kv8_evict_args {
+    i4d_kv8 cache;
+    const float* weights;
+    float* weights_out;
+    int64_t weights_stride, weights_out_stride;
+    const int32_t* lengths;
+    int32_t* lengths_out;
+    int32_t* keep;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int batch, budget, recent, max_length;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} i4d_kv8_evict_args;
+i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* args);
+i4d_status i4d_kv8_evict_workspace(i4d_ctx* ctx, const i4d_kv8_evict_args* args, size_t* bytes_out);
+
+/* Logits processor, rows x vocab, in the order: a token of history[row][0,
+ * history_len) is divided by repetition (logit > 0) or multiplied by it; a
+ * token that occurs n > 0 times from index prompt_len on loses frequency * n,
+ * then presence; bias_values are added at bias_ids (those of one id summed
+ * in their order first); a token whose bit in mask (bit id % 32 of word id / 32) is 0 becomes
+ * -inf.  FP32 steps, each rounded once, stored in the logits' type.  best (may
+ * be NULL) receives the lowest index of the greatest stored logit that is
+ * neither NaN nor -inf, or -1.  Every array but logits and out may be NULL;
+ * ids outside [0, vocab) are ignored; out may be logits with the same stride.
+ * Entries from vocab to the stride are left as they are. */
+typedef struct i4d_logits_args {
+    const void* logits;
+    void* out;
+    int32_t* best;
+    const int32_t* history;
+    const int32_t* history_len;
+    const int32_t* prompt_len; /* NULL: 0 */
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_ids;
+    const float* bias_values;
+    const int32_t* bias_len;
+    const uint32_t* mask;
+    int64_t stride, out_stride, history_stride, bias_stride, mask_stride;
+    int rows, vocab, dtype;
+    void* stream;
+} i4d_logits_args;
+i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* args);
+
+/* Waits for `stream` (as above) and reports the device error bits of the
+ * operators above since the last check: I4D_ERR_ARG and a message naming what
+ * was out of range.  i4d_sync reports them too, for the context's stream. */
+i4d_status i4d_ops_check(i4d_ctx* ctx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
