@@ -1,11 +1,13 @@
 // i4d_kv8_attn.cuh -- attention over the cache of 8-bit codes.
 //
 // k_kv8_attn: eight (or sixteen) query rows of one cache head against a chunk
-// of its tokens.  Codes go from memory to registers in 16-byte pieces and are
-// never staged: the order of the summation index of a matrix instruction is
-// free, so a thread's 16 contiguous codes of a token serve as its part of four
-// steps of K q, and a V^T tile takes the codes of the four tokens whose
-// probabilities the thread holds.  The products are transposed (tokens x rows,
+// of its tokens.  Each warp takes tiles of 16 tokens, which it copies
+// asynchronously into a ring of its own in shared memory, three tiles ahead,
+// so no warp waits for another before the end.  The order of the summation
+// index of a matrix instruction is free, so a thread's 16 contiguous codes of
+// a token serve as its part of four steps of K q, and a V^T tile takes the
+// codes of the four tokens whose probabilities the thread holds: codes go from
+// shared memory to registers in 16-byte pieces without a transposition.  The products are transposed (tokens x rows,
 // then dims x rows), which wastes half as much of a 16 x 8 tile on few rows.
 //   scores   S^T [16 tokens x 8 rows] = K [16 x dim] Q^T     (m16n8k16, FP16 in, FP32 sums)
 //   output   O^T [16 dims x 8 rows]  += V^T [16 x 16 tokens] P^T
@@ -48,6 +50,7 @@ struct AttnDev {
     int splits, chunk; // token chunks of a tile
     float* part;       // workspace: [tile][split][rows][dim + 4]: O, M, l, R
     float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
+    float* scores;     // workspace (few rows, with weights): [tile][rows][max_length], log2 scale
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -179,12 +182,54 @@ __device__ __forceinline__ void load_ktile(const uint8_t* k, int dim, int n, KTi
         }
 }
 
+// Where 16-byte piece c of row r of a tile lies in its shared-memory row, so
+// that the eight lanes of an access phase hit all banks: they read pieces of
+// two rows of K, and of four even (or odd) rows of V.
+template <int DT>
+__device__ __forceinline__ int k_piece(int r, int c) {
+    return DT == 64 ? c : c ^ ((r & 1) << 2);
+}
+template <int DT>
+__device__ __forceinline__ int v_piece(int r, int c) {
+    return DT == 64 ? c ^ ((r >> 1) & 2) : DT == 128 ? c ^ (r & 6) : c ^ (((r >> 1) & 1) | (r & 4));
+}
+
+// Copies n of the 16 tokens at k and v into a ring slot [K: 16][DT], [V: 16][DT]; zeros elsewhere.
+template <int DT>
+__device__ __forceinline__ void copy_tile(uint32_t slot, const uint8_t* k, const uint8_t* v, int dim, int n) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < DT / 32; ++i) {
+        const int e = i * 32 + lane, r = e / (DT / 16), c = e % (DT / 16);
+        const int bytes = r < n && c * 16 < dim ? 16 : 0;
+        const int from = bytes ? r * dim + c * 16 : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + r * DT + k_piece<DT>(r, c) * 16), "l"(k + from), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + 16 * DT + r * DT + v_piece<DT>(r, c) * 16), "l"(v + from), "r"(bytes) : "memory");
+    }
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void read_ktile(uint32_t slot, KTile<DT>& kt) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < DT / 64; ++c) kt.w[r][c] = lds16(slot + (g + 8 * r) * DT + k_piece<DT>(g + 8 * r, t + 4 * c) * 16);
+}
+
 template <int DT, int CODE, int NT, bool HL>
 __device__ __forceinline__ void score_tile(const KTile<DT>& kt, const QTile<DT, NT, HL>& q, float s[NT][4]) {
+    float odd[NT][4];  // two chains of dependent sums
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+        for (int i = 0; i < 4; ++i) s[nt][i] = odd[nt][i] = 0.f;
 #pragma unroll
     for (int c = 0; c < DT / 64; ++c) {
         const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&kt.w[0][c]);
@@ -195,11 +240,16 @@ __device__ __forceinline__ void score_tile(const KTile<DT>& kt, const QTile<DT, 
             const uint32_t f[4] = {halves<CODE, 0>(x), halves<CODE, 0>(y), halves<CODE, 1>(x), halves<CODE, 1>(y)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                mma(s[nt], f, q.hi[nt][c * 4 + i][0], q.hi[nt][c * 4 + i][1]);
-                if constexpr (HL) mma(s[nt], f, q.lo[nt][c * 4 + i][0], q.lo[nt][c * 4 + i][1]);
+                float* sum = i & 1 ? odd[nt] : s[nt];
+                mma(sum, f, q.hi[nt][c * 4 + i][0], q.hi[nt][c * 4 + i][1]);
+                if constexpr (HL) mma(sum, f, q.lo[nt][c * 4 + i][0], q.lo[nt][c * 4 + i][1]);
             }
         }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] += odd[nt][i];
 }
 
 // V codes of 16 tokens: the thread's DT / 8 dims (from (lane / 4) * DT / 8) of
@@ -210,21 +260,18 @@ struct VTile {
 };
 
 template <int DT>
-__device__ __forceinline__ void load_vtile(const uint8_t* v, int dim, int n, VTile<DT>& vt) {
+__device__ __forceinline__ void read_vtile(uint32_t slot, VTile<DT>& vt) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int tok = 2 * t + (r & 1) + (r >> 1) * 8;
+        const uint32_t row = slot + 16 * DT + tok * DT;
         if constexpr (DT == 64) {
-            const bool live = tok < n && g * 8 < dim;
-            const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(v + tok * dim + g * 8)) : make_uint2(0, 0);
-            vt.w[r][0] = x.x;
-            vt.w[r][1] = x.y;
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vt.w[r][0]), "=r"(vt.w[r][1]) : "r"(row + v_piece<DT>(tok, g >> 1) * 16 + (g & 1) * 8) : "memory");
         } else {
 #pragma unroll
             for (int c = 0; c < DT / 128; ++c) {
-                const int d0 = g * (DT / 8) + c * 16;
-                const uint4 x = tok < n && d0 < dim ? __ldg(reinterpret_cast<const uint4*>(v + tok * dim + d0)) : make_uint4(0, 0, 0, 0);
+                const uint4 x = lds16(row + v_piece<DT>(tok, g * (DT / 128) + c) * 16);
                 vt.w[r][4 * c] = x.x;
                 vt.w[r][4 * c + 1] = x.y;
                 vt.w[r][4 * c + 2] = x.z;
@@ -258,12 +305,25 @@ __device__ __forceinline__ int2 row_span(const AttnDev& a, int pos) {
     return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, pos + 1);
 }
 
-template <int DT, int CODE, int NT, bool HL>
-__global__ void __launch_bounds__(kAttnThreads) k_kv8_attn(AttnDev a) {
-    constexpr int kRows = 8 * NT;
-    constexpr int kSub = DT == 256 ? 1 : 2;  // 16-token tiles a step
-    constexpr int kStep = 16 * kSub;
-    __shared__ float merge[kAttnWarps][kRows][DT + 4];
+template <int DT>
+constexpr int kAttnSlots = DT == 256 ? 3 : DT == 128 ? 4 : 6;  // ring slots of a warp
+constexpr int kAttnBlocks = 256; // table entries a chunk can hold
+
+template <int DT, int NT>
+constexpr size_t attn_smem() {
+    const size_t ring = static_cast<size_t>(kAttnWarps) * kAttnSlots<DT> * 32 * DT;
+    const size_t merge = static_cast<size_t>(kAttnWarps) * 8 * NT * (DT + 4) * sizeof(float);
+    return ring > merge ? ring : merge;
+}
+
+// HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
+template <int DT, int CODE, int NT, bool HLQ, bool HLP>
+__global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_kv8_attn(AttnDev a) {
+    constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
+    extern __shared__ __align__(16) unsigned char attn_ring[];
+    __shared__ int s_id[kAttnBlocks];
+    __shared__ float2 s_scale[kAttnBlocks];
+    float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % a.splits;
     const int64_t tile = blockIdx.x / a.splits;
@@ -281,13 +341,8 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_attn(AttnDev a) {
     const int last_row = min(row0 + kRows, s.n * a.group) - 1;
     // tokens that any row of the tile sees, and that all of them see
     const int2 lo_span = row_span(a, first + row0 / a.group), hi_span = row_span(a, first + last_row / a.group);
-    const int begin = max(lo_span.x, split * a.chunk), end = min(hi_span.y, (split + 1) * a.chunk);
+    const int begin = max(lo_span.x, split * a.chunk) & ~15, end = min(hi_span.y, (split + 1) * a.chunk);
     const int all_from = hi_span.x, all_to = lo_span.y;
-    int2 span[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) span[nt][j] = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
 
     float M[NT][2], R[NT][2], l[NT][2], to_r[NT][2], acc[DT / 16][NT][4];
 #pragma unroll
@@ -305,113 +360,126 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_attn(AttnDev a) {
             for (int j = 0; j < 4; ++j) acc[i][nt][j] = 0.f;
 
     if (begin < end) {
-        QTile<DT, NT, HL> q;
-        load_qtile<DT, NT, HL>(a, s, h, row0, q);
-        const int bs = a.cache.block_tokens, dim = a.cache.dim;
-        for (int tok = (begin & ~15) + warp * kStep; tok < end; tok += kAttnWarps * kStep) {
-            KTile<DT> kt[kSub];
-            VTile<DT> vt[kSub];
-            float ks[kSub], vs[kSub];
-            int live[kSub];  // tokens of the 16 that are there
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                const int at = tok + 16 * u;
-                int id = -1;
-                if (at < end) id = load_block(a.seq, b, at / bs, lane == 0);
-                live[u] = id < 0 ? 0 : min(16, end - at);
-                ks[u] = vs[u] = 0.f;
-                const uint8_t *kp = nullptr, *vp = nullptr;
-                if (id >= 0) {
-                    const int64_t off = code_offset(a.cache, id, h) + static_cast<int64_t>(at % bs) * dim;
-                    kp = a.cache.codes[0] + off;
-                    vp = a.cache.codes[1] + off;
-                    ks[u] = __ldg(a.cache.scale[0] + static_cast<int64_t>(id) * a.cache.heads + h);
-                    vs[u] = __ldg(a.cache.scale[1] + static_cast<int64_t>(id) * a.cache.heads + h);
-                }
-                load_ktile<DT>(kp, dim, live[u], kt[u]);
-                load_vtile<DT>(vp, dim, live[u], vt[u]);
+        const int bs = a.cache.block_tokens, dim = a.cache.dim, shift = 31 - __clz(bs);
+        const int blk0 = begin >> shift;
+        for (int i = threadIdx.x; i <= ((end - 1) >> shift) - blk0; i += kAttnThreads) {
+            const int id = load_block(a.seq, b, blk0 + i, true);
+            s_id[i] = id;
+            if (id >= 0) {
+                const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
+                s_scale[i] = make_float2(__ldg(a.cache.scale[0] + at), __ldg(a.cache.scale[1] + at));
             }
-            float x[kSub][NT][4];
-            float top[NT][2], rtop[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) top[nt][j] = rtop[nt][j] = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                const int at = tok + 16 * u;
-                score_tile<DT, CODE, NT, HL>(kt[u], q, x[u]);
-                const float lvs = __log2f(vs[u]);  // only a bound: its rounding cancels
-                const bool whole = live[u] == 16 && at >= all_from && at + 16 <= all_to;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = i & 1, n = g + (i >> 1) * 8;
-                        float y = x[u][nt][i] * (q.factor[nt][j] * ks[u]);
-                        if (!whole && !(n < live[u] && at + n >= span[nt][j].x && at + n < span[nt][j].y)) y = -INFINITY;
-                        x[u][nt][i] = y;
-                        top[nt][j] = fmaxf(top[nt][j], y);
-                        rtop[nt][j] = fmaxf(rtop[nt][j], y + lvs);
-                    }
+        }
+        __syncthreads();
+        const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(attn_ring)) + warp * kSlots * 32 * DT;
+        const int tiles = (end - begin + 15) / 16;
+        auto issue = [&](int i, int slot) {
+            if (i < tiles) {
+                const int at = begin + 16 * i, id = s_id[(at >> shift) - blk0];
+                const int64_t off = id < 0 ? 0 : code_offset(a.cache, id, h) + static_cast<int64_t>(at & (bs - 1)) * dim;
+                copy_tile<DT>(ring + slot * 32 * DT, a.cache.codes[0] + off, a.cache.codes[1] + off, dim, id < 0 ? 0 : min(16, end - at));
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
+        QTile<DT, NT, HLQ> q;
+        load_qtile<DT, NT, HLQ>(a, s, h, row0, q);
+        int slot = 0;
+        for (int i = warp; i < tiles; i += kAttnWarps) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+            __syncwarp();  // this slot's copies of all lanes have landed; all lanes are done with the one to fill
+            issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
+            const uint32_t at_slot = ring + slot * 32 * DT;
+            slot = slot == kSlots - 1 ? 0 : slot + 1;
+            const int at = begin + 16 * i, entry = (at >> shift) - blk0;
+            if (s_id[entry] < 0) continue;
+            const float2 scale = s_scale[entry];
+            const int live = min(16, end - at);
+            float x[NT][4];
+            {
+                KTile<DT> kt;
+                read_ktile<DT>(at_slot, kt);
+                score_tile<DT, CODE, NT, HLQ>(kt, q, x);
+            }
+            VTile<DT> vt;
+            read_vtile<DT>(at_slot, vt);
+            float top[NT][2], lvs = __log2f(scale.y);  // only a bound: its rounding cancels
+            const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
             bool raise = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) raise |= top[nt][j] > M[nt][j] + kSlack || rtop[nt][j] > R[nt][j] + kSlack;
+                for (int j = 0; j < 2; ++j) {
+                    const float f = q.factor[nt][j] * scale.x;
+                    float y0 = x[nt][j] * f, y1 = x[nt][j + 2] * f;
+                    if (!whole) {
+                        const int2 span = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
+                        if (!(g < live && at + g >= span.x && at + g < span.y)) y0 = -INFINITY;
+                        if (!(g + 8 < live && at + g + 8 >= span.x && at + g + 8 < span.y)) y1 = -INFINITY;
+                    }
+                    x[nt][j] = y0;
+                    x[nt][j + 2] = y1;
+                    top[nt][j] = fmaxf(y0, y1);
+                    raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + kSlack;
+                }
             if (__any_sync(~0u, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float m = top[nt][j], r = rtop[nt][j];
+                        float m = top[nt][j];
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) {
-                            m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                            r = fmaxf(r, __shfl_xor_sync(~0u, r, o));
-                        }
+                        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                        const float r = fmaxf(m + lvs, R[nt][j]);
                         m = fmaxf(m, M[nt][j]);
-                        r = fmaxf(r, R[nt][j]);
                         const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
                         l[nt][j] *= fm;
 #pragma unroll
-                        for (int i = 0; i < DT / 16; ++i) {
-                            acc[i][nt][j] *= fr;
-                            acc[i][nt][j + 2] *= fr;
+                        for (int i2 = 0; i2 < DT / 16; ++i2) {
+                            acc[i2][nt][j] *= fr;
+                            acc[i2][nt][j + 2] *= fr;
                         }
                         M[nt][j] = m;
                         R[nt][j] = r;
                         to_r[nt][j] = r == -INFINITY ? 0.f : ex2(m - r);
                     }
             }
+            if (a.scores) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                uint32_t p[NT][2], pl[NT][2];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = i & 1;
-                        const float e = ex2(x[u][nt][i] - (M[nt][j] == -INFINITY ? 0.f : M[nt][j]));
-                        l[nt][j] += e;
-                        w[i] = e * (to_r[nt][j] * vs[u]);
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = nt * 8 + 2 * t + (k & 1), n = g + (k >> 1) * 8;
+                        if (n < live) a.scores[(tile * kRows + r) * a.max_length + at + n] = x[nt][k];
                     }
+            }
+            uint32_t p[NT][2], pl[NT][2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
-                        p[nt][r] = transpose8(hi);
-                        pl[nt][r] = 0;
-                        if constexpr (HL) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
-                        }
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = k & 1;
+                    const float e = ex2(x[nt][k] - (M[nt][j] == -INFINITY ? 0.f : M[nt][j]));
+                    l[nt][j] += e;
+                    w[k] = e * (to_r[nt][j] * scale.y);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
+                    p[nt][r] = transpose8(hi);
+                    pl[nt][r] = 0;
+                    if constexpr (HLP) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
                     }
                 }
-                value_tile<DT, CODE, NT, HL>(vt[u], p, pl, acc);
             }
+            value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the ring is free for the join
     }
 
     // Join the four warps.
@@ -520,6 +588,26 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
         if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
         if (a.weights) a.lse2[tok * a.heads + head] = l2;
     }
+}
+
+// Probabilities summed over a head's few rows for each token, from the scores
+// that k_kv8_attn kept: one thread for a token, rows in order.
+__global__ void __launch_bounds__(256) k_kv8_weights_kept(AttnDev a, int rows_per_tile, int chunks) {
+    const int64_t bh = blockIdx.x / chunks;
+    const int n = (blockIdx.x % chunks) * 256 + threadIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
+    const Seq s = load_seq(a.seq, b, false);
+    if (s.len > a.max_length || s.n == 0 || n >= s.len) return;
+    if (load_block(a.seq, b, n / a.cache.block_tokens, false) < 0) return;
+    const int rows = s.n * a.group, first = s.len - s.n;
+    float sum = 0.f;
+    for (int row = 0; row < rows; ++row) {
+        const int2 sp = row_span(a, first + row / a.group);
+        if (n < sp.x || n >= sp.y) continue;  // not written
+        const int64_t at = (bh * a.row_tiles + row / rows_per_tile) * rows_per_tile + row % rows_per_tile;
+        const float l2 = a.lse2[(s.first + row / a.group) * static_cast<int64_t>(a.heads) + h * a.group + row % a.group];
+        sum += ex2(a.scores[at * a.max_length + n] - l2);
+    }
+    a.weights[bh * a.weights_stride + n] += sum;
 }
 
 // Probabilities summed over a head's rows for each token: the scores again,

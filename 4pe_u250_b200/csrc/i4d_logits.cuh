@@ -46,9 +46,9 @@ __device__ __forceinline__ unsigned long long logit_key(float x, int index) {
 
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas) {
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
-    int* counts = reinterpret_cast<int*>(smem);                  // bit 0: seen in the prompt, above: 2 * occurrences after it
+    int* counts = reinterpret_cast<int*>(logits_smem);                  // bit 0: seen in the prompt, above: 2 * occurrences after it
     float* bias = reinterpret_cast<float*>(counts + kLogitsSlice);
     __shared__ unsigned long long keys[kLogitsThreads / 32];
     __shared__ unsigned long long cta_key[16];

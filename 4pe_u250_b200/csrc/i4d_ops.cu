@@ -165,7 +165,8 @@ struct AttnPlan {
     int dt, nt;  // padded dim, row tiles of eight a CTA
     int row_tiles, splits, chunk;
     int64_t tiles;
-    size_t part_bytes, lse2_bytes;
+    size_t part_bytes, lse2_bytes, score_bytes;
+    size_t bytes() const { return part_bytes + lse2_bytes + score_bytes; }
 };
 
 AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
@@ -176,15 +177,22 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     p.nt = rows > 8 && a.dtype != I4D_F32 && p.dt <= 128 ? 2 : 1;
     p.row_tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
     p.tiles = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
-    // Chunks: enough CTAs for four on every SM, none under 256 tokens.
-    const int64_t want = std::max<int64_t>(1, 4 * o.num_sms / std::max<int64_t>(1, p.tiles));
+    // Chunks: a few CTAs for each place on the GPU, so that ragged lengths even
+    // out, but none under 128 tokens (two tiles a warp) nor above what the
+    // kernel's table of blocks holds.
+    const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 3) * static_cast<int64_t>(o.num_sms);
+    const int64_t want = std::max<int64_t>(1, 4 * places / std::max<int64_t>(1, p.tiles));
     int64_t chunk = (a.max_length + want - 1) / want;
-    chunk = std::max<int64_t>(256, (chunk + 127) / 128 * 128);
+    chunk = std::min<int64_t>(std::max<int64_t>(128, (chunk + 127) / 128 * 128), kAttnBlocks * c.block_tokens / 2);
     p.chunk = static_cast<int>(chunk);
     p.splits = static_cast<int>(std::max<int64_t>(1, (a.max_length + chunk - 1) / chunk));
-    if (p.splits > 1) p.part_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * (c.dim + 4) * sizeof(float);
-    if (a.weights) p.lse2_bytes = static_cast<size_t>(a.tokens) * a.heads * sizeof(float);
-    p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+    const auto round16 = [](size_t n) { return (n + 15) / 16 * 16; };
+    if (p.splits > 1) p.part_bytes = round16(static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * (c.dim + 4) * sizeof(float));
+    if (a.weights) {
+        p.lse2_bytes = round16(static_cast<size_t>(a.tokens) * a.heads * sizeof(float));
+        // Few rows: their scores are kept (4 bytes a row against a token's codes read again).
+        if (rows <= 32) p.score_bytes = static_cast<size_t>(p.tiles) * 8 * p.nt * a.max_length * sizeof(float);
+    }
     return p;
 }
 
@@ -204,19 +212,37 @@ i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     return I4D_OK;
 }
 
-template <int DT, int CODE, int NT, bool HL>
+template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 cudaError_t launch_attn(const AttnDev& d, int64_t grid, cudaStream_t st) {
-    k_kv8_attn<DT, CODE, NT, HL><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d);
+    static_assert(attn_smem<DT, NT>() <= 114688, "two CTAs an SM");
+    k_kv8_attn<DT, CODE, NT, HLQ, HLP><<<static_cast<unsigned>(grid), kAttnThreads, attn_smem<DT, NT>(), st>>>(d);
     return cudaGetLastError();
 }
 
 template <int DT, int CODE>
 cudaError_t launch_attn_d(const AttnDev& d, const AttnPlan& p, int64_t grid, cudaStream_t st) {
-    if (d.dtype == I4D_F32) return launch_attn<DT, CODE, 1, true>(d, grid, st);
+    if (d.dtype == I4D_F32) return launch_attn<DT, CODE, 1, true, true>(d, grid, st);
     if constexpr (DT <= 128) {
-        if (p.nt == 2) return launch_attn<DT, CODE, 2, false>(d, grid, st);
+        if (p.nt == 2) return d.dtype == I4D_F16 ? launch_attn<DT, CODE, 2, false, true>(d, grid, st) : launch_attn<DT, CODE, 2, false, false>(d, grid, st);
     }
-    return launch_attn<DT, CODE, 1, false>(d, grid, st);
+    return d.dtype == I4D_F16 ? launch_attn<DT, CODE, 1, false, true>(d, grid, st) : launch_attn<DT, CODE, 1, false, false>(d, grid, st);
+}
+
+template <int DT, int CODE, int NT, bool HLQ, bool HLP>
+cudaError_t attn_attr() {
+    return cudaFuncSetAttribute(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(attn_smem<DT, NT>()));
+}
+
+template <int DT, int CODE>
+cudaError_t attn_attrs() {
+    cudaError_t e = attn_attr<DT, CODE, 1, true, true>();
+    if (e == cudaSuccess) e = attn_attr<DT, CODE, 1, false, true>();
+    if (e == cudaSuccess) e = attn_attr<DT, CODE, 1, false, false>();
+    if constexpr (DT <= 128) {
+        if (e == cudaSuccess) e = attn_attr<DT, CODE, 2, false, true>();
+        if (e == cudaSuccess) e = attn_attr<DT, CODE, 2, false, false>();
+    }
+    return e;
 }
 
 template <int CODE>
@@ -265,6 +291,12 @@ cudaError_t ops_init() {
     cudaError_t e = cudaFuncSetAttribute(k_logits<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
+    if (e == cudaSuccess) e = attn_attrs<64, I4D_CODE_INT8>();
+    if (e == cudaSuccess) e = attn_attrs<64, I4D_CODE_E4M3>();
+    if (e == cudaSuccess) e = attn_attrs<128, I4D_CODE_INT8>();
+    if (e == cudaSuccess) e = attn_attrs<128, I4D_CODE_E4M3>();
+    if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_INT8>();
+    if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_E4M3>();
     return e;
 }
 
@@ -455,7 +487,7 @@ i4d_status i4d_kv8_attention_workspace(i4d_ctx* ctx, const i4d_kv8_attention_arg
     if (st != I4D_OK) return st;
     OP_ARG(bytes_out, "null bytes_out");
     const AttnPlan p = attn_plan(op_context(ctx), *a);
-    *bytes_out = p.part_bytes + p.lse2_bytes;
+    *bytes_out = p.bytes();
     return I4D_OK;
 }
 
@@ -476,7 +508,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     OP_ARG(!a->weights || a->weights_stride >= a->max_length, "weights' rows are shorter than max_length");
     const OpContext o = op_context(ctx);
     const AttnPlan p = attn_plan(o, *a);
-    const size_t need = p.part_bytes + p.lse2_bytes;
+    const size_t need = p.bytes();
     OP_ARG(need == 0 || (a->workspace && aligned(a->workspace, 16)), "null or misaligned workspace (%zu bytes needed)", need);
     if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
     AttnDev d = {};
@@ -502,6 +534,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.chunk = p.chunk;
     d.part = static_cast<float*>(a->workspace);
     d.lse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + p.part_bytes);
+    if (p.score_bytes) d.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + p.part_bytes + p.lse2_bytes);
     const int64_t grid = p.tiles * p.splits;
     const int64_t joins = (p.tiles * 8 * p.nt + kAttnWarps - 1) / kAttnWarps;
     const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
@@ -516,7 +549,13 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
         k_kv8_join<<<static_cast<unsigned>(joins), kAttnThreads, 0, s>>>(d, 8 * p.nt, p.tiles * 8 * p.nt);
         OP_CK(cudaGetLastError());
     }
-    if (a->weights && wgrid > 0)
+    if (d.scores) {
+        const int chunks = (a->max_length + 255) / 256;
+        if (chunks > 0) {
+            k_kv8_weights_kept<<<static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 256, 0, s>>>(d, 8 * p.nt, chunks);
+            OP_CK(cudaGetLastError());
+        }
+    } else if (a->weights && wgrid > 0)
         OP_CK(int8 ? launch_weights_c<I4D_CODE_INT8>(d, p, wtiles, wgrid, s) : launch_weights_c<I4D_CODE_E4M3>(d, p, wtiles, wgrid, s));
     return I4D_OK;
 }
