@@ -2,6 +2,7 @@
 
   libi4d.so        the CUDA decode library (sm_100a) behind include/i4d.h
   libi4d_synth.so  seeded synthetic model images in the reference format
+  _i4d_torch.so    torch binding of the long-context operators
   i4d_decode       C++ host program over libi4d (replaces decode_host)
   csrc/gen/*       build-time tables (expf constants and exceptions)
 
@@ -103,6 +104,24 @@ def build_i4d():
     return out
 
 
+def build_torch():
+    """The torch binding of the long-context operators, against this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    src = os.path.join(CSRC, "i4d_torch.cpp")
+    out = os.path.join(HERE, "_i4d_torch.so")
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    if _newer(out, [src, os.path.join(ROOT, "include", "i4d.h"), os.path.join(HERE, "libi4d.so")]):
+        inc = [sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), *include_paths()]
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+              *[f"-I{i}" for i in inc], src, "-o", out, "-L" + HERE, "-l:libi4d.so", "-Wl,-rpath,$ORIGIN", "-L" + lib,
+              "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"])
+    return out
+
+
 def build_host():
     src = os.path.join(CSRC, "host", "i4d_decode.cpp")
     out = os.path.join(HERE, "i4d_decode")
@@ -126,6 +145,7 @@ def build_oracle():
 def main():
     build_synth()
     build_i4d()
+    build_torch()
     build_host()
     build_oracle()
 

@@ -33,7 +33,7 @@ struct LogitsDev {
     const int32_t* bias_len;
     const uint32_t* mask;
     int64_t stride, out_stride, history_stride, bias_stride, mask_stride;
-    int vocab;
+    int vocab, history_max, bias_max;
 };
 
 // Greater value, greater key; of equal values the lower index.  0: none.
@@ -58,9 +58,9 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
     const int32_t* hist = a.history ? a.history + row * a.history_stride : nullptr;
-    const int n_hist = hist ? static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.history_len + row), 0)), a.history_stride)) : 0;
+    const int n_hist = hist ? min(max(__ldg(a.history_len + row), 0), a.history_max) : 0;
     const int n_prompt = hist && a.prompt_len ? __ldg(a.prompt_len + row) : 0;
-    const int n_bias = a.bias_ids ? static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.bias_len + row), 0)), a.bias_stride)) : 0;
+    const int n_bias = a.bias_ids ? min(max(__ldg(a.bias_len + row), 0), a.bias_max) : 0;
     const float rep = a.repetition ? __ldg(a.repetition + row) : 1.f;
     const float freq = a.frequency ? __ldg(a.frequency + row) : 0.f;
     const float pres = a.presence ? __ldg(a.presence + row) : 0.f;

@@ -93,21 +93,22 @@ Kv8Dev cache_dev(const i4d_kv8& c) {
 }
 
 i4d_status check_batch(i4d_ctx* ctx, const int32_t* q_start, const int32_t* lengths, const int32_t* table,
-                       int64_t table_stride, int batch, int tokens, int max_q) {
+                       int64_t table_stride, int table_blocks, int batch, int tokens, int max_q) {
     OP_ARG(batch >= 0 && tokens >= 0 && max_q >= 0, "negative batch, tokens or max_q");
     OP_ARG(batch == 0 || (q_start && lengths && table), "null q_start, lengths or block_table");
     OP_ARG(aligned(q_start, 4) && aligned(lengths, 4) && aligned(table, 4), "index arrays need 4-byte alignment");
-    OP_ARG(table_stride >= 0, "negative table_stride");
+    OP_ARG(table_blocks >= 0 && table_stride >= 0, "negative table_stride or table_blocks");
     return I4D_OK;
 }
 
 SeqArrays seq_arrays(const OpContext& o, const i4d_kv8& c, const int32_t* q_start, const int32_t* lengths,
-                     const int32_t* table, int64_t table_stride, int tokens, int max_q) {
+                     const int32_t* table, int64_t table_stride, int table_blocks, int tokens, int max_q) {
     SeqArrays s = {};
     s.q_start = q_start;
     s.lengths = lengths;
     s.table = table;
     s.table_stride = table_stride;
+    s.table_blocks = table_blocks;
     s.tokens = tokens;
     s.max_q = max_q;
     s.block_tokens = c.block_tokens;
@@ -199,14 +200,14 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
 i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     OP_ARG(a, "null arguments");
     i4d_status st = check_cache(ctx, a->cache);
-    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->batch, a->tokens, a->max_q);
     if (st != I4D_OK) return st;
     OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
     OP_ARG(a->heads > 0 && a->heads % a->cache.heads == 0, "%d query heads over %d cache heads", a->heads, a->cache.heads);
     OP_ARG(a->max_length >= 0 && a->max_length <= kMaxTokens, "max_length %d", a->max_length);
     OP_ARG(a->window >= 0 && a->window <= kMaxTokens, "window %d", a->window);
-    OP_ARG(a->table_stride * a->cache.block_tokens >= a->max_length, "block_table rows of %lld blocks hold fewer than max_length %d tokens",
-           static_cast<long long>(a->table_stride), a->max_length);
+    OP_ARG(static_cast<int64_t>(a->table_blocks) * a->cache.block_tokens >= a->max_length,
+           "block_table rows of %d blocks hold fewer than max_length %d tokens", a->table_blocks, a->max_length);
     OP_ARG(std::isfinite(a->scale), "scale is not finite");
     OP_ARG(static_cast<int64_t>(a->max_q) * (a->heads / a->cache.heads) <= kMaxTokens, "too many rows");
     return I4D_OK;
@@ -276,8 +277,8 @@ i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     OP_ARG(a->batch >= 0, "negative batch");
     OP_ARG(a->max_length >= 0 && a->max_length <= kMaxTokens, "max_length %d", a->max_length);
     OP_ARG(a->budget > 0 && a->recent >= 0 && a->recent <= a->budget, "budget %d, recent %d (0 <= recent <= budget, 0 < budget)", a->budget, a->recent);
-    OP_ARG(a->table_stride >= 0 && a->table_stride * a->cache.block_tokens >= a->max_length,
-           "block_table rows of %lld blocks hold fewer than max_length %d tokens", static_cast<long long>(a->table_stride), a->max_length);
+    OP_ARG(a->table_stride >= 0 && a->table_blocks >= 0 && static_cast<int64_t>(a->table_blocks) * a->cache.block_tokens >= a->max_length,
+           "block_table rows of %d blocks hold fewer than max_length %d tokens", a->table_blocks, a->max_length);
     OP_ARG(a->weights_stride >= a->max_length && a->weights_out_stride >= a->max_length, "weights' rows are shorter than max_length");
     return I4D_OK;
 }
@@ -417,7 +418,7 @@ i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* a) {
     if (!ctx) return I4D_ERR_ARG;
     OP_ARG(a, "null arguments");
     i4d_status st = check_cache(ctx, a->cache);
-    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->batch, a->tokens, a->max_q);
     if (st != I4D_OK) return st;
     OP_ARG(is_dtype(a->dtype), "unknown dtype %d", a->dtype);
     if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
@@ -428,7 +429,7 @@ i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* a) {
     const OpContext o = op_context(ctx);
     AppendDev d = {};
     d.cache = cache_dev(a->cache);
-    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->tokens, a->max_q);
     d.in[0] = a->k;
     d.in[1] = a->v;
     d.tok[0] = a->k_stride;
@@ -459,14 +460,14 @@ i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* a) {
     if (!ctx) return I4D_ERR_ARG;
     OP_ARG(a, "null arguments");
     i4d_status st = check_cache(ctx, a->cache);
-    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->batch, a->tokens, a->max_q);
+    if (st == I4D_OK) st = check_batch(ctx, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->batch, a->tokens, a->max_q);
     if (st != I4D_OK) return st;
     if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
     OP_ARG(a->k_out && a->v_out && aligned(a->k_out, 16) && aligned(a->v_out, 16), "k_out and v_out need 16-byte alignment");
     const OpContext o = op_context(ctx);
     ReadDev d = {};
     d.cache = cache_dev(a->cache);
-    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->tokens, a->max_q);
     d.out[0] = static_cast<__nv_bfloat16*>(a->k_out);
     d.out[1] = static_cast<__nv_bfloat16*>(a->v_out);
     const int chunks = (a->max_q + kReadTokens - 1) / kReadTokens;
@@ -513,7 +514,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
     AttnDev d = {};
     d.cache = cache_dev(a->cache);
-    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->tokens, a->max_q);
+    d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->tokens, a->max_q);
     d.q = a->q;
     d.out = a->out;
     d.lse = a->lse;
@@ -588,7 +589,7 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     const OpContext o = op_context(ctx);
     EvictDev d = {};
     d.cache = cache_dev(a->cache);
-    d.seq = seq_arrays(o, a->cache, nullptr, a->lengths, a->block_table, a->table_stride, 0, 0);
+    d.seq = seq_arrays(o, a->cache, nullptr, a->lengths, a->block_table, a->table_stride, a->table_blocks, 0, 0);
     d.weights = a->weights;
     d.weights_out = a->weights_out;
     d.weights_stride = a->weights_stride;
@@ -631,10 +632,10 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     OP_ARG((a->logits == a->out && a->stride == a->out_stride) ||
                !overlap(span_of(a->logits, a->rows, a->stride, 1, 0, a->vocab, bytes), span_of(a->out, a->rows, a->out_stride, 1, 0, a->vocab, bytes)),
            "out overlaps logits");
-    OP_ARG(!a->history || (a->history_len && a->history_stride >= 0 && a->history_stride <= kMaxTokens), "history without history_len, or bad history_stride");
+    OP_ARG(!a->history || (a->history_len && a->history_stride >= 0 && a->history_max >= 0 && a->history_max <= kMaxTokens), "history without history_len, or bad history_stride or history_max");
     OP_ARG(a->history || !(a->repetition || a->frequency || a->presence || a->prompt_len), "penalties without a history");
     OP_ARG(!a->bias_ids == !a->bias_values && !a->bias_ids == !a->bias_len, "bias_ids, bias_values and bias_len go together");
-    OP_ARG(!a->bias_ids || (a->bias_stride >= 0 && a->bias_stride <= kMaxTokens), "bad bias_stride");
+    OP_ARG(!a->bias_ids || (a->bias_stride >= 0 && a->bias_max >= 0 && a->bias_max <= kMaxTokens), "bad bias_stride or bias_max");
     OP_ARG(!a->mask || a->mask_stride >= 0, "negative mask_stride");
     LogitsDev d = {};
     d.in = a->logits;
@@ -656,6 +657,8 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     d.bias_stride = a->bias_stride;
     d.mask_stride = a->mask_stride;
     d.vocab = a->vocab;
+    d.history_max = a->history_max;
+    d.bias_max = a->bias_max;
     // CTAs of a row: slices of at least 2048 entries, eight at most (the
     // portable cluster size), fewer where the rows fill the GPU by themselves.
     const OpContext o = op_context(ctx);

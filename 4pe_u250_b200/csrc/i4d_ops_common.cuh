@@ -80,7 +80,7 @@ struct SeqArrays {
     const int32_t* lengths;
     const int32_t* table;
     int64_t table_stride;
-    int tokens, max_q, block_tokens, blocks;
+    int tokens, max_q, block_tokens, blocks, table_blocks;
     unsigned* err;
 };
 
@@ -92,7 +92,7 @@ struct Seq {
 __device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) {
     const int q0 = __ldg(a.q_start + b), q1 = __ldg(a.q_start + b + 1), len = __ldg(a.lengths + b);
     const bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.tokens && q1 - q0 <= a.max_q && len >= q1 - q0 &&
-                    len <= a.table_stride * a.block_tokens && len <= kMaxTokens;
+                    len <= static_cast<int64_t>(a.table_blocks) * a.block_tokens && len <= kMaxTokens;
     if (!ok && report) atomicOr(a.err, kBadSequence);
     return {q0, ok ? q1 - q0 : 0, ok ? len : 0};
 }

@@ -422,7 +422,8 @@ i4d_status i4d_profile_attention(i4d_ctx* ctx, int layer, uint32_t position, con
  * new ones included: row i of the n rows of sequence b stands at cache index
  * lengths[b] - n + i.  max_q bounds every n, max_length every length.  Token
  * t of sequence b lies in block block_table[b * table_stride + t /
- * block_tokens]; the blocks that a call writes must differ from each other. */
+ * block_tokens], a row of table_blocks entries; the blocks that a call writes
+ * must differ from each other. */
 #define I4D_F32 0
 #define I4D_BF16 1
 #define I4D_F16 2
@@ -491,7 +492,7 @@ typedef struct i4d_kv8_append_args {
     const int32_t* lengths;
     const int32_t* block_table;
     int64_t table_stride;
-    int batch, tokens, max_q, dtype;
+    int table_blocks, batch, tokens, max_q, dtype;
     void* stream;
 } i4d_kv8_append_args;
 i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* args);
@@ -508,7 +509,7 @@ typedef struct i4d_kv8_read_args {
     const int32_t* lengths;
     const int32_t* block_table;
     int64_t table_stride;
-    int batch, tokens, max_q;
+    int table_blocks, batch, tokens, max_q;
     void* stream;
 } i4d_kv8_read_args;
 i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* args);
@@ -535,7 +536,7 @@ typedef struct i4d_kv8_attention_args {
     const int32_t* lengths;
     const int32_t* block_table;
     int64_t table_stride;
-    int batch, tokens, heads, max_q, max_length, window, dtype;
+    int table_blocks, batch, tokens, heads, max_q, max_length, window, dtype;
     float scale;
     void* workspace;
     size_t workspace_bytes;
@@ -566,7 +567,7 @@ typedef struct i4d_kv8_evict_args {
     int32_t* keep;
     const int32_t* block_table;
     int64_t table_stride;
-    int batch, budget, recent, max_length;
+    int table_blocks, batch, budget, recent, max_length;
     void* workspace;
     size_t workspace_bytes;
     void* stream;
@@ -599,7 +600,7 @@ typedef struct i4d_logits_args {
     const int32_t* bias_len;
     const uint32_t* mask;
     int64_t stride, out_stride, history_stride, bias_stride, mask_stride;
-    int rows, vocab, dtype;
+    int rows, vocab, history_max, bias_max, dtype; /* _max: entries of a row, which bound the lengths */
     void* stream;
 } i4d_logits_args;
 i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* args);
