@@ -44,11 +44,12 @@ struct AttnDev {
     float* lse;
     float* weights;
     int64_t q_tok, q_head, out_tok, out_head, weights_stride;
-    int heads, group, window, dtype, max_length;
+    int heads, group, window, dtype, max_length, wide_q;
     float scale_log2;  // softmax scale * log2(e)
     int row_tiles;     // tiles of a (sequence, cache head)
     int splits, chunk; // token chunks of a tile
-    float* part;       // workspace: [tile][split][rows][dim + 4]: O, M, l, R
+    float* part;       // workspace: [tile][split][rows][dim]: O
+    float4* stats;     // workspace: [tile][rows][split]: M, l, R
     float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
     float* scores;     // workspace (few rows, with weights): [tile][rows][max_length], log2 scale
 };
@@ -98,10 +99,34 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ float load_q(const AttnDev& a, int64_t i) {
-    if (a.dtype == I4D_F32) return static_cast<const float*>(a.q)[i];
-    if (a.dtype == I4D_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[i]);
-    return __half2float(static_cast<const __half*>(a.q)[i]);
+// 16 elements of q from element i (wide: 16-byte aligned rows).
+__device__ __forceinline__ void load_q16(const AttnDev& a, int64_t i, float out[16]) {
+    if (a.dtype == I4D_F32) {
+        const float* p = static_cast<const float*>(a.q) + i;
+        if (a.wide_q) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(out + 4 * k) = __ldg(reinterpret_cast<const float4*>(p) + k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) out[k] = __ldg(p + k);
+        }
+        return;
+    }
+    const unsigned short* p = static_cast<const unsigned short*>(a.q) + i;
+    union {
+        uint4 v[2];
+        unsigned short h[16];
+    } x;
+    if (a.wide_q) {
+        x.v[0] = __ldg(reinterpret_cast<const uint4*>(p));
+        x.v[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x.h[k] = __ldg(p + k);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+        out[k] = a.dtype == I4D_BF16 ? __uint_as_float(static_cast<uint32_t>(x.h[k]) << 16) : __half2float(__ushort_as_half(x.h[k]));
 }
 
 __device__ __forceinline__ void store_out(const AttnDev& a, int64_t i, float v) {
@@ -129,12 +154,18 @@ __device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h
         const int row = row0 + nt * 8 + g;
         const bool live = row < s.n * a.group;
         const int64_t base = live ? (s.first + row / a.group) * a.q_tok + (h * a.group + row % a.group) * a.q_head : 0;
-        float top = 0.f;
+        float top = 0.f, x[DT / 64][16];
 #pragma unroll
         for (int c = 0; c < DT / 64; ++c) {
             const int d0 = (t + 4 * c) * 16;
-            if (live && d0 < dim)
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(load_q(a, base + d0 + i)));
+            if (live && d0 < dim) {
+                load_q16(a, base + d0, x[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[c][i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[c][i]));
         }
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
@@ -142,23 +173,17 @@ __device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h
         const int e = max(-115, min(126, 13 - ((__float_as_int(top) >> 23) - 127)));
         const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
 #pragma unroll
-        for (int c = 0; c < DT / 64; ++c) {
-            const int d0 = (t + 4 * c) * 16;
+        for (int c = 0; c < DT / 64; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float x = 0.f, y = 0.f;
-                if (live && d0 < dim) {
-                    x = load_q(a, base + d0 + 2 * i) * up;
-                    y = load_q(a, base + d0 + 2 * i + 1) * up;
-                }
-                const uint32_t w = pack_h2(x, y);
+                const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
+                const uint32_t w = pack_h2(u, v);
                 q.hi[nt][c * 4 + i / 2][i & 1] = w;
                 if constexpr (HL) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-                    q.lo[nt][c * 4 + i / 2][i & 1] = pack_h2(x - f.x, y - f.y);
+                    q.lo[nt][c * 4 + i / 2][i & 1] = pack_h2(u - f.x, v - f.y);
                 }
             }
-        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) q.factor[nt][j] = __shfl_sync(~0u, down, (2 * t + j) * 4) * a.scale_log2;
     }
@@ -533,13 +558,8 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
                 if (a.weights) a.lse2[tok * a.heads + head] = l2;
             }
         } else {
-            float* p = a.part + ((tile * a.splits + split) * kRows + r) * (dim + 4);
-            p[d] = o;
-            if (d == 0) {
-                p[dim] = m;
-                p[dim + 1] = sum;
-                p[dim + 2] = rr;
-            }
+            a.part[((tile * a.splits + split) * kRows + r) * dim + d] = o;
+            if (d == 0) a.stats[(tile * kRows + r) * a.splits + split] = make_float4(m, sum, rr, 0.f);
         }
     }
 }
@@ -558,30 +578,59 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
     const int2 sp = row_span(a, s.len - s.n + row / a.group);
     // chunks that the row's tile looked at (a tile's first row may begin earlier; its chunk holds no token of this row then)
     const int c0 = sp.x / a.chunk, c1 = (sp.y + a.chunk - 1) / a.chunk, dim = a.cache.dim;
-    const float* part = a.part + (tile * a.splits * rows_per_tile + r) * (dim + 4);
-    const int64_t step = static_cast<int64_t>(rows_per_tile) * (dim + 4);
+    const float4* stats = a.stats + (tile * rows_per_tile + r) * a.splits;
     float m = -INFINITY, rr = -INFINITY, sum = 0.f;
     for (int c = c0 + lane; c < c1; c += 32) {
-        m = fmaxf(m, part[c * step + dim]);
-        rr = fmaxf(rr, part[c * step + dim + 2]);
+        const float4 x = stats[c];
+        m = fmaxf(m, x.x);
+        rr = fmaxf(rr, x.z);
     }
     m = warp_max(m);
     rr = warp_max(rr);
-    for (int c = c0 + lane; c < c1; c += 32) {
-        const float pm = part[c * step + dim];
-        sum += part[c * step + dim + 1] * (pm == -INFINITY ? 1.f : ex2(pm - m));
-    }
-    sum = warp_sum(sum);
     const int64_t tok = s.first + row / a.group;
     const int head = h * a.group + row % a.group;
-    const float back = rr == -INFINITY || sum == 0.f ? 0.f : ex2(rr - m) / sum;
-    for (int d = lane; d < dim; d += 32) {
-        float o = 0.f;
-        for (int c = c0; c < c1; ++c) {
-            const float pr = part[c * step + dim + 2];
-            o += part[c * step + d] * (pr == -INFINITY ? 1.f : ex2(pr - rr));
+    float4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // dims 4 lane and 128 + 4 lane
+    const float* part = a.part + (tile * a.splits * rows_per_tile + r) * dim + 4 * lane;
+    const int64_t step = static_cast<int64_t>(rows_per_tile) * dim;
+    const bool low = 4 * lane < dim, high = 128 + 4 * lane < dim;
+    for (int base = c0; base < c1; base += 32) {
+        float f = 0.f;  // the factor of chunk base + lane
+        if (base + lane < c1) {
+            const float4 x = stats[base + lane];
+            sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
+            f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
         }
-        store_out(a, tok * a.out_tok + head * a.out_head + d, sum == 0.f ? 0.f : o * back);
+        const int n = min(32, c1 - base);
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+            const float fk = __shfl_sync(~0u, f, k);
+            const float* p = part + (base + k) * step;
+            if (low) {
+                const float4 x = *reinterpret_cast<const float4*>(p);
+                o[0].x += x.x * fk;
+                o[0].y += x.y * fk;
+                o[0].z += x.z * fk;
+                o[0].w += x.w * fk;
+            }
+            if (high) {
+                const float4 x = *reinterpret_cast<const float4*>(p + 128);
+                o[1].x += x.x * fk;
+                o[1].y += x.y * fk;
+                o[1].z += x.z * fk;
+                o[1].w += x.w * fk;
+            }
+        }
+    }
+    sum = warp_sum(sum);
+    const float back = sum == 0.f ? 0.f : rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (k ? !high : !low) continue;
+        const int64_t at = tok * a.out_tok + head * a.out_head + 128 * k + 4 * lane;
+        store_out(a, at, sum == 0.f ? 0.f : o[k].x * back);
+        store_out(a, at + 1, sum == 0.f ? 0.f : o[k].y * back);
+        store_out(a, at + 2, sum == 0.f ? 0.f : o[k].z * back);
+        store_out(a, at + 3, sum == 0.f ? 0.f : o[k].w * back);
     }
     if (lane == 0) {
         const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);

@@ -8,6 +8,8 @@
 // one step of the last scale (1/2 + 1/4 + ...).
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "i4d_ops_common.cuh"
 
 namespace i4d_ops {
@@ -122,26 +124,28 @@ struct ReadDev {
     __nv_bfloat16* out[2];
 };
 
-constexpr int kReadTokens = 16;
+constexpr int kReadItems = 512;  // of a CTA of 256 threads
 
-// One CTA for kReadTokens rows of a sequence: 16 codes in, 16 BF16 values out
-// an item.  Bound: bytes.
+// An item: 16 codes of K and of V in, 16 BF16 values each out.  Bound: bytes;
+// two items a thread, so that short reads spread over the GPU (16 tokens a CTA
+// took 30 us for 1024 tokens of 32 heads).
 template <int CODE>
 __global__ void __launch_bounds__(256) k_kv8_read(ReadDev a, int chunks) {
-    const int b = blockIdx.x / chunks, t0 = blockIdx.x % chunks * kReadTokens;
-    const Seq s = load_seq(a.seq, b, threadIdx.x == 0 && t0 == 0);
-    if (t0 >= s.n) return;
-    const int rows = min(kReadTokens, s.n - t0), first = s.len - s.n + t0;
-    const int bs = a.cache.block_tokens, per_head = a.cache.dim / 16, per_tok = a.cache.heads * per_head;
-    for (int i = threadIdx.x; i < rows * per_tok; i += 256) {
-        const int r = i / per_tok, e = i % per_tok, h = e / per_head, c = e % per_head;
-        const int p = first + r, id = load_block(a.seq, b, p / bs, true);
+    const int b = blockIdx.x / chunks, i0 = blockIdx.x % chunks * kReadItems;
+    const Seq s = load_seq(a.seq, b, threadIdx.x == 0 && i0 == 0);
+    const int bs = a.cache.block_tokens, shift = 31 - __clz(bs), per_head = a.cache.dim / 16, per_tok = a.cache.heads * per_head;
+#pragma unroll
+    for (int u = 0; u < kReadItems / 256; ++u) {
+        const int i = i0 + u * 256 + threadIdx.x;
+        const int r = i / per_tok, e = i - r * per_tok, h = e / per_head, c = e - h * per_head;
+        if (r >= s.n) continue;
+        const int p = s.len - s.n + r, id = load_block(a.seq, b, p >> shift, true);
         if (id < 0) continue;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const float scale = __ldg(a.cache.scale[which] + static_cast<int64_t>(id) * a.cache.heads + h);
             const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.cache.codes[which] + code_offset(a.cache, id, h) +
-                                                                 static_cast<int64_t>(p % bs) * a.cache.dim) + c);
+                                                                 static_cast<int64_t>(p & (bs - 1)) * a.cache.dim) + c);
             const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
             Vec<__nv_bfloat16, 16> o;
 #pragma unroll
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(ReadDev a, int chunks) {
 #pragma unroll
                 for (int m = 0; m < 4; ++m) o.v[4 * k + m] = __float2bfloat16_rn(f[m] * scale);
             }
-            store_vec<__nv_bfloat16, 16>(a.out[which] + (static_cast<int64_t>(s.first + t0 + r) * a.cache.heads + h) * a.cache.dim + c * 16, o);
+            store_vec<__nv_bfloat16, 16>(a.out[which] + (static_cast<int64_t>(s.first + r) * a.cache.heads + h) * a.cache.dim + c * 16, o);
         }
     }
 }
@@ -212,29 +216,39 @@ __device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
     return x + (w ? warp_sums[w - 1] : 0);
 }
 
-// One CTA for each (sequence, head): the key of the (budget - recent)-th
-// greatest weight by four passes over 8 bits each, then the kept indices in
-// order (of equal keys the first ones), their weights, and a copy of the
-// scales, which the move overwrites.
-__global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a) {
-    __shared__ int hist[256];
+constexpr int kSelectBits = 11;  // 11 + 11 + 10 bits of a key
+constexpr int kSelectBins = 1 << kSelectBits;
+
+// One cluster for each (sequence, head), whose CTAs take consecutive parts of
+// the weights: the key of the (budget - recent)-th greatest weight in three
+// passes over its digits, each a histogram that the cluster adds up through
+// distributed shared memory, then the kept indices in order (of equal keys the
+// first ones), their weights, and a copy of the scales, which the move
+// overwrites.  Bound: the weights read once from memory (the later passes hit
+// L2), then the chain of barriers.
+__global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int ctas) {
+    __shared__ int hist[kSelectBins];
     __shared__ int sums[32];
     __shared__ int chosen, above;
-    const int b = blockIdx.x / a.cache.heads, h = blockIdx.x % a.cache.heads, tid = threadIdx.x;
-    const int len = evict_length(a, b, tid == 0 && h == 0);
-    const float* w = a.weights + (static_cast<int64_t>(b) * a.cache.heads + h) * a.weights_stride;
-    float* wo = a.weights_out + (static_cast<int64_t>(b) * a.cache.heads + h) * a.weights_out_stride;
-    int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.cache.heads + h) * a.budget;
-    if (h == 0 && tid == 0) a.lengths_out[b] = min(len, a.budget);
-    if (len <= a.budget) {
-        for (int i = tid; i < a.budget; i += kSelectThreads) keep[i] = i < len ? i : -1;
+    __shared__ int counts[2];
+    cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
+    const int b = row / a.cache.heads, h = row % a.cache.heads, tid = threadIdx.x;
+    const int len = evict_length(a, b, tid == 0 && h == 0 && rank == 0);
+    const float* w = a.weights + row * a.weights_stride;
+    float* wo = a.weights_out + row * a.weights_out_stride;
+    int32_t* keep = a.keep + static_cast<int64_t>(row) * a.budget;
+    if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = min(len, a.budget);
+    const int first = rank * kSelectThreads + tid, stride = ctas * kSelectThreads;
+    if (len <= a.budget) {  // the whole cluster leaves
+        for (int i = first; i < a.budget; i += stride) keep[i] = i < len ? i : -1;
         if (w != wo)
-            for (int i = tid; i < len; i += kSelectThreads) wo[i] = w[i];
+            for (int i = first; i < len; i += stride) wo[i] = w[i];
         return;
     }
-    const int bs = a.cache.block_tokens, nblk = (len + bs - 1) / bs;
-    float* old = a.old_scale + (static_cast<int64_t>(b) * a.cache.heads + h) * 2 * a.old_blocks;
-    for (int i = tid; i < nblk; i += kSelectThreads) {
+    const int nblk = (len + a.cache.block_tokens - 1) / a.cache.block_tokens;
+    float* old = a.old_scale + static_cast<int64_t>(row) * 2 * a.old_blocks;
+    for (int i = first; i < nblk; i += stride) {
         const int id = load_block(a.seq, b, i, h == 0);
         const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
         old[i] = id < 0 ? 0.f : a.cache.scale[0][at];
@@ -242,120 +256,197 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a) {
     }
     const int free_len = len - a.recent;
     int want = a.budget - a.recent;  // of the tokens before free_len; want < free_len
-    uint32_t key = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    const int part = (len + ctas - 1) / ctas, lo = min(len, rank * part), hi = min(len, lo + part);
+    const bool none = want == 0;
+    uint32_t key = 0, high = 0;
+    for (int shift = 21; !none; shift = max(0, shift - kSelectBits)) {
+        const int bits = shift == 0 ? 10 : kSelectBits;
+        for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t high = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int i = tid; i < free_len; i += kSelectThreads) {
+        for (int i = lo + tid; i < min(hi, free_len); i += kSelectThreads) {
             const uint32_t k = weight_key(w[i]);
-            if ((k & high) == (key & high)) atomicAdd(&hist[(k >> shift) & 255u], 1);
+            if ((k & high) == key) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
         }
-        __syncthreads();
-        // bins from the greatest: the one in which the want-th falls
-        const int mine = tid < 256 ? hist[255 - tid] : 0;
+        cl.sync();
+        // the cluster's sum of the two bins from the greatest that are this thread's
+        const int bin = kSelectBins - 1 - 2 * tid;
+        int n0 = 0, n1 = 0;
+        for (int c = 0; c < ctas; ++c) {
+            const int* other = cl.map_shared_rank(hist, c);
+            n0 += other[bin];
+            n1 += other[bin - 1];
+        }
         int total;
-        const int upto = cta_scan(mine, sums, &total);
-        if (tid < 256 && want > 0 && upto >= want && upto - mine < want) {
-            chosen = 255 - tid;
-            above = upto - mine;
+        const int upto = cta_scan(n0 + n1, sums, &total), before = upto - n0 - n1;
+        if (upto >= want && before < want) {
+            const bool second = before + n0 < want;
+            chosen = bin - second;
+            above = before + (second ? n0 : 0);
         }
-        __syncthreads();
-        if (want > 0) {
-            key |= static_cast<uint32_t>(chosen) << shift;
-            want -= above;
-        }
+        cl.sync();  // hist is read, chosen is written
+        key |= static_cast<uint32_t>(chosen) << shift;
+        high |= static_cast<uint32_t>((1 << bits) - 1) << shift;
+        want -= above;
+        if (shift == 0) break;
     }
-    // `want` of the weights equal to key are kept, all above it; if nothing
-    // but the recent ones is kept, none.
-    const bool none = a.budget == a.recent;
-    int kept = 0, equal = 0;
-    for (int base = 0; base < len; base += kSelectThreads) {
+    // `want` of the weights equal to key are kept and all above it.  This
+    // CTA's places follow those of the CTAs before it.
+    int same_n = 0, more_n = 0;
+    for (int i = lo + tid; i < hi; i += kSelectThreads) {
+        const uint32_t k = weight_key(w[i]);
+        same_n += i < free_len && !none && k == key;
+        more_n += i >= free_len || (!none && k > key);
+    }
+    int all_same, all_more;
+    cta_scan(same_n, sums, &all_same);
+    __syncthreads();
+    cta_scan(more_n, sums, &all_more);
+    if (tid == 0) {
+        counts[0] = all_same;
+        counts[1] = all_more;
+    }
+    cl.sync();
+    int equal = 0, kept = 0;
+    for (int c = 0; c < rank; ++c) {
+        const int* other = cl.map_shared_rank(counts, c);
+        const int e = other[0];
+        kept += other[1] + min(e, max(0, want - equal));
+        equal += e;
+    }
+    for (int base = lo; base < hi; base += kSelectThreads) {
         const int i = base + tid;
-        const bool inside = i < len, free_tok = i < free_len;
+        const bool inside = i < hi, free_tok = i < free_len;
         const float wi = inside ? w[i] : 0.f;
         const uint32_t k = weight_key(wi);
         const bool same = inside && free_tok && !none && k == key;
         int n_same, n_kept;
-        const int rank = equal + cta_scan(same, sums, &n_same);
-        const bool take = inside && (!free_tok || (!none && (k > key || (same && rank <= want))));
+        const int rank_same = equal + cta_scan(same, sums, &n_same);
+        const bool take = inside && (!free_tok || (!none && (k > key || (same && rank_same <= want))));
         const int place = kept + cta_scan(take, sums, &n_kept);
-        __syncthreads();  // every weight of this range is read before any is overwritten in place
         if (take) {
             keep[place - 1] = i;
-            wo[place - 1] = wi;
+            if (w != wo) wo[place - 1] = wi;
         }
         equal += n_same;
         kept += n_kept;
     }
-    __syncthreads();
-    for (int i = a.budget + tid; i < len; i += kSelectThreads) wo[i] = 0.f;
+    if (w != wo) {
+        for (int i = a.budget + first; i < len; i += stride) wo[i] = 0.f;
+        cl.sync();
+        return;
+    }
+    // In place: eight destinations a thread at a time go through registers.
+    cl.sync();  // keep is written; no CTA reads its part of w in the loop above any more
+    for (int base = 0; base < a.budget; base += stride * 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = base + u * stride + first;
+            x[u] = i < a.budget ? __ldcg(w + keep[i]) : 0.f;
+        }
+        cl.sync();  // the sources of this round are read; those of later rounds lie behind its destinations
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = base + u * stride + first;
+            if (i < a.budget) wo[i] = x[u];
+        }
+    }
+    cl.sync();
+    for (int i = a.budget + first; i < len; i += stride) wo[i] = 0.f;
 }
 
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 512;
+constexpr int kMoveVecs = 4;  // 16-byte pieces a thread holds
+constexpr int kMoveRound = kMoveThreads / 2 * kMoveVecs;  // destination tokens a round
 
 // Moves the kept tokens up, in place.  One CTA for each (sequence, head, K or
-// V, slice of 32 code bytes) walks its destination tokens in order: a kept
-// token's index is never below its destination, so once a group's codes are
-// in registers its destinations can be written, and what the next groups read
-// lies behind them.  Slices are independent because a block's new scale comes
-// from the old scales alone (k_kv8_select copied them).
-// Bound: kept codes read and written; 32-byte sectors, one CTA's loads in
-// flight at a time.
+// V, slice of 32 code bytes) walks its destination tokens in order, kMoveRound
+// at a time: a kept token's index is never below its destination, so a round's
+// destinations are written once its own codes are in registers, and what later
+// rounds read lies behind them; their loads may start before.  Slices are
+// independent because a block's new scale comes from the old scales alone
+// (k_kv8_select copied them); sixteen tokens are a warp's, so a block's
+// greatest scale is joined from the maxima of its warps at the one barrier.
+// Bound: kept codes read and written.
 template <int CODE>
 __global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int slices) {
-    constexpr int kRound = kMoveThreads / 2;  // destination tokens a pass: two threads of 16 bytes each
-    __shared__ float dst_scale[kRound / 16];
-    __shared__ float src_scale[kRound];
+    __shared__ float warp_scale[2][kMoveVecs * kMoveThreads / 32];
     const int slice = blockIdx.x % slices, rest = blockIdx.x / slices;
     const int which = rest & 1, h = (rest >> 1) % a.cache.heads, b = (rest >> 1) / a.cache.heads;
     const int len = evict_length(a, b, false);
     if (len <= a.budget) return;
-    const int tid = threadIdx.x, bs = a.cache.block_tokens, dim = a.cache.dim;
+    const int tid = threadIdx.x, bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
     const int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.cache.heads + h) * a.budget;
     const float* old = a.old_scale + ((static_cast<int64_t>(b) * a.cache.heads + h) * 2 + which) * a.old_blocks;
+    uint8_t* codes = a.cache.codes[which];
     const int col = slice * 32 + (tid & 1) * 16;
-    const int group = max(bs, kRound) / bs * bs;  // whole blocks a pass (bs divides kRound or equals it)
-    for (int base = 0; base < a.budget; base += group) {
-        const int i = base + tid / 2;
-        const bool live = i < a.budget;
-        uint4 x = {0, 0, 0, 0};
-        float scale = 0.f;
-        int to = -1;
-        if (live) {
-            const int from = keep[i];
-            const int src = load_block(a.seq, b, from / bs, false);
-            to = load_block(a.seq, b, i / bs, false);
-            scale = old[from / bs];
-            if (src >= 0 && col < dim)
-                x = __ldcg(reinterpret_cast<const uint4*>(a.cache.codes[which] + code_offset(a.cache, src, h) +
-                                                          static_cast<int64_t>(from % bs) * dim + col));
+    int from[kMoveVecs], from_next[kMoveVecs];
+    uint4 x[kMoveVecs], x_next[kMoveVecs];
+    float scale[kMoveVecs], scale_next[kMoveVecs];
+    auto indices = [&](int base, int* f) {
+#pragma unroll
+        for (int u = 0; u < kMoveVecs; ++u) {
+            const int i = base + u * (kMoveThreads / 2) + tid / 2;
+            f[u] = i < a.budget ? __ldg(keep + i) : -1;
         }
-        if ((tid & 1) == 0) src_scale[tid / 2] = scale;
-        __syncthreads();
-        if (tid < kRound / bs) {
-            float m = 0.f;
-            for (int k = 0; k < bs; ++k) m = fmaxf(m, src_scale[tid * bs + k]);
-            dst_scale[tid] = m;
+    };
+    auto pieces = [&](const int* f, uint4* v, float* sc) {
+#pragma unroll
+        for (int u = 0; u < kMoveVecs; ++u) {
+            v[u] = make_uint4(0, 0, 0, 0);
+            sc[u] = 0.f;
+            if (f[u] >= 0) {
+                const int id = load_block(a.seq, b, f[u] >> shift, false);
+                sc[u] = __ldg(old + (f[u] >> shift));
+                if (id >= 0 && col < dim)
+                    v[u] = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) +
+                                                                 static_cast<int64_t>(f[u] & (bs - 1)) * dim + col));
+            }
         }
-        __syncthreads();
-        if (live && to >= 0) {
-            const float now = dst_scale[(i - base) / bs];
-            if (scale != now) {
-                const float ratio = now > 0.f ? __fdiv_rn(scale, now) : 0.f;
-                x.x = rescale4<CODE>(x.x, ratio);
-                x.y = rescale4<CODE>(x.y, ratio);
-                x.z = rescale4<CODE>(x.z, ratio);
-                x.w = rescale4<CODE>(x.w, ratio);
+    };
+    indices(0, from);
+    pieces(from, x, scale);
+    indices(kMoveRound, from_next);
+    int flip = 0;
+    for (int base = 0; base < a.budget; base += kMoveRound, flip ^= 1) {
+        pieces(from_next, x_next, scale_next);
+        indices(base + 2 * kMoveRound, from);
+#pragma unroll
+        for (int u = 0; u < kMoveVecs; ++u) {
+            const float m = warp_max(scale[u]);
+            if ((tid & 31) == 0) warp_scale[flip][u * (kMoveThreads / 32) + tid / 32] = m;
+        }
+        __syncthreads();  // this round's codes are in registers everywhere, its maxima in place
+#pragma unroll
+        for (int u = 0; u < kMoveVecs; ++u) {
+            const int i = base + u * (kMoveThreads / 2) + tid / 2;
+            if (i >= a.budget) continue;
+            const int per = bs / 16, w0 = (u * (kMoveThreads / 32) + tid / 32) / per * per;
+            float now = 0.f;
+            for (int k = 0; k < per; ++k) now = fmaxf(now, warp_scale[flip][w0 + k]);
+            const int to = load_block(a.seq, b, i >> shift, false);
+            if (to < 0) continue;
+            uint4 v = x[u];
+            if (scale[u] != now) {
+                const float ratio = __fdiv_rn(scale[u], now);
+                v.x = rescale4<CODE>(v.x, ratio);
+                v.y = rescale4<CODE>(v.y, ratio);
+                v.z = rescale4<CODE>(v.z, ratio);
+                v.w = rescale4<CODE>(v.w, ratio);
             }
             if (col < dim)
-                *reinterpret_cast<uint4*>(a.cache.codes[which] + code_offset(a.cache, to, h) +
-                                          static_cast<int64_t>(i % bs) * dim + col) = x;
-            if (slice == 0 && (tid & 1) == 0 && i % bs == 0)
+                *reinterpret_cast<uint4*>(codes + code_offset(a.cache, to, h) + static_cast<int64_t>(i & (bs - 1)) * dim + col) = v;
+            if (slice == 0 && (tid & 1) == 0 && (i & (bs - 1)) == 0)
                 a.cache.scale[which][static_cast<int64_t>(to) * a.cache.heads + h] = now;
         }
-        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kMoveVecs; ++u) {
+            x[u] = x_next[u];
+            scale[u] = scale_next[u];
+            const int t = from[u];
+            from[u] = from_next[u];
+            from_next[u] = t;
+        }
     }
 }
 

@@ -73,21 +73,40 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
     const int per_cta = (vecs + ctas - 1) / ctas;
     const int v_end = min(vecs, (rank + 1) * per_cta);
     unsigned long long key = 0;
+    // A thread's vectors of the next slice are loaded before the counting of
+    // its tokens, which hides the wait for them.
+    constexpr int kVecs = kLogitsSlice / V / kLogitsThreads;
     for (int v0 = rank * per_cta; v0 < v_end; v0 += kLogitsSlice / V) {
         const int v1 = min(v_end, v0 + kLogitsSlice / V);
         const int e0 = v0 * V - skew, span = (v1 - v0) * V;
+        Vec<T, V> x[kVecs];
+        uint2 words[kVecs];
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            const int v = v0 + u * kLogitsThreads + tid, e = v * V - skew;
+            words[u] = make_uint2(~0u, ~0u);
+            if (v >= v1) continue;
+            if (e >= 0 && e + V <= a.vocab) {
+                x[u] = *reinterpret_cast<const Vec<T, V>*>(in + e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e + i >= 0 && e + i < a.vocab) x[u].v[i] = in[e + i];
+            }
+            if (mask) words[u] = make_uint2(__ldg(mask + max(e, 0) / 32), __ldg(mask + min(e + V - 1, a.vocab - 1) / 32));
+        }
         __syncthreads();
         if (n_hist)
-            for (int i = tid; i < span; i += kLogitsThreads) counts[i] = 0;
+            for (int i = tid; i < kLogitsSlice / 4; i += kLogitsThreads) reinterpret_cast<int4*>(counts)[i] = make_int4(0, 0, 0, 0);
         if (n_bias)
-            for (int i = tid; i < span; i += kLogitsThreads) bias[i] = 0.f;
+            for (int i = tid; i < kLogitsSlice / 4; i += kLogitsThreads) reinterpret_cast<int4*>(bias)[i] = make_int4(0, 0, 0, 0);
         __syncthreads();
+#pragma unroll 4
         for (int i = tid; i < n_hist; i += kLogitsThreads) {
             const int id = __ldg(hist + i);
-            const unsigned at = static_cast<unsigned>(id) - static_cast<unsigned>(e0);
-            if (id >= 0 && id < a.vocab && id >= e0 && at < static_cast<unsigned>(span)) {
-                if (i < n_prompt) atomicOr(&counts[at], 1);
-                else atomicAdd(&counts[at], 2);
+            if (id >= max(e0, 0) && id < a.vocab && id - e0 < span) {
+                if (i < n_prompt) atomicOr(&counts[id - e0], 1);
+                else atomicAdd(&counts[id - e0], 2);
             }
         }
         if (tid < 32) {  // one warp, so that the values of one id are added in their order
@@ -95,7 +114,7 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
                 const bool live = i + tid < n_bias;
                 const int id = live ? __ldg(a.bias_ids + row * a.bias_stride + i + tid) : -1;
                 const float val = live ? __ldg(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
-                const bool mine = live && id >= 0 && id < a.vocab && id >= e0 && id - e0 < span;
+                const bool mine = live && id >= max(e0, 0) && id < a.vocab && id - e0 < span;
                 const unsigned peers = __match_any_sync(~0u, mine ? id : -1 - tid);
                 const bool leader = __ffs(peers) - 1 == tid;
                 float sum = mine && leader ? bias[id - e0] : 0.f;
@@ -112,44 +131,40 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
             }
         }
         __syncthreads();
-        for (int v = v0 + tid; v < v1; v += kLogitsThreads) {
-            const int e = v * V - skew;
-            const bool whole = e >= 0 && e + V <= a.vocab;
-            Vec<T, V> x;
-            if (whole) {
-                x = *reinterpret_cast<const Vec<T, V>*>(in + e);
-            } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (e + i >= 0 && e + i < a.vocab) x.v[i] = in[e + i];
-            }
-            uint32_t w0 = ~0u, w1 = ~0u;
-            if (mask) {
-                w0 = __ldg(mask + max(e, 0) / 32);
-                w1 = __ldg(mask + min(e + V - 1, a.vocab - 1) / 32);
+        for (int u = 0; u < kVecs; ++u) {
+            const int v = v0 + u * kLogitsThreads + tid, e = v * V - skew, at = (v - v0) * V;
+            if (v >= v1) continue;
+            const bool whole = e >= 0 && e + V <= a.vocab;
+            int c[V];
+            float add[V];
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                *reinterpret_cast<int4*>(c + i) = n_hist ? *reinterpret_cast<const int4*>(counts + at + i) : make_int4(0, 0, 0, 0);
+                if (n_bias) *reinterpret_cast<float4*>(add + i) = *reinterpret_cast<const float4*>(bias + at + i);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int id = e + i;
-                if (id < 0 || id >= a.vocab) continue;
-                float y = to_f32(x.v[i]);
-                if (n_hist) {
-                    const int c = counts[id - e0], n = c >> 1;
-                    if (c) y = a.repetition ? (y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep)) : y;
+                if (!whole && (id < 0 || id >= a.vocab)) continue;
+                float y = to_f32(x[u].v[i]);
+                if (c[i]) {
+                    const int n = c[i] >> 1;
+                    if (a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
                     if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
                 }
-                if (n_bias) y = __fadd_rn(y, bias[id - e0]);
-                const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? w0 : w1;
+                if (n_bias) y = __fadd_rn(y, add[i]);
+                const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? words[u].x : words[u].y;
                 if (!(w >> (id & 31) & 1)) y = -INFINITY;
-                x.v[i] = from_f32<T>(y);
-                key = max(key, logit_key(to_f32(x.v[i]), id));
+                x[u].v[i] = from_f32<T>(y);
+                key = max(key, logit_key(to_f32(x[u].v[i]), id));
             }
             if (whole && aligned_out) {
-                *reinterpret_cast<Vec<T, V>*>(out + e) = x;
+                *reinterpret_cast<Vec<T, V>*>(out + e) = x[u];
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (e + i >= 0 && e + i < a.vocab) out[e + i] = x.v[i];
+                    if (e + i >= 0 && e + i < a.vocab) out[e + i] = x[u].v[i];
             }
         }
     }

@@ -166,8 +166,8 @@ struct AttnPlan {
     int dt, nt;  // padded dim, row tiles of eight a CTA
     int row_tiles, splits, chunk;
     int64_t tiles;
-    size_t part_bytes, lse2_bytes, score_bytes;
-    size_t bytes() const { return part_bytes + lse2_bytes + score_bytes; }
+    size_t part_bytes, stat_bytes, lse2_bytes, score_bytes;
+    size_t bytes() const { return part_bytes + stat_bytes + lse2_bytes + score_bytes; }
 };
 
 AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
@@ -182,13 +182,16 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     // out, but none under 128 tokens (two tiles a warp) nor above what the
     // kernel's table of blocks holds.
     const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 3) * static_cast<int64_t>(o.num_sms);
-    const int64_t want = std::max<int64_t>(1, 4 * places / std::max<int64_t>(1, p.tiles));
+    const int64_t want = std::max<int64_t>(1, 12 * places / std::max<int64_t>(1, p.tiles));
     int64_t chunk = (a.max_length + want - 1) / want;
     chunk = std::min<int64_t>(std::max<int64_t>(128, (chunk + 127) / 128 * 128), kAttnBlocks * c.block_tokens / 2);
     p.chunk = static_cast<int>(chunk);
     p.splits = static_cast<int>(std::max<int64_t>(1, (a.max_length + chunk - 1) / chunk));
     const auto round16 = [](size_t n) { return (n + 15) / 16 * 16; };
-    if (p.splits > 1) p.part_bytes = round16(static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * (c.dim + 4) * sizeof(float));
+    if (p.splits > 1) {
+        p.part_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * c.dim * sizeof(float);
+        p.stat_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * sizeof(float4);
+    }
     if (a.weights) {
         p.lse2_bytes = round16(static_cast<size_t>(a.tokens) * a.heads * sizeof(float));
         // Few rows: their scores are kept (4 bytes a row against a token's codes read again).
@@ -470,7 +473,9 @@ i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* a) {
     d.seq = seq_arrays(o, a->cache, a->q_start, a->lengths, a->block_table, a->table_stride, a->table_blocks, a->tokens, a->max_q);
     d.out[0] = static_cast<__nv_bfloat16*>(a->k_out);
     d.out[1] = static_cast<__nv_bfloat16*>(a->v_out);
-    const int chunks = (a->max_q + kReadTokens - 1) / kReadTokens;
+    const int64_t per_seq = static_cast<int64_t>(a->max_q) * a->cache.heads * (a->cache.dim / 16);
+    OP_ARG(per_seq <= kMaxTokens, "too many rows in one call");
+    const int chunks = static_cast<int>((per_seq + kReadItems - 1) / kReadItems);
     const int64_t grid = static_cast<int64_t>(a->batch) * chunks;
     OP_ARG(grid <= kMaxGrid, "too many rows in one call");
     DeviceScope scope(o.device);
@@ -534,8 +539,11 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.splits = p.splits;
     d.chunk = p.chunk;
     d.part = static_cast<float*>(a->workspace);
-    d.lse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + p.part_bytes);
-    if (p.score_bytes) d.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + p.part_bytes + p.lse2_bytes);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    d.stats = reinterpret_cast<float4*>(ws + p.part_bytes);
+    d.lse2 = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes);
+    if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.lse2_bytes);
+    d.wide_q = aligned(a->q, 16) && a->q_stride * bytes % 16 == 0 && a->q_head_stride * bytes % 16 == 0;
     const int64_t grid = p.tiles * p.splits;
     const int64_t joins = (p.tiles * 8 * p.nt + kAttnWarps - 1) / kAttnWarps;
     const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
@@ -607,8 +615,21 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
-    k_kv8_select<<<static_cast<unsigned>(rows), kSelectThreads, 0, s>>>(d);
-    OP_CK(cudaGetLastError());
+    // CTAs of a row: 4096 weights or more each, eight at most.
+    int ctas = 1;
+    while (ctas < 8 && a->max_length / (2 * ctas) >= 2048) ctas *= 2;
+    OP_ARG(rows * ctas <= kMaxGrid, "too many sequences in one call");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    OP_CK(cudaLaunchKernelEx(&cfg, k_kv8_select, d, ctas));
     if (a->max_length > a->budget) {
         const unsigned grid = static_cast<unsigned>(rows * 2 * slices);
         if (a->cache.code == I4D_CODE_INT8) k_kv8_move<I4D_CODE_INT8><<<grid, kMoveThreads, 0, s>>>(d, slices);
