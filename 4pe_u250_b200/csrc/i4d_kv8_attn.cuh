@@ -65,19 +65,49 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Codes 2 PAIR and 2 PAIR + 1 of a word as two halves (INT8 words come with
-// their top bits flipped: 1024 + 128 + code is exact in FP16).
-template <int CODE, int PAIR>
+// Codes to halves.  INT8 with BIAS: byte v + 128 as the low byte of a half, a
+// subnormal worth (v + 128) 2^-24, which the tensor cores take exactly; the
+// 128 leaves again as 128 times the sum of the query row.  That is half the
+// instructions of an exact conversion, for a sum whose terms are up to 255
+// codes large in place of 127: used for the scores of 16-bit rows.  INT8
+// without: 1024 + 128 + v, minus 1152.  E4M3: exact.
+template <int CODE, bool BIAS>
+constexpr bool kBiased = CODE == I4D_CODE_INT8 && BIAS;
+template <int CODE, bool BIAS>
+constexpr float kCodeUnit = kBiased<CODE, BIAS> ? 0x1p24f : 1.f;  // what a product of such halves is multiplied by
+
+// Codes 0 and 2 (PAIR 0) or 1 and 3 of a word.
+template <int CODE, bool BIAS, int PAIR>
 __device__ __forceinline__ uint32_t halves(uint32_t w) {
-    if constexpr (CODE == I4D_CODE_INT8) {
-        const uint32_t m = __byte_perm(w, 0x64646464u, PAIR ? 0x4342 : 0x4140);
+    if constexpr (kBiased<CODE, BIAS>) {
+        return ((PAIR ? w >> 8 : w) ^ 0x00800080u) & 0x00ff00ffu;
+    } else if constexpr (CODE == I4D_CODE_INT8) {
+        const uint32_t m = __byte_perm(w ^ 0x80808080u, 0x64646464u, PAIR ? 0x4341 : 0x4240);
         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
         return *reinterpret_cast<const uint32_t*>(&h);
     } else {
         uint32_t h;
-        const uint16_t p = static_cast<uint16_t>(PAIR ? w >> 16 : w);
+        const uint16_t p = static_cast<uint16_t>(__byte_perm(w, 0, PAIR ? 0x4431 : 0x4420));
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
         return h;
+    }
+}
+
+// Codes 0, 1 (PAIR 0) or 2, 3 (PAIR 1) of words a and b (INT8: with their top
+// bits flipped): out[0] the first code of both, out[1] the second.
+template <int CODE, int PAIR>
+__device__ __forceinline__ void halves2(uint32_t a, uint32_t b, uint32_t out[2]) {
+    const uint32_t x = __byte_perm(a, b, PAIR ? 0x7362 : 0x5140);  // a0 b0 a1 b1
+    if constexpr (CODE == I4D_CODE_INT8) {
+        const uint32_t m0 = __byte_perm(x, 0x64646464u, 0x4140), m1 = __byte_perm(x, 0x64646464u, 0x4342);
+        const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+        const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), bias), h1 = __hsub2(*reinterpret_cast<const __half2*>(&m1), bias);
+        out[0] = *reinterpret_cast<const uint32_t*>(&h0);
+        out[1] = *reinterpret_cast<const uint32_t*>(&h1);
+    } else {
+        const uint16_t lo = static_cast<uint16_t>(x), hi = static_cast<uint16_t>(x >> 16);
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(out[0]) : "h"(lo));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(out[1]) : "h"(hi));
     }
 }
 
@@ -135,18 +165,19 @@ __device__ __forceinline__ void store_out(const AttnDev& a, int64_t i, float v) 
     else static_cast<__half*>(a.out)[i] = __float2half_rn(v);
 }
 
-// The query rows of a tile as B operands: row `nt * 8 + lane / 4`, codes'
-// order of the summation index.  factor[nt][j]: what the score sums of row
-// nt * 8 + 2 (lane % 4) + j are multiplied by (besides the block's scale).
+// The query rows of a tile as B operands: row `nt * 8 + lane / 4`, the codes'
+// order of the summation index (elements 0 and 2, 1 and 3 of four).  Score
+// sums of row nt * 8 + 2 (lane % 4) + j are multiplied by factor[nt][j] (and
+// the block's scale) after offset[nt][j] has been taken off.
 template <int DT, int NT, bool HL>
 struct QTile {
     static constexpr int KS = DT / 16;
     uint32_t hi[NT][KS][2];
     uint32_t lo[HL ? NT : 1][HL ? KS : 1][2];
-    float factor[NT][2];
+    float factor[NT][2], offset[NT][2];
 };
 
-template <int DT, int NT, bool HL>
+template <int DT, int CODE, int NT, bool HL>
 __device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h, int row0, QTile<DT, NT, HL>& q) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dim = a.cache.dim;
 #pragma unroll
@@ -172,20 +203,27 @@ __device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h
         // 2^e with the row's largest value in [2^13, 2^14)
         const int e = max(-115, min(126, 13 - ((__float_as_int(top) >> 23) - 127)));
         const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
+        float total = 0.f;
 #pragma unroll
         for (int c = 0; c < DT / 64; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
+                const int e = i / 2 * 4 + (i & 1);
+                const float u = x[c][e] * up, v = x[c][e + 2] * up;
                 const uint32_t w = pack_h2(u, v);
                 q.hi[nt][c * 4 + i / 2][i & 1] = w;
-                if constexpr (HL) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-                    q.lo[nt][c * 4 + i / 2][i & 1] = pack_h2(u - f.x, v - f.y);
-                }
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                total += f.x + f.y;
+                if constexpr (HL) q.lo[nt][c * 4 + i / 2][i & 1] = pack_h2(u - f.x, v - f.y);
             }
+        total += __shfl_xor_sync(~0u, total, 1);
+        total += __shfl_xor_sync(~0u, total, 2);
+        constexpr float unit = kCodeUnit<CODE, !HL>;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) q.factor[nt][j] = __shfl_sync(~0u, down, (2 * t + j) * 4) * a.scale_log2;
+        for (int j = 0; j < 2; ++j) {
+            q.factor[nt][j] = __shfl_sync(~0u, down, (2 * t + j) * 4) * a.scale_log2 * unit;
+            q.offset[nt][j] = kBiased<CODE, !HL> ? __shfl_sync(~0u, total, (2 * t + j) * 4) * (128.f / unit) : 0.f;
+        }
     }
 }
 
@@ -219,13 +257,29 @@ __device__ __forceinline__ int v_piece(int r, int c) {
     return DT == 64 ? c ^ ((r >> 1) & 2) : DT == 128 ? c ^ (r & 6) : c ^ (((r >> 1) & 1) | (r & 4));
 }
 
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 // Copies n of the 16 tokens at k and v into a ring slot [K: 16][DT], [V: 16][DT]; zeros elsewhere.
 template <int DT>
 __device__ __forceinline__ void copy_tile(uint32_t slot, const uint8_t* k, const uint8_t* v, int dim, int n) {
+    constexpr int kPieces = DT / 16, kRowsAtOnce = 32 / kPieces;  // a warp's 512 bytes are rows, or part of one
     const int lane = threadIdx.x & 31;
+    if (n == 16 && dim == DT) {  // 16 whole rows lie in one piece of memory
+        k += lane * 16;
+        v += lane * 16;
 #pragma unroll
+        for (int i = 0; i < DT / 32; ++i) {
+            const int r = i * kRowsAtOnce + lane / kPieces, c = lane % kPieces;
+            copy16(slot + r * DT + k_piece<DT>(r, c) * 16, k + i * 512);
+            copy16(slot + 16 * DT + r * DT + v_piece<DT>(r, c) * 16, v + i * 512);
+        }
+        return;
+    }
+#pragma unroll 1
     for (int i = 0; i < DT / 32; ++i) {
-        const int e = i * 32 + lane, r = e / (DT / 16), c = e % (DT / 16);
+        const int r = i * kRowsAtOnce + lane / kPieces, c = lane % kPieces;
         const int bytes = r < n && c * 16 < dim ? 16 : 0;
         const int from = bytes ? r * dim + c * 16 : 0;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + r * DT + k_piece<DT>(r, c) * 16), "l"(k + from), "r"(bytes) : "memory");
@@ -261,8 +315,7 @@ __device__ __forceinline__ void score_tile(const KTile<DT>& kt, const QTile<DT, 
         const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&kt.w[1][c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t x = flip<CODE>(w0[i]), y = flip<CODE>(w1[i]);
-            const uint32_t f[4] = {halves<CODE, 0>(x), halves<CODE, 0>(y), halves<CODE, 1>(x), halves<CODE, 1>(y)};
+            const uint32_t f[4] = {halves<CODE, !HL, 0>(w0[i]), halves<CODE, !HL, 0>(w1[i]), halves<CODE, !HL, 1>(w0[i]), halves<CODE, !HL, 1>(w1[i])};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float* sum = i & 1 ? odd[nt] : s[nt];
@@ -306,7 +359,8 @@ __device__ __forceinline__ void read_vtile(uint32_t slot, VTile<DT>& vt) {
     }
 }
 
-// acc[i]: dims (lane / 4) * DT / 8 + 2 i and + 1, rows 2t and 2t + 1 of each tile.
+// acc[i]: dims (lane / 4) * DT / 8 + 2 i and + 1, rows 2t and 2t + 1 of each
+// tile.
 template <int DT, int CODE, int NT, bool HL>
 __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (&p)[NT][2], const uint32_t (&pl)[NT][2], float acc[DT / 16][NT][4]) {
 #pragma unroll
@@ -314,8 +368,15 @@ __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (
         const uint32_t w0 = flip<CODE>(vt.w[0][w]), w1 = flip<CODE>(vt.w[1][w]), w2 = flip<CODE>(vt.w[2][w]), w3 = flip<CODE>(vt.w[3][w]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint32_t x = __byte_perm(w0, w1, half ? 0x7362 : 0x5140), y = __byte_perm(w2, w3, half ? 0x7362 : 0x5140);
-            const uint32_t f[4] = {halves<CODE, 0>(x), halves<CODE, 1>(x), halves<CODE, 0>(y), halves<CODE, 1>(y)};
+            uint32_t x[2], y[2];
+            if (half) {
+                halves2<CODE, 1>(w0, w1, x);
+                halves2<CODE, 1>(w2, w3, y);
+            } else {
+                halves2<CODE, 0>(w0, w1, x);
+                halves2<CODE, 0>(w2, w3, y);
+            }
+            const uint32_t f[4] = {x[0], x[1], y[0], y[1]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 mma(acc[2 * w + half][nt], f, p[nt][0], p[nt][1]);
@@ -331,7 +392,7 @@ __device__ __forceinline__ int2 row_span(const AttnDev& a, int pos) {
 }
 
 template <int DT>
-constexpr int kAttnSlots = DT == 256 ? 3 : DT == 128 ? 4 : 6;  // ring slots of a warp
+constexpr int kAttnSlots = DT == 256 ? 3 : DT == 128 ? 3 : 6;  // ring slots of a warp
 constexpr int kAttnBlocks = 256; // table entries a chunk can hold
 
 template <int DT, int NT>
@@ -341,13 +402,16 @@ constexpr size_t attn_smem() {
     return ring > merge ? ring : merge;
 }
 
+// CTAs an SM: by shared memory and by registers (8 rows of up to 128 values in 128 registers).
+template <int DT, int NT>
+constexpr int kAttnPlaces = DT == 256 || NT == 2 ? 2 : 4;
+
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_kv8_attn(AttnDev a) {
+__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(AttnDev a) {
     constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
     extern __shared__ __align__(16) unsigned char attn_ring[];
-    __shared__ int s_id[kAttnBlocks];
-    __shared__ float2 s_scale[kAttnBlocks];
+    __shared__ float4 s_block[kAttnBlocks];  // id, scale of K, of V, log2 of the latter
     float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % a.splits;
@@ -369,13 +433,13 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
     const int begin = max(lo_span.x, split * a.chunk) & ~15, end = min(hi_span.y, (split + 1) * a.chunk);
     const int all_from = hi_span.x, all_to = lo_span.y;
 
-    float M[NT][2], R[NT][2], l[NT][2], to_r[NT][2], acc[DT / 16][NT][4];
+    float M[NT][2], R[NT][2], l[NT][2], to_r[NT][2], from[NT][2], acc[DT / 16][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             M[nt][j] = R[nt][j] = -INFINITY;
-            l[nt][j] = to_r[nt][j] = 0.f;
+            l[nt][j] = to_r[nt][j] = from[nt][j] = 0.f;
         }
 #pragma unroll
     for (int i = 0; i < DT / 16; ++i)
@@ -389,18 +453,21 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
         const int blk0 = begin >> shift;
         for (int i = threadIdx.x; i <= ((end - 1) >> shift) - blk0; i += kAttnThreads) {
             const int id = load_block(a.seq, b, blk0 + i, true);
-            s_id[i] = id;
+            float4 x = make_float4(__int_as_float(id), 0.f, 0.f, 0.f);
             if (id >= 0) {
                 const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
-                s_scale[i] = make_float2(__ldg(a.cache.scale[0] + at), __ldg(a.cache.scale[1] + at));
+                x.y = __ldg(a.cache.scale[0] + at);
+                x.z = __ldg(a.cache.scale[1] + at);
+                x.w = __log2f(x.z);  // only a bound: its rounding cancels
             }
+            s_block[i] = x;
         }
         __syncthreads();
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(attn_ring)) + warp * kSlots * 32 * DT;
         const int tiles = (end - begin + 15) / 16;
         auto issue = [&](int i, int slot) {
             if (i < tiles) {
-                const int at = begin + 16 * i, id = s_id[(at >> shift) - blk0];
+                const int at = begin + 16 * i, id = __float_as_int(s_block[(at >> shift) - blk0].x);
                 const int64_t off = id < 0 ? 0 : code_offset(a.cache, id, h) + static_cast<int64_t>(at & (bs - 1)) * dim;
                 copy_tile<DT>(ring + slot * 32 * DT, a.cache.codes[0] + off, a.cache.codes[1] + off, dim, id < 0 ? 0 : min(16, end - at));
             }
@@ -409,7 +476,7 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
 #pragma unroll
         for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
         QTile<DT, NT, HLQ> q;
-        load_qtile<DT, NT, HLQ>(a, s, h, row0, q);
+        load_qtile<DT, CODE, NT, HLQ>(a, s, h, row0, q);
         int slot = 0;
         for (int i = warp; i < tiles; i += kAttnWarps) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
@@ -417,9 +484,10 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
             issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
             const uint32_t at_slot = ring + slot * 32 * DT;
             slot = slot == kSlots - 1 ? 0 : slot + 1;
-            const int at = begin + 16 * i, entry = (at >> shift) - blk0;
-            if (s_id[entry] < 0) continue;
-            const float2 scale = s_scale[entry];
+            const int at = begin + 16 * i;
+            const float4 block = s_block[(at >> shift) - blk0];
+            if (__float_as_int(block.x) < 0) continue;
+            const float lvs = block.w;
             const int live = min(16, end - at);
             float x[NT][4];
             {
@@ -429,15 +497,15 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
             }
             VTile<DT> vt;
             read_vtile<DT>(at_slot, vt);
-            float top[NT][2], lvs = __log2f(scale.y);  // only a bound: its rounding cancels
+            float top[NT][2];
             const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
             bool raise = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float f = q.factor[nt][j] * scale.x;
-                    float y0 = x[nt][j] * f, y1 = x[nt][j + 2] * f;
+                    const float f = q.factor[nt][j] * block.y, off = q.offset[nt][j] * f;
+                    float y0 = fmaf(x[nt][j], f, -off), y1 = fmaf(x[nt][j + 2], f, -off);
                     if (!whole) {
                         const int2 span = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
                         if (!(g < live && at + g >= span.x && at + g < span.y)) y0 = -INFINITY;
@@ -467,6 +535,7 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
                         }
                         M[nt][j] = m;
                         R[nt][j] = r;
+                        from[nt][j] = m == -INFINITY ? 0.f : m;
                         to_r[nt][j] = r == -INFINITY ? 0.f : ex2(m - r);
                     }
             }
@@ -486,9 +555,9 @@ __global__ void __launch_bounds__(kAttnThreads, DT == 256 || NT == 2 ? 2 : 3) k_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int j = k & 1;
-                    const float e = ex2(x[nt][k] - (M[nt][j] == -INFINITY ? 0.f : M[nt][j]));
+                    const float e = ex2(x[nt][k] - from[nt][j]);
                     l[nt][j] += e;
-                    w[k] = e * (to_r[nt][j] * scale.y);
+                    w[k] = e * (to_r[nt][j] * block.z);
                 }
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -682,7 +751,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_weights(AttnDev a, int til
     const int to = a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(rows), max(int64_t{0}, (static_cast<int64_t>(at) + 15 + a.window - first)) * a.group)) : rows;
     for (int row0 = from; row0 < to; row0 += 8) {
         QTile<DT, 1, HL> q;
-        load_qtile<DT, 1, HL>(a, s, h, row0, q);
+        load_qtile<DT, CODE, 1, HL>(a, s, h, row0, q);
         float x[1][4];
         score_tile<DT, CODE, 1, HL>(kt, q, x);
 #pragma unroll
@@ -694,7 +763,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_weights(AttnDev a, int til
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int n = at + g + 8 * r;
-                if (n < s.len && n >= sp.x && n < sp.y) sum[r] += ex2(fmaf(x[0][j + 2 * r], q.factor[0][j] * ks, -l2));
+                if (n < s.len && n >= sp.x && n < sp.y) sum[r] += ex2(fmaf(x[0][j + 2 * r] - q.offset[0][j], q.factor[0][j] * ks, -l2));
             }
         }
     }

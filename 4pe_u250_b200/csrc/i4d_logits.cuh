@@ -45,11 +45,13 @@ __device__ __forceinline__ unsigned long long logit_key(float x, int index) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas) {
+__global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int ctas) {
     extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
     int* counts = reinterpret_cast<int*>(logits_smem);                  // bit 0: seen in the prompt, above: 2 * occurrences after it
     float* bias = reinterpret_cast<float*>(counts + kLogitsSlice);
+    __shared__ int found[kLogitsThreads / 32];
+    __shared__ float2 entries[kLogitsThreads];
     __shared__ unsigned long long keys[kLogitsThreads / 32];
     __shared__ unsigned long long cta_key[16];
     cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
@@ -109,25 +111,33 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
                 else atomicAdd(&counts[id - e0], 2);
             }
         }
-        if (tid < 32) {  // one warp, so that the values of one id are added in their order
-            for (int i = 0; i < n_bias; i += 32) {
-                const bool live = i + tid < n_bias;
-                const int id = live ? __ldg(a.bias_ids + row * a.bias_stride + i + tid) : -1;
-                const float val = live ? __ldg(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
-                const bool mine = live && id >= max(e0, 0) && id < a.vocab && id - e0 < span;
-                const unsigned peers = __match_any_sync(~0u, mine ? id : -1 - tid);
-                const bool leader = __ffs(peers) - 1 == tid;
-                float sum = mine && leader ? bias[id - e0] : 0.f;
-                if (__any_sync(~0u, mine && !leader)) {
-                    for (int l = 0; l < 32; ++l) {
-                        const float v = __shfl_sync(~0u, val, l);
-                        if (peers >> l & 1) sum = __fadd_rn(sum, v);
-                    }
-                } else {
-                    sum = __fadd_rn(sum, val);
+        // Biases: the slice's entries of a round in their order, then the first
+        // of each id adds up the values of that id.
+        for (int i = 0; i < n_bias; i += kLogitsThreads) {
+            const bool live = i + tid < n_bias;
+            const int id = live ? __ldg(a.bias_ids + row * a.bias_stride + i + tid) : -1;
+            const bool mine = live && id >= max(e0, 0) && id < a.vocab && id - e0 < span;
+            const unsigned votes = __ballot_sync(~0u, mine);
+            if ((tid & 31) == 0) found[tid >> 5] = __popc(votes);
+            __syncthreads();
+            int at = __popc(votes & ((1u << (tid & 31)) - 1)), total = 0;
+#pragma unroll
+            for (int w = 0; w < kLogitsThreads / 32; ++w) {
+                at += w < tid >> 5 ? found[w] : 0;
+                total += found[w];
+            }
+            if (mine) entries[at] = make_float2(__int_as_float(id - e0), __ldg(a.bias_values + row * a.bias_stride + i + tid));
+            __syncthreads();
+            if (tid < total) {
+                const int slot = __float_as_int(entries[tid].x);
+                bool leads = true;
+                for (int k = 0; k < tid; ++k) leads &= __float_as_int(entries[k].x) != slot;
+                if (leads) {
+                    float sum = bias[slot];
+                    for (int k = tid; k < total; ++k)
+                        if (__float_as_int(entries[k].x) == slot) sum = __fadd_rn(sum, entries[k].y);
+                    bias[slot] = sum;
                 }
-                if (mine && leader) bias[id - e0] = sum;
-                __syncwarp();
             }
         }
         __syncthreads();
@@ -136,28 +146,28 @@ __global__ void __launch_bounds__(kLogitsThreads) k_logits(LogitsDev a, int ctas
             const int v = v0 + u * kLogitsThreads + tid, e = v * V - skew, at = (v - v0) * V;
             if (v >= v1) continue;
             const bool whole = e >= 0 && e + V <= a.vocab;
-            int c[V];
-            float add[V];
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                *reinterpret_cast<int4*>(c + i) = n_hist ? *reinterpret_cast<const int4*>(counts + at + i) : make_int4(0, 0, 0, 0);
-                if (n_bias) *reinterpret_cast<float4*>(add + i) = *reinterpret_cast<const float4*>(bias + at + i);
-            }
+            for (int i0 = 0; i0 < V; i0 += 4) {
+                int c[4];
+                float add[4];
+                *reinterpret_cast<int4*>(c) = n_hist ? *reinterpret_cast<const int4*>(counts + at + i0) : make_int4(0, 0, 0, 0);
+                if (n_bias) *reinterpret_cast<float4*>(add) = *reinterpret_cast<const float4*>(bias + at + i0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int id = e + i;
-                if (!whole && (id < 0 || id >= a.vocab)) continue;
-                float y = to_f32(x[u].v[i]);
-                if (c[i]) {
-                    const int n = c[i] >> 1;
-                    if (a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                    if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                for (int k = 0; k < 4; ++k) {
+                    const int i = i0 + k, id = e + i;
+                    if (!whole && (id < 0 || id >= a.vocab)) continue;
+                    float y = to_f32(x[u].v[i]);
+                    if (c[k]) {
+                        const int n = c[k] >> 1;
+                        if (a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                        if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                    }
+                    if (n_bias) y = __fadd_rn(y, add[k]);
+                    const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? words[u].x : words[u].y;
+                    if (!(w >> (id & 31) & 1)) y = -INFINITY;
+                    x[u].v[i] = from_f32<T>(y);
+                    key = max(key, logit_key(to_f32(x[u].v[i]), id));
                 }
-                if (n_bias) y = __fadd_rn(y, add[i]);
-                const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? words[u].x : words[u].y;
-                if (!(w >> (id & 31) & 1)) y = -INFINITY;
-                x[u].v[i] = from_f32<T>(y);
-                key = max(key, logit_key(to_f32(x[u].v[i]), id));
             }
             if (whole && aligned_out) {
                 *reinterpret_cast<Vec<T, V>*>(out + e) = x[u];

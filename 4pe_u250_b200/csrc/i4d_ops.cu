@@ -181,7 +181,7 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     // Chunks: a few CTAs for each place on the GPU, so that ragged lengths even
     // out, but none under 128 tokens (two tiles a warp) nor above what the
     // kernel's table of blocks holds.
-    const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 3) * static_cast<int64_t>(o.num_sms);
+    const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 4) * static_cast<int64_t>(o.num_sms);
     const int64_t want = std::max<int64_t>(1, 12 * places / std::max<int64_t>(1, p.tiles));
     int64_t chunk = (a.max_length + want - 1) / want;
     chunk = std::min<int64_t>(std::max<int64_t>(128, (chunk + 127) / 128 * 128), kAttnBlocks * c.block_tokens / 2);
