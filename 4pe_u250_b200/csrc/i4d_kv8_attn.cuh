@@ -46,10 +46,10 @@ struct AttnDev {
     int64_t q_tok, q_head, out_tok, out_head, weights_stride;
     int heads, group, window, dtype, max_length, wide_q;
     float scale_log2;  // softmax scale * log2(e)
-    int row_tiles;     // tiles of a (sequence, cache head)
-    int splits, chunk; // token chunks of a tile
-    float* part;       // workspace: [tile][split][rows][dim]: O
-    float4* stats;     // workspace: [tile][rows][split]: M, l, R
+    int batch, row_tiles;  // row tiles of a (sequence, cache head), at most
+    int even;              // CTAs that share the tokens evenly, or 0: one for each (sequence, cache head, row tile)
+    float* part;       // workspace: [even][2][rows][dim]: O of a CTA's pieces that are not whole
+    float4* stats;     // workspace: [even][2][rows]: M, l, R
     float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
     float* scores;     // workspace (few rows, with weights): [tile][rows][max_length], log2 scale
 };
@@ -393,7 +393,7 @@ __device__ __forceinline__ int2 row_span(const AttnDev& a, int pos) {
 
 template <int DT>
 constexpr int kAttnSlots = DT == 256 ? 3 : DT == 128 ? 3 : 6;  // ring slots of a warp
-constexpr int kAttnBlocks = 256; // table entries a chunk can hold
+constexpr int kAttnBlocks = 256; // blocks whose ids and scales are held at a time
 
 template <int DT, int NT>
 constexpr size_t attn_smem() {
@@ -406,31 +406,90 @@ constexpr size_t attn_smem() {
 template <int DT, int NT>
 constexpr int kAttnPlaces = DT == 256 || NT == 2 ? 2 : 4;
 
+// The work of a call in units of 16 tokens: sequence by sequence, its row
+// tiles of each head, the tokens that any row of the sequence sees.
+struct Units {
+    int tiles;     // token tiles of one (head, row tile)
+    int segments;  // heads * row tiles of the sequence
+};
+__device__ __forceinline__ Units seq_units(const AttnDev& a, const Seq& s, int rows_per_tile) {
+    if (s.n == 0 || s.len > a.max_length) return {0, 0};
+    const int lo = row_span(a, s.len - s.n).x & ~15;
+    return {(s.len - lo + 15) >> 4, a.cache.heads * ((s.n * a.group + rows_per_tile - 1) / rows_per_tile)};
+}
+
+struct Place {
+    int64_t before;  // units of the sequences before `seq`
+    int seq;
+};
+
+// Units of the whole batch and, in *at, the sequence in which unit u lies (or
+// those before sequence `want`, u < 0).  The CTA's threads take consecutive
+// sequences each.
+__device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_tile, int64_t u, int want, bool report, Place* at) {
+    __shared__ int64_t s_sum[kAttnWarps];
+    __shared__ Place s_place;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (a.batch + kAttnThreads - 1) / kAttnThreads, b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Seq s = load_seq(a.seq, b, report);
+        if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
+        const Units n = seq_units(a, s, rows_per_tile);
+        mine += static_cast<int64_t>(n.tiles) * n.segments;
+    }
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+        if (w < warp) upto += s_sum[w];
+        total += s_sum[w];
+    }
+    int64_t before = upto - mine;
+    if (u >= 0 ? u >= before && u < upto : want >= b0 && want < b1) {
+        for (int b = b0; b < b1; ++b) {
+            const Units n = seq_units(a, load_seq(a.seq, b, false), rows_per_tile);
+            const int64_t next = before + static_cast<int64_t>(n.tiles) * n.segments;
+            if (u >= 0 ? u < next : b == want) {
+                s_place = {before, b};
+                break;
+            }
+            before = next;
+        }
+    }
+    __syncthreads();
+    *at = s_place;
+    return total;
+}
+
+// One piece of work of a CTA: token tiles [t0, t1) of a segment, whose first
+// tile begins at token lo.
+struct Piece {
+    int b, h, rt;
+    int begin, end;  // tokens, begin a multiple of 16
+    bool whole;      // the segment's only piece
+    int slot;        // where its partial sums go otherwise: 0 the CTA's first piece, 1 its last
+};
+
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(AttnDev a) {
+__device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block) {
     constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
-    extern __shared__ __align__(16) unsigned char attn_ring[];
-    __shared__ float4 s_block[kAttnBlocks];  // id, scale of K, of V, log2 of the latter
     float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % a.splits;
-    const int64_t tile = blockIdx.x / a.splits;
-    const int rt = tile % a.row_tiles, h = tile / a.row_tiles % a.cache.heads;
-    const int b = tile / a.row_tiles / a.cache.heads;
-    const bool report = split == 0 && rt == 0 && h == 0 && threadIdx.x == 0;
-    Seq s = load_seq(a.seq, b, report);
-    if (s.len > a.max_length) {
-        if (report) atomicOr(a.seq.err, kBadSequence);
-        return;
-    }
-    const int row0 = rt * kRows;
-    if (row0 >= s.n * a.group) return;
+    const int b = pc.b, h = pc.h, row0 = pc.rt * kRows;
     const int first = s.len - s.n;  // cache index of row 0's query
     const int last_row = min(row0 + kRows, s.n * a.group) - 1;
     // tokens that any row of the tile sees, and that all of them see
     const int2 lo_span = row_span(a, first + row0 / a.group), hi_span = row_span(a, first + last_row / a.group);
-    const int begin = max(lo_span.x, split * a.chunk) & ~15, end = min(hi_span.y, (split + 1) * a.chunk);
+    const int begin = max(lo_span.x & ~15, pc.begin), end = min(hi_span.y, pc.end);
     const int all_from = hi_span.x, all_to = lo_span.y;
 
     float M[NT][2], R[NT][2], l[NT][2], to_r[NT][2], from[NT][2], acc[DT / 16][NT][4];
@@ -450,129 +509,136 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
 
     if (begin < end) {
         const int bs = a.cache.block_tokens, dim = a.cache.dim, shift = 31 - __clz(bs);
-        const int blk0 = begin >> shift;
-        for (int i = threadIdx.x; i <= ((end - 1) >> shift) - blk0; i += kAttnThreads) {
-            const int id = load_block(a.seq, b, blk0 + i, true);
-            float4 x = make_float4(__int_as_float(id), 0.f, 0.f, 0.f);
-            if (id >= 0) {
-                const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
-                x.y = __ldg(a.cache.scale[0] + at);
-                x.z = __ldg(a.cache.scale[1] + at);
-                x.w = __log2f(x.z);  // only a bound: its rounding cancels
-            }
-            s_block[i] = x;
-        }
-        __syncthreads();
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(attn_ring)) + warp * kSlots * 32 * DT;
-        const int tiles = (end - begin + 15) / 16;
-        auto issue = [&](int i, int slot) {
-            if (i < tiles) {
-                const int at = begin + 16 * i, id = __float_as_int(s_block[(at >> shift) - blk0].x);
-                const int64_t off = id < 0 ? 0 : code_offset(a.cache, id, h) + static_cast<int64_t>(at & (bs - 1)) * dim;
-                copy_tile<DT>(ring + slot * 32 * DT, a.cache.codes[0] + off, a.cache.codes[1] + off, dim, id < 0 ? 0 : min(16, end - at));
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
         QTile<DT, NT, HLQ> q;
-        load_qtile<DT, CODE, NT, HLQ>(a, s, h, row0, q);
-        int slot = 0;
-        for (int i = warp; i < tiles; i += kAttnWarps) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
-            __syncwarp();  // this slot's copies of all lanes have landed; all lanes are done with the one to fill
-            issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
-            const uint32_t at_slot = ring + slot * 32 * DT;
-            slot = slot == kSlots - 1 ? 0 : slot + 1;
-            const int at = begin + 16 * i;
-            const float4 block = s_block[(at >> shift) - blk0];
-            if (__float_as_int(block.x) < 0) continue;
-            const float lvs = block.w;
-            const int live = min(16, end - at);
-            float x[NT][4];
-            {
-                KTile<DT> kt;
-                read_ktile<DT>(at_slot, kt);
-                score_tile<DT, CODE, NT, HLQ>(kt, q, x);
-            }
-            VTile<DT> vt;
-            read_vtile<DT>(at_slot, vt);
-            float top[NT][2];
-            const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
-            bool raise = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float f = q.factor[nt][j] * block.y, off = q.offset[nt][j] * f;
-                    float y0 = fmaf(x[nt][j], f, -off), y1 = fmaf(x[nt][j + 2], f, -off);
-                    if (!whole) {
-                        const int2 span = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
-                        if (!(g < live && at + g >= span.x && at + g < span.y)) y0 = -INFINITY;
-                        if (!(g + 8 < live && at + g + 8 >= span.x && at + g + 8 < span.y)) y1 = -INFINITY;
-                    }
-                    x[nt][j] = y0;
-                    x[nt][j + 2] = y1;
-                    top[nt][j] = fmaxf(y0, y1);
-                    raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + kSlack;
+        const int span = kAttnBlocks << shift;  // tokens whose blocks the table holds
+        for (int from_tok = begin; from_tok < end;) {
+            // [from_tok, to_tok): up to a block's end, so that the table's entries do
+            const int blk0 = from_tok >> shift, to_tok = static_cast<int>(min(static_cast<int64_t>(end), (static_cast<int64_t>(blk0) << shift) + span));
+            if (from_tok != begin) __syncthreads();  // the table is free
+            for (int i = threadIdx.x; i <= ((to_tok - 1) >> shift) - blk0; i += kAttnThreads) {
+                const int id = load_block(a.seq, b, blk0 + i, true);
+                float4 x = make_float4(__int_as_float(id), 0.f, 0.f, 0.f);
+                if (id >= 0) {
+                    const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
+                    x.y = __ldg(a.cache.scale[0] + at);
+                    x.z = __ldg(a.cache.scale[1] + at);
+                    x.w = __log2f(x.z);  // only a bound: its rounding cancels
                 }
-            if (__any_sync(~0u, raise)) {
+                s_block[i] = x;
+            }
+            __syncthreads();
+            const int tiles = (to_tok - from_tok + 15) >> 4;
+            auto issue = [&](int i, int slot) {
+                if (i < tiles) {
+                    const int at = from_tok + 16 * i, id = __float_as_int(s_block[(at >> shift) - blk0].x);
+                    const int64_t off = id < 0 ? 0 : code_offset(a.cache, id, h) + (at & (bs - 1)) * dim;
+                    copy_tile<DT>(ring + slot * 32 * DT, a.cache.codes[0] + off, a.cache.codes[1] + off, dim, id < 0 ? 0 : min(16, to_tok - at));
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll
+            for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
+            if (from_tok == begin) load_qtile<DT, CODE, NT, HLQ>(a, s, h, row0, q);
+            int slot = 0;
+            for (int i = warp; i < tiles; i += kAttnWarps) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+                __syncwarp();  // this slot's copies of all lanes have landed; all lanes are done with the one to fill
+                issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
+                const uint32_t at_slot = ring + slot * 32 * DT;
+                slot = slot == kSlots - 1 ? 0 : slot + 1;
+                const int at = from_tok + 16 * i;
+                const float4 block = s_block[(at >> shift) - blk0];
+                if (__float_as_int(block.x) < 0) continue;
+                const float lvs = block.w;
+                const int live = min(16, to_tok - at);
+                float x[NT][4];
+                {
+                    KTile<DT> kt;
+                    read_ktile<DT>(at_slot, kt);
+                    score_tile<DT, CODE, NT, HLQ>(kt, q, x);
+                }
+                VTile<DT> vt;
+                read_vtile<DT>(at_slot, vt);
+                float top[NT][2];
+                const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
+                bool raise = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float m = top[nt][j];
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                        const float r = fmaxf(m + lvs, R[nt][j]);
-                        m = fmaxf(m, M[nt][j]);
-                        const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
-                        l[nt][j] *= fm;
-#pragma unroll
-                        for (int i2 = 0; i2 < DT / 16; ++i2) {
-                            acc[i2][nt][j] *= fr;
-                            acc[i2][nt][j + 2] *= fr;
+                        const float f = q.factor[nt][j] * block.y, off = q.offset[nt][j] * f;
+                        float y0 = fmaf(x[nt][j], f, -off), y1 = fmaf(x[nt][j + 2], f, -off);
+                        if (!whole) {
+                            const int2 span = row_span(a, first + (row0 + nt * 8 + 2 * t + j) / a.group);
+                            if (!(g < live && at + g >= span.x && at + g < span.y)) y0 = -INFINITY;
+                            if (!(g + 8 < live && at + g + 8 >= span.x && at + g + 8 < span.y)) y1 = -INFINITY;
                         }
-                        M[nt][j] = m;
-                        R[nt][j] = r;
-                        from[nt][j] = m == -INFINITY ? 0.f : m;
-                        to_r[nt][j] = r == -INFINITY ? 0.f : ex2(m - r);
+                        x[nt][j] = y0;
+                        x[nt][j + 2] = y1;
+                        top[nt][j] = fmaxf(y0, y1);
+                        raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + kSlack;
                     }
-            }
-            if (a.scores) {
+                if (__any_sync(~0u, raise)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float m = top[nt][j];
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                            const float r = fmaxf(m + lvs, R[nt][j]);
+                            m = fmaxf(m, M[nt][j]);
+                            const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
+                            l[nt][j] *= fm;
+#pragma unroll
+                            for (int i2 = 0; i2 < DT / 16; ++i2) {
+                                acc[i2][nt][j] *= fr;
+                                acc[i2][nt][j + 2] *= fr;
+                            }
+                            M[nt][j] = m;
+                            R[nt][j] = r;
+                            from[nt][j] = m == -INFINITY ? 0.f : m;
+                            to_r[nt][j] = r == -INFINITY ? 0.f : ex2(m - r);
+                        }
+                }
+                if (a.scores) {
+                    const int64_t tile = (static_cast<int64_t>(b) * a.cache.heads + h) * a.row_tiles + pc.rt;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = nt * 8 + 2 * t + (k & 1), n = g + (k >> 1) * 8;
+                            if (n < live && row0 + r <= last_row) a.scores[(tile * kRows + r) * a.max_length + at + n] = x[nt][k];
+                        }
+                }
+                uint32_t p[NT][2], pl[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int r = nt * 8 + 2 * t + (k & 1), n = g + (k >> 1) * 8;
-                        if (n < live) a.scores[(tile * kRows + r) * a.max_length + at + n] = x[nt][k];
+                        const int j = k & 1;
+                        const float e = ex2(x[nt][k] - from[nt][j]);
+                        l[nt][j] += e;
+                        w[k] = e * (to_r[nt][j] * block.z);
                     }
-            }
-            uint32_t p[NT][2], pl[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int j = k & 1;
-                    const float e = ex2(x[nt][k] - from[nt][j]);
-                    l[nt][j] += e;
-                    w[k] = e * (to_r[nt][j] * block.z);
-                }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
-                    p[nt][r] = transpose8(hi);
-                    pl[nt][r] = 0;
-                    if constexpr (HLP) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                        pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
+                        p[nt][r] = transpose8(hi);
+                        pl[nt][r] = 0;
+                        if constexpr (HLP) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
+                        }
                     }
                 }
+                value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
             }
-            value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            from_tok = to_tok;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // the ring is free for the join
     }
 
@@ -596,121 +662,182 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
             }
         }
     __syncthreads();
-    const int dim = a.cache.dim;
-    for (int i = threadIdx.x; i < kRows * DT; i += kAttnThreads) {
-        const int r = i / DT, d = i % DT, row = row0 + r;
-        if (row >= s.n * a.group || d >= dim) continue;
-        float m = -INFINITY, rr = -INFINITY, sum = 0.f, o = 0.f;
+    const int dim = a.cache.dim, rows = last_row - row0 + 1;
+    if (threadIdx.x < rows) {  // a row's statistics, and what its warps' sums are multiplied by
+        const int r = threadIdx.x, row = row0 + r;
+        float m = -INFINITY, rr = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) {
             m = fmaxf(m, merge[w][r][DT]);
             rr = fmaxf(rr, merge[w][r][DT + 2]);
         }
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) {
-            if (merge[w][r][DT] == -INFINITY) {  // the warp saw nothing of this row (its sums are 0, or NaN with the row's)
-                sum += merge[w][r][DT + 1];
-                o += merge[w][r][d];
-                continue;
-            }
-            sum += merge[w][r][DT + 1] * ex2(merge[w][r][DT] - m);
-            if (merge[w][r][DT + 2] != -INFINITY) o += merge[w][r][d] * ex2(merge[w][r][DT + 2] - rr);
-        }
-        if (a.splits == 1) {
+        for (int w = 0; w < kAttnWarps; ++w)  // (a warp that saw nothing of the row: its sums are 0, or NaN with the row's)
+            sum += merge[w][r][DT + 1] * (merge[w][r][DT] == -INFINITY ? 1.f : ex2(merge[w][r][DT] - m));
+        const float back = !pc.whole ? 1.f : sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w)
+            merge[w][r][DT + 3] = (merge[w][r][DT + 2] == -INFINITY ? 1.f : ex2(merge[w][r][DT + 2] - rr)) * back;
+        if (pc.whole) {
             const int64_t tok = s.first + row / a.group;
             const int head = h * a.group + row % a.group;
-            const float back = rr == -INFINITY ? 0.f : ex2(rr - m);
-            store_out(a, tok * a.out_tok + head * a.out_head + d, sum == 0.f ? 0.f : o * back / sum);
-            if (d == 0) {
-                const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-                if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-                if (a.weights) a.lse2[tok * a.heads + head] = l2;
-            }
+            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+            if (a.weights) a.lse2[tok * a.heads + head] = l2;
         } else {
-            a.part[((tile * a.splits + split) * kRows + r) * dim + d] = o;
-            if (d == 0) a.stats[(tile * kRows + r) * a.splits + split] = make_float4(m, sum, rr, 0.f);
+            a.stats[(static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r] = make_float4(m, sum, rr, 0.f);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (DT / 4); i += kAttnThreads) {
+        const int r = i / (DT / 4), d = i % (DT / 4) * 4, row = row0 + r;
+        if (d >= dim) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(&merge[w][r][d]);
+            const float f = merge[w][r][DT + 3];
+            o.x += x.x * f;
+            o.y += x.y * f;
+            o.z += x.z * f;
+            o.w += x.w * f;
+        }
+        if (pc.whole) {
+            const int64_t at = (s.first + row / a.group) * a.out_tok + (h * a.group + row % a.group) * a.out_head + d;
+            store_out(a, at, o.x);
+            store_out(a, at + 1, o.y);
+            store_out(a, at + 2, o.z);
+            store_out(a, at + 3, o.w);
+        } else {
+            *reinterpret_cast<float4*>(a.part + ((static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r) * dim + d) = o;
         }
     }
 }
 
-// Joins the chunks of a tile: one warp for a row.
-__global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_per_tile, int64_t rows_total) {
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * kAttnWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, r = w % rows_per_tile;
-    const int64_t tile = w / rows_per_tile;
-    const int rt = tile % a.row_tiles, h = tile / a.row_tiles % a.cache.heads;
-    const int64_t b = tile / a.row_tiles / a.cache.heads;
-    if (w >= rows_total) return;
-    const Seq s = load_seq(a.seq, static_cast<int>(b), false);
-    const int row = rt * rows_per_tile + r;
-    if (s.len > a.max_length || row >= s.n * a.group) return;
-    const int2 sp = row_span(a, s.len - s.n + row / a.group);
-    // chunks that the row's tile looked at (a tile's first row may begin earlier; its chunk holds no token of this row then)
-    const int c0 = sp.x / a.chunk, c1 = (sp.y + a.chunk - 1) / a.chunk, dim = a.cache.dim;
-    const float4* stats = a.stats + (tile * rows_per_tile + r) * a.splits;
-    float m = -INFINITY, rr = -INFINITY, sum = 0.f;
-    for (int c = c0 + lane; c < c1; c += 32) {
-        const float4 x = stats[c];
-        m = fmaxf(m, x.x);
-        rr = fmaxf(rr, x.z);
+template <int DT, int CODE, int NT, bool HLQ, bool HLP>
+__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(AttnDev a) {
+    constexpr int kRows = 8 * NT;
+    extern __shared__ __align__(16) unsigned char attn_ring[];
+    __shared__ float4 s_block[kAttnBlocks];  // id, scale of K, of V, log2 of the latter
+    if (!a.even) {
+        const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.cache.heads, b = blockIdx.x / a.row_tiles / a.cache.heads;
+        const bool report = rt == 0 && h == 0 && threadIdx.x == 0;
+        const Seq s = load_seq(a.seq, b, report);
+        if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
+        if (s.len > a.max_length || rt * kRows >= s.n * a.group) return;
+        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, 0, s.len, true, 0}, attn_ring, s_block);
+        return;
     }
-    m = warp_max(m);
-    rr = warp_max(rr);
-    const int64_t tok = s.first + row / a.group;
-    const int head = h * a.group + row % a.group;
-    float4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // dims 4 lane and 128 + 4 lane
-    const float* part = a.part + (tile * a.splits * rows_per_tile + r) * dim + 4 * lane;
-    const int64_t step = static_cast<int64_t>(rows_per_tile) * dim;
-    const bool low = 4 * lane < dim, high = 128 + 4 * lane < dim;
-    for (int base = c0; base < c1; base += 32) {
-        float f = 0.f;  // the factor of chunk base + lane
-        if (base + lane < c1) {
-            const float4 x = stats[base + lane];
-            sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
-            f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
+    Place at;
+    const bool report = blockIdx.x == 0;
+    const int64_t total = find_units(a, kRows, 0, 0, report, &at), share = (total + a.even - 1) / a.even;
+    int64_t u = static_cast<int64_t>(blockIdx.x) * share;
+    const int64_t u_end = min(total, u + share), u0 = u;
+    if (u >= u_end) return;
+    find_units(a, kRows, u, 0, false, &at);
+    while (u < u_end) {
+        const Seq s = load_seq(a.seq, at.seq, false);
+        const Units n = seq_units(a, s, kRows);
+        const int64_t size = static_cast<int64_t>(n.tiles) * n.segments;
+        if (u >= at.before + size) {
+            at.before += size;
+            ++at.seq;
+            continue;
         }
-        const int n = min(32, c1 - base);
+        const int seg = static_cast<int>((u - at.before) / n.tiles), row_tiles = n.segments / a.cache.heads;
+        const int64_t seg0 = at.before + static_cast<int64_t>(seg) * n.tiles;
+        const int t0 = static_cast<int>(u - seg0), t1 = static_cast<int>(min(static_cast<int64_t>(n.tiles), u_end - seg0));
+        const int lo = row_span(a, s.len - s.n).x & ~15;
+        if (u != u0) __syncthreads();  // the previous piece's shared memory is free
+        attend<DT, CODE, NT, HLQ, HLP>(a, s, {at.seq, seg / row_tiles, seg % row_tiles, lo + 16 * t0, min(s.len, lo + 16 * t1), t0 == 0 && t1 == n.tiles, u == u0 ? 0 : 1},
+                                       attn_ring, s_block);
+        u = seg0 + t1;
+    }
+}
+
+// Joins the pieces of the segments that several CTAs shared: one CTA for a
+// segment, a warp for a row at a time.
+__global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_per_tile) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.cache.heads, b = blockIdx.x / a.row_tiles / a.cache.heads;
+    const int lane = threadIdx.x & 31, dim = a.cache.dim;
+    const Seq s = load_seq(a.seq, b, false);
+    const Units n = seq_units(a, s, rows_per_tile);
+    const int row_tiles = n.segments / a.cache.heads;
+    if (rt >= row_tiles) return;
+    Place at;
+    const int64_t total = find_units(a, rows_per_tile, -1, b, false, &at), share = (total + a.even - 1) / a.even;
+    const int64_t seg0 = at.before + (static_cast<int64_t>(h) * row_tiles + rt) * n.tiles, seg1 = seg0 + n.tiles;
+    const int c0 = static_cast<int>(seg0 / share), c1 = static_cast<int>((seg1 - 1) / share);
+    if (c0 == c1) return;  // whole
+    const int rows = min(rows_per_tile, s.n * a.group - rt * rows_per_tile);
+    for (int r = threadIdx.x >> 5; r < rows; r += kAttnWarps) {
+        // piece c: a CTA's first one unless the CTA began in an earlier segment
+        auto index = [&](int c) { return (static_cast<int64_t>(c) * 2 + (static_cast<int64_t>(c) * share < seg0 ? 1 : 0)) * rows_per_tile + r; };
+        float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+        for (int c = c0 + lane; c <= c1; c += 32) {
+            const float4 x = a.stats[index(c)];
+            m = fmaxf(m, x.x);
+            rr = fmaxf(rr, x.z);
+        }
+        m = warp_max(m);
+        rr = warp_max(rr);
+        float4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // dims 4 lane and 128 + 4 lane
+        const bool low = 4 * lane < dim, high = 128 + 4 * lane < dim;
+        for (int base = c0; base <= c1; base += 32) {
+            float f = 0.f;  // the factor of piece base + lane
+            if (base + lane <= c1) {
+                const float4 x = a.stats[index(base + lane)];
+                sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
+                f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
+            }
+            const int k1 = min(32, c1 + 1 - base);
 #pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-            const float fk = __shfl_sync(~0u, f, k);
-            const float* p = part + (base + k) * step;
-            if (low) {
-                const float4 x = *reinterpret_cast<const float4*>(p);
-                o[0].x += x.x * fk;
-                o[0].y += x.y * fk;
-                o[0].z += x.z * fk;
-                o[0].w += x.w * fk;
-            }
-            if (high) {
-                const float4 x = *reinterpret_cast<const float4*>(p + 128);
-                o[1].x += x.x * fk;
-                o[1].y += x.y * fk;
-                o[1].z += x.z * fk;
-                o[1].w += x.w * fk;
+            for (int k = 0; k < k1; ++k) {
+                const float fk = __shfl_sync(~0u, f, k);
+                const float* p = a.part + index(base + k) * dim + 4 * lane;
+                if (low) {
+                    const float4 x = *reinterpret_cast<const float4*>(p);
+                    o[0].x += x.x * fk;
+                    o[0].y += x.y * fk;
+                    o[0].z += x.z * fk;
+                    o[0].w += x.w * fk;
+                }
+                if (high) {
+                    const float4 x = *reinterpret_cast<const float4*>(p + 128);
+                    o[1].x += x.x * fk;
+                    o[1].y += x.y * fk;
+                    o[1].z += x.z * fk;
+                    o[1].w += x.w * fk;
+                }
             }
         }
-    }
-    sum = warp_sum(sum);
-    const float back = sum == 0.f ? 0.f : rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+        sum = warp_sum(sum);
+        const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+        const int row = rt * rows_per_tile + r;
+        const int64_t tok = s.first + row / a.group;
+        const int head = h * a.group + row % a.group;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if (k ? !high : !low) continue;
-        const int64_t at = tok * a.out_tok + head * a.out_head + 128 * k + 4 * lane;
-        store_out(a, at, sum == 0.f ? 0.f : o[k].x * back);
-        store_out(a, at + 1, sum == 0.f ? 0.f : o[k].y * back);
-        store_out(a, at + 2, sum == 0.f ? 0.f : o[k].z * back);
-        store_out(a, at + 3, sum == 0.f ? 0.f : o[k].w * back);
-    }
-    if (lane == 0) {
-        const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-        if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-        if (a.weights) a.lse2[tok * a.heads + head] = l2;
+        for (int k = 0; k < 2; ++k) {
+            if (k ? !high : !low) continue;
+            const int64_t to = tok * a.out_tok + head * a.out_head + 128 * k + 4 * lane;
+            store_out(a, to, o[k].x * back);
+            store_out(a, to + 1, o[k].y * back);
+            store_out(a, to + 2, o[k].z * back);
+            store_out(a, to + 3, o[k].w * back);
+        }
+        if (lane == 0) {
+            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+            if (a.weights) a.lse2[tok * a.heads + head] = l2;
+        }
     }
 }
 
 // Probabilities summed over a head's few rows for each token, from the scores
 // that k_kv8_attn kept: one thread for a token, rows in order.
 __global__ void __launch_bounds__(256) k_kv8_weights_kept(AttnDev a, int rows_per_tile, int chunks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t bh = blockIdx.x / chunks;
     const int n = (blockIdx.x % chunks) * 256 + threadIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const Seq s = load_seq(a.seq, b, false);

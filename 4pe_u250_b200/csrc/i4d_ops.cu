@@ -119,6 +119,22 @@ SeqArrays seq_arrays(const OpContext& o, const i4d_kv8& c, const int32_t* q_star
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
 
+// A kernel that waits for the one before it by itself (griddepcontrol.wait
+// first of all), so that its launch overlaps that one's end.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ------------------------------------------------------------------ rope
 
 template <typename T, int V, bool IL>
@@ -164,8 +180,9 @@ cudaError_t launch_append_t(const AppendDev& d, int code, bool wide, int64_t uni
 
 struct AttnPlan {
     int dt, nt;  // padded dim, row tiles of eight a CTA
-    int row_tiles, splits, chunk;
-    int64_t tiles;
+    int row_tiles;
+    int64_t segments;  // (sequence, cache head, row tile)
+    int even;          // CTAs that share the tokens, or 0
     size_t part_bytes, stat_bytes, lse2_bytes, score_bytes;
     size_t bytes() const { return part_bytes + stat_bytes + lse2_bytes + score_bytes; }
 };
@@ -177,25 +194,23 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     p.dt = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     p.nt = rows > 8 && a.dtype != I4D_F32 && p.dt <= 128 ? 2 : 1;
     p.row_tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
-    p.tiles = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
-    // Chunks: a few CTAs for each place on the GPU, so that ragged lengths even
-    // out, but none under 128 tokens (two tiles a warp) nor above what the
-    // kernel's table of blocks holds.
+    p.segments = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
+    // Few rows: the CTAs that fit the GPU share the tokens evenly, whatever
+    // the lengths are (lengths are known on the device only), but no more of
+    // them than have two tiles a warp.  Many rows are work enough by themselves.
     const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 4) * static_cast<int64_t>(o.num_sms);
-    const int64_t want = std::max<int64_t>(1, 12 * places / std::max<int64_t>(1, p.tiles));
-    int64_t chunk = (a.max_length + want - 1) / want;
-    chunk = std::min<int64_t>(std::max<int64_t>(128, (chunk + 127) / 128 * 128), kAttnBlocks * c.block_tokens / 2);
-    p.chunk = static_cast<int>(chunk);
-    p.splits = static_cast<int>(std::max<int64_t>(1, (a.max_length + chunk - 1) / chunk));
-    const auto round16 = [](size_t n) { return (n + 15) / 16 * 16; };
-    if (p.splits > 1) {
-        p.part_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * c.dim * sizeof(float);
-        p.stat_bytes = static_cast<size_t>(p.tiles) * p.splits * 8 * p.nt * sizeof(float4);
+    if (p.row_tiles <= 4) {
+        const int64_t units = p.segments * ((a.max_length + 15) / 16);
+        p.even = static_cast<int>(std::max<int64_t>(1, std::min(places, (units + 7) / 8)));
+    }
+    if (p.even) {
+        p.part_bytes = static_cast<size_t>(p.even) * 2 * 8 * p.nt * c.dim * sizeof(float);
+        p.stat_bytes = static_cast<size_t>(p.even) * 2 * 8 * p.nt * sizeof(float4);
     }
     if (a.weights) {
-        p.lse2_bytes = round16(static_cast<size_t>(a.tokens) * a.heads * sizeof(float));
+        p.lse2_bytes = (static_cast<size_t>(a.tokens) * a.heads * sizeof(float) + 15) / 16 * 16;
         // Few rows: their scores are kept (4 bytes a row against a token's codes read again).
-        if (rows <= 32) p.score_bytes = static_cast<size_t>(p.tiles) * 8 * p.nt * a.max_length * sizeof(float);
+        if (rows <= 32) p.score_bytes = static_cast<size_t>(p.segments) * 8 * p.nt * a.max_length * sizeof(float);
     }
     return p;
 }
@@ -535,34 +550,29 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.dtype = a->dtype;
     d.max_length = a->max_length;
     d.scale_log2 = a->scale * kLog2e;
+    d.batch = a->batch;
     d.row_tiles = p.row_tiles;
-    d.splits = p.splits;
-    d.chunk = p.chunk;
+    d.even = p.even;
     d.part = static_cast<float*>(a->workspace);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     d.stats = reinterpret_cast<float4*>(ws + p.part_bytes);
     d.lse2 = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes);
     if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.lse2_bytes);
     d.wide_q = aligned(a->q, 16) && a->q_stride * bytes % 16 == 0 && a->q_head_stride * bytes % 16 == 0;
-    const int64_t grid = p.tiles * p.splits;
-    const int64_t joins = (p.tiles * 8 * p.nt + kAttnWarps - 1) / kAttnWarps;
+    const int64_t grid = p.even ? p.even : p.segments;
     const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
     const int64_t wgrid = static_cast<int64_t>(a->batch) * a->cache.heads * wtiles;
-    OP_ARG(grid <= kMaxGrid && joins <= kMaxGrid && wgrid <= kMaxGrid, "too many rows in one call");
+    OP_ARG(p.segments <= kMaxGrid && wgrid <= kMaxGrid, "too many rows in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
     const bool int8 = a->cache.code == I4D_CODE_INT8;
     OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
-    if (p.splits > 1) {
-        k_kv8_join<<<static_cast<unsigned>(joins), kAttnThreads, 0, s>>>(d, 8 * p.nt, p.tiles * 8 * p.nt);
-        OP_CK(cudaGetLastError());
-    }
+    if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
     if (d.scores) {
         const int chunks = (a->max_length + 255) / 256;
         if (chunks > 0) {
-            k_kv8_weights_kept<<<static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 256, 0, s>>>(d, 8 * p.nt, chunks);
-            OP_CK(cudaGetLastError());
+            OP_CK(launch_after(k_kv8_weights_kept, static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 256, s, d, 8 * p.nt, chunks));
         }
     } else if (a->weights && wgrid > 0)
         OP_CK(int8 ? launch_weights_c<I4D_CODE_INT8>(d, p, wtiles, wgrid, s) : launch_weights_c<I4D_CODE_E4M3>(d, p, wtiles, wgrid, s));
