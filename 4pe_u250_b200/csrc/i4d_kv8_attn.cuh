@@ -1,13 +1,15 @@
 // i4d_kv8_attn.cuh -- attention over the cache of 8-bit codes.
 //
 // k_kv8_attn: eight (or sixteen) query rows of one cache head against a chunk
-// of its tokens.  Each warp takes tiles of 16 tokens, which it copies
-// asynchronously into a ring of its own in shared memory, three tiles ahead,
-// so no warp waits for another before the end.  The order of the summation
-// index of a matrix instruction is free, so a thread's 16 contiguous codes of
-// a token serve as its part of four steps of K q, and a V^T tile takes the
-// codes of the four tokens whose probabilities the thread holds: codes go from
-// shared memory to registers in 16-byte pieces without a transposition.  The products are transposed (tokens x rows,
+// of its tokens.  Each warp takes tiles of 16 tokens, which tensor copies
+// bring into a ring of its own in shared memory, two tiles ahead, so no warp
+// waits for another before the end (2 KB tensor copies stream at 6.7 TB/s
+// where 16-byte asynchronous copies stopped at 5.1; 812 MB of codes).  The
+// order of the summation index of a matrix instruction is free, so a thread's
+// 16 contiguous codes of a token serve as its part of four steps of K q, and a
+// V^T tile takes the codes of the four tokens whose probabilities the thread
+// holds: codes go from shared memory to registers in 16-byte pieces without a
+// transposition, and the copies' 128-byte swizzle keeps the banks apart.  The products are transposed (tokens x rows,
 // then dims x rows), which wastes half as much of a 16 x 8 tile on few rows.
 //   scores   S^T [16 tokens x 8 rows] = K [16 x dim] Q^T     (m16n8k16, FP16 in, FP32 sums)
 //   output   O^T [16 dims x 8 rows]  += V^T [16 x 16 tokens] P^T
@@ -26,6 +28,8 @@
 // Bound: the codes of K and V, read once.
 #pragma once
 
+#include <cuda.h>
+
 #include "i4d_kv8_cache.cuh"
 
 namespace i4d_ops {
@@ -37,6 +41,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 6.f;
 
 struct AttnDev {
+    CUtensorMap maps[2];  // K, V codes as rows of dim bytes; boxes of 16 rows x 128 (dim <= 64: 64) bytes
     Kv8Dev cache;
     SeqArrays seq;
     const void* q;
@@ -165,6 +170,14 @@ __device__ __forceinline__ void store_out(const AttnDev& a, int64_t i, float v) 
     else static_cast<__half*>(a.out)[i] = __float2half_rn(v);
 }
 
+// First of the 16 dims of lane t's piece c of a token's codes: neighbouring
+// pieces, so that two rows of an access phase take the even and the odd pieces
+// of a swizzled row and hit all banks.
+template <int DT>
+__device__ __forceinline__ int k_dim(int t, int c) {
+    return DT == 64 ? 16 * t : (c >> 1) * 128 + (2 * t + (c & 1)) * 16;
+}
+
 // The query rows of a tile as B operands: row `nt * 8 + lane / 4`, the codes'
 // order of the summation index (elements 0 and 2, 1 and 3 of four).  Score
 // sums of row nt * 8 + 2 (lane % 4) + j are multiplied by factor[nt][j] (and
@@ -188,7 +201,7 @@ __device__ __forceinline__ void load_qtile(const AttnDev& a, const Seq& s, int h
         float top = 0.f, x[DT / 64][16];
 #pragma unroll
         for (int c = 0; c < DT / 64; ++c) {
-            const int d0 = (t + 4 * c) * 16;
+            const int d0 = k_dim<DT>(t, c);
             if (live && d0 < dim) {
                 load_q16(a, base + d0, x[c]);
             } else {
@@ -240,51 +253,47 @@ __device__ __forceinline__ void load_ktile(const uint8_t* k, int dim, int n, KTi
     for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int c = 0; c < DT / 64; ++c) {
-            const int d0 = (t + 4 * c) * 16;
+            const int d0 = k_dim<DT>(t, c);
             kt.w[r][c] = (g + 8 * r < n && d0 < dim) ? __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * r) * dim + d0)) : make_uint4(0, 0, 0, 0);
         }
 }
 
-// Where 16-byte piece c of row r of a tile lies in its shared-memory row, so
-// that the eight lanes of an access phase hit all banks: they read pieces of
-// two rows of K, and of four even (or odd) rows of V.
+// A ring slot: 16 rows of K, then of V, in boxes of 128 (64) bytes a row with
+// the copies' swizzle: the 16-byte pieces of a row are exchanged by the row's
+// place in the pattern.
 template <int DT>
-__device__ __forceinline__ int k_piece(int r, int c) {
-    return DT == 64 ? c : c ^ ((r & 1) << 2);
-}
-template <int DT>
-__device__ __forceinline__ int v_piece(int r, int c) {
-    return DT == 64 ? c ^ ((r >> 1) & 2) : DT == 128 ? c ^ (r & 6) : c ^ (((r >> 1) & 1) | (r & 4));
+__device__ __forceinline__ uint32_t slot_at(uint32_t slot, int which, int row, int d) {
+    if constexpr (DT == 64) return slot + which * 1024 + row * 64 + (d ^ ((row >> 1 & 3) << 4));
+    return slot + which * 16 * DT + (d >> 7) * 2048 + row * 128 + ((d & 127) ^ ((row & 7) << 4));
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 
-// Copies n of the 16 tokens at k and v into a ring slot [K: 16][DT], [V: 16][DT]; zeros elsewhere.
+// False if the barrier's phase did not end within the limit (about a second).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 20); ++i) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// One lane: the 16 rows from `row` of K and V into a slot.
 template <int DT>
-__device__ __forceinline__ void copy_tile(uint32_t slot, const uint8_t* k, const uint8_t* v, int dim, int n) {
-    constexpr int kPieces = DT / 16, kRowsAtOnce = 32 / kPieces;  // a warp's 512 bytes are rows, or part of one
-    const int lane = threadIdx.x & 31;
-    if (n == 16 && dim == DT) {  // 16 whole rows lie in one piece of memory
-        k += lane * 16;
-        v += lane * 16;
+__device__ __forceinline__ void copy_tile(const AttnDev& a, uint32_t slot, uint32_t bar, int row) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(32 * DT) : "memory");
 #pragma unroll
-        for (int i = 0; i < DT / 32; ++i) {
-            const int r = i * kRowsAtOnce + lane / kPieces, c = lane % kPieces;
-            copy16(slot + r * DT + k_piece<DT>(r, c) * 16, k + i * 512);
-            copy16(slot + 16 * DT + r * DT + v_piece<DT>(r, c) * 16, v + i * 512);
-        }
-        return;
-    }
-#pragma unroll 1
-    for (int i = 0; i < DT / 32; ++i) {
-        const int r = i * kRowsAtOnce + lane / kPieces, c = lane % kPieces;
-        const int bytes = r < n && c * 16 < dim ? 16 : 0;
-        const int from = bytes ? r * dim + c * 16 : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + r * DT + k_piece<DT>(r, c) * 16), "l"(k + from), "r"(bytes) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + 16 * DT + r * DT + v_piece<DT>(r, c) * 16), "l"(v + from), "r"(bytes) : "memory");
-    }
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int x = 0; x < (DT + 127) / 128; ++x)
+            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                             slot + which * 16 * DT + x * 2048),
+                         "l"(&a.maps[which]), "r"(x * 128), "r"(row), "r"(bar)
+                         : "memory");
 }
 
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
@@ -299,7 +308,7 @@ __device__ __forceinline__ void read_ktile(uint32_t slot, KTile<DT>& kt) {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int c = 0; c < DT / 64; ++c) kt.w[r][c] = lds16(slot + (g + 8 * r) * DT + k_piece<DT>(g + 8 * r, t + 4 * c) * 16);
+        for (int c = 0; c < DT / 64; ++c) kt.w[r][c] = lds16(slot_at<DT>(slot, 0, g + 8 * r, k_dim<DT>(t, c)));
 }
 
 template <int DT, int CODE, int NT, bool HL>
@@ -330,8 +339,13 @@ __device__ __forceinline__ void score_tile(const KTile<DT>& kt, const QTile<DT, 
         for (int i = 0; i < 4; ++i) s[nt][i] += odd[nt][i];
 }
 
-// V codes of 16 tokens: the thread's DT / 8 dims (from (lane / 4) * DT / 8) of
-// tokens 2t, 2t + 1, 2t + 8, 2t + 9.
+// V codes of 16 tokens: of tokens 2t, 2t + 1, 2t + 8, 2t + 9, the dims
+// v_dim(lane / 4, word) and the three after it.
+template <int DT>
+__device__ __forceinline__ int v_dim(int g, int w) {
+    return DT == 64 ? g * 8 + w * 4 : (w >> 2) * 128 + g * 16 + (w & 3) * 4;
+}
+
 template <int DT>
 struct VTile {
     uint32_t w[4][DT / 32];
@@ -343,13 +357,13 @@ __device__ __forceinline__ void read_vtile(uint32_t slot, VTile<DT>& vt) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int tok = 2 * t + (r & 1) + (r >> 1) * 8;
-        const uint32_t row = slot + 16 * DT + tok * DT;
         if constexpr (DT == 64) {
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vt.w[r][0]), "=r"(vt.w[r][1]) : "r"(row + v_piece<DT>(tok, g >> 1) * 16 + (g & 1) * 8) : "memory");
+            const uint32_t at = slot_at<DT>(slot, 1, tok, g >> 1 << 4) + (g & 1) * 8;
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vt.w[r][0]), "=r"(vt.w[r][1]) : "r"(at) : "memory");
         } else {
 #pragma unroll
             for (int c = 0; c < DT / 128; ++c) {
-                const uint4 x = lds16(row + v_piece<DT>(tok, g * (DT / 128) + c) * 16);
+                const uint4 x = lds16(slot_at<DT>(slot, 1, tok, c * 128 + g * 16));
                 vt.w[r][4 * c] = x.x;
                 vt.w[r][4 * c + 1] = x.y;
                 vt.w[r][4 * c + 2] = x.z;
@@ -359,8 +373,20 @@ __device__ __forceinline__ void read_vtile(uint32_t slot, VTile<DT>& vt) {
     }
 }
 
-// acc[i]: dims (lane / 4) * DT / 8 + 2 i and + 1, rows 2t and 2t + 1 of each
-// tile.
+// Zeros in place of the tokens from `live` on: their bytes may be anything.
+template <int DT>
+__device__ __forceinline__ void clear_vtile(int live, VTile<DT>& vt) {
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (2 * t + (r & 1) + (r >> 1) * 8 >= live) {
+#pragma unroll
+            for (int w = 0; w < DT / 32; ++w) vt.w[r][w] = 0;
+        }
+}
+
+// acc[i]: dims v_dim(lane / 4, i / 2) + 2 (i % 2) and the next, rows 2t and
+// 2t + 1 of each tile.
 template <int DT, int CODE, int NT, bool HL>
 __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (&p)[NT][2], const uint32_t (&pl)[NT][2], float acc[DT / 16][NT][4]) {
 #pragma unroll
@@ -399,7 +425,7 @@ template <int DT, int NT>
 constexpr size_t attn_smem() {
     const size_t ring = static_cast<size_t>(kAttnWarps) * kAttnSlots<DT> * 32 * DT;
     const size_t merge = static_cast<size_t>(kAttnWarps) * 8 * NT * (DT + 4) * sizeof(float);
-    return ring > merge ? ring : merge;
+    return (ring > merge ? ring : merge) + 1024;
 }
 
 // CTAs an SM: by shared memory and by registers (8 rows of up to 128 values in 128 registers).
@@ -480,7 +506,7 @@ struct Piece {
 
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block) {
+__device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block, uint64_t* s_bar, uint32_t& phases) {
     constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
     float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -510,6 +536,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
     if (begin < end) {
         const int bs = a.cache.block_tokens, dim = a.cache.dim, shift = 31 - __clz(bs);
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(attn_ring)) + warp * kSlots * 32 * DT;
+        const uint32_t bars = static_cast<uint32_t>(__cvta_generic_to_shared(s_bar)) + warp * kSlots * 8;
         QTile<DT, NT, HLQ> q;
         const int span = kAttnBlocks << shift;  // tokens whose blocks the table holds
         for (int from_tok = begin; from_tok < end;) {
@@ -530,21 +557,23 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
             __syncthreads();
             const int tiles = (to_tok - from_tok + 15) >> 4;
             auto issue = [&](int i, int slot) {
-                if (i < tiles) {
-                    const int at = from_tok + 16 * i, id = __float_as_int(s_block[(at >> shift) - blk0].x);
-                    const int64_t off = id < 0 ? 0 : code_offset(a.cache, id, h) + (at & (bs - 1)) * dim;
-                    copy_tile<DT>(ring + slot * 32 * DT, a.cache.codes[0] + off, a.cache.codes[1] + off, dim, id < 0 ? 0 : min(16, to_tok - at));
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (lane != 0 || i >= tiles) return;
+                const int at = from_tok + 16 * i, id = __float_as_int(s_block[(at >> shift) - blk0].x);
+                if (id >= 0) copy_tile<DT>(a, ring + slot * 32 * DT, bars + slot * 8, (id * a.cache.heads + h) * bs + (at & (bs - 1)));
+                else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + slot * 8) : "memory");
             };
-#pragma unroll
+            // the slots are used in turn; `phases` holds the parity of each one's next phase
             for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
             if (from_tok == begin) load_qtile<DT, CODE, NT, HLQ>(a, s, h, row0, q);
             int slot = 0;
             for (int i = warp; i < tiles; i += kAttnWarps) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
-                __syncwarp();  // this slot's copies of all lanes have landed; all lanes are done with the one to fill
+                __syncwarp();  // all lanes are done with the slot to fill
                 issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
+                if (!bar_wait(bars + slot * 8, phases >> slot & 1)) {
+                    if (lane == 0) atomicOr(a.seq.err, kTimeout);
+                    break;
+                }
+                phases ^= 1u << slot;
                 const uint32_t at_slot = ring + slot * 32 * DT;
                 slot = slot == kSlots - 1 ? 0 : slot + 1;
                 const int at = from_tok + 16 * i;
@@ -560,6 +589,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 }
                 VTile<DT> vt;
                 read_vtile<DT>(at_slot, vt);
+                if (live < 16) clear_vtile<DT>(live, vt);
                 float top[NT][2];
                 const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
                 bool raise = false;
@@ -636,7 +666,6 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 }
                 value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
             from_tok = to_tok;
         }
         __syncthreads();  // the ring is free for the join
@@ -652,8 +681,9 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
             float* m = merge[warp][nt * 8 + 2 * t + j];
 #pragma unroll
             for (int i = 0; i < DT / 16; ++i) {
-                m[g * (DT / 8) + 2 * i] = acc[i][nt][j];
-                m[g * (DT / 8) + 2 * i + 1] = acc[i][nt][j + 2];
+                const int d = v_dim<DT>(g, i >> 1) + 2 * (i & 1);
+                m[d] = acc[i][nt][j];
+                m[d + 1] = acc[i][nt][j + 2];
             }
             if (g == 0) {
                 m[DT] = M[nt][j];
@@ -715,9 +745,16 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
 }
 
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(AttnDev a) {
+__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(const __grid_constant__ AttnDev a) {
     constexpr int kRows = 8 * NT;
-    extern __shared__ __align__(16) unsigned char attn_ring[];
+    extern __shared__ unsigned char attn_smem_base[];
+    // the copies' swizzle counts from 1024-byte boundaries
+    unsigned char* attn_ring = attn_smem_base + (-static_cast<uint32_t>(__cvta_generic_to_shared(attn_smem_base)) & 1023u);
+    __shared__ uint64_t s_bar[kAttnWarps * kAttnSlots<DT>];
+    uint32_t phases = 0;
+    if (threadIdx.x < kAttnWarps * kAttnSlots<DT>) bar_init(static_cast<uint32_t>(__cvta_generic_to_shared(s_bar + threadIdx.x)), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
     __shared__ float4 s_block[kAttnBlocks];  // id, scale of K, of V, log2 of the latter
     if (!a.even) {
         const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.cache.heads, b = blockIdx.x / a.row_tiles / a.cache.heads;
@@ -725,7 +762,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
         const Seq s = load_seq(a.seq, b, report);
         if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
         if (s.len > a.max_length || rt * kRows >= s.n * a.group) return;
-        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, 0, s.len, true, 0}, attn_ring, s_block);
+        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, 0, s.len, true, 0}, attn_ring, s_block, s_bar, phases);
         return;
     }
     Place at;
@@ -748,9 +785,12 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
         const int64_t seg0 = at.before + static_cast<int64_t>(seg) * n.tiles;
         const int t0 = static_cast<int>(u - seg0), t1 = static_cast<int>(min(static_cast<int64_t>(n.tiles), u_end - seg0));
         const int lo = row_span(a, s.len - s.n).x & ~15;
-        if (u != u0) __syncthreads();  // the previous piece's shared memory is free
+        if (u != u0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the join wrote where the next copies go
+            __syncthreads();
+        }
         attend<DT, CODE, NT, HLQ, HLP>(a, s, {at.seq, seg / row_tiles, seg % row_tiles, lo + 16 * t0, min(s.len, lo + 16 * t1), t0 == 0 && t1 == n.tiles, u == u0 ? 0 : 1},
-                                       attn_ring, s_block);
+                                       attn_ring, s_block, s_bar, phases);
         u = seg0 + t1;
     }
 }

@@ -178,6 +178,37 @@ cudaError_t launch_append_t(const AppendDev& d, int code, bool wide, int64_t uni
 
 // ------------------------------------------------------------- attention
 
+// cuTensorMapEncodeTiled of the driver, looked up once (it comes with no
+// library that this one links).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+        return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeFn>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// The cache's codes as a matrix of bytes, a row for each (block, head, slot),
+// copied in boxes of `rows` rows of 128 bytes (64 for dims up to 64).
+i4d_status encode_codes(i4d_ctx* ctx, const i4d_kv8& c, const void* codes, int rows, CUtensorMap* map) {
+    const EncodeFn fn = encode_fn();
+    if (!fn) return op_fail(ctx, I4D_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const bool narrow = c.dim <= 64;
+    const cuuint64_t size[2] = {static_cast<cuuint64_t>(c.dim), static_cast<cuuint64_t>(c.blocks) * c.heads * c.block_tokens};
+    const cuuint64_t stride[1] = {static_cast<cuuint64_t>(c.dim)};
+    const cuuint32_t box[2] = {narrow ? 64u : 128u, static_cast<cuuint32_t>(rows)}, step[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), size, stride, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return op_fail(ctx, I4D_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return I4D_OK;
+}
+
 struct AttnPlan {
     int dt, nt;  // padded dim, row tiles of eight a CTA
     int row_tiles;
@@ -226,6 +257,8 @@ i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     OP_ARG(a->window >= 0 && a->window <= kMaxTokens, "window %d", a->window);
     OP_ARG(static_cast<int64_t>(a->table_blocks) * a->cache.block_tokens >= a->max_length,
            "block_table rows of %d blocks hold fewer than max_length %d tokens", a->table_blocks, a->max_length);
+    OP_ARG(static_cast<int64_t>(a->cache.blocks) * a->cache.heads * a->cache.block_tokens <= 0x7fffffff,
+           "a cache of 2^31 or more (token, head) rows");
     OP_ARG(std::isfinite(a->scale), "scale is not finite");
     OP_ARG(static_cast<int64_t>(a->max_q) * (a->heads / a->cache.heads) <= kMaxTokens, "too many rows");
     return I4D_OK;
@@ -327,6 +360,7 @@ i4d_status ops_report(i4d_ctx* ctx) {
     if (!e) return I4D_OK;
     OP_CK(cudaMemsetAsync(o.err, 0, sizeof(e), o.stream));
     OP_CK(cudaStreamSynchronize(o.stream));
+    if (e & kTimeout) return op_fail(ctx, I4D_ERR_TIMEOUT, "a bounded device wait of an operator gave up (error word 0x%x)", e);
     return op_fail(ctx, I4D_ERR_ARG, "an operator skipped tokens:%s%s", e & kBadSequence ? " q_start or lengths out of range;" : "",
                    e & kBadBlock ? " block id outside the pool;" : "");
 }
@@ -567,6 +601,9 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
     const bool int8 = a->cache.code == I4D_CODE_INT8;
+    i4d_status enc = encode_codes(ctx, a->cache, a->cache.k, 16, &d.maps[0]);
+    if (enc == I4D_OK) enc = encode_codes(ctx, a->cache, a->cache.v, 16, &d.maps[1]);
+    if (enc != I4D_OK) return enc;
     OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
     if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
     if (d.scores) {

@@ -18,6 +18,7 @@ namespace i4d_ops {
 // Bits of the operators' device error word.
 constexpr unsigned kBadSequence = 1u;  // q_start or lengths outside what the call's arguments allow
 constexpr unsigned kBadBlock = 2u;     // a block id outside the pool
+constexpr unsigned kTimeout = 4u;      // a bounded wait gave up
 
 constexpr int kMaxTokens = 1 << 30;  // of one sequence, so that a block's end is an int
 
