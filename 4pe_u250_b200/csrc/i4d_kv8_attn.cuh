@@ -49,7 +49,7 @@ struct AttnDev {
     float* lse;
     float* weights;
     int64_t q_tok, q_head, out_tok, out_head, weights_stride;
-    int heads, group, window, dtype, max_length, wide_q;
+    int heads, group, window, dtype, max_length, wide_q, wide_out;
     float scale_log2;  // softmax scale * log2(e)
     int batch, row_tiles;  // row tiles of a (sequence, cache head), at most
     int even;              // CTAs that share the tokens evenly, or 0: one for each (sequence, cache head, row tile)

@@ -1,0 +1,516 @@
+// i4d_kv8_prompt.cuh -- attention of many query rows over the cache of 8-bit
+// codes on the fifth-generation tensor cores.
+//
+// One CTA for up to 256 rows (query, head of the group) of one cache head: two
+// tiles of 128 rows take turns, so that one tile's products run under the
+// other's softmax.  Tiles of 128 tokens go through
+//   producer (1 warp)      codes of 16 tokens a tensor copy, scales of 16 tokens into a table
+//   converters (4 warps)   codes -> FP16 operands in the 128-byte swizzle, a token row a thread
+//   products (1 thread)    S = Q K^T (128 x 128), O += P V, both into tensor memory
+//   softmax (2 x 4 warps)  a row a thread: bounds M and R, P = 2^(x - M) v_scale 2^(M - R) in FP16 over S
+// K is the second operand of S with its dims contiguous, V that of O with its
+// dims contiguous too (the transposed form), so both convert alike; P is the
+// first operand straight from tensor memory.  The arithmetic is
+// i4d_kv8_attn.cuh's: exact codes and query rows, FP32 sums, probabilities in
+// one FP16 part.  A row's statistics stay in its thread, and O is rescaled
+// only where a score passes the bound by more than 2^6.
+// Bound: 4 dim products a visible (row, token) at the tensor rate, and one
+// exponential for each at the rate of the special-function units, which for
+// dim 128 takes as long (16 a cycle and SM against 8192 products).
+#pragma once
+
+#include "i4d_kv8_attn.cuh"
+
+namespace i4d_ops {
+
+constexpr int kPrThreads = 448;
+constexpr int kPrRows = 256;
+constexpr int kPrTokens = 128;
+
+template <int DT>
+struct PromptSmem {
+    static constexpr int kBlock = 16384;                  // 128 rows of 64 halves
+    static constexpr int kOperand = DT / 64 * kBlock;     // 128 rows of DT halves
+    static constexpr int kRaw = kPrTokens * DT;           // codes of a tile
+    static constexpr int q = 0;
+    static constexpr int k = q + 2 * kOperand;            // two buffers
+    static constexpr int v = k + 2 * kOperand;
+    static constexpr int raw = v + kOperand;              // two stages of K, V
+    static constexpr int total = raw + 4 * kRaw;
+};
+
+// Barriers.
+enum {
+    kRawKFull = 0, kRawVFull = 2, kRawKEmpty = 4, kRawVEmpty = 6, kKFull = 8, kKEmpty = 10,
+    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 2, kPvDone = kPFull + 2, kQFull = kPvDone + 2, kODone, kPrBars
+};
+
+struct PrShared {
+    uint64_t bar[kPrBars];
+    float4 table[4][8];  // of 16 tokens: scale of K (-1: not there), of V, log2 of it
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ uint32_t bar_at(const PrShared& sh, int i) { return static_cast<uint32_t>(__cvta_generic_to_shared(&sh.bar[i])); }
+
+// False once the wait, or another one of the CTA, has given up.
+__device__ __forceinline__ bool pr_wait(PrShared& sh, int i, uint32_t parity) {
+    const uint32_t bar = bar_at(sh, i);
+    for (int n = 0; n < (1 << 18); ++n) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((n & 63) == 63 && *reinterpret_cast<volatile int*>(&sh.abort)) return false;
+    }
+    *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+    return false;
+}
+
+__device__ __forceinline__ bool pr_test(const PrShared& sh, int i, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar_at(sh, i)), "r"(parity) : "memory");
+    return ok;
+}
+
+__device__ __forceinline__ void pr_arrive(const PrShared& sh, int i) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at(sh, i)) : "memory");
+}
+
+// The issuing thread's products so far arrive on a barrier when they are done.
+__device__ __forceinline__ void pr_commit(const PrShared& sh, int i) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_at(sh, i)) : "memory");
+}
+
+// Shared-memory operands in the 128-byte swizzle, 1024 bytes between groups of
+// eight rows; `lead` bytes between blocks of 64 along a contiguous non-summed
+// dimension (unused where the summed one is contiguous).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead) {
+    return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+
+// FP16 operands, FP32 sums, 128 rows, n columns.
+__host__ __device__ constexpr uint32_t product_desc(int n, bool b_transposed) {
+    return 1u << 4 | (b_transposed ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
+                 "r"(desc), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
+                 "r"(desc), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+
+#define I4D_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
+#define I4D_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+
+// 32 columns of the warp's 32 lanes of tensor memory, a lane a thread.
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t x[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : I4D_R8(x, 0), I4D_R8(x, 8), I4D_R8(x, 16), I4D_R8(x, 24)
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t x[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+        "%27,%28,%29,%30,%31,%32};" ::"r"(at),
+        I4D_W8(x, 0), I4D_W8(x, 8), I4D_W8(x, 16), I4D_W8(x, 24)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t x[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), I4D_W8(x, 0),
+                 I4D_W8(x, 8)
+                 : "memory");
+}
+// The loaded registers hold their values behind this point.
+__device__ __forceinline__ void tmem_wait_load(uint32_t x[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]),
+                   "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]), "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]),
+                   "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]),
+                   "+r"(x[31])::"memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One token row of codes (128 or 64 bytes with the copy's swizzle) to halves
+// in an operand's row; zeros for a row that is not there.
+template <int DT, int CODE>
+__device__ __forceinline__ void convert_row(uint32_t raw, uint32_t to, int row, bool there) {
+#pragma unroll
+    for (int c = 0; c < DT / 16; ++c) {
+        const uint32_t from = DT == 64 ? raw + row * 64 + ((c ^ (row >> 1 & 3)) << 4) : raw + row * 128 + ((c ^ (row & 7)) << 4);
+        uint4 w = lds16(from);
+        if (!there) w = make_uint4(0, 0, 0, 0);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (CODE == I4D_CODE_INT8) {
+                const uint32_t x = ws[i] ^ 0x80808080u;
+                const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+                const uint32_t m0 = __byte_perm(x, 0x64646464u, 0x4140), m1 = __byte_perm(x, 0x64646464u, 0x4342);
+                const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), bias), h1 = __hsub2(*reinterpret_cast<const __half2*>(&m1), bias);
+                h[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+                h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+            } else {
+                const uint16_t lo = static_cast<uint16_t>(ws[i]), hi = static_cast<uint16_t>(ws[i] >> 16);
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[2 * i]) : "h"(lo));
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[2 * i + 1]) : "h"(hi));
+            }
+        }
+        const uint32_t line = to + (c >> 2) * 16384 + row * 128;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((((c & 3) * 2 + p) ^ (row & 7)) << 4)), "r"(h[4 * p]), "r"(h[4 * p + 1]),
+                         "r"(h[4 * p + 2]), "r"(h[4 * p + 3])
+                         : "memory");
+    }
+}
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <int DT, int CODE>
+__global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_constant__ AttnDev a) {
+    using L = PromptSmem<DT>;
+    extern __shared__ unsigned char pr_base[];
+    __shared__ PrShared sh;
+    const uint32_t base_raw = static_cast<uint32_t>(__cvta_generic_to_shared(pr_base));
+    const uint32_t base = (base_raw + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the last row tiles see the most tokens: they start first
+    const int rt = a.row_tiles - 1 - static_cast<int>(blockIdx.x / (a.cache.heads * a.batch));
+    const int bh = blockIdx.x % (a.cache.heads * a.batch), h = bh % a.cache.heads, b = bh / a.cache.heads;
+    const bool report = rt == 0 && h == 0 && threadIdx.x == 0;
+    const Seq s = load_seq(a.seq, b, report);
+    if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
+    const int rows = s.n * a.group, row0 = rt * kPrRows;
+    if (s.len > a.max_length || row0 >= rows) return;
+    const int first = s.len - s.n, live = min(kPrRows, rows - row0);
+    const bool both = live > 128;
+    const int2 first_span = row_span(a, first + row0 / a.group), last_span = row_span(a, first + (row0 + live - 1) / a.group);
+    const int t0 = first_span.x & ~15, end = last_span.y;
+    const int tiles = (end - t0 + kPrTokens - 1) / kPrTokens;
+    const int bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPrBars; ++i) {
+            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i == kPFull || i == kPFull + 1 ? 4 : i == kQFull ? 8 : 1;
+            bar_init(bar_at(sh, i), count);
+        }
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&sh.tmem))) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 12) {  // ------------------------------------------- producer
+        constexpr int kBoxBytes = 16 * DT;
+        int done = 0;
+        for (int j = 0; j < tiles; ++j, ++done) {
+            const int st = j & 1, at = t0 + kPrTokens * j + 16 * lane;
+            int id = -1;
+            float4 entry = make_float4(-1.f, 0.f, 0.f, 0.f);
+            if (lane < 8 && at < end) {
+                id = load_block(a.seq, b, at >> shift, true);
+                if (id >= 0) {
+                    const int64_t sc = static_cast<int64_t>(id) * a.cache.heads + h;
+                    entry.x = __ldg(a.cache.scale[0] + sc);
+                    entry.y = __ldg(a.cache.scale[1] + sc);
+                    entry.z = __log2f(entry.y);  // only a bound: its rounding cancels
+                }
+            }
+            const int row = (id * a.cache.heads + h) * bs + (at & (bs - 1));
+            const int bytes = __popc(__ballot_sync(~0u, id >= 0)) * kBoxBytes;
+            if (!pr_wait(sh, kRawKEmpty + st, (j >> 1 & 1) ^ 1)) break;
+            if (lane < 8) sh.table[j & 3][lane] = entry;
+            __syncwarp();
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                if (which && !pr_wait(sh, kRawVEmpty + st, (j >> 1 & 1) ^ 1)) break;
+                const uint32_t bar = bar_at(sh, (which ? kRawVFull : kRawKFull) + st);
+                if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+                __syncwarp();
+                if (id >= 0)
+                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                                     base + L::raw + (st * 2 + which) * L::kRaw + lane * kBoxBytes),
+                                 "l"(&a.maps[which]), "r"(0), "r"(row), "r"(bar)
+                                 : "memory");
+            }
+        }
+        if (sh.abort)  // copies in flight land before the CTA leaves
+            for (int j = max(0, done - 1); j < min(tiles, done + 1); ++j) {
+                bar_wait(bar_at(sh, kRawKFull + (j & 1)), j >> 1 & 1);
+                bar_wait(bar_at(sh, kRawVFull + (j & 1)), j >> 1 & 1);
+            }
+    } else if (warp == 13) {  // ------------------------------------- products
+        if (lane == 0 && pr_wait(sh, kQFull, 0)) {
+            constexpr uint32_t kScores = product_desc(128, false), kValues = product_desc(DT, true);
+            auto scores = [&](int tile, int j) {
+#pragma unroll
+                for (int i = 0; i < DT / 16; ++i) {
+                    const uint32_t step = (i >> 2) * L::kBlock + (i & 3) * 32;
+                    product_ss(tmem + tile * 128, operand_desc(base + L::q + tile * L::kOperand + step, 16),
+                               operand_desc(base + L::k + (j & 1) * L::kOperand + step, 16), kScores, i > 0);
+                }
+                pr_commit(sh, kSFull + tile);
+            };
+            auto values = [&](int tile, int j) {
+#pragma unroll
+                for (int i = 0; i < kPrTokens / 16; ++i)
+                    product_ts(tmem + 256 + tile * 128, tmem + tile * 128 + i * 8, operand_desc(base + L::v + i * 2048, L::kBlock), kValues, j > 0 || i > 0);
+            };
+            // Whichever tile's next product has its operands: S of token tile j
+            // once O has taken P of tile j - 1 from the same tensor memory.
+            const int n = both ? 2 : 1;
+            int s_done[2] = {0, 0}, o_done[2] = {0, 0}, idle = 0;
+            bool ok = true;
+            while (o_done[0] < tiles || (both && o_done[1] < tiles)) {
+                bool moved = false;
+                for (int t = 0; t < n; ++t) {
+                    int j = s_done[t];
+                    if (j < tiles && j == o_done[t] && pr_test(sh, kKFull + (j & 1), j >> 1 & 1) && (j == 0 || pr_test(sh, kPvDone + t, (j - 1) & 1))) {
+                        fence_after();
+                        scores(t, j);
+                        s_done[t] = j + 1;
+                        if (s_done[n - 1 - t] > j) pr_commit(sh, kKEmpty + (j & 1));
+                        moved = true;
+                    }
+                    j = o_done[t];
+                    if (j < s_done[t] && pr_test(sh, kVFull, j & 1) && pr_test(sh, kPFull + t, j & 1)) {
+                        fence_after();
+                        values(t, j);
+                        pr_commit(sh, kPvDone + t);
+                        o_done[t] = j + 1;
+                        if (o_done[n - 1 - t] > j) pr_commit(sh, kVEmpty);
+                        moved = true;
+                    }
+                }
+                if (moved) {
+                    idle = 0;
+                } else if (++idle > (1 << 22) || *reinterpret_cast<volatile int*>(&sh.abort)) {
+                    *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+                    ok = false;
+                    break;
+                }
+            }
+            pr_commit(sh, kODone);
+            if (!ok) bar_wait(bar_at(sh, kODone), 0);  // products in flight end before the CTA leaves
+        }
+        __syncwarp();
+    } else if (warp >= 8) {  // --------------------------------------- converters
+        const int row = threadIdx.x - 256;
+        for (int j = 0; j < tiles; ++j) {
+            const int st = j & 1;
+            if (!pr_wait(sh, kRawKFull + st, j >> 1 & 1) || !pr_wait(sh, kKEmpty + st, (j >> 1 & 1) ^ 1)) break;
+            const bool there = t0 + kPrTokens * j + row < s.len && sh.table[j & 3][row >> 4].x >= 0.f;
+            convert_row<DT, CODE>(base + L::raw + st * 2 * L::kRaw, base + L::k + st * L::kOperand, row, true);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                pr_arrive(sh, kKFull + st);
+                pr_arrive(sh, kRawKEmpty + st);
+            }
+            if (!pr_wait(sh, kRawVFull + st, j >> 1 & 1) || !pr_wait(sh, kVEmpty, (j & 1) ^ 1)) break;
+            convert_row<DT, CODE>(base + L::raw + (st * 2 + 1) * L::kRaw, base + L::v, row, there);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                pr_arrive(sh, kVFull);
+                pr_arrive(sh, kRawVEmpty + st);
+            }
+        }
+    } else {  // ------------------------------------------------------- softmax
+        const int tile = warp >> 2, r = threadIdx.x & 127, row = row0 + tile * 128 + r;
+        const bool mine = row < rows;
+        const int64_t tok = s.first + row / a.group;
+        const int head = h * a.group + row % a.group;
+        float down = 0.f;
+        {  // the row to FP16: two passes over memory, the largest value, then the halves
+            const int64_t at = mine ? tok * a.q_tok + head * a.q_head : 0;
+            float top = 0.f, x[16];
+            for (int c = 0; mine && c < dim / 16; ++c) {
+                load_q16(a, at + 16 * c, x);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+            }
+            const int e = max(-115, min(126, 13 - ((__float_as_int(top) >> 23) - 127)));
+            float up = __int_as_float((e + 127) << 23);
+            down = __int_as_float((127 - e) << 23) * fabsf(a.scale_log2);
+            if (a.scale_log2 < 0.f) up = -up;
+            for (int c = 0; c < DT / 16; ++c) {
+                uint32_t w[8];
+                if (mine && 16 * c < dim) {
+                    load_q16(a, at + 16 * c, x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = pack_h2(x[2 * i] * up, x[2 * i + 1] * up);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = 0;
+                }
+                const uint32_t line = base + L::q + tile * L::kOperand + (c >> 2) * L::kBlock + r * 128;
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((((c & 3) * 2 + p) ^ (r & 7)) << 4)), "r"(w[4 * p]), "r"(w[4 * p + 1]),
+                                 "r"(w[4 * p + 2]), "r"(w[4 * p + 3])
+                                 : "memory");
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) pr_arrive(sh, kQFull);
+        }
+        const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lanes 32 (warp % 4) of tensor memory
+        const uint32_t s_at = tmem + quarter + tile * 128, o_at = tmem + quarter + 256 + tile * 128;
+        const int2 span = row_span(a, first + row / a.group);
+        const int tile_last = min(row0 + tile * 128 + 127, row0 + live - 1);
+        const int all_from = row_span(a, first + tile_last / a.group).x, all_to = min(s.len, row_span(a, first + (row0 + tile * 128) / a.group).y);
+        float M = -INFINITY, R = -INFINITY, l = 0.f, to_r = 0.f;
+        bool ok = tile == 0 || both;
+        for (int j = 0; ok && j < tiles; ++j) {
+            ok = pr_wait(sh, kSFull + tile, j & 1);
+            if (!ok) break;
+            fence_after();
+            const int at = t0 + kPrTokens * j;
+            const bool whole = at >= all_from && at + kPrTokens <= all_to;
+            const int from = span.x - at, width = min(span.y, s.len) - span.x;  // column c is seen if c - from < width, unsigned
+            const float4* table = sh.table[j & 3];
+            uint32_t x[2][32];
+            // the greatest score of the row, and the greatest with its block's value scale
+            float top = -INFINITY, rtop = -INFINITY;
+            tmem_load32(s_at, x[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_wait_load(x[c & 1]);
+                if (c < 3) tmem_load32(s_at + 32 * (c + 1), x[c + 1 & 1]);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const float4 block = table[2 * c + g];
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float y = __uint_as_float(x[c & 1][16 * g + i]);
+                        if (!whole && static_cast<unsigned>(32 * c + 16 * g + i - from) >= static_cast<unsigned>(width)) y = -INFINITY;
+                        m = fmaxf(m, y);
+                    }
+                    m = block.x < 0.f || m == -INFINITY ? -INFINITY : m * (down * block.x);
+                    top = fmaxf(top, m);
+                    rtop = fmaxf(rtop, m + block.z);
+                }
+            }
+            const bool raise = top > M + kSlack || rtop > R + kSlack;
+            if (__any_sync(~0u, raise)) {
+                const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(rtop, R) : R;
+                l *= M == m ? 1.f : ex2(M - m);
+                const float f = R == rr ? 1.f : ex2(R - rr);
+                M = m;
+                R = rr;
+                to_r = R == -INFINITY ? 0.f : ex2(M - R);
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < DT / 32; ++c) {
+                        tmem_load32(o_at + 32 * c, x[0]);
+                        tmem_wait_load(x[0]);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * f);
+                        tmem_store32(o_at + 32 * c, x[0]);
+                    }
+                }
+            }
+            const float off = M == -INFINITY ? 0.f : M;
+            tmem_load32(s_at, x[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_wait_load(x[c & 1]);
+                if (c < 3) tmem_load32(s_at + 32 * (c + 1), x[c + 1 & 1]);
+                uint32_t p[16];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const float4 block = table[2 * c + g];
+                    const float f = down * block.x, w = to_r * block.y;
+                    const bool gone = block.x < 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float e0 = ex2(fmaf(__uint_as_float(x[c & 1][16 * g + i]), f, -off));
+                        float e1 = ex2(fmaf(__uint_as_float(x[c & 1][16 * g + i + 1]), f, -off));
+                        if (!whole) {
+                            if (gone || static_cast<unsigned>(32 * c + 16 * g + i - from) >= static_cast<unsigned>(width)) e0 = 0.f;
+                            if (gone || static_cast<unsigned>(32 * c + 16 * g + i + 1 - from) >= static_cast<unsigned>(width)) e1 = 0.f;
+                        } else if (gone) {
+                            e0 = e1 = 0.f;
+                        }
+                        l += e0 + e1;
+                        p[8 * g + i / 2] = pack_h2(e0 * w, e1 * w);
+                    }
+                }
+                tmem_store16(s_at + 16 * c, p);
+            }
+            tmem_wait_store();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) pr_arrive(sh, kPFull + tile);
+        }
+        if (ok && pr_wait(sh, kODone, 0)) {
+            fence_after();
+            const float back = l == 0.f || R == -INFINITY ? 0.f : ex2(R - M) / l;
+            uint32_t x[32];
+#pragma unroll
+            for (int c = 0; c < DT / 32; ++c) {
+                tmem_load32(o_at + 32 * c, x);
+                tmem_wait_load(x);
+                if (!mine) continue;
+                const int64_t to = tok * a.out_tok + head * a.out_head + 32 * c;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (32 * c + i >= dim) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float u = __uint_as_float(x[i + 2 * k]) * back, v = __uint_as_float(x[i + 2 * k + 1]) * back;
+                        if (a.dtype == I4D_BF16) {
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(u, v);
+                            w[k] = *reinterpret_cast<const uint32_t*>(&y);
+                        } else {
+                            w[k] = pack_h2(u, v);
+                        }
+                    }
+                    unsigned short* out = static_cast<unsigned short*>(a.out) + to + i;
+                    if (a.wide_out) {
+                        *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) out[k] = static_cast<unsigned short>(w[k / 2] >> (16 * (k & 1)));
+                    }
+                }
+            }
+            if (mine) {
+                const float l2 = l == 0.f ? -INFINITY : M + log2f(l);
+                if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+                if (a.weights) a.lse2[tok * a.heads + head] = l2;
+            }
+        }
+        fence_before();
+    }
+    __syncthreads();
+    if (warp == 13) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (threadIdx.x == 0 && sh.abort) atomicOr(a.seq.err, kTimeout);
+}
+
+}  // namespace i4d_ops

@@ -10,6 +10,7 @@
 #include "i4d_internal.h"
 #include "i4d_kv8_attn.cuh"
 #include "i4d_kv8_cache.cuh"
+#include "i4d_kv8_prompt.cuh"
 #include "i4d_logits.cuh"
 #include "i4d_rope.cuh"
 
@@ -214,6 +215,7 @@ struct AttnPlan {
     int row_tiles;
     int64_t segments;  // (sequence, cache head, row tile)
     int even;          // CTAs that share the tokens, or 0
+    bool prompt;       // k_kv8_prompt: row tiles of kPrRows
     size_t part_bytes, stat_bytes, lse2_bytes, score_bytes;
     size_t bytes() const { return part_bytes + stat_bytes + lse2_bytes + score_bytes; }
 };
@@ -224,13 +226,15 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     const int64_t rows = static_cast<int64_t>(a.max_q) * (a.heads / c.heads);
     p.dt = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     p.nt = rows > 8 && a.dtype != I4D_F32 && p.dt <= 128 ? 2 : 1;
-    p.row_tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.prompt = rows > 64 && a.dtype != I4D_F32 && p.dt <= 128;
+    const int tile = p.prompt ? kPrRows : 8 * p.nt;
+    p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
     p.segments = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
     // Few rows: the CTAs that fit the GPU share the tokens evenly, whatever
     // the lengths are (lengths are known on the device only), but no more of
     // them than have two tiles a warp.  Many rows are work enough by themselves.
     const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 4) * static_cast<int64_t>(o.num_sms);
-    if (p.row_tiles <= 4) {
+    if (!p.prompt && p.row_tiles <= 4) {
         const int64_t units = p.segments * ((a.max_length + 15) / 16);
         p.even = static_cast<int>(std::max<int64_t>(1, std::min(places, (units + 7) / 8)));
     }
@@ -297,8 +301,23 @@ cudaError_t attn_attrs() {
     return e;
 }
 
+template <int DT>
+constexpr int kPromptSmem = PromptSmem<DT>::total + 1024;
+
+template <int DT, int CODE>
+cudaError_t launch_prompt(const AttnDev& d, int64_t grid, cudaStream_t st) {
+    k_kv8_prompt<DT, CODE><<<static_cast<unsigned>(grid), kPrThreads, kPromptSmem<DT>, st>>>(d);
+    return cudaGetLastError();
+}
+
+template <int DT, int CODE>
+cudaError_t prompt_attr() {
+    return cudaFuncSetAttribute(k_kv8_prompt<DT, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
+}
+
 template <int CODE>
 cudaError_t launch_attn_c(const AttnDev& d, const AttnPlan& p, int64_t grid, cudaStream_t st) {
+    if (p.prompt) return p.dt == 64 ? launch_prompt<64, CODE>(d, grid, st) : launch_prompt<128, CODE>(d, grid, st);
     return p.dt == 64 ? launch_attn_d<64, CODE>(d, p, grid, st) : p.dt == 128 ? launch_attn_d<128, CODE>(d, p, grid, st) : launch_attn_d<256, CODE>(d, p, grid, st);
 }
 
@@ -349,6 +368,10 @@ cudaError_t ops_init() {
     if (e == cudaSuccess) e = attn_attrs<128, I4D_CODE_E4M3>();
     if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_INT8>();
     if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_E4M3>();
+    if (e == cudaSuccess) e = prompt_attr<64, I4D_CODE_INT8>();
+    if (e == cudaSuccess) e = prompt_attr<64, I4D_CODE_E4M3>();
+    if (e == cudaSuccess) e = prompt_attr<128, I4D_CODE_INT8>();
+    if (e == cudaSuccess) e = prompt_attr<128, I4D_CODE_E4M3>();
     return e;
 }
 
@@ -592,6 +615,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.stats = reinterpret_cast<float4*>(ws + p.part_bytes);
     d.lse2 = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes);
     if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.lse2_bytes);
+    d.wide_out = aligned(a->out, 16) && a->out_stride * bytes % 16 == 0 && a->out_head_stride * bytes % 16 == 0;
     d.wide_q = aligned(a->q, 16) && a->q_stride * bytes % 16 == 0 && a->q_head_stride * bytes % 16 == 0;
     const int64_t grid = p.even ? p.even : p.segments;
     const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
