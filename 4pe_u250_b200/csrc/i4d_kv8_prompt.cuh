@@ -6,7 +6,7 @@
 // other's softmax.  Tiles of 128 tokens go through
 //   producer (1 warp)      codes of 16 tokens a tensor copy, scales of 16 tokens into a table
 //   converters (4 warps)   codes -> FP16 operands in the 128-byte swizzle, a token row a thread
-//   products (1 thread)    S = Q K^T (128 x 128), O += P V, both into tensor memory
+//   products (2 threads)   a row tile each: S = Q K^T (128 x 128), O += P V, both into tensor memory
 //   softmax (2 x 4 warps)  a row a thread: bounds M and R, P = 2^(x - M) v_scale 2^(M - R) in FP16 over S
 // K is the second operand of S with its dims contiguous, V that of O with its
 // dims contiguous too (the transposed form), so both convert alike; P is the
@@ -23,7 +23,7 @@
 
 namespace i4d_ops {
 
-constexpr int kPrThreads = 448;
+constexpr int kPrThreads = 480;
 constexpr int kPrRows = 256;
 constexpr int kPrTokens = 128;
 
@@ -47,7 +47,8 @@ enum {
 
 struct PrShared {
     uint64_t bar[kPrBars];
-    float4 table[4][8];  // of 16 tokens: scale of K (-1: not there), of V, log2 of it
+    float4 table[4][8];  // of 16 tokens: scale of K, of V, log2 of it
+    int missing[4];      // bit g: the table's 16 tokens g are not there
     uint32_t tmem;
     int abort;
 };
@@ -66,13 +67,6 @@ __device__ __forceinline__ bool pr_wait(PrShared& sh, int i, uint32_t parity) {
     }
     *reinterpret_cast<volatile int*>(&sh.abort) = 1;
     return false;
-}
-
-__device__ __forceinline__ bool pr_test(const PrShared& sh, int i, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar_at(sh, i)), "r"(parity) : "memory");
-    return ok;
 }
 
 __device__ __forceinline__ void pr_arrive(const PrShared& sh, int i) {
@@ -138,18 +132,59 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t x[32]) {
                    "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]),
                    "+r"(x[31])::"memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t x[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];" : I4D_R8(x, 0), I4D_R8(x, 8) : "r"(at));
+}
+__device__ __forceinline__ void tmem_wait_load16(uint32_t x[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]),
+                   "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15])::"memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max16(const uint32_t* x) {
+    const float* y = reinterpret_cast<const float*>(x);
+    const float a = max3(y[0], y[1], y[2]), b = max3(y[3], y[4], y[5]), c = max3(y[6], y[7], y[8]), d = max3(y[9], y[10], y[11]), e = max3(y[12], y[13], y[14]);
+    return max3(max3(a, b, c), max3(d, e, y[15]), c);
+}
+// Two FP32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One token row of codes (128 or 64 bytes with the copy's swizzle) to halves
 // in an operand's row; zeros for a row that is not there.
 template <int DT, int CODE>
 __device__ __forceinline__ void convert_row(uint32_t raw, uint32_t to, int row, bool there) {
+    uint4 w[DT / 16];
 #pragma unroll
     for (int c = 0; c < DT / 16; ++c) {
         const uint32_t from = DT == 64 ? raw + row * 64 + ((c ^ (row >> 1 & 3)) << 4) : raw + row * 128 + ((c ^ (row & 7)) << 4);
-        uint4 w = lds16(from);
-        if (!there) w = make_uint4(0, 0, 0, 0);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        w[c] = lds16(from);
+    }
+#pragma unroll
+    for (int c = 0; c < DT / 16; ++c) {
+        if (!there) w[c] = make_uint4(0, 0, 0, 0);
+        const uint32_t ws[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
         uint32_t h[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -204,7 +239,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPrBars; ++i) {
-            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i == kPFull || i == kPFull + 1 ? 4 : i == kQFull ? 8 : 1;
+            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i == kPFull || i == kPFull + 1 ? 4 : i == kQFull ? 8 : (i >= kKEmpty && i < kVFull) || i == kVEmpty || i == kODone ? (both ? 2 : 1) : 1;
             bar_init(bar_at(sh, i), count);
         }
         sh.abort = 0;
@@ -225,7 +260,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
         for (int j = 0; j < tiles; ++j, ++done) {
             const int st = j & 1, at = t0 + kPrTokens * j + 16 * lane;
             int id = -1;
-            float4 entry = make_float4(-1.f, 0.f, 0.f, 0.f);
+            float4 entry = make_float4(0.f, 0.f, -INFINITY, 0.f);
             if (lane < 8 && at < end) {
                 id = load_block(a.seq, b, at >> shift, true);
                 if (id >= 0) {
@@ -236,9 +271,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                 }
             }
             const int row = (id * a.cache.heads + h) * bs + (at & (bs - 1));
-            const int bytes = __popc(__ballot_sync(~0u, id >= 0)) * kBoxBytes;
+            const unsigned found = __ballot_sync(~0u, id >= 0);
+            const int bytes = __popc(found) * kBoxBytes;
             if (!pr_wait(sh, kRawKEmpty + st, (j >> 1 & 1) ^ 1)) break;
             if (lane < 8) sh.table[j & 3][lane] = entry;
+            if (lane == 0) sh.missing[j & 3] = ~found & 0xff;
             __syncwarp();
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
@@ -258,56 +295,40 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                 bar_wait(bar_at(sh, kRawKFull + (j & 1)), j >> 1 & 1);
                 bar_wait(bar_at(sh, kRawVFull + (j & 1)), j >> 1 & 1);
             }
-    } else if (warp == 13) {  // ------------------------------------- products
-        if (lane == 0 && pr_wait(sh, kQFull, 0)) {
+    } else if (warp >= 13) {  // ------------------------------------- products
+        const int t = warp - 13;  // the row tile
+        if (lane == 0 && (t == 0 || both) && pr_wait(sh, kQFull, 0)) {
             constexpr uint32_t kScores = product_desc(128, false), kValues = product_desc(DT, true);
-            auto scores = [&](int tile, int j) {
+            const uint32_t s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
+            const uint64_t q_desc = operand_desc(base + L::q + t * L::kOperand, 16), k_desc = operand_desc(base + L::k, 16),
+                           v_desc = operand_desc(base + L::v, L::kBlock);
+            bool ok = true;
+            for (int j = 0; j <= tiles; ++j) {
+                // O takes P of token tile j - 1 from the tensor memory that the
+                // scores of tile j then go to.
+                if (j > 0) {
+                    ok = pr_wait(sh, kVFull, (j - 1) & 1) && pr_wait(sh, kPFull + t, (j - 1) & 1);
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll
+                    for (int i = 0; i < kPrTokens / 16; ++i) product_ts(o_at, s_at + i * 8, v_desc + (i * 2048 >> 4), kValues, j > 1 || i > 0);
+                    pr_commit(sh, kVEmpty);
+                    pr_commit(sh, kPvDone + t);
+                    if (j == tiles) break;
+                    ok = pr_wait(sh, kPvDone + t, (j - 1) & 1);
+                    if (!ok) break;
+                }
+                ok = pr_wait(sh, kKFull + (j & 1), j >> 1 & 1);
+                if (!ok) break;
+                fence_after();
+                const uint64_t kd = k_desc + ((j & 1) * L::kOperand >> 4);
 #pragma unroll
                 for (int i = 0; i < DT / 16; ++i) {
-                    const uint32_t step = (i >> 2) * L::kBlock + (i & 3) * 32;
-                    product_ss(tmem + tile * 128, operand_desc(base + L::q + tile * L::kOperand + step, 16),
-                               operand_desc(base + L::k + (j & 1) * L::kOperand + step, 16), kScores, i > 0);
+                    const int step = ((i >> 2) * L::kBlock + (i & 3) * 32) >> 4;
+                    product_ss(s_at, q_desc + step, kd + step, kScores, i > 0);
                 }
-                pr_commit(sh, kSFull + tile);
-            };
-            auto values = [&](int tile, int j) {
-#pragma unroll
-                for (int i = 0; i < kPrTokens / 16; ++i)
-                    product_ts(tmem + 256 + tile * 128, tmem + tile * 128 + i * 8, operand_desc(base + L::v + i * 2048, L::kBlock), kValues, j > 0 || i > 0);
-            };
-            // Whichever tile's next product has its operands: S of token tile j
-            // once O has taken P of tile j - 1 from the same tensor memory.
-            const int n = both ? 2 : 1;
-            int s_done[2] = {0, 0}, o_done[2] = {0, 0}, idle = 0;
-            bool ok = true;
-            while (o_done[0] < tiles || (both && o_done[1] < tiles)) {
-                bool moved = false;
-                for (int t = 0; t < n; ++t) {
-                    int j = s_done[t];
-                    if (j < tiles && j == o_done[t] && pr_test(sh, kKFull + (j & 1), j >> 1 & 1) && (j == 0 || pr_test(sh, kPvDone + t, (j - 1) & 1))) {
-                        fence_after();
-                        scores(t, j);
-                        s_done[t] = j + 1;
-                        if (s_done[n - 1 - t] > j) pr_commit(sh, kKEmpty + (j & 1));
-                        moved = true;
-                    }
-                    j = o_done[t];
-                    if (j < s_done[t] && pr_test(sh, kVFull, j & 1) && pr_test(sh, kPFull + t, j & 1)) {
-                        fence_after();
-                        values(t, j);
-                        pr_commit(sh, kPvDone + t);
-                        o_done[t] = j + 1;
-                        if (o_done[n - 1 - t] > j) pr_commit(sh, kVEmpty);
-                        moved = true;
-                    }
-                }
-                if (moved) {
-                    idle = 0;
-                } else if (++idle > (1 << 22) || *reinterpret_cast<volatile int*>(&sh.abort)) {
-                    *reinterpret_cast<volatile int*>(&sh.abort) = 1;
-                    ok = false;
-                    break;
-                }
+                pr_commit(sh, kSFull + t);
+                pr_commit(sh, kKEmpty + (j & 1));
             }
             pr_commit(sh, kODone);
             if (!ok) bar_wait(bar_at(sh, kODone), 0);  // products in flight end before the CTA leaves
@@ -318,7 +339,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1;
             if (!pr_wait(sh, kRawKFull + st, j >> 1 & 1) || !pr_wait(sh, kKEmpty + st, (j >> 1 & 1) ^ 1)) break;
-            const bool there = t0 + kPrTokens * j + row < s.len && sh.table[j & 3][row >> 4].x >= 0.f;
+            const bool there = t0 + kPrTokens * j + row < s.len && !(sh.missing[j & 3] >> (row >> 4) & 1);
             convert_row<DT, CODE>(base + L::raw + st * 2 * L::kRaw, base + L::k + st * L::kOperand, row, true);
             fence_async();
             __syncwarp();
@@ -379,91 +400,108 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
         const int2 span = row_span(a, first + row / a.group);
         const int tile_last = min(row0 + tile * 128 + 127, row0 + live - 1);
         const int all_from = row_span(a, first + tile_last / a.group).x, all_to = min(s.len, row_span(a, first + (row0 + tile * 128) / a.group).y);
-        float M = -INFINITY, R = -INFINITY, l = 0.f, to_r = 0.f;
+        float M = -INFINITY, R = -INFINITY, to_r = 0.f, off = 0.f;
+        float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = tile == 0 || both;
         for (int j = 0; ok && j < tiles; ++j) {
             ok = pr_wait(sh, kSFull + tile, j & 1);
             if (!ok) break;
             fence_after();
             const int at = t0 + kPrTokens * j;
-            const bool whole = at >= all_from && at + kPrTokens <= all_to;
-            const int from = span.x - at, width = min(span.y, s.len) - span.x;  // column c is seen if c - from < width, unsigned
+            const int missing = sh.missing[j & 3];
+            const bool whole = at >= all_from && at + kPrTokens <= all_to && !missing;
             const float4* table = sh.table[j & 3];
-            uint32_t x[2][32];
-            // the greatest score of the row, and the greatest with its block's value scale
-            float top = -INFINITY, rtop = -INFINITY;
-            tmem_load32(s_at, x[0]);
+            // 32 scores to probabilities: their bound first, then P over S.
+            auto chunk = [&](uint32_t (&x)[32], int c) {
+                if (!whole) {  // scores that the row does not see
+                    const int lo = min(32, max(0, span.x - at - 32 * c)), hi = min(32, max(lo, min(span.y, s.len) - at - 32 * c));
+                    uint32_t seen = static_cast<uint32_t>((1ull << hi) - (1ull << lo));
+                    if (missing >> (2 * c) & 1) seen &= 0xffff0000u;
+                    if (missing >> (2 * c + 1) & 1) seen &= 0x0000ffffu;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_wait_load(x[c & 1]);
-                if (c < 3) tmem_load32(s_at + 32 * (c + 1), x[c + 1 & 1]);
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const float4 block = table[2 * c + g];
-                    float m = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float y = __uint_as_float(x[c & 1][16 * g + i]);
-                        if (!whole && static_cast<unsigned>(32 * c + 16 * g + i - from) >= static_cast<unsigned>(width)) y = -INFINITY;
-                        m = fmaxf(m, y);
-                    }
-                    m = block.x < 0.f || m == -INFINITY ? -INFINITY : m * (down * block.x);
-                    top = fmaxf(top, m);
-                    rtop = fmaxf(rtop, m + block.z);
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1)) x[i] = 0xff800000u;
                 }
-            }
-            const bool raise = top > M + kSlack || rtop > R + kSlack;
-            if (__any_sync(~0u, raise)) {
-                const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(rtop, R) : R;
-                l *= M == m ? 1.f : ex2(M - m);
-                const float f = R == rr ? 1.f : ex2(R - rr);
-                M = m;
-                R = rr;
-                to_r = R == -INFINITY ? 0.f : ex2(M - R);
-                if (j > 0) {
-#pragma unroll
-                    for (int c = 0; c < DT / 32; ++c) {
-                        tmem_load32(o_at + 32 * c, x[0]);
-                        tmem_wait_load(x[0]);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * f);
-                        tmem_store32(o_at + 32 * c, x[0]);
-                    }
-                }
-            }
-            const float off = M == -INFINITY ? 0.f : M;
-            tmem_load32(s_at, x[0]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_wait_load(x[c & 1]);
-                if (c < 3) tmem_load32(s_at + 32 * (c + 1), x[c + 1 & 1]);
+                const float4 b0 = table[2 * c], b1 = table[2 * c + 1];
+                // (a factor of zero would make NaN of what is not seen)
+                const float f0 = fmaxf(down * b0.x, 1e-37f), f1 = fmaxf(down * b1.x, 1e-37f);
+                const float m0 = max16(x) * f0, m1 = max16(x + 16) * f1;
+                const float top = fmaxf(m0, m1), rtop = fmaxf(m0 + b0.z, m1 + b1.z);
                 uint32_t p[16];
+                float2 part[2];
+                for (;;) {
+                    // With the bounds as they are; if a score passes them, again with raised ones.
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const float4 block = table[2 * c + g];
-                    const float f = down * block.x, w = to_r * block.y;
-                    const bool gone = block.x < 0.f;
+                    for (int g = 0; g < 2; ++g) {
+                        const float2 f = g ? make_float2(f1, f1) : make_float2(f0, f0), o = make_float2(-off, -off);
+                        const float wv = to_r * (g ? b1.y : b0.y);
+                        const float2 w = make_float2(wv, wv);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float e0 = ex2(fmaf(__uint_as_float(x[c & 1][16 * g + i]), f, -off));
-                        float e1 = ex2(fmaf(__uint_as_float(x[c & 1][16 * g + i + 1]), f, -off));
-                        if (!whole) {
-                            if (gone || static_cast<unsigned>(32 * c + 16 * g + i - from) >= static_cast<unsigned>(width)) e0 = 0.f;
-                            if (gone || static_cast<unsigned>(32 * c + 16 * g + i + 1 - from) >= static_cast<unsigned>(width)) e1 = 0.f;
-                        } else if (gone) {
-                            e0 = e1 = 0.f;
+                        for (int i = 0; i < 8; ++i) {
+                            const float2 y = fma2(make_float2(__uint_as_float(x[16 * g + 2 * i]), __uint_as_float(x[16 * g + 2 * i + 1])), f, o);
+                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                            part[g] = i ? add2(part[g], e) : e;
+                            const float2 z = mul2(e, w);
+                            p[8 * g + i] = pack_h2(z.x, z.y);
                         }
-                        l += e0 + e1;
-                        p[8 * g + i / 2] = pack_h2(e0 * w, e1 * w);
+                    }
+                    const bool raise = top > M + kSlack || rtop > R + kSlack;
+                    if (!__any_sync(~0u, raise)) break;
+                    const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(rtop, R) : R;
+                    const float fm = M == m ? 1.f : ex2(M - m), f = R == rr ? 1.f : ex2(R - rr);
+                    sum[0].x *= fm;
+                    sum[0].y *= fm;
+                    sum[1].x *= fm;
+                    sum[1].y *= fm;
+                    M = m;
+                    R = rr;
+                    off = M == -INFINITY ? 0.f : M;
+                    to_r = R == -INFINITY ? 0.f : ex2(M - R);
+                    // O so far, and the tile's P so far
+                    tmem_wait_store();
+                    uint32_t y[16];
+#pragma unroll 1
+                    for (int k = 0; j > 0 && k < DT / 16; ++k) {
+                        tmem_load16(o_at + 16 * k, y);
+                        tmem_wait_load16(y);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                        tmem_store16(o_at + 16 * k, y);
+                    }
+                    const __half2 fh = __float2half2_rn(f);
+#pragma unroll 1
+                    for (int k = 0; k < c; ++k) {
+                        tmem_load16(s_at + 16 * k, y);
+                        tmem_wait_load16(y);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y[i]), fh);
+                            y[i] = *reinterpret_cast<const uint32_t*>(&z);
+                        }
+                        tmem_store16(s_at + 16 * k, y);
                     }
                 }
+                sum[0] = add2(sum[0], part[0]);
+                sum[1] = add2(sum[1], part[1]);
                 tmem_store16(s_at + 16 * c, p);
+            };
+            uint32_t x0[32], x1[32];
+            tmem_load32(s_at, x0);
+#pragma unroll 1
+            for (int c = 0; c < 4; c += 2) {
+                tmem_wait_load(x0);
+                tmem_load32(s_at + 32 * (c + 1), x1);
+                chunk(x0, c);
+                tmem_wait_load(x1);
+                if (c == 0) tmem_load32(s_at + 64, x0);
+                chunk(x1, c + 1);
             }
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) pr_arrive(sh, kPFull + tile);
         }
+        const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         if (ok && pr_wait(sh, kODone, 0)) {
             fence_after();
             const float back = l == 0.f || R == -INFINITY ? 0.f : ex2(R - M) / l;
