@@ -42,7 +42,7 @@ struct PromptSmem {
 // Barriers.
 enum {
     kRawKFull = 0, kRawVFull = 2, kRawKEmpty = 4, kRawVEmpty = 6, kKFull = 8, kKEmpty = 10,
-    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 2, kPvDone = kPFull + 2, kQFull = kPvDone + 2, kODone, kPrBars
+    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 4, kPvDone = kPFull + 4, kQFull = kPvDone + 4, kODone, kPrBars
 };
 
 struct PrShared {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPrBars; ++i) {
-            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i == kPFull || i == kPFull + 1 ? 4 : i == kQFull ? 8 : (i >= kKEmpty && i < kVFull) || i == kVEmpty || i == kODone ? (both ? 2 : 1) : 1;
+            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i >= kPFull && i < kPvDone ? 4 : i == kQFull ? 8 : (i >= kKEmpty && i < kVFull) || i == kVEmpty || i == kODone ? (both ? 2 : 1) : 1;
             bar_init(bar_at(sh, i), count);
         }
         sh.abort = 0;
@@ -298,37 +298,44 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
     } else if (warp >= 13) {  // ------------------------------------- products
         const int t = warp - 13;  // the row tile
         if (lane == 0 && (t == 0 || both) && pr_wait(sh, kQFull, 0)) {
-            constexpr uint32_t kScores = product_desc(128, false), kValues = product_desc(DT, true);
+            constexpr uint32_t kScores = product_desc(64, false), kValues = product_desc(DT, true);
             const uint32_t s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
             const uint64_t q_desc = operand_desc(base + L::q + t * L::kOperand, 16), k_desc = operand_desc(base + L::k, 16),
                            v_desc = operand_desc(base + L::v, L::kBlock);
             bool ok = true;
-            for (int j = 0; j <= tiles; ++j) {
-                // O takes P of token tile j - 1 from the tensor memory that the
-                // scores of tile j then go to.
-                if (j > 0) {
-                    ok = pr_wait(sh, kVFull, (j - 1) & 1) && pr_wait(sh, kPFull + t, (j - 1) & 1);
+            // Tile 1 begins when tile 0 has its first probabilities: the one's
+            // products then run under the other's softmax.
+            if (t == 1) ok = pr_wait(sh, kPFull, 0);
+            for (int j = 0; ok && j <= tiles; ++j) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int at = 2 * t + half;
+                    // O takes P of 64 tokens from the tensor memory that the
+                    // scores of the next tile's 64 then go to.
+                    if (j > 0) {
+                        ok = ok && pr_wait(sh, kVFull, (j - 1) & 1) && pr_wait(sh, kPFull + at, (j - 1) & 1);
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            product_ts(o_at, s_at + half * 64 + i * 8, v_desc + ((4 * half + i) * 2048 >> 4), kValues, j > 1 || half > 0 || i > 0);
+                        pr_commit(sh, kPvDone + at);
+                        if (half) pr_commit(sh, kVEmpty);
+                        if (j == tiles) continue;
+                        ok = pr_wait(sh, kPvDone + at, (j - 1) & 1);
+                    }
+                    ok = ok && pr_wait(sh, kKFull + (j & 1), j >> 1 & 1);
                     if (!ok) break;
                     fence_after();
+                    const uint64_t kd = k_desc + (((j & 1) * L::kOperand + half * 8192) >> 4);
 #pragma unroll
-                    for (int i = 0; i < kPrTokens / 16; ++i) product_ts(o_at, s_at + i * 8, v_desc + (i * 2048 >> 4), kValues, j > 1 || i > 0);
-                    pr_commit(sh, kVEmpty);
-                    pr_commit(sh, kPvDone + t);
-                    if (j == tiles) break;
-                    ok = pr_wait(sh, kPvDone + t, (j - 1) & 1);
-                    if (!ok) break;
+                    for (int i = 0; i < DT / 16; ++i) {
+                        const int step = ((i >> 2) * L::kBlock + (i & 3) * 32) >> 4;
+                        product_ss(s_at + half * 64, q_desc + step, kd + step, kScores, i > 0);
+                    }
+                    pr_commit(sh, kSFull + at);
+                    if (half) pr_commit(sh, kKEmpty + (j & 1));
                 }
-                ok = pr_wait(sh, kKFull + (j & 1), j >> 1 & 1);
-                if (!ok) break;
-                fence_after();
-                const uint64_t kd = k_desc + ((j & 1) * L::kOperand >> 4);
-#pragma unroll
-                for (int i = 0; i < DT / 16; ++i) {
-                    const int step = ((i >> 2) * L::kBlock + (i & 3) * 32) >> 4;
-                    product_ss(s_at, q_desc + step, kd + step, kScores, i > 0);
-                }
-                pr_commit(sh, kSFull + t);
-                pr_commit(sh, kKEmpty + (j & 1));
             }
             pr_commit(sh, kODone);
             if (!ok) bar_wait(bar_at(sh, kODone), 0);  // products in flight end before the CTA leaves
@@ -404,14 +411,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = tile == 0 || both;
         for (int j = 0; ok && j < tiles; ++j) {
-            ok = pr_wait(sh, kSFull + tile, j & 1);
-            if (!ok) break;
-            fence_after();
             const int at = t0 + kPrTokens * j;
-            const int missing = sh.missing[j & 3];
-            const bool whole = at >= all_from && at + kPrTokens <= all_to && !missing;
+            int missing = 0;
+            bool whole = false;
             const float4* table = sh.table[j & 3];
-            // 32 scores to probabilities: their bound first, then P over S.
+            // 32 scores to probabilities, which overlay those of their half of the tile.
+            auto p_at = [&](int c) { return s_at + (c >> 1) * 64 + (c & 1) * 16; };
             auto chunk = [&](uint32_t (&x)[32], int c) {
                 if (!whole) {  // scores that the row does not see
                     const int lo = min(32, max(0, span.x - at - 32 * c)), hi = min(32, max(lo, min(span.y, s.len) - at - 32 * c));
@@ -457,49 +462,57 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                     R = rr;
                     off = M == -INFINITY ? 0.f : M;
                     to_r = R == -INFINITY ? 0.f : ex2(M - R);
-                    // O so far, and the tile's P so far
+                    // O so far (with the products before this half of the tile), and the half's P so far
                     tmem_wait_store();
+                    const bool any_o = j > 0 || c > 1;
+                    if (any_o) {
+                        ok = pr_wait(sh, kPvDone + 2 * tile + (c < 2), (c < 2 ? j - 1 : j) & 1);
+                        fence_after();
+                    }
                     uint32_t y[16];
 #pragma unroll 1
-                    for (int k = 0; j > 0 && k < DT / 16; ++k) {
+                    for (int k = 0; any_o && k < DT / 16; ++k) {
                         tmem_load16(o_at + 16 * k, y);
                         tmem_wait_load16(y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
                         tmem_store16(o_at + 16 * k, y);
                     }
-                    const __half2 fh = __float2half2_rn(f);
-#pragma unroll 1
-                    for (int k = 0; k < c; ++k) {
-                        tmem_load16(s_at + 16 * k, y);
+                    if (c & 1) {
+                        const __half2 fh = __float2half2_rn(f);
+                        tmem_load16(p_at(c - 1), y);
                         tmem_wait_load16(y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y[i]), fh);
                             y[i] = *reinterpret_cast<const uint32_t*>(&z);
                         }
-                        tmem_store16(s_at + 16 * k, y);
+                        tmem_store16(p_at(c - 1), y);
                     }
                 }
                 sum[0] = add2(sum[0], part[0]);
                 sum[1] = add2(sum[1], part[1]);
-                tmem_store16(s_at + 16 * c, p);
+                tmem_store16(p_at(c), p);
             };
-            uint32_t x0[32], x1[32];
-            tmem_load32(s_at, x0);
 #pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
-                tmem_wait_load(x0);
-                tmem_load32(s_at + 32 * (c + 1), x1);
-                chunk(x0, c);
-                tmem_wait_load(x1);
-                if (c == 0) tmem_load32(s_at + 64, x0);
-                chunk(x1, c + 1);
+            for (int half = 0; half < 2; ++half) {
+                ok = ok && pr_wait(sh, kSFull + 2 * tile + half, j & 1);
+                if (!ok) break;
+                fence_after();
+                missing = sh.missing[j & 3];
+                whole = at >= all_from && at + kPrTokens <= all_to && !missing;
+#pragma unroll 1
+                for (int c = 2 * half; c < 2 * half + 2; ++c) {
+                    uint32_t x[32];
+                    tmem_load32(s_at + 32 * c, x);
+                    tmem_wait_load(x);
+                    chunk(x, c);
+                }
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) pr_arrive(sh, kPFull + 2 * tile + half);
             }
-            tmem_wait_store();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) pr_arrive(sh, kPFull + tile);
         }
         const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         if (ok && pr_wait(sh, kODone, 0)) {
