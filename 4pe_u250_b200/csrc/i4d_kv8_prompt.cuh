@@ -1,8 +1,8 @@
 // i4d_kv8_prompt.cuh -- attention of many query rows over the cache of 8-bit
 // codes on the fifth-generation tensor cores.
 //
-// One CTA for up to 256 rows (query, head of the group) of one cache head: two
-// tiles of 128 rows take turns, so that one tile's products run under the
+// A CTA takes up to 256 rows (query, head of the group) of one cache head at a
+// time: two tiles of 128 rows take turns, so that one tile's products run under the
 // other's softmax.  Tiles of 128 tokens go through
 //   producer (1 warp)      codes of 16 tokens a tensor copy, scales of 16 tokens into a table
 //   converters (4 warps)   codes -> FP16 operands in the 128-byte swizzle, a token row a thread
@@ -42,11 +42,15 @@ struct PromptSmem {
 // Barriers.
 enum {
     kRawKFull = 0, kRawVFull = 2, kRawKEmpty = 4, kRawVEmpty = 6, kKFull = 8, kKEmpty = 10,
-    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 4, kPvDone = kPFull + 4, kQFull = kPvDone + 4, kODone, kPrBars
+    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 4, kPvDone = kPFull + 4, kQFull = kPvDone + 4, kODone = kQFull + 2, kPrBars = kODone + 2
 };
+
+constexpr int kPrWarps = kPrThreads / 32;
 
 struct PrShared {
     uint64_t bar[kPrBars];
+    int64_t sums[kPrWarps], before;  // units of work (find_prompt)
+    int pair;
     float4 table[4][8];  // of 16 tokens: scale of K, of V, log2 of it
     int missing[4];      // bit g: the table's 16 tokens g are not there
     uint32_t tmem;
@@ -214,6 +218,98 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// Token tiles of row tile rt of a sequence, from token `begin`.
+struct PrSpan {
+    int tiles, begin, end, live;  // live rows
+};
+__device__ __forceinline__ PrSpan prompt_span(const AttnDev& a, const Seq& s, int rt) {
+    const int rows = s.n * a.group, row0 = rt * kPrRows, first = s.len - s.n;
+    if (s.len > a.max_length || row0 >= rows) return {0, 0, 0, 0};
+    const int live = min(kPrRows, rows - row0);
+    const int begin = row_span(a, first + row0 / a.group).x & ~15, end = row_span(a, first + (row0 + live - 1) / a.group).y;
+    return {(end - begin + kPrTokens - 1) / kPrTokens, begin, end, live};
+}
+
+// Units of the batch (token tiles of 128 for each sequence, row tile, head, in
+// this order) and the pair (sequence * row tiles + row tile) in which unit
+// u(total) lies, with the units before it.  WARPS warps take consecutive pairs.
+template <int WARPS, typename U>
+__device__ __forceinline__ int64_t find_prompt(const AttnDev& a, U&& unit, bool report, int64_t* sums, int64_t* before_out, int* pair_out) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t pairs = static_cast<int64_t>(a.batch) * a.row_tiles, per = (pairs + WARPS * 32 - 1) / (WARPS * 32);
+    const int64_t p0 = min(pairs, threadIdx.x * per), p1 = min(pairs, p0 + per);
+    auto size = [&](int64_t p, bool tell) {
+        const int b = static_cast<int>(p / a.row_tiles), rt = static_cast<int>(p % a.row_tiles);
+        const Seq s = load_seq(a.seq, b, tell && rt == 0);
+        if (tell && rt == 0 && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
+        return static_cast<int64_t>(prompt_span(a, s, rt).tiles) * a.cache.heads;
+    };
+    int64_t mine = 0;
+    for (int64_t p = p0; p < p1; ++p) mine += size(p, report);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) upto += sums[w];
+        total += sums[w];
+    }
+    const int64_t u = unit(total);
+    int64_t before = upto - mine;
+    if (u >= before && u < upto)
+        for (int64_t p = p0; p < p1; ++p) {
+            const int64_t next = before + size(p, false);
+            if (u < next) {
+                *before_out = before;
+                *pair_out = static_cast<int>(p);
+                break;
+            }
+            before = next;
+        }
+    __syncthreads();
+    return total;
+}
+
+// Calls f for each of a CTA's pieces in turn until it returns false: token
+// tiles [j0, j1) of a (sequence, row tile, head).
+struct PrPiece {
+    Seq s;
+    PrSpan span;
+    int b, rt, h, j0, j1, slot;  // slot: where partial sums go, 0 the CTA's first piece, 1 its last
+    bool whole;
+};
+template <typename F>
+__device__ __forceinline__ void each_piece(const AttnDev& a, int64_t u, int64_t u_end, int64_t before, int pair, F&& f) {
+    const int64_t u0 = u;
+    while (u < u_end) {
+        PrPiece p;
+        p.b = pair / a.row_tiles;
+        p.rt = pair % a.row_tiles;
+        p.s = load_seq(a.seq, p.b, false);
+        p.span = prompt_span(a, p.s, p.rt);
+        const int64_t next = before + static_cast<int64_t>(p.span.tiles) * a.cache.heads;
+        if (u >= next) {
+            before = next;
+            ++pair;
+            continue;
+        }
+        p.h = static_cast<int>((u - before) / p.span.tiles);
+        const int64_t first = before + static_cast<int64_t>(p.h) * p.span.tiles;
+        p.j0 = static_cast<int>(u - first);
+        p.j1 = static_cast<int>(min(static_cast<int64_t>(p.span.tiles), u_end - first));
+        p.whole = p.j0 == 0 && p.j1 == p.span.tiles;
+        p.slot = u == u0 ? 0 : 1;
+        if (!f(p)) return;
+        u = first + p.j1;
+    }
+}
+
 template <int DT, int CODE>
 __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_constant__ AttnDev a) {
     using L = PromptSmem<DT>;
@@ -222,24 +318,26 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
     const uint32_t base_raw = static_cast<uint32_t>(__cvta_generic_to_shared(pr_base));
     const uint32_t base = (base_raw + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the last row tiles see the most tokens: they start first
-    const int rt = a.row_tiles - 1 - static_cast<int>(blockIdx.x / (a.cache.heads * a.batch));
-    const int bh = blockIdx.x % (a.cache.heads * a.batch), h = bh % a.cache.heads, b = bh / a.cache.heads;
-    const bool report = rt == 0 && h == 0 && threadIdx.x == 0;
-    const Seq s = load_seq(a.seq, b, report);
-    if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
-    const int rows = s.n * a.group, row0 = rt * kPrRows;
-    if (s.len > a.max_length || row0 >= rows) return;
-    const int first = s.len - s.n, live = min(kPrRows, rows - row0);
-    const bool both = live > 128;
-    const int2 first_span = row_span(a, first + row0 / a.group), last_span = row_span(a, first + (row0 + live - 1) / a.group);
-    const int t0 = first_span.x & ~15, end = last_span.y;
-    const int tiles = (end - t0 + kPrTokens - 1) / kPrTokens;
     const int bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
+    // The CTA's even share of the units.
+    int64_t u, u_end;
+    {
+        int64_t share = 0;
+        const int64_t total = find_prompt<kPrWarps>(a, [&](int64_t n) {
+            share = (n + gridDim.x - 1) / gridDim.x;
+            return share * blockIdx.x;
+        }, blockIdx.x == 0, sh.sums, &sh.before, &sh.pair);
+        u = share * blockIdx.x;
+        u_end = min(total, u + share);
+    }
+    if (u >= u_end) return;
+    const int64_t before = sh.before;
+    const int pair = sh.pair;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPrBars; ++i) {
-            const int count = i >= kRawKEmpty && i < kKEmpty ? 4 : i == kVFull ? 4 : i >= kPFull && i < kPvDone ? 4 : i == kQFull ? 8 : (i >= kKEmpty && i < kVFull) || i == kVEmpty || i == kODone ? (both ? 2 : 1) : 1;
+            const bool warps = (i >= kRawKEmpty && i < kKEmpty) || i == kVFull || (i >= kPFull && i < kPvDone) || i == kQFull || i == kQFull + 1;
+            const int count = warps ? 4 : (i >= kKEmpty && i < kVFull) || i == kVEmpty ? 2 : 1;
             bar_init(bar_at(sh, i), count);
         }
         sh.abort = 0;
@@ -256,115 +354,153 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 
     if (warp == 12) {  // ------------------------------------------- producer
         constexpr int kBoxBytes = 16 * DT;
-        int done = 0;
-        for (int j = 0; j < tiles; ++j, ++done) {
-            const int st = j & 1, at = t0 + kPrTokens * j + 16 * lane;
-            int id = -1;
-            float4 entry = make_float4(0.f, 0.f, -INFINITY, 0.f);
-            if (lane < 8 && at < end) {
-                id = load_block(a.seq, b, at >> shift, true);
-                if (id >= 0) {
-                    const int64_t sc = static_cast<int64_t>(id) * a.cache.heads + h;
-                    entry.x = __ldg(a.cache.scale[0] + sc);
-                    entry.y = __ldg(a.cache.scale[1] + sc);
-                    entry.z = __log2f(entry.y);  // only a bound: its rounding cancels
+        int n = 0;  // tiles so far, over all pieces
+        each_piece(a, u, u_end, before, pair, [&](const PrPiece& p) {
+            bool ok = true;
+            for (int j = p.j0; ok && j < p.j1; ++j, ++n) {
+                const int st = n & 1, at = p.span.begin + kPrTokens * j + 16 * lane;
+                int id = -1;
+                float4 entry = make_float4(0.f, 0.f, -INFINITY, 0.f);
+                if (lane < 8 && at < p.span.end) {
+                    id = load_block(a.seq, p.b, at >> shift, true);
+                    if (id >= 0) {
+                        const int64_t sc = static_cast<int64_t>(id) * a.cache.heads + p.h;
+                        entry.x = __ldg(a.cache.scale[0] + sc);
+                        entry.y = __ldg(a.cache.scale[1] + sc);
+                        entry.z = __log2f(entry.y);  // only a bound: its rounding cancels
+                    }
+                }
+                const int row = (id * a.cache.heads + p.h) * bs + (at & (bs - 1));
+                const unsigned found = __ballot_sync(~0u, id >= 0);
+                const int bytes = __popc(found) * kBoxBytes;
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    ok = __all_sync(~0u, pr_wait(sh, (which ? kRawVEmpty : kRawKEmpty) + st, (n >> 1 & 1) ^ 1));
+                    if (!ok) break;
+                    if (!which) {
+                        if (lane < 8) sh.table[n & 3][lane] = entry;
+                        if (lane == 0) sh.missing[n & 3] = ~found & 0xff;
+                        __syncwarp();
+                    }
+                    const uint32_t bar = bar_at(sh, (which ? kRawVFull : kRawKFull) + st);
+                    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+                    __syncwarp();
+                    if (id >= 0)
+                        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                                         base + L::raw + (st * 2 + which) * L::kRaw + lane * kBoxBytes),
+                                     "l"(&a.maps[which]), "r"(0), "r"(row), "r"(bar)
+                                     : "memory");
                 }
             }
-            const int row = (id * a.cache.heads + h) * bs + (at & (bs - 1));
-            const unsigned found = __ballot_sync(~0u, id >= 0);
-            const int bytes = __popc(found) * kBoxBytes;
-            if (!pr_wait(sh, kRawKEmpty + st, (j >> 1 & 1) ^ 1)) break;
-            if (lane < 8) sh.table[j & 3][lane] = entry;
-            if (lane == 0) sh.missing[j & 3] = ~found & 0xff;
-            __syncwarp();
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                if (which && !pr_wait(sh, kRawVEmpty + st, (j >> 1 & 1) ^ 1)) break;
-                const uint32_t bar = bar_at(sh, (which ? kRawVFull : kRawKFull) + st);
-                if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-                __syncwarp();
-                if (id >= 0)
-                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                                     base + L::raw + (st * 2 + which) * L::kRaw + lane * kBoxBytes),
-                                 "l"(&a.maps[which]), "r"(0), "r"(row), "r"(bar)
-                                 : "memory");
-            }
-        }
+            return ok;
+        });
         if (sh.abort)  // copies in flight land before the CTA leaves
-            for (int j = max(0, done - 1); j < min(tiles, done + 1); ++j) {
+            for (int j = max(0, n - 2); j < n; ++j) {
                 bar_wait(bar_at(sh, kRawKFull + (j & 1)), j >> 1 & 1);
                 bar_wait(bar_at(sh, kRawVFull + (j & 1)), j >> 1 & 1);
             }
     } else if (warp >= 13) {  // ------------------------------------- products
         const int t = warp - 13;  // the row tile
-        if (lane == 0 && (t == 0 || both) && pr_wait(sh, kQFull, 0)) {
+        if (lane == 0) {
             constexpr uint32_t kScores = product_desc(64, false), kValues = product_desc(DT, true);
             const uint32_t s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
             const uint64_t q_desc = operand_desc(base + L::q + t * L::kOperand, 16), k_desc = operand_desc(base + L::k, 16),
                            v_desc = operand_desc(base + L::v, L::kBlock);
+            // Token tiles of all pieces; of those with rows in this row tile,
+            // whose barriers count them; pieces with such rows.
+            int n = 0, m = 0, pieces = 0;
             bool ok = true;
-            // Tile 1 begins when tile 0 has its first probabilities: the one's
-            // products then run under the other's softmax.
-            if (t == 1) ok = pr_wait(sh, kPFull, 0);
-            for (int j = 0; ok && j <= tiles; ++j) {
+            each_piece(a, u, u_end, before, pair, [&](const PrPiece& p) {
+                const int count = p.j1 - p.j0;
+                if (t * 128 >= p.span.live) {  // nothing here for this row tile: it only gives the buffers on
+                    for (int j = 0; ok && j < count; ++j, ++n) {
+                        ok = pr_wait(sh, kKFull + (n & 1), n >> 1 & 1);
+                        if (ok) pr_arrive(sh, kKEmpty + (n & 1));
+                        ok = ok && pr_wait(sh, kVFull, n & 1);
+                        if (ok) pr_arrive(sh, kVEmpty);
+                    }
+                    return ok;
+                }
+                ok = pr_wait(sh, kQFull + t, pieces++ & 1);
+                // Tile 1 begins when tile 0 has its first probabilities: the
+                // one's products then run under the other's softmax.
+                if (t == 1 && n == 0) ok = ok && pr_wait(sh, kPFull, 0);
+                for (int j = 0; ok && j <= count; ++j) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int at = 2 * t + half;
-                    // O takes P of 64 tokens from the tensor memory that the
-                    // scores of the next tile's 64 then go to.
-                    if (j > 0) {
-                        ok = ok && pr_wait(sh, kVFull, (j - 1) & 1) && pr_wait(sh, kPFull + at, (j - 1) & 1);
+                    for (int half = 0; half < 2; ++half) {
+                        const int at = 2 * t + half;
+                        // O takes P of 64 tokens from the tensor memory that the
+                        // scores of the next tile's 64 then go to.
+                        if (j > 0) {
+                            ok = ok && pr_wait(sh, kVFull, (n + j - 1) & 1) && pr_wait(sh, kPFull + at, (m + j - 1) & 1);
+                            if (!ok) break;
+                            fence_after();
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                product_ts(o_at, s_at + half * 64 + i * 8, v_desc + ((4 * half + i) * 2048 >> 4), kValues, j > 1 || half > 0 || i > 0);
+                            pr_commit(sh, kPvDone + at);
+                            if (half) pr_commit(sh, kVEmpty);
+                            if (j == count) continue;
+                            ok = pr_wait(sh, kPvDone + at, (m + j - 1) & 1);
+                        }
+                        ok = ok && pr_wait(sh, kKFull + ((n + j) & 1), (n + j) >> 1 & 1);
                         if (!ok) break;
                         fence_after();
+                        const uint64_t kd = k_desc + ((((n + j) & 1) * L::kOperand + half * 8192) >> 4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            product_ts(o_at, s_at + half * 64 + i * 8, v_desc + ((4 * half + i) * 2048 >> 4), kValues, j > 1 || half > 0 || i > 0);
-                        pr_commit(sh, kPvDone + at);
-                        if (half) pr_commit(sh, kVEmpty);
-                        if (j == tiles) continue;
-                        ok = pr_wait(sh, kPvDone + at, (j - 1) & 1);
+                        for (int i = 0; i < DT / 16; ++i) {
+                            const int step = ((i >> 2) * L::kBlock + (i & 3) * 32) >> 4;
+                            product_ss(s_at + half * 64, q_desc + step, kd + step, kScores, i > 0);
+                        }
+                        pr_commit(sh, kSFull + at);
+                        if (half) pr_commit(sh, kKEmpty + ((n + j) & 1));
                     }
-                    ok = ok && pr_wait(sh, kKFull + (j & 1), j >> 1 & 1);
-                    if (!ok) break;
-                    fence_after();
-                    const uint64_t kd = k_desc + (((j & 1) * L::kOperand + half * 8192) >> 4);
-#pragma unroll
-                    for (int i = 0; i < DT / 16; ++i) {
-                        const int step = ((i >> 2) * L::kBlock + (i & 3) * 32) >> 4;
-                        product_ss(s_at + half * 64, q_desc + step, kd + step, kScores, i > 0);
-                    }
-                    pr_commit(sh, kSFull + at);
-                    if (half) pr_commit(sh, kKEmpty + (j & 1));
                 }
-            }
-            pr_commit(sh, kODone);
-            if (!ok) bar_wait(bar_at(sh, kODone), 0);  // products in flight end before the CTA leaves
+                pr_commit(sh, kODone + t);
+                n += count;
+                m += count;
+                return ok;
+            });
+            if (!ok && pieces) bar_wait(bar_at(sh, kODone + t), (pieces - 1) & 1);  // products in flight end before the CTA leaves
         }
         __syncwarp();
     } else if (warp >= 8) {  // --------------------------------------- converters
         const int row = threadIdx.x - 256;
-        for (int j = 0; j < tiles; ++j) {
-            const int st = j & 1;
-            if (!pr_wait(sh, kRawKFull + st, j >> 1 & 1) || !pr_wait(sh, kKEmpty + st, (j >> 1 & 1) ^ 1)) break;
-            const bool there = t0 + kPrTokens * j + row < s.len && !(sh.missing[j & 3] >> (row >> 4) & 1);
-            convert_row<DT, CODE>(base + L::raw + st * 2 * L::kRaw, base + L::k + st * L::kOperand, row, true);
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                pr_arrive(sh, kKFull + st);
-                pr_arrive(sh, kRawKEmpty + st);
+        int n = 0;
+        each_piece(a, u, u_end, before, pair, [&](const PrPiece& p) {
+            for (int j = p.j0; j < p.j1; ++j, ++n) {
+                const int st = n & 1;
+                if (!__all_sync(~0u, pr_wait(sh, kRawKFull + st, n >> 1 & 1) && pr_wait(sh, kKEmpty + st, (n >> 1 & 1) ^ 1))) return false;
+                const bool there = p.span.begin + kPrTokens * j + row < p.s.len && !(sh.missing[n & 3] >> (row >> 4) & 1);
+                convert_row<DT, CODE>(base + L::raw + st * 2 * L::kRaw, base + L::k + st * L::kOperand, row, true);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    pr_arrive(sh, kKFull + st);
+                    pr_arrive(sh, kRawKEmpty + st);
+                }
+                if (!__all_sync(~0u, pr_wait(sh, kRawVFull + st, n >> 1 & 1) && pr_wait(sh, kVEmpty, (n & 1) ^ 1))) return false;
+                convert_row<DT, CODE>(base + L::raw + (st * 2 + 1) * L::kRaw, base + L::v, row, there);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    pr_arrive(sh, kVFull);
+                    pr_arrive(sh, kRawVEmpty + st);
+                }
             }
-            if (!pr_wait(sh, kRawVFull + st, j >> 1 & 1) || !pr_wait(sh, kVEmpty, (j & 1) ^ 1)) break;
-            convert_row<DT, CODE>(base + L::raw + (st * 2 + 1) * L::kRaw, base + L::v, row, there);
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                pr_arrive(sh, kVFull);
-                pr_arrive(sh, kRawVEmpty + st);
-            }
-        }
+            return true;
+        });
     } else {  // ------------------------------------------------------- softmax
-        const int tile = warp >> 2, r = threadIdx.x & 127, row = row0 + tile * 128 + r;
+        const int tile = warp >> 2, r = threadIdx.x & 127;
+        int n = 0, m = 0, pieces = 0;  // as in the products' threads
+        each_piece(a, u, u_end, before, pair, [&](const PrPiece& piece) {
+        const int count = piece.j1 - piece.j0;
+        if (tile * 128 >= piece.span.live) {
+            n += count;
+            return true;
+        }
+        const Seq& s = piece.s;
+        const int first = s.len - s.n, row0 = piece.rt * kPrRows, row = row0 + tile * 128 + r, rows = s.n * a.group, h = piece.h;
         const bool mine = row < rows;
         const int64_t tok = s.first + row / a.group;
         const int head = h * a.group + row % a.group;
@@ -400,21 +536,21 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) pr_arrive(sh, kQFull);
+            if (lane == 0) pr_arrive(sh, kQFull + tile);
         }
         const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lanes 32 (warp % 4) of tensor memory
         const uint32_t s_at = tmem + quarter + tile * 128, o_at = tmem + quarter + 256 + tile * 128;
         const int2 span = row_span(a, first + row / a.group);
-        const int tile_last = min(row0 + tile * 128 + 127, row0 + live - 1);
+        const int tile_last = min(row0 + tile * 128 + 127, row0 + piece.span.live - 1);
         const int all_from = row_span(a, first + tile_last / a.group).x, all_to = min(s.len, row_span(a, first + (row0 + tile * 128) / a.group).y);
         float M = -INFINITY, R = -INFINITY, to_r = 0.f, off = 0.f;
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        bool ok = tile == 0 || both;
-        for (int j = 0; ok && j < tiles; ++j) {
-            const int at = t0 + kPrTokens * j;
+        bool ok = true;
+        for (int j = 0; ok && j < count; ++j) {
+            const int at = piece.span.begin + kPrTokens * (piece.j0 + j), parity = (m + j) & 1;
             int missing = 0;
             bool whole = false;
-            const float4* table = sh.table[j & 3];
+            const float4* table = sh.table[(n + j) & 3];
             // 32 scores to probabilities, which overlay those of their half of the tile.
             auto p_at = [&](int c) { return s_at + (c >> 1) * 64 + (c & 1) * 16; };
             auto chunk = [&](uint32_t (&x)[32], int c) {
@@ -466,7 +602,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                     tmem_wait_store();
                     const bool any_o = j > 0 || c > 1;
                     if (any_o) {
-                        ok = pr_wait(sh, kPvDone + 2 * tile + (c < 2), (c < 2 ? j - 1 : j) & 1);
+                        ok = __all_sync(~0u, pr_wait(sh, kPvDone + 2 * tile + (c < 2), c < 2 ? parity ^ 1 : parity)) && ok;
                         fence_after();
                     }
                     uint32_t y[16];
@@ -496,10 +632,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
             };
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
-                ok = ok && pr_wait(sh, kSFull + 2 * tile + half, j & 1);
+                ok = ok && __all_sync(~0u, pr_wait(sh, kSFull + 2 * tile + half, parity));
                 if (!ok) break;
                 fence_after();
-                missing = sh.missing[j & 3];
+                missing = sh.missing[(n + j) & 3];
                 whole = at >= all_from && at + kPrTokens <= all_to && !missing;
 #pragma unroll 1
                 for (int c = 2 * half; c < 2 * half + 2; ++c) {
@@ -515,53 +651,136 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
             }
         }
         const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        if (ok && pr_wait(sh, kODone, 0)) {
-            fence_after();
-            const float back = l == 0.f || R == -INFINITY ? 0.f : ex2(R - M) / l;
+        if (!ok || !__all_sync(~0u, pr_wait(sh, kODone + tile, pieces & 1))) return false;
+        fence_after();
+        const float back = !piece.whole ? 1.f : l == 0.f || R == -INFINITY ? 0.f : ex2(R - M) / l;
+        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + piece.slot) * kPrRows + tile * 128 + r;
+#pragma unroll
+        for (int c = 0; c < DT / 32; ++c) {
             uint32_t x[32];
+            __syncwarp();
+            tmem_load32(o_at + 32 * c, x);
+            tmem_wait_load(x);
+            if (!mine) continue;
+            if (!piece.whole) {
 #pragma unroll
-            for (int c = 0; c < DT / 32; ++c) {
-                tmem_load32(o_at + 32 * c, x);
-                tmem_wait_load(x);
-                if (!mine) continue;
-                const int64_t to = tok * a.out_tok + head * a.out_head + 32 * c;
+                for (int i = 0; i < 32; i += 4)
+                    if (32 * c + i < dim) *reinterpret_cast<uint4*>(a.part + part * dim + 32 * c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                continue;
+            }
+            const int64_t to = tok * a.out_tok + head * a.out_head + 32 * c;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (32 * c + i >= dim) break;
-                    uint32_t w[4];
+            for (int i = 0; i < 32; i += 8) {
+                if (32 * c + i >= dim) break;
+                uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float u = __uint_as_float(x[i + 2 * k]) * back, v = __uint_as_float(x[i + 2 * k + 1]) * back;
-                        if (a.dtype == I4D_BF16) {
-                            const __nv_bfloat162 y = __floats2bfloat162_rn(u, v);
-                            w[k] = *reinterpret_cast<const uint32_t*>(&y);
-                        } else {
-                            w[k] = pack_h2(u, v);
-                        }
-                    }
-                    unsigned short* out = static_cast<unsigned short*>(a.out) + to + i;
-                    if (a.wide_out) {
-                        *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < 4; ++k) {
+                    const float y0 = __uint_as_float(x[i + 2 * k]) * back, y1 = __uint_as_float(x[i + 2 * k + 1]) * back;
+                    if (a.dtype == I4D_BF16) {
+                        const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
+                        w[k] = *reinterpret_cast<const uint32_t*>(&y);
                     } else {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) out[k] = static_cast<unsigned short>(w[k / 2] >> (16 * (k & 1)));
+                        w[k] = pack_h2(y0, y1);
                     }
                 }
+                unsigned short* out = static_cast<unsigned short*>(a.out) + to + i;
+                if (a.wide_out) {
+                    *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) out[k] = static_cast<unsigned short>(w[k / 2] >> (16 * (k & 1)));
+                }
             }
-            if (mine) {
+        }
+        if (mine) {
+            if (piece.whole) {
                 const float l2 = l == 0.f ? -INFINITY : M + log2f(l);
                 if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
                 if (a.weights) a.lse2[tok * a.heads + head] = l2;
+            } else {
+                a.stats[part] = make_float4(M, l, R, 0.f);
             }
         }
         fence_before();
+        n += count;
+        m += count;
+        ++pieces;
+        __syncwarp();
+        return true;
+        });
     }
+    fence_before();
     __syncthreads();
     if (warp == 13) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
     if (threadIdx.x == 0 && sh.abort) atomicOr(a.seq.err, kTimeout);
+}
+
+// Joins the pieces of a segment that several CTAs of k_kv8_prompt shared:
+// blockIdx.x / 8 + 1 is the first CTA whose share begins inside the segment,
+// blockIdx.x % 8 the 32 rows; a warp for a row at a time.
+__global__ void __launch_bounds__(256) k_kv8_prompt_join(AttnDev a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ int64_t s_sums[8], s_before;
+    __shared__ int s_pair;
+    const int c = blockIdx.x / 8 + 1, lane = threadIdx.x & 31, dim = a.cache.dim;
+    int64_t share = 0;
+    const int64_t total = find_prompt<8>(a, [&](int64_t n) {
+        share = (n + a.even - 1) / a.even;
+        return share * c;
+    }, false, s_sums, &s_before, &s_pair);
+    const int64_t u = share * c;
+    if (u >= total) return;
+    const int b = s_pair / a.row_tiles, rt = s_pair % a.row_tiles;
+    const Seq s = load_seq(a.seq, b, false);
+    const PrSpan span = prompt_span(a, s, rt);
+    const int h = static_cast<int>((u - s_before) / span.tiles);
+    const int64_t seg0 = s_before + static_cast<int64_t>(h) * span.tiles, seg1 = seg0 + span.tiles;
+    if (u == seg0 || u - share > seg0) return;  // no CTA's share begins inside, or an earlier one's does
+    const int c0 = c - 1, c1 = static_cast<int>((seg1 - 1) / share);
+    for (int r = (blockIdx.x & 7) * 32 + (threadIdx.x >> 5); r < min(span.live, (static_cast<int>(blockIdx.x) & 7) * 32 + 32); r += 8) {
+        // the first CTA's last piece (or its only one), the others' first
+        auto index = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 && share * c0 < seg0 ? 1 : 0)) * kPrRows + r; };
+        float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+        for (int k = c0 + lane; k <= c1; k += 32) {
+            const float4 x = a.stats[index(k)];
+            m = fmaxf(m, x.x);
+            rr = fmaxf(rr, x.z);
+        }
+        m = warp_max(m);
+        rr = warp_max(rr);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = c0; k <= c1; ++k) {
+            const float4 x = a.stats[index(k)];
+            sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
+            const float f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
+            if (4 * lane < dim) {
+                const float4 y = *reinterpret_cast<const float4*>(a.part + index(k) * dim + 4 * lane);
+                o.x += y.x * f;
+                o.y += y.y * f;
+                o.z += y.z * f;
+                o.w += y.w * f;
+            }
+        }
+        const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+        const int row = rt * kPrRows + r;
+        const int64_t tok = s.first + row / a.group;
+        const int head = h * a.group + row % a.group;
+        if (4 * lane < dim) {
+            const int64_t to = tok * a.out_tok + head * a.out_head + 4 * lane;
+            store_out(a, to, o.x * back);
+            store_out(a, to + 1, o.y * back);
+            store_out(a, to + 2, o.z * back);
+            store_out(a, to + 3, o.w * back);
+        }
+        if (lane == 0) {
+            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+            if (a.weights) a.lse2[tok * a.heads + head] = l2;
+        }
+    }
 }
 
 }  // namespace i4d_ops

@@ -238,9 +238,10 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
         const int64_t units = p.segments * ((a.max_length + 15) / 16);
         p.even = static_cast<int>(std::max<int64_t>(1, std::min(places, (units + 7) / 8)));
     }
+    if (p.prompt) p.even = static_cast<int>(std::min<int64_t>(o.num_sms, p.segments * ((a.max_length + kPrTokens - 1) / kPrTokens + 1)));
     if (p.even) {
-        p.part_bytes = static_cast<size_t>(p.even) * 2 * 8 * p.nt * c.dim * sizeof(float);
-        p.stat_bytes = static_cast<size_t>(p.even) * 2 * 8 * p.nt * sizeof(float4);
+        p.part_bytes = static_cast<size_t>(p.even) * 2 * tile * c.dim * sizeof(float);
+        p.stat_bytes = static_cast<size_t>(p.even) * 2 * tile * sizeof(float4);
     }
     if (a.weights) {
         p.lse2_bytes = (static_cast<size_t>(a.tokens) * a.heads * sizeof(float) + 15) / 16 * 16;
@@ -629,7 +630,9 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     if (enc == I4D_OK) enc = encode_codes(ctx, a->cache, a->cache.v, 16, &d.maps[1]);
     if (enc != I4D_OK) return enc;
     OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
-    if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
+    if (p.prompt) {
+        if (p.even > 1) OP_CK(launch_after(k_kv8_prompt_join, static_cast<unsigned>(8 * (p.even - 1)), 256, s, d));
+    } else if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
     if (d.scores) {
         const int chunks = (a->max_length + 255) / 256;
         if (chunks > 0) {
