@@ -218,14 +218,15 @@ __device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
 
 constexpr int kSelectBits = 11;  // 11 + 11 + 10 bits of a key
 constexpr int kSelectBins = 1 << kSelectBits;
+constexpr int kSelectHeld = 8;   // weights that a thread holds in registers
 
 // One cluster for each (sequence, head), whose CTAs take consecutive parts of
-// the weights: the key of the (budget - recent)-th greatest weight in three
-// passes over its digits, each a histogram that the cluster adds up through
-// distributed shared memory, then the kept indices in order (of equal keys the
-// first ones), their weights, and a copy of the scales, which the move
-// overwrites.  Bound: the weights read once from memory (the later passes hit
-// L2), then the chain of barriers.
+// the weights and their threads consecutive weights: the key of the (budget -
+// recent)-th greatest weight in three passes over its digits, each a histogram
+// that the cluster adds up through distributed shared memory, then the kept
+// indices in order (of equal keys the first ones), their weights, and a copy
+// of the scales, which the move overwrites.  Rows of up to 65536 weights are
+// read once into registers.  Bound: the chain of cluster barriers.
 __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int ctas) {
     __shared__ int hist[kSelectBins];
     __shared__ int sums[32];
@@ -246,6 +247,17 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
             for (int i = first; i < len; i += stride) wo[i] = w[i];
         return;
     }
+    // This thread's weights [lo, lo + n).
+    const int per = (len + stride - 1) / stride, lo = min(len, first * per), n = min(len, lo + per) - lo;
+    float held[kSelectHeld];
+#pragma unroll
+    for (int k = 0; k < kSelectHeld; ++k) held[k] = k < n ? w[lo + k] : 0.f;
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < kSelectHeld; ++k)
+            if (k < n) f(lo + k, held[k]);
+        for (int k = kSelectHeld; k < n; ++k) f(lo + k, w[lo + k]);
+    };
     const int nblk = (len + a.cache.block_tokens - 1) / a.cache.block_tokens;
     float* old = a.old_scale + static_cast<int64_t>(row) * 2 * a.old_blocks;
     for (int i = first; i < nblk; i += stride) {
@@ -256,22 +268,23 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
     }
     const int free_len = len - a.recent;
     int want = a.budget - a.recent;  // of the tokens before free_len; want < free_len
-    const int part = (len + ctas - 1) / ctas, lo = min(len, rank * part), hi = min(len, lo + part);
     const bool none = want == 0;
     uint32_t key = 0, high = 0;
     for (int shift = 21; !none; shift = max(0, shift - kSelectBits)) {
         const int bits = shift == 0 ? 10 : kSelectBits;
         for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        for (int i = lo + tid; i < min(hi, free_len); i += kSelectThreads) {
-            const uint32_t k = weight_key(w[i]);
-            if ((k & high) == key) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
-        }
+        each([&](int i, float x) {
+            const uint32_t k = weight_key(x);
+            if (i < free_len && (k & high) == key) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+        });
         cl.sync();
         // the cluster's sum of the two bins from the greatest that are this thread's
         const int bin = kSelectBins - 1 - 2 * tid;
         int n0 = 0, n1 = 0;
-        for (int c = 0; c < ctas; ++c) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c >= ctas) break;
             const int* other = cl.map_shared_rank(hist, c);
             n0 += other[bin];
             n1 += other[bin - 1];
@@ -289,66 +302,57 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
         want -= above;
         if (shift == 0) break;
     }
-    // `want` of the weights equal to key are kept and all above it.  This
-    // CTA's places follow those of the CTAs before it.
-    int same_n = 0, more_n = 0;
-    for (int i = lo + tid; i < hi; i += kSelectThreads) {
-        const uint32_t k = weight_key(w[i]);
-        same_n += i < free_len && !none && k == key;
-        more_n += i >= free_len || (!none && k > key);
-    }
+    // `want` of the weights equal to key are kept and all above it.  A
+    // thread's places follow those of the threads and CTAs before it.
+    int same = 0, more = 0;
+    each([&](int i, float x) {
+        const uint32_t k = weight_key(x);
+        same += i < free_len && !none && k == key;
+        more += i >= free_len || (!none && k > key);
+    });
     int all_same, all_more;
-    cta_scan(same_n, sums, &all_same);
-    __syncthreads();
-    cta_scan(more_n, sums, &all_more);
+    const int same_upto = cta_scan(same, sums, &all_same);
+    const int more_upto = cta_scan(more, sums, &all_more);
     if (tid == 0) {
         counts[0] = all_same;
         counts[1] = all_more;
     }
     cl.sync();
-    int equal = 0, kept = 0;
+    int equal = same_upto - same, larger = more_upto - more;
     for (int c = 0; c < rank; ++c) {
         const int* other = cl.map_shared_rank(counts, c);
-        const int e = other[0];
-        kept += other[1] + min(e, max(0, want - equal));
-        equal += e;
+        equal += other[0];
+        larger += other[1];
     }
-    for (int base = lo; base < hi; base += kSelectThreads) {
-        const int i = base + tid;
-        const bool inside = i < hi, free_tok = i < free_len;
-        const float wi = inside ? w[i] : 0.f;
-        const uint32_t k = weight_key(wi);
-        const bool same = inside && free_tok && !none && k == key;
-        int n_same, n_kept;
-        const int rank_same = equal + cta_scan(same, sums, &n_same);
-        const bool take = inside && (!free_tok || (!none && (k > key || (same && rank_same <= want))));
-        const int place = kept + cta_scan(take, sums, &n_kept);
-        if (take) {
-            keep[place - 1] = i;
-            if (w != wo) wo[place - 1] = wi;
+    int place = larger + min(equal, want);
+    // In place and more than the registers hold: the weights move after the
+    // indices are known (below); otherwise every weight has been read by now.
+    const bool late = w == wo && per > kSelectHeld;
+    each([&](int i, float x) {
+        const uint32_t k = weight_key(x);
+        const bool is_same = i < free_len && !none && k == key;
+        if (i >= free_len || (!none && k > key) || (is_same && equal < want)) {
+            keep[place] = i;
+            if (!late) wo[place] = x;
+            ++place;
         }
-        equal += n_same;
-        kept += n_kept;
-    }
-    if (w != wo) {
-        for (int i = a.budget + first; i < len; i += stride) wo[i] = 0.f;
-        cl.sync();
-        return;
-    }
-    // In place: eight destinations a thread at a time go through registers.
-    cl.sync();  // keep is written; no CTA reads its part of w in the loop above any more
-    for (int base = 0; base < a.budget; base += stride * 8) {
-        float x[8];
+        equal += is_same;
+    });
+    if (late) {
+        cl.sync();  // keep is written; no CTA reads its part of w in the loop above any more
+        for (int base = 0; base < a.budget; base += stride * 8) {
+            float x[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = base + u * stride + first;
-            x[u] = i < a.budget ? __ldcg(w + keep[i]) : 0.f;
-        }
-        cl.sync();  // the sources of this round are read; those of later rounds lie behind its destinations
+            for (int u = 0; u < 8; ++u) {
+                const int i = base + u * stride + first;
+                x[u] = i < a.budget ? __ldcg(w + keep[i]) : 0.f;
+            }
+            cl.sync();  // the sources of this round are read; those of later rounds lie behind its destinations
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = base + u * stride + first;
-            if (i < a.budget) wo[i] = x[u];
+            for (int u = 0; u < 8; ++u) {
+                const int i = base + u * stride + first;
+                if (i < a.budget) wo[i] = x[u];
+            }
         }
     }
     cl.sync();
@@ -357,75 +361,64 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
 
 constexpr int kMoveThreads = 512;
 constexpr int kMoveVecs = 4;  // 16-byte pieces a thread holds
-constexpr int kMoveRound = kMoveThreads / 2 * kMoveVecs;  // destination tokens a round
 
-// Moves the kept tokens up, in place.  One CTA for each (sequence, head, K or
-// V, slice of 32 code bytes) walks its destination tokens in order, kMoveRound
-// at a time: a kept token's index is never below its destination, so a round's
-// destinations are written once its own codes are in registers, and what later
-// rounds read lies behind them; their loads may start before.  Slices are
-// independent because a block's new scale comes from the old scales alone
-// (k_kv8_select copied them); sixteen tokens are a warp's, so a block's
-// greatest scale is joined from the maxima of its warps at the one barrier.
-// Bound: kept codes read and written.
+// Destination tokens of a CTA in a round: whole blocks.
+__host__ __device__ __forceinline__ int move_tokens(int dim) { return kMoveThreads * kMoveVecs / (dim / 16) / 128 * 128; }
+
+// Moves the kept tokens up, in place.  One cluster for each (sequence, head, K
+// or V) walks its destination tokens in order, a round of all its CTAs at a
+// time: a kept token's index is never below its destination, so a round's
+// destinations can be written once all of the round's codes are in registers
+// (the cluster's barrier), and what later rounds read lies behind them.  A
+// block's new scale comes from the old scales, which k_kv8_select copied.
+// Bound: kept codes read and written in whole rows.
 template <int CODE>
-__global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int slices) {
-    __shared__ float warp_scale[2][kMoveVecs * kMoveThreads / 32];
-    const int slice = blockIdx.x % slices, rest = blockIdx.x / slices;
+__global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int ctas) {
+    __shared__ float token_scale[kMoveThreads * kMoveVecs];
+    __shared__ float block_scale[kMoveThreads * kMoveVecs / 16];
+    cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    const int rank = blockIdx.x % ctas, rest = blockIdx.x / ctas;
     const int which = rest & 1, h = (rest >> 1) % a.cache.heads, b = (rest >> 1) / a.cache.heads;
     const int len = evict_length(a, b, false);
-    if (len <= a.budget) return;
-    const int tid = threadIdx.x, bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
+    if (len <= a.budget) return;  // the whole cluster leaves
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
+    const int pieces = dim / 16, tokens = move_tokens(dim);
     const int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.cache.heads + h) * a.budget;
     const float* old = a.old_scale + ((static_cast<int64_t>(b) * a.cache.heads + h) * 2 + which) * a.old_blocks;
     uint8_t* codes = a.cache.codes[which];
-    const int col = slice * 32 + (tid & 1) * 16;
-    int from[kMoveVecs], from_next[kMoveVecs];
-    uint4 x[kMoveVecs], x_next[kMoveVecs];
-    float scale[kMoveVecs], scale_next[kMoveVecs];
-    auto indices = [&](int base, int* f) {
+    for (int base = 0; base < a.budget; base += ctas * tokens) {
+        const int mine = base + rank * tokens, count = min(tokens, a.budget - mine);  // may be negative
+        uint4 x[kMoveVecs];
+        float scale[kMoveVecs];
 #pragma unroll
         for (int u = 0; u < kMoveVecs; ++u) {
-            const int i = base + u * (kMoveThreads / 2) + tid / 2;
-            f[u] = i < a.budget ? __ldg(keep + i) : -1;
-        }
-    };
-    auto pieces = [&](const int* f, uint4* v, float* sc) {
-#pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-            v[u] = make_uint4(0, 0, 0, 0);
-            sc[u] = 0.f;
-            if (f[u] >= 0) {
-                const int id = load_block(a.seq, b, f[u] >> shift, false);
-                sc[u] = __ldg(old + (f[u] >> shift));
-                if (id >= 0 && col < dim)
-                    v[u] = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) +
-                                                                 static_cast<int64_t>(f[u] & (bs - 1)) * dim + col));
+            const int e = u * kMoveThreads + tid, i = e / pieces, c = e - i * pieces;
+            x[u] = make_uint4(0, 0, 0, 0);
+            scale[u] = 0.f;
+            if (i < count) {
+                const int from = __ldg(keep + mine + i);
+                const int id = load_block(a.seq, b, from >> shift, false);
+                scale[u] = __ldg(old + (from >> shift));
+                if (id >= 0)
+                    x[u] = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) + static_cast<int64_t>(from & (bs - 1)) * dim) + c);
             }
+            if (i < tokens && c == 0) token_scale[i] = scale[u];
         }
-    };
-    indices(0, from);
-    pieces(from, x, scale);
-    indices(kMoveRound, from_next);
-    int flip = 0;
-    for (int base = 0; base < a.budget; base += kMoveRound, flip ^= 1) {
-        pieces(from_next, x_next, scale_next);
-        indices(base + 2 * kMoveRound, from);
+        __syncthreads();
+        for (int k = warp; k < tokens >> shift; k += kMoveThreads / 32) {
+            float m = 0.f;
+            for (int i = lane; i < bs; i += 32) m = fmaxf(m, token_scale[(k << shift) + i]);
+            m = warp_max(m);
+            if (lane == 0) block_scale[k] = m;
+        }
+        cl.sync();  // the round's codes are in registers everywhere
 #pragma unroll
         for (int u = 0; u < kMoveVecs; ++u) {
-            const float m = warp_max(scale[u]);
-            if ((tid & 31) == 0) warp_scale[flip][u * (kMoveThreads / 32) + tid / 32] = m;
-        }
-        __syncthreads();  // this round's codes are in registers everywhere, its maxima in place
-#pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-            const int i = base + u * (kMoveThreads / 2) + tid / 2;
-            if (i >= a.budget) continue;
-            const int per = bs / 16, w0 = (u * (kMoveThreads / 32) + tid / 32) / per * per;
-            float now = 0.f;
-            for (int k = 0; k < per; ++k) now = fmaxf(now, warp_scale[flip][w0 + k]);
-            const int to = load_block(a.seq, b, i >> shift, false);
+            const int e = u * kMoveThreads + tid, i = e / pieces, c = e - i * pieces;
+            if (i >= count) continue;
+            const int to = load_block(a.seq, b, (mine + i) >> shift, false);
             if (to < 0) continue;
+            const float now = block_scale[i >> shift];
             uint4 v = x[u];
             if (scale[u] != now) {
                 const float ratio = __fdiv_rn(scale[u], now);
@@ -434,19 +427,11 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int slice
                 v.z = rescale4<CODE>(v.z, ratio);
                 v.w = rescale4<CODE>(v.w, ratio);
             }
-            if (col < dim)
-                *reinterpret_cast<uint4*>(codes + code_offset(a.cache, to, h) + static_cast<int64_t>(i & (bs - 1)) * dim + col) = v;
-            if (slice == 0 && (tid & 1) == 0 && (i & (bs - 1)) == 0)
-                a.cache.scale[which][static_cast<int64_t>(to) * a.cache.heads + h] = now;
+            const int at = (mine + i) & (bs - 1);
+            *(reinterpret_cast<uint4*>(codes + code_offset(a.cache, to, h) + static_cast<int64_t>(at) * dim) + c) = v;
+            if (c == 0 && at == 0) a.cache.scale[which][static_cast<int64_t>(to) * a.cache.heads + h] = now;
         }
-#pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-            x[u] = x_next[u];
-            scale[u] = scale_next[u];
-            const int t = from[u];
-            from[u] = from_next[u];
-            from_next[u] = t;
-        }
+        __syncthreads();  // the scales are used
     }
 }
 

@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t bar_at(const PrShared& sh, int i) { return s
 // False once the wait, or another one of the CTA, has given up.
 __device__ __forceinline__ bool pr_wait(PrShared& sh, int i, uint32_t parity) {
     const uint32_t bar = bar_at(sh, i);
-    for (int n = 0; n < (1 << 18); ++n) {
+    for (int n = 0; n < (1 << 16); ++n) {
         uint32_t ok;
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");

@@ -1,11 +1,13 @@
 // i4d_logits.cuh -- penalties, biases and masks on rows of logits.
 //
-// One cluster of CTAs for a row.  A CTA walks slices of the row: the counts of
-// the history's tokens that fall in the slice are gathered in shared memory
-// with integer atomics (their sum does not depend on the order), the biases
-// beside them, then each logit is read, changed and written once.  The row's
-// best index is joined over the cluster through distributed shared memory, so
-// nothing is kept in global memory between launches.
+// One cluster of CTAs for a row, each with a part of it.  The tokens that the
+// history or the biases touch are few, so a CTA marks them in a bitmap, gives
+// each a place by counting bits, and gathers counts (integer atomics, whose sum
+// does not depend on the order) and biases there.  Then it streams its part,
+// where an untouched logit only meets the mask, and last works out the touched
+// ones, a thread each, so that no warp runs the penalties' division for one
+// lane.  The row's best index is joined over the cluster through distributed
+// shared memory; nothing is kept in global memory between launches.
 // Bound: the logits in and out; for one row the chain of barriers.
 #pragma once
 
@@ -16,7 +18,9 @@
 namespace i4d_ops {
 
 constexpr int kLogitsThreads = 512;
-constexpr int kLogitsSlice = 8192;  // entries: 32 KB of counts and 32 KB of biases
+constexpr int kLogitsTouched = 8192;  // touched tokens that a CTA can hold
+constexpr int kLogitsPart = 65536;    // logits of a part, with no more than that many ids in the lists
+constexpr int kLogitsSmem = kLogitsTouched * (4 + 4 + 2) + kLogitsPart / 32 * (4 + 2);
 
 struct LogitsDev {
     const void* in;
@@ -44,25 +48,45 @@ __device__ __forceinline__ unsigned long long logit_key(float x, int index) {
     return static_cast<unsigned long long>(k) << 32 | (0xffffffffu - index);
 }
 
+// Marks, places and values of the touched tokens of a part.
+struct Touched {
+    int* counts;          // [place] bit 0: in the prompt, above: 2 * occurrences after it
+    float* bias;          // [place]
+    uint32_t* bits;       // [part / 32]
+    uint16_t* ids;        // [place] id - first
+    uint16_t* before;     // [part / 32] places before a word
+    int first, span;      // ids [first, first + span), span <= kLogitsPart
+    __device__ __forceinline__ bool holds(int id) const { return static_cast<unsigned>(id - first) < static_cast<unsigned>(span); }
+    __device__ __forceinline__ int place(int id) const {
+        const int at = id - first;
+        return before[at >> 5] + __popc(bits[at >> 5] & ((1u << (at & 31)) - 1));
+    }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int ctas) {
     extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
-    int* counts = reinterpret_cast<int*>(logits_smem);                  // bit 0: seen in the prompt, above: 2 * occurrences after it
-    float* bias = reinterpret_cast<float*>(counts + kLogitsSlice);
+    Touched t;
+    t.counts = reinterpret_cast<int*>(logits_smem);
+    t.bias = reinterpret_cast<float*>(t.counts + kLogitsTouched);
+    t.bits = reinterpret_cast<uint32_t*>(t.bias + kLogitsTouched);
+    t.ids = reinterpret_cast<uint16_t*>(t.bits + kLogitsPart / 32);
+    t.before = t.ids + kLogitsTouched;
     __shared__ int found[kLogitsThreads / 32];
     __shared__ float2 entries[kLogitsThreads];
     __shared__ unsigned long long keys[kLogitsThreads / 32];
     __shared__ unsigned long long cta_key[16];
     cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
     if (a.best) cl.barrier_arrive();  // the wait stands before the first access to another CTA's memory
-    const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x;
+    const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
     const int32_t* hist = a.history ? a.history + row * a.history_stride : nullptr;
     const int n_hist = hist ? min(max(__ldg(a.history_len + row), 0), a.history_max) : 0;
     const int n_prompt = hist && a.prompt_len ? __ldg(a.prompt_len + row) : 0;
-    const int n_bias = a.bias_ids ? min(max(__ldg(a.bias_len + row), 0), a.bias_max) : 0;
+    const int32_t* bias_ids = a.bias_ids ? a.bias_ids + row * a.bias_stride : nullptr;
+    const int n_bias = bias_ids ? min(max(__ldg(a.bias_len + row), 0), a.bias_max) : 0;
     const float rep = a.repetition ? __ldg(a.repetition + row) : 1.f;
     const float freq = a.frequency ? __ldg(a.frequency + row) : 0.f;
     const float pres = a.presence ? __ldg(a.presence + row) : 0.f;
@@ -74,114 +98,158 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
     const int vecs = (a.vocab + skew + V - 1) / V;
     const int per_cta = (vecs + ctas - 1) / ctas;
     const int v_end = min(vecs, (rank + 1) * per_cta);
+    // More ids than places: parts of so many logits that no more can be touched.
+    const int part = (static_cast<int64_t>(n_hist) + n_bias <= kLogitsTouched ? kLogitsPart : kLogitsTouched) / V;
     unsigned long long key = 0;
-    // A thread's vectors of the next slice are loaded before the counting of
-    // its tokens, which hides the wait for them.
-    constexpr int kVecs = kLogitsSlice / V / kLogitsThreads;
-    for (int v0 = rank * per_cta; v0 < v_end; v0 += kLogitsSlice / V) {
-        const int v1 = min(v_end, v0 + kLogitsSlice / V);
-        const int e0 = v0 * V - skew, span = (v1 - v0) * V;
-        Vec<T, V> x[kVecs];
-        uint2 words[kVecs];
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            const int v = v0 + u * kLogitsThreads + tid, e = v * V - skew;
-            words[u] = make_uint2(~0u, ~0u);
-            if (v >= v1) continue;
-            if (e >= 0 && e + V <= a.vocab) {
-                x[u] = *reinterpret_cast<const Vec<T, V>*>(in + e);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (e + i >= 0 && e + i < a.vocab) x[u].v[i] = in[e + i];
-            }
-            if (mask) words[u] = make_uint2(__ldg(mask + max(e, 0) / 32), __ldg(mask + min(e + V - 1, a.vocab - 1) / 32));
-        }
-        __syncthreads();
-        if (n_hist)
-            for (int i = tid; i < kLogitsSlice / 4; i += kLogitsThreads) reinterpret_cast<int4*>(counts)[i] = make_int4(0, 0, 0, 0);
-        if (n_bias)
-            for (int i = tid; i < kLogitsSlice / 4; i += kLogitsThreads) reinterpret_cast<int4*>(bias)[i] = make_int4(0, 0, 0, 0);
-        __syncthreads();
-#pragma unroll 4
-        for (int i = tid; i < n_hist; i += kLogitsThreads) {
-            const int id = __ldg(hist + i);
-            if (id >= max(e0, 0) && id < a.vocab && id - e0 < span) {
-                if (i < n_prompt) atomicOr(&counts[id - e0], 1);
-                else atomicAdd(&counts[id - e0], 2);
-            }
-        }
-        // Biases: the slice's entries of a round in their order, then the first
-        // of each id adds up the values of that id.
-        for (int i = 0; i < n_bias; i += kLogitsThreads) {
-            const bool live = i + tid < n_bias;
-            const int id = live ? __ldg(a.bias_ids + row * a.bias_stride + i + tid) : -1;
-            const bool mine = live && id >= max(e0, 0) && id < a.vocab && id - e0 < span;
-            const unsigned votes = __ballot_sync(~0u, mine);
-            if ((tid & 31) == 0) found[tid >> 5] = __popc(votes);
+    float best = -INFINITY;  // of this thread's streamed logits, whose ids only grow
+    int best_id = -1;
+    for (int v0 = rank * per_cta; v0 < v_end; v0 += part) {
+        const int v1 = min(v_end, v0 + part);
+        t.first = max(0, v0 * V - skew);
+        t.span = min(a.vocab, v1 * V - skew) - t.first;
+        const int words = (t.span + 31) / 32;
+        int touched = 0;
+        if (n_hist | n_bias) {
             __syncthreads();
-            int at = __popc(votes & ((1u << (tid & 31)) - 1)), total = 0;
+            for (int i = tid; i < words; i += kLogitsThreads) t.bits[i] = 0;
+            __syncthreads();
+#pragma unroll 4
+            for (int i = tid; i < n_hist; i += kLogitsThreads) {
+                const int id = __ldg(hist + i);
+                if (t.holds(id)) atomicOr(&t.bits[(id - t.first) >> 5], 1u << ((id - t.first) & 31));
+            }
+            for (int i = tid; i < n_bias; i += kLogitsThreads) {
+                const int id = __ldg(bias_ids + i);
+                if (t.holds(id)) atomicOr(&t.bits[(id - t.first) >> 5], 1u << ((id - t.first) & 31));
+            }
+            __syncthreads();
+            // places: each thread's words follow those of the threads before it
+            const int per = (words + kLogitsThreads - 1) / kLogitsThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+            int mine = 0;
+            for (int w = w0; w < w1; ++w) mine += __popc(t.bits[w]);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(~0u, upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (lane == 31) found[warp] = upto;
+            __syncthreads();
 #pragma unroll
             for (int w = 0; w < kLogitsThreads / 32; ++w) {
-                at += w < tid >> 5 ? found[w] : 0;
-                total += found[w];
+                if (w < warp) upto += found[w];
+                touched += found[w];
             }
-            if (mine) entries[at] = make_float2(__int_as_float(id - e0), __ldg(a.bias_values + row * a.bias_stride + i + tid));
+            int at = upto - mine;
+            for (int w = w0; w < w1; ++w) {
+                t.before[w] = static_cast<uint16_t>(at);
+                for (uint32_t x = t.bits[w]; x; x &= x - 1) {
+                    t.ids[at] = static_cast<uint16_t>(w * 32 + __ffs(x) - 1);
+                    t.counts[at] = 0;
+                    t.bias[at++] = 0.f;
+                }
+            }
             __syncthreads();
-            if (tid < total) {
-                const int slot = __float_as_int(entries[tid].x);
-                bool leads = true;
-                for (int k = 0; k < tid; ++k) leads &= __float_as_int(entries[k].x) != slot;
-                if (leads) {
-                    float sum = bias[slot];
-                    for (int k = tid; k < total; ++k)
-                        if (__float_as_int(entries[k].x) == slot) sum = __fadd_rn(sum, entries[k].y);
-                    bias[slot] = sum;
+#pragma unroll 4
+            for (int i = tid; i < n_hist; i += kLogitsThreads) {
+                const int id = __ldg(hist + i);
+                if (t.holds(id)) {
+                    if (i < n_prompt) atomicOr(&t.counts[t.place(id)], 1);
+                    else atomicAdd(&t.counts[t.place(id)], 2);
+                }
+            }
+            // Biases: the part's entries of a round in their order, then the
+            // first of each id adds up the values of that id.
+            for (int i = 0; i < n_bias; i += kLogitsThreads) {
+                const int id = i + tid < n_bias ? __ldg(bias_ids + i + tid) : -1;
+                const bool in_part = t.holds(id);
+                const unsigned votes = __ballot_sync(~0u, in_part);
+                __syncthreads();
+                if (lane == 0) found[warp] = __popc(votes);
+                __syncthreads();
+                int to = __popc(votes & ((1u << lane) - 1)), total = 0;
+#pragma unroll
+                for (int w = 0; w < kLogitsThreads / 32; ++w) {
+                    to += w < warp ? found[w] : 0;
+                    total += found[w];
+                }
+                if (in_part) entries[to] = make_float2(__int_as_float(t.place(id)), __ldg(a.bias_values + row * a.bias_stride + i + tid));
+                __syncthreads();
+                if (tid < total) {
+                    const int slot = __float_as_int(entries[tid].x);
+                    bool leads = true;
+                    for (int k = 0; k < tid; ++k) leads &= __float_as_int(entries[k].x) != slot;
+                    if (leads) {
+                        float sum = t.bias[slot];
+                        for (int k = tid; k < total; ++k)
+                            if (__float_as_int(entries[k].x) == slot) sum = __fadd_rn(sum, entries[k].y);
+                        t.bias[slot] = sum;
+                    }
                 }
             }
         }
-        __syncthreads();
+        // The stream: touched logits go out as they came.
+#pragma unroll 2
+        for (int v = v0 + tid; v < v1; v += kLogitsThreads) {
+            const int e = v * V - skew;
+            if (e >= 0 && e + V <= a.vocab) {
+                Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(in + e);
+                uint32_t skip = 0, seen = ~0u;
+                if (touched) {
+                    const int at = e - t.first, w = at >> 5;
+                    skip = __funnelshift_r(t.bits[w], w + 1 < words ? t.bits[w + 1] : 0u, at & 31);
+                }
+                if (mask) seen = __funnelshift_r(__ldg(mask + (e >> 5)), __ldg(mask + ((e + V - 1) >> 5)), e & 31);
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            const int v = v0 + u * kLogitsThreads + tid, e = v * V - skew, at = (v - v0) * V;
-            if (v >= v1) continue;
-            const bool whole = e >= 0 && e + V <= a.vocab;
-#pragma unroll
-            for (int i0 = 0; i0 < V; i0 += 4) {
-                int c[4];
-                float add[4];
-                *reinterpret_cast<int4*>(c) = n_hist ? *reinterpret_cast<const int4*>(counts + at + i0) : make_int4(0, 0, 0, 0);
-                if (n_bias) *reinterpret_cast<float4*>(add) = *reinterpret_cast<const float4*>(bias + at + i0);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i = i0 + k, id = e + i;
-                    if (!whole && (id < 0 || id >= a.vocab)) continue;
-                    float y = to_f32(x[u].v[i]);
-                    if (c[k]) {
-                        const int n = c[k] >> 1;
-                        if (a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                        if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                for (int i = 0; i < V; ++i) {
+                    const float y = to_f32(x.v[i]);
+                    const bool gone = !(seen >> i & 1), raw = skip >> i & 1;
+                    if (gone && !raw) x.v[i] = from_f32<T>(-INFINITY);
+                    if (y > best && !gone && !raw) {
+                        best = y;
+                        best_id = e + i;
                     }
-                    if (n_bias) y = __fadd_rn(y, add[k]);
-                    const uint32_t w = (id >> 5) == (max(e, 0) >> 5) ? words[u].x : words[u].y;
-                    if (!(w >> (id & 31) & 1)) y = -INFINITY;
-                    x[u].v[i] = from_f32<T>(y);
-                    key = max(key, logit_key(to_f32(x[u].v[i]), id));
+                }
+                if (aligned_out) {
+                    *reinterpret_cast<Vec<T, V>*>(out + e) = x;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) out[e + i] = x.v[i];
+                }
+            } else {
+                for (int id = max(e, 0); id < min(e + V, a.vocab); ++id) {
+                    const T x = in[id];
+                    const int at = id - t.first;
+                    const bool raw = touched && (t.bits[at >> 5] >> (at & 31) & 1);
+                    const bool gone = mask && !(__ldg(mask + (id >> 5)) >> (id & 31) & 1);
+                    out[id] = gone && !raw ? from_f32<T>(-INFINITY) : x;
+                    if (to_f32(x) > best && !gone && !raw) {
+                        best = to_f32(x);
+                        best_id = id;
+                    }
                 }
             }
-            if (whole && aligned_out) {
-                *reinterpret_cast<Vec<T, V>*>(out + e) = x[u];
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (e + i >= 0 && e + i < a.vocab) out[e + i] = x[u].v[i];
+        }
+        if (touched) {
+            __syncthreads();  // counts and biases are complete, the touched logits lie in `out`
+            for (int k = tid; k < touched; k += kLogitsThreads) {
+                const int id = t.first + t.ids[k], c = t.counts[k], n = c >> 1;
+                float y = to_f32(out[id]);
+                if (c && a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                y = __fadd_rn(y, t.bias[k]);
+                if (mask && !(__ldg(mask + (id >> 5)) >> (id & 31) & 1)) y = -INFINITY;
+                const T z = from_f32<T>(y);
+                out[id] = z;
+                key = max(key, logit_key(to_f32(z), id));
             }
         }
     }
     if (!a.best) return;
+    key = max(key, logit_key(best, best_id));
 #pragma unroll
     for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(~0u, key, o));
-    if ((tid & 31) == 0) keys[tid >> 5] = key;
+    if (lane == 0) keys[warp] = key;
     __syncthreads();
     cl.barrier_wait();
     if (tid == 0) {

@@ -120,6 +120,23 @@ SeqArrays seq_arrays(const OpContext& o, const i4d_kv8& c, const int32_t* q_star
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
 
+// A kernel in clusters of `ctas` CTAs.
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, int ctas, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // A kernel that waits for the one before it by itself (griddepcontrol.wait
 // first of all), so that its launch overlaps that one's end.
 template <typename... Params, typename... Args>
@@ -359,7 +376,7 @@ i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
 namespace i4d_ops {
 
 cudaError_t ops_init() {
-    const int logits_smem = 2 * kLogitsSlice * 4;
+    const int logits_smem = kLogitsSmem;
     cudaError_t e = cudaFuncSetAttribute(k_logits<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
@@ -683,32 +700,21 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     d.budget = a->budget;
     d.recent = a->recent;
     d.max_length = a->max_length;
-    const int slices = (a->cache.dim + 31) / 32;
     const int64_t rows = static_cast<int64_t>(a->batch) * heads;
-    OP_ARG(rows * 2 * slices <= kMaxGrid, "too many sequences in one call");
+    // CTAs of a row of weights: two thousand or more each; of a moved row: a
+    // round's tokens each; eight at most (the portable cluster size).
+    int ctas = 1, movers = 1;
+    while (ctas < 8 && a->max_length / (2 * ctas) >= 2048) ctas *= 2;
+    while (movers < 8 && a->budget > movers * move_tokens(a->cache.dim)) movers *= 2;
+    OP_ARG(rows * 2 * 8 <= kMaxGrid, "too many sequences in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
-    // CTAs of a row: 4096 weights or more each, eight at most.
-    int ctas = 1;
-    while (ctas < 8 && a->max_length / (2 * ctas) >= 2048) ctas *= 2;
-    OP_ARG(rows * ctas <= kMaxGrid, "too many sequences in one call");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
-    cfg.blockDim = dim3(kSelectThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    OP_CK(cudaLaunchKernelEx(&cfg, k_kv8_select, d, ctas));
+    OP_CK(launch_cluster(k_kv8_select, static_cast<unsigned>(rows * ctas), kSelectThreads, 0, ctas, s, d, ctas));
     if (a->max_length > a->budget) {
-        const unsigned grid = static_cast<unsigned>(rows * 2 * slices);
-        if (a->cache.code == I4D_CODE_INT8) k_kv8_move<I4D_CODE_INT8><<<grid, kMoveThreads, 0, s>>>(d, slices);
-        else k_kv8_move<I4D_CODE_E4M3><<<grid, kMoveThreads, 0, s>>>(d, slices);
-        OP_CK(cudaGetLastError());
+        const unsigned grid = static_cast<unsigned>(rows * 2 * movers);
+        OP_CK(a->cache.code == I4D_CODE_INT8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8>, grid, kMoveThreads, 0, movers, s, d, movers)
+                                             : launch_cluster(k_kv8_move<I4D_CODE_E4M3>, grid, kMoveThreads, 0, movers, s, d, movers));
     }
     return I4D_OK;
 }
@@ -762,21 +768,12 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     OP_ARG(static_cast<int64_t>(a->rows) * ctas <= kMaxGrid, "too many rows in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(a->rows * ctas));
-    cfg.blockDim = dim3(kLogitsThreads);
-    cfg.dynamicSmemBytes = 2 * kLogitsSlice * 4;
-    cfg.stream = stream_of(o, a->stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const unsigned grid = static_cast<unsigned>(a->rows * ctas);
+    const cudaStream_t s = stream_of(o, a->stream);
     switch (a->dtype) {
-        case I4D_F32: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<float>, d, ctas)); break;
-        case I4D_BF16: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<__nv_bfloat16>, d, ctas)); break;
-        default: OP_CK(cudaLaunchKernelEx(&cfg, k_logits<__half>, d, ctas)); break;
+        case I4D_F32: OP_CK(launch_cluster(k_logits<float>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
+        case I4D_BF16: OP_CK(launch_cluster(k_logits<__nv_bfloat16>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
+        default: OP_CK(launch_cluster(k_logits<__half>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
     }
     return I4D_OK;
 }
