@@ -189,7 +189,8 @@ __device__ __forceinline__ int evict_length(const EvictDev& a, int b, bool repor
     return ok ? len : 0;
 }
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
 
 // Inclusive sum over the CTA of one value a thread; *total receives the sum.
 __device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
@@ -203,22 +204,22 @@ __device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
     if (lane == 31) warp_sums[w] = x;
     __syncthreads();
     if (w == 0) {
-        int y = warp_sums[lane];
+        int y = lane < kSelectWarps ? warp_sums[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int z = __shfl_up_sync(~0u, y, o);
             if (lane >= o) y += z;
         }
-        warp_sums[lane] = y;
+        if (lane < kSelectWarps) warp_sums[lane] = y;
     }
     __syncthreads();
-    *total = warp_sums[31];
+    *total = warp_sums[kSelectWarps - 1];
     return x + (w ? warp_sums[w - 1] : 0);
 }
 
 constexpr int kSelectBits = 11;  // 11 + 11 + 10 bits of a key
 constexpr int kSelectBins = 1 << kSelectBits;
-constexpr int kSelectHeld = 8;   // weights that a thread holds in registers
+constexpr int kSelectHeld = 16;  // weights that a thread holds in registers
 
 // One cluster for each (sequence, head), whose CTAs take consecutive parts of
 // the weights and their threads consecutive weights: the key of the (budget -
@@ -227,8 +228,8 @@ constexpr int kSelectHeld = 8;   // weights that a thread holds in registers
 // indices in order (of equal keys the first ones), their weights, and a copy
 // of the scales, which the move overwrites.  Rows of up to 65536 weights are
 // read once into registers.  Bound: the chain of cluster barriers.
-__global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int ctas) {
-    __shared__ int hist[kSelectBins];
+__global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, int ctas) {
+    __shared__ __align__(16) int hist[kSelectBins];
     __shared__ int sums[32];
     __shared__ int chosen, above;
     __shared__ int counts[2];
@@ -258,14 +259,6 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
             if (k < n) f(lo + k, held[k]);
         for (int k = kSelectHeld; k < n; ++k) f(lo + k, w[lo + k]);
     };
-    const int nblk = (len + a.cache.block_tokens - 1) / a.cache.block_tokens;
-    float* old = a.old_scale + static_cast<int64_t>(row) * 2 * a.old_blocks;
-    for (int i = first; i < nblk; i += stride) {
-        const int id = load_block(a.seq, b, i, h == 0);
-        const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
-        old[i] = id < 0 ? 0.f : a.cache.scale[0][at];
-        old[a.old_blocks + i] = id < 0 ? 0.f : a.cache.scale[1][at];
-    }
     const int free_len = len - a.recent;
     int want = a.budget - a.recent;  // of the tokens before free_len; want < free_len
     const bool none = want == 0;
@@ -279,22 +272,32 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
             if (i < free_len && (k & high) == key) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
         });
         cl.sync();
-        // the cluster's sum of the two bins from the greatest that are this thread's
-        const int bin = kSelectBins - 1 - 2 * tid;
-        int n0 = 0, n1 = 0;
+        // the cluster's sums of the four bins from the greatest that are this thread's
+        const int bin = kSelectBins - 4 - 4 * tid;  // bin + 3 is the greatest
+        int4 n4 = make_int4(0, 0, 0, 0);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             if (c >= ctas) break;
-            const int* other = cl.map_shared_rank(hist, c);
-            n0 += other[bin];
-            n1 += other[bin - 1];
+            const int4 x = *reinterpret_cast<const int4*>(cl.map_shared_rank(hist, c) + bin);
+            n4.x += x.x;
+            n4.y += x.y;
+            n4.z += x.z;
+            n4.w += x.w;
         }
+        const int sum = n4.x + n4.y + n4.z + n4.w;
         int total;
-        const int upto = cta_scan(n0 + n1, sums, &total), before = upto - n0 - n1;
+        const int upto = cta_scan(sum, sums, &total), before = upto - sum;
         if (upto >= want && before < want) {
-            const bool second = before + n0 < want;
-            chosen = bin - second;
-            above = before + (second ? n0 : 0);
+            int at = before, k = 3;
+            const int size[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+            for (int i = 3; i > 0; --i)
+                if (k == i && at + size[i] < want) {
+                    at += size[i];
+                    --k;
+                }
+            chosen = bin + k;
+            above = at;
         }
         cl.sync();  // hist is read, chosen is written
         key |= static_cast<uint32_t>(chosen) << shift;
@@ -338,6 +341,14 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
         }
         equal += is_same;
     });
+    const int nblk = (len + a.cache.block_tokens - 1) / a.cache.block_tokens;
+    float* old = a.old_scale + static_cast<int64_t>(row) * 2 * a.old_blocks;
+    for (int i = first; i < nblk; i += stride) {
+        const int id = load_block(a.seq, b, i, h == 0);
+        const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
+        old[i] = id < 0 ? 0.f : a.cache.scale[0][at];
+        old[a.old_blocks + i] = id < 0 ? 0.f : a.cache.scale[1][at];
+    }
     if (late) {
         cl.sync();  // keep is written; no CTA reads its part of w in the loop above any more
         for (int base = 0; base < a.budget; base += stride * 8) {
@@ -360,49 +371,71 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv8_select(EvictDev a, int c
 }
 
 constexpr int kMoveThreads = 512;
-constexpr int kMoveVecs = 4;  // 16-byte pieces a thread holds
 
-// Destination tokens of a CTA in a round: whole blocks.
-__host__ __device__ __forceinline__ int move_tokens(int dim) { return kMoveThreads * kMoveVecs / (dim / 16) / 128 * 128; }
+// 16-byte pieces that a thread holds, and destination tokens of a CTA in a
+// round: whole blocks.
+__host__ __device__ constexpr int move_pieces(int dim) { return dim <= 128 ? 2 : 4; }
+__host__ __device__ constexpr int move_tokens(int dim) { return kMoveThreads * move_pieces(dim) / (dim / 16) / 128 * 128; }
 
 // Moves the kept tokens up, in place.  One cluster for each (sequence, head, K
 // or V) walks its destination tokens in order, a round of all its CTAs at a
 // time: a kept token's index is never below its destination, so a round's
 // destinations can be written once all of the round's codes are in registers
-// (the cluster's barrier), and what later rounds read lies behind them.  A
-// block's new scale comes from the old scales, which k_kv8_select copied.
+// (the cluster's barrier), and what later rounds read lies behind them, so
+// their loads start before.  A block's new scale comes from the old scales,
+// which k_kv8_select copied.
 // Bound: kept codes read and written in whole rows.
-template <int CODE>
-__global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int ctas) {
-    __shared__ float token_scale[kMoveThreads * kMoveVecs];
-    __shared__ float block_scale[kMoveThreads * kMoveVecs / 16];
+template <int CODE, int VECS>
+__global__ void __launch_bounds__(kMoveThreads, 2) k_kv8_move(EvictDev a, int ctas) {
+    __shared__ float token_scale[kMoveThreads * VECS];
+    __shared__ float block_scale[kMoveThreads * VECS / 16];
     cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
     const int rank = blockIdx.x % ctas, rest = blockIdx.x / ctas;
     const int which = rest & 1, h = (rest >> 1) % a.cache.heads, b = (rest >> 1) / a.cache.heads;
     const int len = evict_length(a, b, false);
     if (len <= a.budget) return;  // the whole cluster leaves
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = a.cache.block_tokens, shift = 31 - __clz(bs), dim = a.cache.dim;
-    const int pieces = dim / 16, tokens = move_tokens(dim);
-    const int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.cache.heads + h) * a.budget;
+    const int pieces = dim / 16, tokens = move_tokens(dim), round = ctas * tokens;
+    const int32_t* keep = a.keep + (static_cast<int64_t>(b) * a.cache.heads + h) * a.budget + rank * tokens;
     const float* old = a.old_scale + ((static_cast<int64_t>(b) * a.cache.heads + h) * 2 + which) * a.old_blocks;
     uint8_t* codes = a.cache.codes[which];
-    for (int base = 0; base < a.budget; base += ctas * tokens) {
-        const int mine = base + rank * tokens, count = min(tokens, a.budget - mine);  // may be negative
-        uint4 x[kMoveVecs];
-        float scale[kMoveVecs];
+    int tok[VECS], col[VECS];  // this thread's pieces of a round
 #pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-            const int e = u * kMoveThreads + tid, i = e / pieces, c = e - i * pieces;
-            x[u] = make_uint4(0, 0, 0, 0);
-            scale[u] = 0.f;
-            if (i < count) {
-                const int from = __ldg(keep + mine + i);
-                const int id = load_block(a.seq, b, from >> shift, false);
-                scale[u] = __ldg(old + (from >> shift));
-                if (id >= 0)
-                    x[u] = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) + static_cast<int64_t>(from & (bs - 1)) * dim) + c);
-            }
-            if (i < tokens && c == 0) token_scale[i] = scale[u];
+    for (int u = 0; u < VECS; ++u) {
+        const int e = u * kMoveThreads + tid;
+        tok[u] = e / pieces;
+        col[u] = (e - tok[u] * pieces) * 16;
+        if (tok[u] >= tokens) tok[u] = -1;
+    }
+    // kept index of a piece's token (-1: none), its code's place, its scale
+    auto kept = [&](int base, int u) { return tok[u] >= 0 && base + rank * tokens + tok[u] < a.budget ? __ldg(keep + base + tok[u]) : -1; };
+    auto piece = [&](int from, int u, float& scale) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        scale = 0.f;
+        if (from >= 0) {
+            const int id = load_block(a.seq, b, from >> shift, false);
+            scale = __ldg(old + (from >> shift));
+            if (id >= 0) x = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) + static_cast<int64_t>(from & (bs - 1)) * dim + col[u]));
+        }
+        return x;
+    };
+    uint4 x[VECS];
+    float scale[VECS];
+    int next[VECS];
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+        x[u] = piece(kept(0, u), u, scale[u]);
+        next[u] = kept(round, u);
+    }
+    for (int base = 0; base < a.budget; base += round) {
+        const int mine = base + rank * tokens;
+        uint4 ahead[VECS];
+        float ahead_scale[VECS];
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) {
+            ahead[u] = piece(next[u], u, ahead_scale[u]);
+            next[u] = kept(base + 2 * round, u);
+            if (tok[u] >= 0 && col[u] == 0) token_scale[tok[u]] = scale[u];
         }
         __syncthreads();
         for (int k = warp; k < tokens >> shift; k += kMoveThreads / 32) {
@@ -413,23 +446,25 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv8_move(EvictDev a, int ctas)
         }
         cl.sync();  // the round's codes are in registers everywhere
 #pragma unroll
-        for (int u = 0; u < kMoveVecs; ++u) {
-            const int e = u * kMoveThreads + tid, i = e / pieces, c = e - i * pieces;
-            if (i >= count) continue;
-            const int to = load_block(a.seq, b, (mine + i) >> shift, false);
-            if (to < 0) continue;
-            const float now = block_scale[i >> shift];
-            uint4 v = x[u];
-            if (scale[u] != now) {
-                const float ratio = __fdiv_rn(scale[u], now);
-                v.x = rescale4<CODE>(v.x, ratio);
-                v.y = rescale4<CODE>(v.y, ratio);
-                v.z = rescale4<CODE>(v.z, ratio);
-                v.w = rescale4<CODE>(v.w, ratio);
+        for (int u = 0; u < VECS; ++u) {
+            if (tok[u] >= 0 && mine + tok[u] < a.budget) {
+                const int to = load_block(a.seq, b, (mine + tok[u]) >> shift, false), at = (mine + tok[u]) & (bs - 1);
+                if (to >= 0) {
+                    const float now = block_scale[tok[u] >> shift];
+                    uint4 v = x[u];
+                    if (scale[u] != now) {
+                        const float ratio = __fdiv_rn(scale[u], now);
+                        v.x = rescale4<CODE>(v.x, ratio);
+                        v.y = rescale4<CODE>(v.y, ratio);
+                        v.z = rescale4<CODE>(v.z, ratio);
+                        v.w = rescale4<CODE>(v.w, ratio);
+                    }
+                    *reinterpret_cast<uint4*>(codes + code_offset(a.cache, to, h) + static_cast<int64_t>(at) * dim + col[u]) = v;
+                    if (col[u] == 0 && at == 0) a.cache.scale[which][static_cast<int64_t>(to) * a.cache.heads + h] = now;
+                }
             }
-            const int at = (mine + i) & (bs - 1);
-            *(reinterpret_cast<uint4*>(codes + code_offset(a.cache, to, h) + static_cast<int64_t>(at) * dim) + c) = v;
-            if (c == 0 && at == 0) a.cache.scale[which][static_cast<int64_t>(to) * a.cache.heads + h] = now;
+            x[u] = ahead[u];
+            scale[u] = ahead_scale[u];
         }
         __syncthreads();  // the scales are used
     }

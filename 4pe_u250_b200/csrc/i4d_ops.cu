@@ -713,8 +713,13 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     OP_CK(launch_cluster(k_kv8_select, static_cast<unsigned>(rows * ctas), kSelectThreads, 0, ctas, s, d, ctas));
     if (a->max_length > a->budget) {
         const unsigned grid = static_cast<unsigned>(rows * 2 * movers);
-        OP_CK(a->cache.code == I4D_CODE_INT8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8>, grid, kMoveThreads, 0, movers, s, d, movers)
-                                             : launch_cluster(k_kv8_move<I4D_CODE_E4M3>, grid, kMoveThreads, 0, movers, s, d, movers));
+        const bool int8 = a->cache.code == I4D_CODE_INT8;
+        if (move_pieces(a->cache.dim) == 2)
+            OP_CK(int8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8, 2>, grid, kMoveThreads, 0, movers, s, d, movers)
+                       : launch_cluster(k_kv8_move<I4D_CODE_E4M3, 2>, grid, kMoveThreads, 0, movers, s, d, movers));
+        else
+            OP_CK(int8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8, 4>, grid, kMoveThreads, 0, movers, s, d, movers)
+                       : launch_cluster(k_kv8_move<I4D_CODE_E4M3, 4>, grid, kMoveThreads, 0, movers, s, d, movers));
     }
     return I4D_OK;
 }
