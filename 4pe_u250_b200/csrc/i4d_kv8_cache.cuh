@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_kv8_append(Ap
     if (tid == 0) *scale = now;  // every thread has read `had` (the barrier above, or the shuffles)
     uint8_t* codes = a.cache.codes[which] + code_offset(a.cache, id, h);
     if (old && now > had) {
-        const float ratio = __fdiv_rn(had, now);
+        const Rescale ratio = make_rescale(__fdiv_rn(had, now));
         uint2* p = reinterpret_cast<uint2*>(codes);
         for (int i = tid; i < old * per_tok; i += THREADS) {
             uint2 w = p[i];
@@ -374,7 +374,7 @@ constexpr int kMoveThreads = 512;
 
 // 16-byte pieces that a thread holds, and destination tokens of a CTA in a
 // round: whole blocks.
-__host__ __device__ constexpr int move_pieces(int dim) { return dim <= 128 ? 2 : 4; }
+__host__ __device__ constexpr int move_pieces(int) { return 4; }
 __host__ __device__ constexpr int move_tokens(int dim) { return kMoveThreads * move_pieces(dim) / (dim / 16) / 128 * 128; }
 
 // Moves the kept tokens up, in place.  One cluster for each (sequence, head, K
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) k_kv8_move(EvictDev a, int ct
                     const float now = block_scale[tok[u] >> shift];
                     uint4 v = x[u];
                     if (scale[u] != now) {
-                        const float ratio = __fdiv_rn(scale[u], now);
+                        const Rescale ratio = make_rescale(__fdiv_rn(scale[u], now));
                         v.x = rescale4<CODE>(v.x, ratio);
                         v.y = rescale4<CODE>(v.y, ratio);
                         v.z = rescale4<CODE>(v.z, ratio);

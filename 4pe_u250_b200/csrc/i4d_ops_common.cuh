@@ -157,11 +157,40 @@ __device__ __forceinline__ void decode4(uint32_t w, float out[4]) {
     }
 }
 
+// round(code * ratio) of a word's codes, 0 <= ratio <= 1.  Powers of two down to
+// 2^-14 keep every product exact in FP16, where an INT8 code is rounded by the
+// sum with 1536 (whose steps are 1): a third of the instructions of FP32.
+struct Rescale {
+    float ratio;
+    __half2 half;
+    bool fast;
+};
+__device__ __forceinline__ Rescale make_rescale(float r) { return {r, __float2half2_rn(r), (__float_as_int(r) & 0x7fffff) == 0 && r >= 0x1p-14f}; }
+
 template <int CODE>
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, const Rescale& r) {
+    if (r.fast) {
+        if constexpr (CODE == I4D_CODE_INT8) {
+            const uint32_t x = w ^ 0x80808080u, m0 = __byte_perm(x, 0x64646464u, 0x4140), m1 = __byte_perm(x, 0x64646464u, 0x4342);
+            const __half2 bias = __half2half2(__ushort_as_half(0x6480)), whole = __half2half2(__ushort_as_half(0x6600));
+            const __half2 h0 = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&m0), bias), r.half, whole);
+            const __half2 h1 = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&m1), bias), r.half, whole);
+            return __byte_perm(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1), 0x6420);
+        } else {
+            uint32_t h[2];
+            uint16_t e[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[i]) : "h"(static_cast<uint16_t>(w >> (16 * i))));
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), r.half);
+                asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(e[i]) : "r"(*reinterpret_cast<const uint32_t*>(&y)));
+            }
+            return e[0] | static_cast<uint32_t>(e[1]) << 16;
+        }
+    }
     float f[4];
     decode4<CODE>(w, f);
-    return encode4<CODE>(__fmul_rn(f[0], ratio), __fmul_rn(f[1], ratio), __fmul_rn(f[2], ratio), __fmul_rn(f[3], ratio));
+    return encode4<CODE>(__fmul_rn(f[0], r.ratio), __fmul_rn(f[1], r.ratio), __fmul_rn(f[2], r.ratio), __fmul_rn(f[3], r.ratio));
 }
 
 __device__ __forceinline__ float warp_max(float x) {
