@@ -52,7 +52,8 @@ struct AttnDev {
     int heads, group, window, dtype, max_length, wide_q, wide_out;
     float scale_log2;  // softmax scale * log2(e)
     int batch, row_tiles;  // row tiles of a (sequence, cache head), at most
-    int even;              // CTAs that share the tokens evenly, or 0: one for each (sequence, cache head, row tile)
+    int even;              // CTAs that share the tokens evenly, or 0: a cluster for each (sequence, cache head, row tile)
+    int cluster;           // its CTAs, which share the segment's tokens and join through distributed shared memory
     float* part;       // workspace: [even][2][rows][dim]: O of a CTA's pieces that are not whole
     float4* stats;     // workspace: [even][2][rows]: M, l, R
     float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
@@ -449,21 +450,23 @@ struct Place {
     int seq;
 };
 
-// Units of the whole batch and, in *at, the sequence in which unit u lies (or
-// those before sequence `want`, u < 0).  The CTA's threads take consecutive
-// sequences each.
-__device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_tile, int64_t u, int want, bool report, Place* at) {
+// Units of the whole batch and, in *at, the sequence in which unit u(total)
+// lies (or those before sequence `want`, u < 0).  The CTA's threads take
+// consecutive sequences each.
+template <typename U>
+__device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_tile, U&& unit, int want, bool report, Place* at) {
     __shared__ int64_t s_sum[kAttnWarps];
     __shared__ Place s_place;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (a.batch + kAttnThreads - 1) / kAttnThreads, b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Seq s = load_seq(a.seq, b, report);
-        if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
+    auto size = [&](int b, bool tell) {
+        const Seq s = load_seq(a.seq, b, tell);
+        if (tell && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
         const Units n = seq_units(a, s, rows_per_tile);
-        mine += static_cast<int64_t>(n.tiles) * n.segments;
-    }
+        return static_cast<int64_t>(n.tiles) * n.segments;
+    };
+    int64_t mine = 0, last = 0;
+    for (int b = b0; b < b1; ++b) mine += last = size(b, report);
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -478,11 +481,11 @@ __device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_til
         if (w < warp) upto += s_sum[w];
         total += s_sum[w];
     }
+    const int64_t u = unit(total);
     int64_t before = upto - mine;
     if (u >= 0 ? u >= before && u < upto : want >= b0 && want < b1) {
         for (int b = b0; b < b1; ++b) {
-            const Units n = seq_units(a, load_seq(a.seq, b, false), rows_per_tile);
-            const int64_t next = before + static_cast<int64_t>(n.tiles) * n.segments;
+            const int64_t next = before + (b1 - b0 == 1 ? last : size(b, false));
             if (u >= 0 ? u < next : b == want) {
                 s_place = {before, b};
                 break;
@@ -500,9 +503,26 @@ __device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_til
 struct Piece {
     int b, h, rt;
     int begin, end;  // tokens, begin a multiple of 16
-    bool whole;      // the segment's only piece
+    bool whole;      // the segment's only piece (of the cluster, if there is one)
     int slot;        // where its partial sums go otherwise: 0 the CTA's first piece, 1 its last
 };
+
+// Four values of a finished row from dim d on.
+__device__ __forceinline__ void store_row(const AttnDev& a, const Seq& s, int h, int row, int d, float4 o) {
+    const int64_t at = (s.first + row / a.group) * a.out_tok + (h * a.group + row % a.group) * a.out_head + d;
+    store_out(a, at, o.x);
+    store_out(a, at + 1, o.y);
+    store_out(a, at + 2, o.z);
+    store_out(a, at + 3, o.w);
+}
+
+// stats: M, l of a finished row.
+__device__ __forceinline__ void store_lse(const AttnDev& a, const Seq& s, int h, int row, float4 stats) {
+    const int64_t at = (s.first + row / a.group) * static_cast<int64_t>(a.heads) + h * a.group + row % a.group;
+    const float l2 = stats.y == 0.f ? -INFINITY : stats.x + log2f(stats.y);
+    if (a.lse) a.lse[at] = l2 * kLn2;
+    if (a.weights) a.lse2[at] = l2;
+}
 
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
@@ -704,19 +724,15 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w)  // (a warp that saw nothing of the row: its sums are 0, or NaN with the row's)
             sum += merge[w][r][DT + 1] * (merge[w][r][DT] == -INFINITY ? 1.f : ex2(merge[w][r][DT] - m));
-        const float back = !pc.whole ? 1.f : sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+        const bool done = pc.whole && a.cluster <= 1;
+        const float back = !done ? 1.f : sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w)
             merge[w][r][DT + 3] = (merge[w][r][DT + 2] == -INFINITY ? 1.f : ex2(merge[w][r][DT + 2] - rr)) * back;
-        if (pc.whole) {
-            const int64_t tok = s.first + row / a.group;
-            const int head = h * a.group + row % a.group;
-            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-            if (a.weights) a.lse2[tok * a.heads + head] = l2;
-        } else {
-            a.stats[(static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r] = make_float4(m, sum, rr, 0.f);
-        }
+        const float4 stats = make_float4(m, sum, rr, 0.f);
+        if (done) store_lse(a, s, h, row, stats);
+        else if (pc.whole) s_block[r] = stats;
+        else a.stats[(static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r] = stats;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (DT / 4); i += kAttnThreads) {
@@ -732,15 +748,43 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
             o.z += x.z * f;
             o.w += x.w * f;
         }
-        if (pc.whole) {
-            const int64_t at = (s.first + row / a.group) * a.out_tok + (h * a.group + row % a.group) * a.out_head + d;
-            store_out(a, at, o.x);
-            store_out(a, at + 1, o.y);
-            store_out(a, at + 2, o.z);
-            store_out(a, at + 3, o.w);
-        } else {
-            *reinterpret_cast<float4*>(a.part + ((static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r) * dim + d) = o;
+        if (!pc.whole) *reinterpret_cast<float4*>(a.part + ((static_cast<int64_t>(blockIdx.x) * 2 + pc.slot) * kRows + r) * dim + d) = o;
+        else if (a.cluster > 1) *reinterpret_cast<float4*>(&merge[0][r][d]) = o;  // (only this thread reads it above)
+        else store_row(a, s, h, row, d, o);
+    }
+    if (pc.whole && a.cluster > 1) {
+        cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+        const int ctas = a.cluster, rank = blockIdx.x % ctas;
+        cl.sync();
+        for (int i = rank * kAttnThreads + threadIdx.x; i < rows * (DT / 4); i += ctas * kAttnThreads) {
+            const int r = i / (DT / 4), d = i % (DT / 4) * 4, row = row0 + r;
+            float4 stats[8];
+            float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                stats[c] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+                if (c < ctas) stats[c] = cl.map_shared_rank(s_block, c)[r];
+                m = fmaxf(m, stats[c].x);
+                rr = fmaxf(rr, stats[c].z);
+            }
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c >= ctas) break;
+                sum += stats[c].y * (stats[c].x == -INFINITY ? 1.f : ex2(stats[c].x - m));
+                if (d >= dim) continue;
+                const float4 x = *reinterpret_cast<const float4*>(&cl.map_shared_rank(&merge[0][0][0], c)[r * (DT + 4) + d]);
+                const float f = stats[c].z == -INFINITY ? 1.f : ex2(stats[c].z - rr);
+                o.x += x.x * f;
+                o.y += x.y * f;
+                o.z += x.z * f;
+                o.w += x.w * f;
+            }
+            const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+            if (d < dim) store_row(a, s, h, row, d, make_float4(o.x * back, o.y * back, o.z * back, o.w * back));
+            if (d == 0) store_lse(a, s, h, row, make_float4(m, sum, rr, 0.f));
         }
+        cl.sync();  // no CTA leaves while another reads its memory
     }
 }
 
@@ -757,21 +801,26 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
     __syncthreads();
     __shared__ float4 s_block[kAttnBlocks];  // id, scale of K, of V, log2 of the latter
     if (!a.even) {
-        const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.cache.heads, b = blockIdx.x / a.row_tiles / a.cache.heads;
-        const bool report = rt == 0 && h == 0 && threadIdx.x == 0;
+        const int segment = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;
+        const int rt = segment % a.row_tiles, h = segment / a.row_tiles % a.cache.heads, b = segment / a.row_tiles / a.cache.heads;
+        const bool report = rt == 0 && h == 0 && rank == 0 && threadIdx.x == 0;
         const Seq s = load_seq(a.seq, b, report);
         if (report && s.len > a.max_length) atomicOr(a.seq.err, kBadSequence);
-        if (s.len > a.max_length || rt * kRows >= s.n * a.group) return;
-        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, 0, s.len, true, 0}, attn_ring, s_block, s_bar, phases);
+        if (s.len > a.max_length || rt * kRows >= s.n * a.group) return;  // the whole cluster
+        const int first = s.len - s.n, lo = row_span(a, first + rt * kRows / a.group).x & ~15;
+        const int share = ((s.len - lo + 15) / 16 + a.cluster - 1) / a.cluster * 16;
+        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, lo + rank * share, min(s.len, lo + (rank + 1) * share), true, 0}, attn_ring, s_block, s_bar, phases);
         return;
     }
     Place at;
-    const bool report = blockIdx.x == 0;
-    const int64_t total = find_units(a, kRows, 0, 0, report, &at), share = (total + a.even - 1) / a.even;
-    int64_t u = static_cast<int64_t>(blockIdx.x) * share;
+    int64_t share = 0;
+    const int64_t total = find_units(a, kRows, [&](int64_t n) {
+        share = (n + a.even - 1) / a.even;
+        return share * blockIdx.x;
+    }, 0, blockIdx.x == 0, &at);
+    int64_t u = share * blockIdx.x;
     const int64_t u_end = min(total, u + share), u0 = u;
     if (u >= u_end) return;
-    find_units(a, kRows, u, 0, false, &at);
     while (u < u_end) {
         const Seq s = load_seq(a.seq, at.seq, false);
         const Units n = seq_units(a, s, kRows);
@@ -806,7 +855,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
     const int row_tiles = n.segments / a.cache.heads;
     if (rt >= row_tiles) return;
     Place at;
-    const int64_t total = find_units(a, rows_per_tile, -1, b, false, &at), share = (total + a.even - 1) / a.even;
+    const int64_t total = find_units(a, rows_per_tile, [](int64_t) { return int64_t{-1}; }, b, false, &at), share = (total + a.even - 1) / a.even;
     const int64_t seg0 = at.before + (static_cast<int64_t>(h) * row_tiles + rt) * n.tiles, seg1 = seg0 + n.tiles;
     const int c0 = static_cast<int>(seg0 / share), c1 = static_cast<int>((seg1 - 1) / share);
     if (c0 == c1) return;  // whole
@@ -866,11 +915,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
             store_out(a, to + 2, o[k].z * back);
             store_out(a, to + 3, o[k].w * back);
         }
-        if (lane == 0) {
-            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-            if (a.weights) a.lse2[tok * a.heads + head] = l2;
-        }
+        if (lane == 0) store_lse(a, s, h, row, make_float4(m, sum, rr, 0.f));
     }
 }
 

@@ -232,6 +232,7 @@ struct AttnPlan {
     int row_tiles;
     int64_t segments;  // (sequence, cache head, row tile)
     int even;          // CTAs that share the tokens, or 0
+    int cluster;       // else the CTAs of a segment, 1 to 8
     bool prompt;       // k_kv8_prompt: row tiles of kPrRows
     size_t part_bytes, stat_bytes, lse2_bytes, score_bytes;
     size_t bytes() const { return part_bytes + stat_bytes + lse2_bytes + score_bytes; }
@@ -247,13 +248,21 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     const int tile = p.prompt ? kPrRows : 8 * p.nt;
     p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
     p.segments = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
-    // Few rows: the CTAs that fit the GPU share the tokens evenly, whatever
-    // the lengths are (lengths are known on the device only), but no more of
-    // them than have two tiles a warp.  Many rows are work enough by themselves.
+    // Few segments of moderate length: as many CTAs of a cluster for each as
+    // fit the GPU at once, which need no second kernel (one stream of 2047
+    // tokens, 32 heads: 20.5 us through partial sums in memory, 13 so).  Long
+    // ones: the CTAs that fit the GPU share all tokens evenly, whatever the
+    // lengths are (which the device alone knows), but no more of them than have
+    // two tiles a warp.  Many rows are work enough by themselves.
     const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 4) * static_cast<int64_t>(o.num_sms);
+    p.cluster = 1;
     if (!p.prompt && p.row_tiles <= 4) {
-        const int64_t units = p.segments * ((a.max_length + 15) / 16);
-        p.even = static_cast<int>(std::max<int64_t>(1, std::min(places, (units + 7) / 8)));
+        while (p.cluster < 8 && p.segments * p.cluster * 2 <= places && a.max_length > 128 * p.cluster) p.cluster *= 2;
+        if (p.segments > places || a.max_length > 1024 * p.cluster) {
+            const int64_t units = p.segments * ((a.max_length + 15) / 16);
+            p.even = static_cast<int>(std::max<int64_t>(1, std::min(places, (units + 7) / 8)));
+            p.cluster = 1;
+        }
     }
     if (p.prompt) p.even = static_cast<int>(std::min<int64_t>(o.num_sms, p.segments * ((a.max_length + kPrTokens - 1) / kPrTokens + 1)));
     if (p.even) {
@@ -289,8 +298,7 @@ i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 cudaError_t launch_attn(const AttnDev& d, int64_t grid, cudaStream_t st) {
     static_assert(attn_smem<DT, NT>() <= 114688, "two CTAs an SM");
-    k_kv8_attn<DT, CODE, NT, HLQ, HLP><<<static_cast<unsigned>(grid), kAttnThreads, attn_smem<DT, NT>(), st>>>(d);
-    return cudaGetLastError();
+    return launch_cluster(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, static_cast<unsigned>(grid), kAttnThreads, attn_smem<DT, NT>(), d.cluster, st, d);
 }
 
 template <int DT, int CODE>
@@ -628,6 +636,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.batch = a->batch;
     d.row_tiles = p.row_tiles;
     d.even = p.even;
+    d.cluster = p.cluster;
     d.part = static_cast<float*>(a->workspace);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     d.stats = reinterpret_cast<float4*>(ws + p.part_bytes);
@@ -635,10 +644,10 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.lse2_bytes);
     d.wide_out = aligned(a->out, 16) && a->out_stride * bytes % 16 == 0 && a->out_head_stride * bytes % 16 == 0;
     d.wide_q = aligned(a->q, 16) && a->q_stride * bytes % 16 == 0 && a->q_head_stride * bytes % 16 == 0;
-    const int64_t grid = p.even ? p.even : p.segments;
+    const int64_t grid = p.even ? p.even : p.segments * p.cluster;
     const int wtiles = (a->max_length + 16 * kAttnWarps - 1) / (16 * kAttnWarps);
     const int64_t wgrid = static_cast<int64_t>(a->batch) * a->cache.heads * wtiles;
-    OP_ARG(p.segments <= kMaxGrid && wgrid <= kMaxGrid, "too many rows in one call");
+    OP_ARG(p.segments * 8 <= kMaxGrid && wgrid <= kMaxGrid, "too many rows in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
