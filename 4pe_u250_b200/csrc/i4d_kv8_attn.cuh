@@ -57,7 +57,9 @@ struct AttnDev {
     float* part;       // workspace: [even][2][rows][dim]: O of a CTA's pieces that are not whole
     float4* stats;     // workspace: [even][2][rows]: M, l, R
     float* lse2;       // workspace: [tokens][heads], log2 of the softmax sum (with weights)
-    float* scores;     // workspace (few rows, with weights): [tile][rows][max_length], log2 scale
+    int4* segments;    // workspace: [segment]: first and last CTA of its pieces, slot of the first
+    float* scores;     // workspace (few rows, with weights): [segment][rows][score_stride], log2 scale
+    int64_t score_stride;  // a multiple of 4
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -451,10 +453,9 @@ struct Place {
 };
 
 // Units of the whole batch and, in *at, the sequence in which unit u(total)
-// lies (or those before sequence `want`, u < 0).  The CTA's threads take
-// consecutive sequences each.
+// lies.  The CTA's threads take consecutive sequences each.
 template <typename U>
-__device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_tile, U&& unit, int want, bool report, Place* at) {
+__device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_tile, U&& unit, bool report, Place* at) {
     __shared__ int64_t s_sum[kAttnWarps];
     __shared__ Place s_place;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -483,10 +484,10 @@ __device__ __forceinline__ int64_t find_units(const AttnDev& a, int rows_per_til
     }
     const int64_t u = unit(total);
     int64_t before = upto - mine;
-    if (u >= 0 ? u >= before && u < upto : want >= b0 && want < b1) {
+    if (u >= before && u < upto) {
         for (int b = b0; b < b1; ++b) {
             const int64_t next = before + (b1 - b0 == 1 ? last : size(b, false));
-            if (u >= 0 ? u < next : b == want) {
+            if (u < next) {
                 s_place = {before, b};
                 break;
             }
@@ -598,9 +599,9 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 slot = slot == kSlots - 1 ? 0 : slot + 1;
                 const int at = from_tok + 16 * i;
                 const float4 block = s_block[(at >> shift) - blk0];
-                if (__float_as_int(block.x) < 0) continue;
                 const float lvs = block.w;
-                const int live = min(16, to_tok - at);
+                const int live = __float_as_int(block.x) < 0 ? 0 : min(16, to_tok - at);
+                if (live == 0 && !a.scores) continue;  // (the kept scores of a bad block are -inf)
                 float x[NT][4];
                 {
                     KTile<DT> kt;
@@ -659,7 +660,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int r = nt * 8 + 2 * t + (k & 1), n = g + (k >> 1) * 8;
-                            if (n < live && row0 + r <= last_row) a.scores[(tile * kRows + r) * a.max_length + at + n] = x[nt][k];
+                            if (at + n < to_tok && row0 + r <= last_row) a.scores[(tile * kRows + r) * a.score_stride + at + n] = x[nt][k];
                         }
                 }
                 uint32_t p[NT][2], pl[NT][2];
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
     const int64_t total = find_units(a, kRows, [&](int64_t n) {
         share = (n + a.even - 1) / a.even;
         return share * blockIdx.x;
-    }, 0, blockIdx.x == 0, &at);
+    }, blockIdx.x == 0, &at);
     int64_t u = share * blockIdx.x;
     const int64_t u_end = min(total, u + share), u0 = u;
     if (u >= u_end) return;
@@ -834,6 +835,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
         const int64_t seg0 = at.before + static_cast<int64_t>(seg) * n.tiles;
         const int t0 = static_cast<int>(u - seg0), t1 = static_cast<int>(min(static_cast<int64_t>(n.tiles), u_end - seg0));
         const int lo = row_span(a, s.len - s.n).x & ~15;
+        if (t0 == 0 && threadIdx.x == 0)
+            a.segments[(static_cast<int64_t>(at.seq) * a.cache.heads + seg / row_tiles) * a.row_tiles + seg % row_tiles] =
+                make_int4(blockIdx.x, static_cast<int>((seg0 + n.tiles - 1) / share), u == u0 ? 0 : 1, 0);
         if (u != u0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the join wrote where the next copies go
             __syncthreads();
@@ -854,15 +858,13 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
     const Units n = seq_units(a, s, rows_per_tile);
     const int row_tiles = n.segments / a.cache.heads;
     if (rt >= row_tiles) return;
-    Place at;
-    const int64_t total = find_units(a, rows_per_tile, [](int64_t) { return int64_t{-1}; }, b, false, &at), share = (total + a.even - 1) / a.even;
-    const int64_t seg0 = at.before + (static_cast<int64_t>(h) * row_tiles + rt) * n.tiles, seg1 = seg0 + n.tiles;
-    const int c0 = static_cast<int>(seg0 / share), c1 = static_cast<int>((seg1 - 1) / share);
+    const int4 segment = a.segments[blockIdx.x];
+    const int c0 = segment.x, c1 = segment.y;
     if (c0 == c1) return;  // whole
     const int rows = min(rows_per_tile, s.n * a.group - rt * rows_per_tile);
     for (int r = threadIdx.x >> 5; r < rows; r += kAttnWarps) {
-        // piece c: a CTA's first one unless the CTA began in an earlier segment
-        auto index = [&](int c) { return (static_cast<int64_t>(c) * 2 + (static_cast<int64_t>(c) * share < seg0 ? 1 : 0)) * rows_per_tile + r; };
+        // the first CTA's piece may be its last, those of the others are their first
+        auto index = [&](int c) { return (static_cast<int64_t>(c) * 2 + (c == c0 ? segment.z : 0)) * rows_per_tile + r; };
         float m = -INFINITY, rr = -INFINITY, sum = 0.f;
         for (int c = c0 + lane; c <= c1; c += 32) {
             const float4 x = a.stats[index(c)];
@@ -920,24 +922,32 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
 }
 
 // Probabilities summed over a head's few rows for each token, from the scores
-// that k_kv8_attn kept: one thread for a token, rows in order.
-__global__ void __launch_bounds__(256) k_kv8_weights_kept(AttnDev a, int rows_per_tile, int chunks) {
+// that k_kv8_attn kept: four tokens a thread, rows in order.
+__global__ void __launch_bounds__(128) k_kv8_weights_kept(AttnDev a, int rows_per_tile, int chunks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t bh = blockIdx.x / chunks;
-    const int n = (blockIdx.x % chunks) * 256 + threadIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
+    const int n = ((blockIdx.x % chunks) * 128 + threadIdx.x) * 4, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const Seq s = load_seq(a.seq, b, false);
     if (s.len > a.max_length || s.n == 0 || n >= s.len) return;
-    if (load_block(a.seq, b, n / a.cache.block_tokens, false) < 0) return;
     const int rows = s.n * a.group, first = s.len - s.n;
-    float sum = 0.f;
+    float* to = a.weights + bh * a.weights_stride + n;
+    float w[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = n + i < s.len ? to[i] : 0.f;
+#pragma unroll 4
     for (int row = 0; row < rows; ++row) {
         const int2 sp = row_span(a, first + row / a.group);
-        if (n < sp.x || n >= sp.y) continue;  // not written
         const int64_t at = (bh * a.row_tiles + row / rows_per_tile) * rows_per_tile + row % rows_per_tile;
         const float l2 = a.lse2[(s.first + row / a.group) * static_cast<int64_t>(a.heads) + h * a.group + row % a.group];
-        sum += ex2(a.scores[at * a.max_length + n] - l2);
+        const float4 x = *reinterpret_cast<const float4*>(a.scores + at * a.score_stride + n);
+        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (scores outside the row's span may not have been written)
+            sum[i] += n + i >= sp.x && n + i < sp.y ? ex2(y[i] - l2) : 0.f;
     }
-    a.weights[bh * a.weights_stride + n] += sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < s.len) to[i] = w[i] + sum[i];
 }
 
 // Probabilities summed over a head's rows for each token: the scores again,

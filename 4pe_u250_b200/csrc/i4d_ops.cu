@@ -234,9 +234,11 @@ struct AttnPlan {
     int even;          // CTAs that share the tokens, or 0
     int cluster;       // else the CTAs of a segment, 1 to 8
     bool prompt;       // k_kv8_prompt: row tiles of kPrRows
-    size_t part_bytes, stat_bytes, lse2_bytes, score_bytes;
-    size_t bytes() const { return part_bytes + stat_bytes + lse2_bytes + score_bytes; }
+    size_t part_bytes, stat_bytes, segment_bytes, lse2_bytes, score_bytes;  // multiples of 16
+    size_t bytes() const { return part_bytes + stat_bytes + segment_bytes + lse2_bytes + score_bytes; }
 };
+
+int64_t score_stride(int max_length) { return (static_cast<int64_t>(max_length) + 3) / 4 * 4; }
 
 AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     AttnPlan p = {};
@@ -268,11 +270,12 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     if (p.even) {
         p.part_bytes = static_cast<size_t>(p.even) * 2 * tile * c.dim * sizeof(float);
         p.stat_bytes = static_cast<size_t>(p.even) * 2 * tile * sizeof(float4);
+        if (!p.prompt) p.segment_bytes = static_cast<size_t>(p.segments) * sizeof(int4);
     }
     if (a.weights) {
         p.lse2_bytes = (static_cast<size_t>(a.tokens) * a.heads * sizeof(float) + 15) / 16 * 16;
         // Few rows: their scores are kept (4 bytes a row against a token's codes read again).
-        if (rows <= 32) p.score_bytes = static_cast<size_t>(p.segments) * 8 * p.nt * a.max_length * sizeof(float);
+        if (rows <= 32) p.score_bytes = static_cast<size_t>(p.segments) * 8 * p.nt * score_stride(a.max_length) * sizeof(float);
     }
     return p;
 }
@@ -640,8 +643,10 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     d.part = static_cast<float*>(a->workspace);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     d.stats = reinterpret_cast<float4*>(ws + p.part_bytes);
-    d.lse2 = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes);
-    if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.lse2_bytes);
+    d.segments = reinterpret_cast<int4*>(ws + p.part_bytes + p.stat_bytes);
+    d.lse2 = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.segment_bytes);
+    if (p.score_bytes) d.scores = reinterpret_cast<float*>(ws + p.part_bytes + p.stat_bytes + p.segment_bytes + p.lse2_bytes);
+    d.score_stride = score_stride(a->max_length);
     d.wide_out = aligned(a->out, 16) && a->out_stride * bytes % 16 == 0 && a->out_head_stride * bytes % 16 == 0;
     d.wide_q = aligned(a->q, 16) && a->q_stride * bytes % 16 == 0 && a->q_head_stride * bytes % 16 == 0;
     const int64_t grid = p.even ? p.even : p.segments * p.cluster;
@@ -660,9 +665,9 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
         if (p.even > 1) OP_CK(launch_after(k_kv8_prompt_join, static_cast<unsigned>(8 * (p.even - 1)), 256, s, d));
     } else if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
     if (d.scores) {
-        const int chunks = (a->max_length + 255) / 256;
+        const int chunks = (a->max_length + 511) / 512;
         if (chunks > 0) {
-            OP_CK(launch_after(k_kv8_weights_kept, static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 256, s, d, 8 * p.nt, chunks));
+            OP_CK(launch_after(k_kv8_weights_kept, static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 128, s, d, 8 * p.nt, chunks));
         }
     } else if (a->weights && wgrid > 0)
         OP_CK(int8 ? launch_weights_c<I4D_CODE_INT8>(d, p, wtiles, wgrid, s) : launch_weights_c<I4D_CODE_E4M3>(d, p, wtiles, wgrid, s));
