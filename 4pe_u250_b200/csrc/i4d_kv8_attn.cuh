@@ -848,24 +848,32 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
     }
 }
 
+constexpr int kJoinThreads = 512;
+
 // Joins the pieces of the segments that several CTAs shared: one CTA for a
-// segment, a warp for a row at a time.
-__global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_per_tile) {
+// segment, whose warps take rows and, if there are fewer rows than warps,
+// every so-manieth piece of one, so that the pieces are read at once.
+__global__ void __launch_bounds__(kJoinThreads) k_kv8_join(AttnDev a, int rows_per_tile) {
+    constexpr int kWarps = kJoinThreads / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ float4 s_o[kWarps][64];
+    __shared__ float s_sum[kWarps];
+    const int4 segment = a.segments[blockIdx.x];
     const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.cache.heads, b = blockIdx.x / a.row_tiles / a.cache.heads;
-    const int lane = threadIdx.x & 31, dim = a.cache.dim;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim;
     const Seq s = load_seq(a.seq, b, false);
     const Units n = seq_units(a, s, rows_per_tile);
-    const int row_tiles = n.segments / a.cache.heads;
-    if (rt >= row_tiles) return;
-    const int4 segment = a.segments[blockIdx.x];
+    if (rt >= n.segments / a.cache.heads) return;  // (its entry in the table was not written)
     const int c0 = segment.x, c1 = segment.y;
     if (c0 == c1) return;  // whole
-    const int rows = min(rows_per_tile, s.n * a.group - rt * rows_per_tile);
-    for (int r = threadIdx.x >> 5; r < rows; r += kAttnWarps) {
-        // the first CTA's piece may be its last, those of the others are their first
-        auto index = [&](int c) { return (static_cast<int64_t>(c) * 2 + (c == c0 ? segment.z : 0)) * rows_per_tile + r; };
-        float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+    const int rows = min(rows_per_tile, s.n * a.group - rt * rows_per_tile), parts = kWarps / rows;
+    const int r = warp / parts, part = warp % parts;  // rows <= 16
+    float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+    float4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // dims 4 lane and 128 + 4 lane
+    const bool low = 4 * lane < dim, high = 128 + 4 * lane < dim;
+    // the first CTA's piece may be its last, those of the others are their first
+    auto index = [&](int c) { return (static_cast<int64_t>(c) * 2 + (c == c0 ? segment.z : 0)) * rows_per_tile + r; };
+    if (r < rows) {
         for (int c = c0 + lane; c <= c1; c += 32) {
             const float4 x = a.stats[index(c)];
             m = fmaxf(m, x.x);
@@ -873,52 +881,46 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_join(AttnDev a, int rows_p
         }
         m = warp_max(m);
         rr = warp_max(rr);
-        float4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // dims 4 lane and 128 + 4 lane
-        const bool low = 4 * lane < dim, high = 128 + 4 * lane < dim;
-        for (int base = c0; base <= c1; base += 32) {
-            float f = 0.f;  // the factor of piece base + lane
-            if (base + lane <= c1) {
-                const float4 x = a.stats[index(base + lane)];
-                sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
-                f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
-            }
-            const int k1 = min(32, c1 + 1 - base);
-#pragma unroll 8
-            for (int k = 0; k < k1; ++k) {
-                const float fk = __shfl_sync(~0u, f, k);
-                const float* p = a.part + index(base + k) * dim + 4 * lane;
-                if (low) {
-                    const float4 x = *reinterpret_cast<const float4*>(p);
-                    o[0].x += x.x * fk;
-                    o[0].y += x.y * fk;
-                    o[0].z += x.z * fk;
-                    o[0].w += x.w * fk;
-                }
-                if (high) {
-                    const float4 x = *reinterpret_cast<const float4*>(p + 128);
-                    o[1].x += x.x * fk;
-                    o[1].y += x.y * fk;
-                    o[1].z += x.z * fk;
-                    o[1].w += x.w * fk;
-                }
-            }
+#pragma unroll 4
+        for (int c = c0 + part; c <= c1; c += parts) {
+            const float4 x = a.stats[index(c)];
+            const float* p = a.part + index(c) * dim + 4 * lane;
+            const float4 y = low ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 z = high ? *reinterpret_cast<const float4*>(p + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
+            sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
+            o[0].x += y.x * f;
+            o[0].y += y.y * f;
+            o[0].z += y.z * f;
+            o[0].w += y.w * f;
+            o[1].x += z.x * f;
+            o[1].y += z.y * f;
+            o[1].z += z.z * f;
+            o[1].w += z.w * f;
         }
-        sum = warp_sum(sum);
-        const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
-        const int row = rt * rows_per_tile + r;
-        const int64_t tok = s.first + row / a.group;
-        const int head = h * a.group + row % a.group;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k ? !high : !low) continue;
-            const int64_t to = tok * a.out_tok + head * a.out_head + 128 * k + 4 * lane;
-            store_out(a, to, o[k].x * back);
-            store_out(a, to + 1, o[k].y * back);
-            store_out(a, to + 2, o[k].z * back);
-            store_out(a, to + 3, o[k].w * back);
-        }
-        if (lane == 0) store_lse(a, s, h, row, make_float4(m, sum, rr, 0.f));
     }
+    s_o[warp][lane] = o[0];
+    s_o[warp][32 + lane] = o[1];
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (part || r >= rows) return;
+    for (int k = 1; k < parts; ++k) {
+        sum += s_sum[warp + k];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 x = s_o[warp + k][32 * i + lane];
+            o[i].x += x.x;
+            o[i].y += x.y;
+            o[i].z += x.z;
+            o[i].w += x.w;
+        }
+    }
+    const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+    const int row = rt * rows_per_tile + r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (i ? high : low) store_row(a, s, h, row, 128 * i + 4 * lane, make_float4(o[i].x * back, o[i].y * back, o[i].z * back, o[i].w * back));
+    if (lane == 0) store_lse(a, s, h, row, make_float4(m, sum, rr, 0.f));
 }
 
 // Probabilities summed over a head's few rows for each token, from the scores

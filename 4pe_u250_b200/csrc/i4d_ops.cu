@@ -663,7 +663,7 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
     if (p.prompt) {
         if (p.even > 1) OP_CK(launch_after(k_kv8_prompt_join, static_cast<unsigned>(8 * (p.even - 1)), 256, s, d));
-    } else if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kAttnThreads, s, d, 8 * p.nt));
+    } else if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kJoinThreads, s, d, 8 * p.nt));
     if (d.scores) {
         const int chunks = (a->max_length + 511) / 512;
         if (chunks > 0) {
