@@ -20,7 +20,8 @@ namespace i4d_ops {
 constexpr int kLogitsThreads = 512;
 constexpr int kLogitsTouched = 8192;  // touched tokens that a CTA can hold
 constexpr int kLogitsPart = 65536;    // logits of a part, with no more than that many ids in the lists
-constexpr int kLogitsSmem = kLogitsTouched * (4 + 4 + 2) + kLogitsPart / 32 * (4 + 2);
+// Shared memory for `places` touched tokens (a multiple of 8) of parts of `words` words (a multiple of 4).
+__host__ __device__ constexpr int logits_smem_bytes(int places, int words) { return places * (4 + 4 + 2) + words * (4 + 2); }
 
 struct LogitsDev {
     const void* in;
@@ -38,6 +39,7 @@ struct LogitsDev {
     const uint32_t* mask;
     int64_t stride, out_stride, history_stride, bias_stride, mask_stride;
     int vocab, history_max, bias_max;
+    int places, words;  // touched tokens and bitmap words that the launch has shared memory for
 };
 
 // Greater value, greater key; of equal values the lower index.  0: none.
@@ -57,6 +59,12 @@ struct Touched {
     uint16_t* before;     // [part / 32] places before a word
     int first, span;      // ids [first, first + span), span <= kLogitsPart
     __device__ __forceinline__ bool holds(int id) const { return static_cast<unsigned>(id - first) < static_cast<unsigned>(span); }
+    // (Few tokens are most of a text: a mark that stands is not written again.)
+    __device__ __forceinline__ void mark(int id) const {
+        const int at = id - first;
+        const uint32_t bit = 1u << (at & 31);
+        if (!(*static_cast<volatile uint32_t*>(bits + (at >> 5)) & bit)) atomicOr(bits + (at >> 5), bit);
+    }
     __device__ __forceinline__ int place(int id) const {
         const int at = id - first;
         return before[at >> 5] + __popc(bits[at >> 5] & ((1u << (at & 31)) - 1));
@@ -64,15 +72,15 @@ struct Touched {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int ctas) {
+__global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int ctas) {
     extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
     Touched t;
     t.counts = reinterpret_cast<int*>(logits_smem);
-    t.bias = reinterpret_cast<float*>(t.counts + kLogitsTouched);
-    t.bits = reinterpret_cast<uint32_t*>(t.bias + kLogitsTouched);
-    t.ids = reinterpret_cast<uint16_t*>(t.bits + kLogitsPart / 32);
-    t.before = t.ids + kLogitsTouched;
+    t.bias = reinterpret_cast<float*>(t.counts + a.places);
+    t.bits = reinterpret_cast<uint32_t*>(t.bias + a.places);
+    t.ids = reinterpret_cast<uint16_t*>(t.bits + a.words);
+    t.before = t.ids + a.places;
     __shared__ int found[kLogitsThreads / 32];
     __shared__ float2 entries[kLogitsThreads];
     __shared__ unsigned long long keys[kLogitsThreads / 32];
@@ -99,12 +107,16 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
     const int per_cta = (vecs + ctas - 1) / ctas;
     const int v_end = min(vecs, (rank + 1) * per_cta);
     // More ids than places: parts of so many logits that no more can be touched.
-    const int part = (static_cast<int64_t>(n_hist) + n_bias <= kLogitsTouched ? kLogitsPart : kLogitsTouched) / V;
+    const int part = (n_hist + n_bias <= a.places ? a.words * 32 : min(a.places, a.words * 32)) / V;
+    constexpr int kAhead = 2;  // vectors that a thread loads before it works on them
     unsigned long long key = 0;
     float best = -INFINITY;  // of this thread's streamed logits, whose ids only grow
     int best_id = -1;
     for (int v0 = rank * per_cta; v0 < v_end; v0 += part) {
         const int v1 = min(v_end, v0 + part);
+        // the stream's cache lines, on their way while the tokens are counted
+        for (int v = v0 + tid * (128 / 16); v < v1; v += kLogitsThreads * (128 / 16))
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(in + max(v * V - skew, 0)));
         t.first = max(0, v0 * V - skew);
         t.span = min(a.vocab, v1 * V - skew) - t.first;
         const int words = (t.span + 31) / 32;
@@ -116,11 +128,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
 #pragma unroll 4
             for (int i = tid; i < n_hist; i += kLogitsThreads) {
                 const int id = __ldg(hist + i);
-                if (t.holds(id)) atomicOr(&t.bits[(id - t.first) >> 5], 1u << ((id - t.first) & 31));
+                if (t.holds(id)) t.mark(id);
             }
             for (int i = tid; i < n_bias; i += kLogitsThreads) {
                 const int id = __ldg(bias_ids + i);
-                if (t.holds(id)) atomicOr(&t.bits[(id - t.first) >> 5], 1u << ((id - t.first) & 31));
+                if (t.holds(id)) t.mark(id);
             }
             __syncthreads();
             // places: each thread's words follow those of the threads before it
@@ -154,8 +166,13 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
             for (int i = tid; i < n_hist; i += kLogitsThreads) {
                 const int id = __ldg(hist + i);
                 if (t.holds(id)) {
-                    if (i < n_prompt) atomicOr(&t.counts[t.place(id)], 1);
-                    else atomicAdd(&t.counts[t.place(id)], 2);
+                    int* count = &t.counts[t.place(id)];
+                    if (i < n_prompt) {
+                        if (!(*static_cast<volatile int*>(count) & 1)) atomicOr(count, 1);
+                    } else {  // one lane adds for all lanes with its token
+                        const unsigned peers = __match_any_sync(__activemask(), id);
+                        if (__ffs(peers) - 1 == lane) atomicAdd(count, 2 * __popc(peers));
+                    }
                 }
             }
             // Biases: the part's entries of a round in their order, then the
@@ -189,17 +206,30 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
             }
         }
         // The stream: touched logits go out as they came.
-#pragma unroll 2
-        for (int v = v0 + tid; v < v1; v += kLogitsThreads) {
-            const int e = v * V - skew;
+        for (int vb = v0; vb < v1; vb += kLogitsThreads * kAhead) {
+        Vec<T, V> ahead[kAhead];
+        uint2 words_ahead[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int v = vb + u * kLogitsThreads + tid, e = v * V - skew;
+            words_ahead[u] = make_uint2(~0u, ~0u);
+            if (v < v1 && e >= 0 && e + V <= a.vocab) {
+                ahead[u] = *reinterpret_cast<const Vec<T, V>*>(in + e);
+                if (mask) words_ahead[u] = make_uint2(__ldg(mask + (e >> 5)), __ldg(mask + ((e + V - 1) >> 5)));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int v = vb + u * kLogitsThreads + tid, e = v * V - skew;
+            if (v >= v1) continue;
             if (e >= 0 && e + V <= a.vocab) {
-                Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(in + e);
-                uint32_t skip = 0, seen = ~0u;
+                Vec<T, V> x = ahead[u];
+                uint32_t skip = 0;
+                const uint32_t seen = __funnelshift_r(words_ahead[u].x, words_ahead[u].y, e & 31);
                 if (touched) {
                     const int at = e - t.first, w = at >> 5;
                     skip = __funnelshift_r(t.bits[w], w + 1 < words ? t.bits[w + 1] : 0u, at & 31);
                 }
-                if (mask) seen = __funnelshift_r(__ldg(mask + (e >> 5)), __ldg(mask + ((e + V - 1) >> 5)), e & 31);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float y = to_f32(x.v[i]);
@@ -229,6 +259,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
                     }
                 }
             }
+        }
         }
         if (touched) {
             __syncthreads();  // counts and biases are complete, the touched logits lie in `out`

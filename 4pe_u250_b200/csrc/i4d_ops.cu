@@ -160,9 +160,12 @@ cudaError_t launch_rope(const RopeDev& d, int num_sms, cudaStream_t st) {
     const int rot_items = (IL ? d.rot : d.rot / 2) / V;
     const int items = (d.heads[0] + d.heads[1]) * (rot_items + (d.copy_tail ? (d.dim - d.rot) / V : 0));
     // Few tokens: their heads are spread over CTAs, up to two waves of them.
+    if (d.tokens >= 16 * num_sms) {
+        k_rope_many<T, V, IL><<<(d.tokens + kRopeWarps - 1) / kRopeWarps, 32 * kRopeWarps, 0, st>>>(d);
+        return cudaGetLastError();
+    }
     const int most = (items + kRopeThreads - 1) / kRopeThreads;
     const int groups = std::max(1, std::min(most, 2 * num_sms / d.tokens));
-    if (static_cast<int64_t>(d.tokens) * groups > kMaxGrid) return cudaErrorInvalidValue;
     k_rope<T, V, IL><<<d.tokens * groups, kRopeThreads, 0, st>>>(d, groups);
     return cudaGetLastError();
 }
@@ -387,7 +390,7 @@ i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
 namespace i4d_ops {
 
 cudaError_t ops_init() {
-    const int logits_smem = kLogitsSmem;
+    const int logits_smem = logits_smem_bytes(kLogitsTouched, kLogitsPart / 32);
     cudaError_t e = cudaFuncSetAttribute(k_logits<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
@@ -789,10 +792,15 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     OP_CK(scope.error());
     const unsigned grid = static_cast<unsigned>(a->rows * ctas);
     const cudaStream_t s = stream_of(o, a->stream);
+    // Shared memory for the ids that the lists can hold and a CTA's part of the row.
+    const int64_t ids = static_cast<int64_t>(a->history ? a->history_max : 0) + (a->bias_ids ? a->bias_max : 0);
+    d.places = static_cast<int>(std::min<int64_t>(kLogitsTouched, (ids + 255) / 256 * 256));
+    d.words = std::min(kLogitsPart / 32, ((a->vocab + ctas - 1) / ctas + 32 + 127) / 128 * 4);
+    const int smem = logits_smem_bytes(d.places, d.words);
     switch (a->dtype) {
-        case I4D_F32: OP_CK(launch_cluster(k_logits<float>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
-        case I4D_BF16: OP_CK(launch_cluster(k_logits<__nv_bfloat16>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
-        default: OP_CK(launch_cluster(k_logits<__half>, grid, kLogitsThreads, kLogitsSmem, ctas, s, d, ctas)); break;
+        case I4D_F32: OP_CK(launch_cluster(k_logits<float>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        case I4D_BF16: OP_CK(launch_cluster(k_logits<__nv_bfloat16>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        default: OP_CK(launch_cluster(k_logits<__half>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
     }
     return I4D_OK;
 }
