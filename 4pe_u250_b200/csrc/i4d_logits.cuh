@@ -8,10 +8,15 @@
 // ones, a thread each, so that no warp runs the penalties' division for one
 // lane.  The row's best index is joined over the cluster through distributed
 // shared memory; nothing is kept in global memory between launches.
-// Bound: the logits in and out; for one row the chain of barriers.
+// Bound: the logits in and out; but a list of thousands of ids costs a CTA's
+// phases, each with its barriers, as much again (192 rows of 128001 in bf16:
+// 32 us without lists, 60 with histories and biases, 15 at the copy's rate),
+// and one row the chain of those phases (10 us).
 #pragma once
 
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "i4d_ops_common.cuh"
 
@@ -50,6 +55,46 @@ __device__ __forceinline__ unsigned long long logit_key(float x, int index) {
     return static_cast<unsigned long long>(k) << 32 | (0xffffffffu - index);
 }
 
+// Puts -inf in place of the logits whose bit in `seen` is 0, but for those
+// whose bit in `raw` is 1, which stay; returns the greatest of those that are
+// seen and not raw (-inf: none; NaN passed over).
+__device__ __forceinline__ float mask_vec(Vec<float, 4>& x, uint32_t seen, uint32_t raw) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (seen & ~raw & 1u << i) top = fmaxf(top, x.v[i]);
+        if (!((seen | raw) & 1u << i)) x.v[i] = -INFINITY;
+    }
+    return top;
+}
+// 16-bit logits two at a time.
+template <typename T>
+__device__ __forceinline__ float mask_vec(Vec<T, 8>& x, uint32_t seen, uint32_t raw) {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr uint32_t kNone = kBf16 ? 0xff80ff80u : 0xfc00fc00u;  // two of -inf
+    // bit 2 i and bit 2 i + 1 to two masks of 16
+    auto both = [](uint32_t bits, int i) {
+        return __byte_perm(static_cast<int>(bits << (31 - 2 * i)) >> 31, static_cast<int>(bits << (30 - 2 * i)) >> 31, 0x5410);
+    };
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+    uint32_t top = kNone;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t counts = both(seen & ~raw, i), stays = both(raw, i);
+        const uint32_t y = (w[i] & counts) | (kNone & ~counts);
+        w[i] = (w[i] & stays) | (y & ~stays);
+        if constexpr (kBf16) {
+            const __nv_bfloat162 z = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&top), *reinterpret_cast<const __nv_bfloat162*>(&y));
+            top = *reinterpret_cast<const uint32_t*>(&z);
+        } else {
+            const __half2 z = __hmax2(*reinterpret_cast<const __half2*>(&top), *reinterpret_cast<const __half2*>(&y));
+            top = *reinterpret_cast<const uint32_t*>(&z);
+        }
+    }
+    const T* y = reinterpret_cast<const T*>(&top);
+    return fmaxf(to_f32(y[0]), to_f32(y[1]));
+}
+
 // Marks, places and values of the touched tokens of a part.
 struct Touched {
     int* counts;          // [place] bit 0: in the prompt, above: 2 * occurrences after it
@@ -59,11 +104,9 @@ struct Touched {
     uint16_t* before;     // [part / 32] places before a word
     int first, span;      // ids [first, first + span), span <= kLogitsPart
     __device__ __forceinline__ bool holds(int id) const { return static_cast<unsigned>(id - first) < static_cast<unsigned>(span); }
-    // (Few tokens are most of a text: a mark that stands is not written again.)
     __device__ __forceinline__ void mark(int id) const {
         const int at = id - first;
-        const uint32_t bit = 1u << (at & 31);
-        if (!(*static_cast<volatile uint32_t*>(bits + (at >> 5)) & bit)) atomicOr(bits + (at >> 5), bit);
+        atomicOr(bits + (at >> 5), 1u << (at & 31));
     }
     __device__ __forceinline__ int place(int id) const {
         const int at = id - first;
@@ -72,7 +115,7 @@ struct Touched {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int ctas) {
+__global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int ctas) {
     extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
     Touched t;
@@ -109,6 +152,23 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
     // More ids than places: parts of so many logits that no more can be touched.
     const int part = (n_hist + n_bias <= a.places ? a.words * 32 : min(a.places, a.words * 32)) / V;
     constexpr int kAhead = 2;  // vectors that a thread loads before it works on them
+    // The lists' ids, read once into registers as far as they hold them; each is
+    // looked at twice for every part.
+    constexpr int kHeld = 6;
+    constexpr int kFew = 8;  // bits of a word that one thread takes
+    int held[kHeld], held_bias = -1;
+    float held_value = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) held[k] = k * kLogitsThreads + tid < n_hist ? __ldg(hist + k * kLogitsThreads + tid) : -1;
+    if (tid < n_bias) {
+        held_bias = __ldg(bias_ids + tid);
+        held_value = __ldg(a.bias_values + row * a.bias_stride + tid);
+    }
+    auto each_id = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) f(k * kLogitsThreads + tid, held[k]);
+        for (int i = kHeld * kLogitsThreads + tid; i < n_hist; i += kLogitsThreads) f(i, __ldg(hist + i));
+    };
     unsigned long long key = 0;
     float best = -INFINITY;  // of this thread's streamed logits, whose ids only grow
     int best_id = -1;
@@ -125,20 +185,21 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
             __syncthreads();
             for (int i = tid; i < words; i += kLogitsThreads) t.bits[i] = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int i = tid; i < n_hist; i += kLogitsThreads) {
-                const int id = __ldg(hist + i);
+            each_id([&](int, int id) {
                 if (t.holds(id)) t.mark(id);
-            }
-            for (int i = tid; i < n_bias; i += kLogitsThreads) {
+            });
+            if (t.holds(held_bias)) t.mark(held_bias);
+            for (int i = kLogitsThreads + tid; i < n_bias; i += kLogitsThreads) {
                 const int id = __ldg(bias_ids + i);
                 if (t.holds(id)) t.mark(id);
             }
             __syncthreads();
-            // places: each thread's words follow those of the threads before it
-            const int per = (words + kLogitsThreads - 1) / kLogitsThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+            // places: each thread's words follow those of the threads before it.  A
+            // warp's words lie 33 apart: the full ones, of frequent tokens, are
+            // neighbours (and an odd distance reaches every bank).
+            const int w0 = tid * 33 % kLogitsThreads;
             int mine = 0;
-            for (int w = w0; w < w1; ++w) mine += __popc(t.bits[w]);
+            for (int w = w0; w < words; w += kLogitsThreads) mine += __popc(t.bits[w]);
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -153,33 +214,53 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
                 touched += found[w];
             }
             int at = upto - mine;
-            for (int w = w0; w < w1; ++w) {
-                t.before[w] = static_cast<uint16_t>(at);
-                for (uint32_t x = t.bits[w]; x; x &= x - 1) {
-                    t.ids[at] = static_cast<uint16_t>(w * 32 + __ffs(x) - 1);
-                    t.counts[at] = 0;
-                    t.bias[at++] = 0.f;
+            for (int wb = 0; wb < words; wb += kLogitsThreads) {
+                const int w = wb + w0;
+                const uint32_t x = w < words ? t.bits[w] : 0u;
+                if (w < words) t.before[w] = static_cast<uint16_t>(at);
+                const bool full = __popc(x) > kFew;
+                if (!full)
+                    for (uint32_t y = x, to = at; y; y &= y - 1) t.ids[to++] = static_cast<uint16_t>(w * 32 + __ffs(y) - 1);
+                for (unsigned todo = __ballot_sync(~0u, full); todo; todo &= todo - 1) {  // a lane for each bit
+                    const int from = __ffs(todo) - 1;
+                    const uint32_t y = __shfl_sync(~0u, x, from);
+                    const int to = __shfl_sync(~0u, at, from) + __popc(y & ((1u << lane) - 1)), word = __shfl_sync(~0u, w, from);
+                    if (y >> lane & 1) t.ids[to] = static_cast<uint16_t>(word * 32 + lane);
                 }
+                at += __popc(x);
+            }
+            for (int k = tid; k < touched; k += kLogitsThreads) {
+                t.counts[k] = 0;
+                t.bias[k] = 0.f;
             }
             __syncthreads();
-#pragma unroll 4
-            for (int i = tid; i < n_hist; i += kLogitsThreads) {
-                const int id = __ldg(hist + i);
+            each_id([&](int i, int id) {
                 if (t.holds(id)) {
                     int* count = &t.counts[t.place(id)];
-                    if (i < n_prompt) {
-                        if (!(*static_cast<volatile int*>(count) & 1)) atomicOr(count, 1);
-                    } else {  // one lane adds for all lanes with its token
-                        const unsigned peers = __match_any_sync(__activemask(), id);
-                        if (__ffs(peers) - 1 == lane) atomicAdd(count, 2 * __popc(peers));
-                    }
+                    if (i < n_prompt) atomicOr(count, 1);
+                    else atomicAdd(count, 2);
                 }
-            }
-            // Biases: the part's entries of a round in their order, then the
-            // first of each id adds up the values of that id.
+            });
+            // Biases, a thread for each.  A thread that finds its own mark in its
+            // place adds alone; else the part's entries of the round are listed in
+            // their order, and the first of each id adds up the values of that id.
             for (int i = 0; i < n_bias; i += kLogitsThreads) {
-                const int id = i + tid < n_bias ? __ldg(bias_ids + i + tid) : -1;
+                const int id = i == 0 ? held_bias : i + tid < n_bias ? __ldg(bias_ids + i + tid) : -1;
+                const float value = i == 0 ? held_value : i + tid < n_bias ? __ldg(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
                 const bool in_part = t.holds(id);
+                float* sum_of = &t.bias[in_part ? t.place(id) : 0];
+                float prior = 0.f;
+                if (i) {
+                    __syncthreads();
+                    if (in_part) prior = *sum_of;
+                    __syncthreads();
+                }
+                if (in_part) *sum_of = __int_as_float(tid);
+                __syncthreads();
+                const bool shared = in_part && __float_as_int(*sum_of) != tid;
+                const int several = __syncthreads_or(shared);
+                if (in_part) *sum_of = several ? prior : __fadd_rn(prior, value);
+                if (!several) continue;
                 const unsigned votes = __ballot_sync(~0u, in_part);
                 __syncthreads();
                 if (lane == 0) found[warp] = __popc(votes);
@@ -190,7 +271,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
                     to += w < warp ? found[w] : 0;
                     total += found[w];
                 }
-                if (in_part) entries[to] = make_float2(__int_as_float(t.place(id)), __ldg(a.bias_values + row * a.bias_stride + i + tid));
+                if (in_part) entries[to] = make_float2(__int_as_float(t.place(id)), value);
                 __syncthreads();
                 if (tid < total) {
                     const int slot = __float_as_int(entries[tid].x);
@@ -224,21 +305,18 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
             if (v >= v1) continue;
             if (e >= 0 && e + V <= a.vocab) {
                 Vec<T, V> x = ahead[u];
-                uint32_t skip = 0;
+                uint32_t raw = 0;
                 const uint32_t seen = __funnelshift_r(words_ahead[u].x, words_ahead[u].y, e & 31);
                 if (touched) {
                     const int at = e - t.first, w = at >> 5;
-                    skip = __funnelshift_r(t.bits[w], w + 1 < words ? t.bits[w + 1] : 0u, at & 31);
+                    raw = __funnelshift_r(t.bits[w], w + 1 < words ? t.bits[w + 1] : 0u, at & 31);
                 }
+                const float top = mask_vec(x, seen, raw);
+                if (top > best) {
+                    best = top;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float y = to_f32(x.v[i]);
-                    const bool gone = !(seen >> i & 1), raw = skip >> i & 1;
-                    if (gone && !raw) x.v[i] = from_f32<T>(-INFINITY);
-                    if (y > best && !gone && !raw) {
-                        best = y;
-                        best_id = e + i;
-                    }
+                    for (int i = V - 1; i >= 0; --i)
+                        if ((seen & ~raw) >> i & 1 && to_f32(x.v[i]) == top) best_id = e + i;
                 }
                 if (aligned_out) {
                     *reinterpret_cast<Vec<T, V>*>(out + e) = x;
@@ -263,16 +341,32 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits(LogitsDev a, int c
         }
         if (touched) {
             __syncthreads();  // counts and biases are complete, the touched logits lie in `out`
-            for (int k = tid; k < touched; k += kLogitsThreads) {
-                const int id = t.first + t.ids[k], c = t.counts[k], n = c >> 1;
-                float y = to_f32(out[id]);
-                if (c && a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
-                y = __fadd_rn(y, t.bias[k]);
-                if (mask && !(__ldg(mask + (id >> 5)) >> (id & 31) & 1)) y = -INFINITY;
-                const T z = from_f32<T>(y);
-                out[id] = z;
-                key = max(key, logit_key(to_f32(z), id));
+            constexpr int kLate = 4;  // logits that a thread loads before it works on them
+            for (int kb = tid; kb < touched; kb += kLogitsThreads * kLate) {
+                float ys[kLate];
+                int ids[kLate];
+                uint32_t seen[kLate];
+#pragma unroll
+                for (int u = 0; u < kLate; ++u) {
+                    const int k = kb + u * kLogitsThreads;
+                    ids[u] = k < touched ? t.first + t.ids[k] : t.first;
+                    ys[u] = k < touched ? to_f32(out[ids[u]]) : 0.f;
+                    seen[u] = mask ? __ldg(mask + (ids[u] >> 5)) >> (ids[u] & 31) & 1 : 1;
+                }
+#pragma unroll
+                for (int u = 0; u < kLate; ++u) {
+                    const int k = kb + u * kLogitsThreads;
+                    if (k >= touched) break;
+                    const int c = t.counts[k], n = c >> 1;
+                    float y = ys[u];
+                    if (c && a.repetition) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                    if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n))), pres);
+                    y = __fadd_rn(y, t.bias[k]);
+                    if (!seen[u]) y = -INFINITY;
+                    const T z = from_f32<T>(y);
+                    out[ids[u]] = z;
+                    key = max(key, logit_key(to_f32(z), ids[u]));
+                }
             }
         }
     }

@@ -782,11 +782,13 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     d.vocab = a->vocab;
     d.history_max = a->history_max;
     d.bias_max = a->bias_max;
-    // CTAs of a row: slices of at least 2048 entries, eight at most (the
-    // portable cluster size), fewer where the rows fill the GPU by themselves.
+    // CTAs of a row: parts of at least 2048 entries, eight at most (the portable
+    // cluster size), no more than fill the places of two CTAs an SM once, since
+    // each reads the row's whole lists (192 rows of 128001 with histories: 60 us
+    // with two a row, 64 with one, 71 with four, 101 with eight).
     const OpContext o = op_context(ctx);
     int ctas = 1;
-    while (ctas < 8 && a->vocab / (2 * ctas) >= 2048 && static_cast<int64_t>(a->rows) * ctas < 4 * o.num_sms) ctas *= 2;
+    while (ctas < 8 && a->vocab / (2 * ctas) >= 2048 && static_cast<int64_t>(a->rows) * ctas < 2 * o.num_sms) ctas *= 2;
     OP_ARG(static_cast<int64_t>(a->rows) * ctas <= kMaxGrid, "too many rows in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());

@@ -58,7 +58,8 @@ def _rope_bound(x, y, magnitude, t, interleaved, half):
 @pytest.mark.parametrize("interleaved", [True, False])
 @pytest.mark.parametrize("tokens,heads,kv,dim,rot,scaling", [
     (1, 1, 1, 64, 64, "none"), (3, 5, 2, 96, 32, "parts"), (33, 4, 4, 80, 80, "base"), (7, 32, 8, 128, 128, "linear"),
-    (2, 3, 1, 256, 256, "none"), (5, 2, 2, 20, 6, "none"), (4, 2, 1, 18, 18, "parts")])
+    (2, 3, 1, 256, 256, "none"), (5, 2, 2, 20, 6, "none"), (4, 2, 1, 18, 18, "parts"),
+    (2401, 3, 1, 64, 32, "none"), (2401, 2, 1, 20, 6, "none"), (2401, 1, 2, 256, 256, "base")])
 def test_rope(pkg, ctx, name, interleaved, tokens, heads, kv, dim, rot, scaling):
     torch = _torch()
     t = _type(name)
