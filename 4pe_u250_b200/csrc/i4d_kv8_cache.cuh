@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 __device__ __forceinline__ int evict_length(const EvictDev& a, int b, bool report) {
     const int len = __ldg(a.seq.lengths + b);
-    const bool ok = len >= 0 && len <= a.max_length;
+    const bool ok = length_ok(len, a.max_length);
     if (!ok && report) atomicOr(a.seq.err, kBadSequence);
     return ok ? len : 0;
 }
@@ -374,8 +374,8 @@ constexpr int kMoveThreads = 512;
 
 // 16-byte pieces that a thread holds, and destination tokens of a CTA in a
 // round: whole blocks.
-__host__ __device__ constexpr int move_pieces(int) { return 4; }
-__host__ __device__ constexpr int move_tokens(int dim) { return kMoveThreads * move_pieces(dim) / (dim / 16) / 128 * 128; }
+constexpr int kMovePieces = 4;
+__host__ __device__ constexpr int move_tokens(int dim) { return kMoveThreads * kMovePieces / (dim / 16) / 128 * 128; }
 
 // Moves the kept tokens up, in place.  One cluster for each (sequence, head, K
 // or V) walks its destination tokens in order, a round of all its CTAs at a
@@ -385,8 +385,9 @@ __host__ __device__ constexpr int move_tokens(int dim) { return kMoveThreads * m
 // their loads start before.  A block's new scale comes from the old scales,
 // which k_kv8_select copied.
 // Bound: kept codes read and written in whole rows.
-template <int CODE, int VECS>
+template <int CODE>
 __global__ void __launch_bounds__(kMoveThreads, 2) k_kv8_move(EvictDev a, int ctas) {
+    constexpr int VECS = kMovePieces;
     __shared__ float token_scale[kMoveThreads * VECS];
     __shared__ float block_scale[kMoveThreads * VECS / 16];
     cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 #include "i4d.h"
 #include "i4d_internal.h"
@@ -60,14 +61,69 @@ cudaStream_t stream_of(const OpContext& o, void* stream) {
 
 // Bytes [lo, hi) that `n` rows of `heads` heads touch.
 struct Span {
+    const char* name;
     uintptr_t lo, hi;
 };
-Span span_of(const void* p, int64_t n, int64_t stride, int64_t heads, int64_t head_stride, int64_t inner, int bytes) {
+Span span_of(const char* name, const void* p, int64_t n, int64_t stride, int64_t heads, int64_t head_stride, int64_t inner, int64_t bytes) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    if (!p || n <= 0 || heads <= 0) return {at, at};
-    return {at, at + static_cast<uintptr_t>(((n - 1) * stride + (heads - 1) * head_stride + inner) * bytes)};
+    if (!p || n <= 0 || heads <= 0) return {name, at, at};
+    return {name, at, at + static_cast<uintptr_t>(((n - 1) * stride + (heads - 1) * head_stride + inner) * bytes)};
 }
+Span span_of(const char* name, const void* p, int64_t n, int64_t bytes) { return span_of(name, p, 1, 0, 1, 0, n, bytes); }
 bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// What a call writes must not lie in what else it reads or writes.
+i4d_status check_apart(i4d_ctx* ctx, std::initializer_list<Span> writes, std::initializer_list<Span> reads) {
+    for (const Span* w = writes.begin(); w != writes.end(); ++w) {
+        for (const Span* x = w + 1; x != writes.end(); ++x) OP_ARG(!overlap(*w, *x), "%s overlaps %s", w->name, x->name);
+        for (const Span& r : reads) OP_ARG(!overlap(*w, r), "%s overlaps %s", w->name, r.name);
+    }
+    return I4D_OK;
+}
+
+// Rows of heads in one buffer, as [tokens][heads][dim] with strides.
+struct View {
+    const char* name;
+    const void* p;
+    int64_t n, stride, heads, head_stride, inner;
+    int bytes;
+    Span span() const { return span_of(name, p, n, stride, heads, head_stride, inner, bytes); }
+    bool same(const View& o) const { return p == o.p && stride == o.stride && head_stride == o.head_stride; }
+};
+
+// False where no element of one view is one of the other: apart in memory, or
+// parts of one buffer's rows (the q, k and v of a fused projection), which lie
+// apart in each period of a stride that all their steps are multiples of.
+bool overlap(const View& a, const View& b) {
+    if (!overlap(a.span(), b.span())) return false;
+    for (const int64_t period : {a.stride, a.head_stride, b.stride, b.head_stride}) {
+        if (period <= 0) continue;
+        const auto extent = [&](const View& v) {
+            return v.inner + (v.stride % period ? (v.n - 1) * v.stride : 0) + (v.head_stride % period ? (v.heads - 1) * v.head_stride : 0);
+        };
+        const int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p)) / a.bytes % period;
+        const int64_t delta = from < 0 ? from + period : from;
+        if (extent(a) <= delta && delta + extent(b) <= period) return false;
+    }
+    return true;
+}
+
+// Every element has a place of its own.
+bool rows_apart(const View& v) {
+    if (v.n == 1) return v.heads == 1 || v.head_stride >= v.inner;
+    if (v.heads == 1) return v.stride >= v.inner;
+    return (v.head_stride >= v.inner && v.stride >= (v.heads - 1) * v.head_stride + v.inner) ||
+           (v.stride >= v.inner && v.head_stride >= (v.n - 1) * v.stride + v.inner);
+}
+
+int64_t cache_bytes(const i4d_kv8& c) { return static_cast<int64_t>(c.blocks) * c.heads * c.block_tokens * c.dim; }
+int64_t cache_scales(const i4d_kv8& c) { return static_cast<int64_t>(c.blocks) * c.heads; }
+#define CACHE_SPANS(c)                                                                              \
+    span_of("cache k", (c).k, cache_bytes(c), 1), span_of("cache v", (c).v, cache_bytes(c), 1),     \
+        span_of("k_scale", (c).k_scale, cache_scales(c), 4), span_of("v_scale", (c).v_scale, cache_scales(c), 4)
+#define BATCH_SPANS(a)                                                                              \
+    span_of("q_start", (a)->q_start, (a)->batch + 1, 4), span_of("lengths", (a)->lengths, (a)->batch, 4), \
+        span_of("block_table", (a)->block_table, (a)->batch, (a)->table_stride, 1, 0, (a)->table_blocks, 4)
 
 i4d_status check_cache(i4d_ctx* ctx, const i4d_kv8& c) {
     OP_ARG(c.k && c.v && c.k_scale && c.v_scale, "null cache buffer");
@@ -463,7 +519,7 @@ i4d_status i4d_rope(i4d_ctx* ctx, const i4d_rope_args* a) {
     void* out[2] = {a->q_out, has_k ? a->k_out : nullptr};
     const int64_t in_s[2] = {a->q_stride, a->k_stride}, in_h[2] = {a->q_head_stride, a->k_head_stride};
     const int64_t out_s[2] = {a->q_out_stride, a->k_out_stride}, out_h[2] = {a->q_out_head_stride, a->k_out_head_stride};
-    Span si[2], so[2];
+    View vi[2] = {}, vo[2] = {};
     const int vec = 16 / bytes;
     bool wide = a->dim % vec == 0 && a->rot_dim % (a->interleaved ? vec : 2 * vec) == 0;
     bool copy = false;
@@ -476,30 +532,26 @@ i4d_status i4d_rope(i4d_ctx* ctx, const i4d_rope_args* a) {
         d.out_tok[i] = out_s[i];
         d.out_head[i] = out_h[i];
         d.heads[i] = heads;
-        if (!heads) {
-            si[i] = so[i] = {0, 0};
-            continue;
-        }
-        OP_ARG(aligned(in[i], bytes) && aligned(out[i], bytes), "misaligned buffer");
-        OP_ARG(in_s[i] >= 0 && in_h[i] >= 0, "negative input stride");
-        // every output element has a place of its own
-        const bool head_inner = out_h[i] >= a->dim && out_s[i] >= (heads - 1) * out_h[i] + a->dim;
-        const bool token_inner = out_s[i] >= a->dim && out_h[i] >= (a->tokens - 1) * out_s[i] + a->dim;
-        OP_ARG(head_inner || token_inner || (heads == 1 && out_s[i] >= a->dim) || (a->tokens == 1 && out_h[i] >= a->dim), "output rows overlap");
-        si[i] = span_of(in[i], a->tokens, in_s[i], heads, in_h[i], a->dim, bytes);
-        so[i] = span_of(out[i], a->tokens, out_s[i], heads, out_h[i], a->dim, bytes);
+        vi[i] = {i ? "k" : "q", in[i], a->tokens, in_s[i], heads, in_h[i], a->dim, bytes};
+        vo[i] = {i ? "k_out" : "q_out", out[i], a->tokens, out_s[i], heads, out_h[i], a->dim, bytes};
+        if (!heads) continue;
+        OP_ARG(aligned(in[i], bytes) && aligned(out[i], bytes), "misaligned %s or %s", vi[i].name, vo[i].name);
+        OP_ARG(in_s[i] >= 0 && in_h[i] >= 0, "negative stride of %s", vi[i].name);
+        OP_ARG(out_s[i] >= 0 && out_h[i] >= 0 && rows_apart(vo[i]), "rows of %s overlap", vo[i].name);
         wide = wide && aligned(in[i], 16) && aligned(out[i], 16) && in_s[i] % vec == 0 && in_h[i] % vec == 0 && out_s[i] % vec == 0 && out_h[i] % vec == 0;
     }
     for (int i = 0; i < 2; ++i) {
         if (!d.heads[i]) continue;
-        const bool same = in[i] == out[i] && in_s[i] == out_s[i] && in_h[i] == out_h[i];
-        OP_ARG(same || !overlap(si[i], so[i]), "an output overlaps its input");
-        copy = copy || !same;
+        OP_ARG(vi[i].same(vo[i]) || !overlap(vi[i], vo[i]), "%s overlaps %s", vo[i].name, vi[i].name);
+        OP_ARG(!d.heads[1 - i] || !overlap(vo[i], vi[1 - i]), "%s overlaps %s", vo[i].name, vi[1 - i].name);
+        copy = copy || !vi[i].same(vo[i]);
     }
-    if (has_k) {
-        // q and k may be interleaved parts of one buffer; only plain overlap of different tensors is refused
-        OP_ARG(out[0] != out[1], "q_out is k_out");
+    OP_ARG(!has_k || !overlap(vo[0], vo[1]), "q_out overlaps k_out");
+    for (const View& v : vo) {
+        const i4d_status st = check_apart(ctx, {v.span()}, {span_of("positions", a->positions, a->tokens, 4), span_of("turns", a->turns, a->rot_dim / 2, 8)});
+        if (st != I4D_OK) return st;
     }
+    OP_ARG(aligned(a->positions, 4) && aligned(a->turns, 8), "misaligned positions or turns");
     d.positions = a->positions;
     d.turns = a->turns;
     d.tokens = a->tokens;
@@ -508,11 +560,11 @@ i4d_status i4d_rope(i4d_ctx* ctx, const i4d_rope_args* a) {
     d.inverse = a->inverse != 0;
     d.copy_tail = copy && a->dim > a->rot_dim;
     d.magnitude = a->magnitude;
+    if (!wide && a->interleaved) OP_ARG((a->dim - a->rot_dim) % 2 == 0 || !d.copy_tail, "dim %d must be even", a->dim);
     const OpContext o = op_context(ctx);
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t st = stream_of(o, a->stream);
-    if (!wide && a->interleaved) OP_ARG((a->dim - a->rot_dim) % 2 == 0 || !d.copy_tail, "dim %d must be even", a->dim);
     switch (a->dtype) {
         case I4D_F32: OP_CK(launch_rope_t<float>(d, a->interleaved != 0, wide, o.num_sms, st)); break;
         case I4D_BF16: OP_CK(launch_rope_t<__nv_bfloat16>(d, a->interleaved != 0, wide, o.num_sms, st)); break;
@@ -533,6 +585,10 @@ i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* a) {
     const int bytes = dtype_bytes(a->dtype);
     OP_ARG(aligned(a->k, bytes) && aligned(a->v, bytes), "misaligned k or v");
     OP_ARG(a->k_stride >= 0 && a->k_head_stride >= 0 && a->v_stride >= 0 && a->v_head_stride >= 0, "negative stride");
+    st = check_apart(ctx, {CACHE_SPANS(a->cache)},
+                     {span_of("k", a->k, a->tokens, a->k_stride, a->cache.heads, a->k_head_stride, a->cache.dim, bytes),
+                      span_of("v", a->v, a->tokens, a->v_stride, a->cache.heads, a->v_head_stride, a->cache.dim, bytes), BATCH_SPANS(a)});
+    if (st != I4D_OK) return st;
     const OpContext o = op_context(ctx);
     AppendDev d = {};
     d.cache = cache_dev(a->cache);
@@ -571,6 +627,9 @@ i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* a) {
     if (st != I4D_OK) return st;
     if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
     OP_ARG(a->k_out && a->v_out && aligned(a->k_out, 16) && aligned(a->v_out, 16), "k_out and v_out need 16-byte alignment");
+    const int64_t rows = static_cast<int64_t>(a->tokens) * a->cache.heads * a->cache.dim;
+    st = check_apart(ctx, {span_of("k_out", a->k_out, rows, 2), span_of("v_out", a->v_out, rows, 2)}, {CACHE_SPANS(a->cache), BATCH_SPANS(a)});
+    if (st != I4D_OK) return st;
     const OpContext o = op_context(ctx);
     ReadDev d = {};
     d.cache = cache_dev(a->cache);
@@ -603,22 +662,26 @@ i4d_status i4d_kv8_attention_workspace(i4d_ctx* ctx, const i4d_kv8_attention_arg
 
 i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     if (!ctx) return I4D_ERR_ARG;
-    const i4d_status st = check_attention(ctx, a);
+    i4d_status st = check_attention(ctx, a);
     if (st != I4D_OK) return st;
     if (a->batch == 0 || a->tokens == 0 || a->max_q == 0) return I4D_OK;
     OP_ARG(a->q && a->out, "null q or out");
     const int bytes = dtype_bytes(a->dtype), dim = a->cache.dim;
     OP_ARG(aligned(a->q, bytes) && aligned(a->out, bytes) && aligned(a->lse, 4) && aligned(a->weights, 4), "misaligned buffer");
     OP_ARG(a->q_stride >= 0 && a->q_head_stride >= 0, "negative q stride");
-    const bool head_inner = a->out_head_stride >= dim && a->out_stride >= (a->heads - 1) * a->out_head_stride + dim;
-    const bool token_inner = a->out_stride >= dim && a->out_head_stride >= (a->tokens - 1) * a->out_stride + dim;
-    OP_ARG(head_inner || token_inner || (a->heads == 1 && a->out_stride >= dim) || (a->tokens == 1 && a->out_head_stride >= dim), "rows of out overlap");
-    OP_ARG(!overlap(span_of(a->q, a->tokens, a->q_stride, a->heads, a->q_head_stride, dim, bytes),
-                    span_of(a->out, a->tokens, a->out_stride, a->heads, a->out_head_stride, dim, bytes)), "out overlaps q");
+    const View vq = {"q", a->q, a->tokens, a->q_stride, a->heads, a->q_head_stride, dim, bytes};
+    const View vout = {"out", a->out, a->tokens, a->out_stride, a->heads, a->out_head_stride, dim, bytes};
+    OP_ARG(a->out_stride >= 0 && a->out_head_stride >= 0 && rows_apart(vout), "rows of out overlap");
+    OP_ARG(!overlap(vq, vout), "out overlaps q");
     OP_ARG(!a->weights || a->weights_stride >= a->max_length, "weights' rows are shorter than max_length");
     const OpContext o = op_context(ctx);
     const AttnPlan p = attn_plan(o, *a);
     const size_t need = p.bytes();
+    const Span weights = span_of("weights", a->weights, static_cast<int64_t>(a->batch) * a->cache.heads, a->weights_stride, 1, 0, a->max_length, 4);
+    const Span lse = span_of("lse", a->lse, static_cast<int64_t>(a->tokens) * a->heads, 4), space = span_of("workspace", a->workspace, need, 1);
+    st = check_apart(ctx, {vout.span(), lse, weights, space}, {CACHE_SPANS(a->cache), BATCH_SPANS(a)});
+    if (st == I4D_OK) st = check_apart(ctx, {lse, weights, space}, {vq.span()});
+    if (st != I4D_OK) return st;
     OP_ARG(need == 0 || (a->workspace && aligned(a->workspace, 16)), "null or misaligned workspace (%zu bytes needed)", need);
     if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
     AttnDev d = {};
@@ -688,20 +751,26 @@ i4d_status i4d_kv8_evict_workspace(i4d_ctx* ctx, const i4d_kv8_evict_args* a, si
 
 i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     if (!ctx) return I4D_ERR_ARG;
-    const i4d_status st = check_evict(ctx, a);
+    i4d_status st = check_evict(ctx, a);
     if (st != I4D_OK) return st;
     if (a->batch == 0) return I4D_OK;
     OP_ARG(a->lengths && a->lengths_out && a->keep && a->block_table && a->weights && a->weights_out, "null buffer");
     OP_ARG(aligned(a->lengths, 4) && aligned(a->lengths_out, 4) && aligned(a->keep, 4) && aligned(a->block_table, 4) &&
                aligned(a->weights, 4) && aligned(a->weights_out, 4), "arrays need 4-byte alignment");
     const int heads = a->cache.heads;
-    OP_ARG(!overlap(span_of(a->lengths, 1, 0, 1, 0, a->batch, 4), span_of(a->lengths_out, 1, 0, 1, 0, a->batch, 4)), "lengths_out overlaps lengths");
-    const Span win = span_of(a->weights, static_cast<int64_t>(a->batch) * heads, a->weights_stride, 1, 0, a->max_length, 4);
-    const Span wout = span_of(a->weights_out, static_cast<int64_t>(a->batch) * heads, a->weights_out_stride, 1, 0, a->max_length, 4);
-    OP_ARG((a->weights == a->weights_out && a->weights_stride == a->weights_out_stride) || !overlap(win, wout), "weights_out overlaps weights");
     const size_t need = evict_workspace(*a);
     OP_ARG(need == 0 || (a->workspace && aligned(a->workspace, 16)), "null or misaligned workspace (%zu bytes needed)", need);
     if (a->workspace_bytes < need) return op_fail(ctx, I4D_ERR_SIZE, "workspace of %zu bytes; %zu needed", a->workspace_bytes, need);
+    const int64_t weight_rows = static_cast<int64_t>(a->batch) * heads;
+    const Span win = span_of("weights", a->weights, weight_rows, a->weights_stride, 1, 0, a->max_length, 4);
+    const Span wout = span_of("weights_out", a->weights_out, weight_rows, a->weights_out_stride, 1, 0, a->max_length, 4);
+    OP_ARG((a->weights == a->weights_out && a->weights_stride == a->weights_out_stride) || !overlap(win, wout), "weights_out overlaps weights");
+    st = check_apart(ctx, {wout, span_of("lengths_out", a->lengths_out, a->batch, 4), span_of("keep", a->keep, weight_rows * a->budget, 4),
+                           span_of("workspace", a->workspace, need, 1), CACHE_SPANS(a->cache)},
+                     {span_of("lengths", a->lengths, a->batch, 4), span_of("block_table", a->block_table, a->batch, a->table_stride, 1, 0, a->table_blocks, 4)});
+    if (st == I4D_OK) st = check_apart(ctx, {span_of("lengths_out", a->lengths_out, a->batch, 4), span_of("keep", a->keep, weight_rows * a->budget, 4),
+                                             span_of("workspace", a->workspace, need, 1), CACHE_SPANS(a->cache)}, {win});
+    if (st != I4D_OK) return st;
     const OpContext o = op_context(ctx);
     EvictDev d = {};
     d.cache = cache_dev(a->cache);
@@ -730,13 +799,8 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     OP_CK(launch_cluster(k_kv8_select, static_cast<unsigned>(rows * ctas), kSelectThreads, 0, ctas, s, d, ctas));
     if (a->max_length > a->budget) {
         const unsigned grid = static_cast<unsigned>(rows * 2 * movers);
-        const bool int8 = a->cache.code == I4D_CODE_INT8;
-        if (move_pieces(a->cache.dim) == 2)
-            OP_CK(int8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8, 2>, grid, kMoveThreads, 0, movers, s, d, movers)
-                       : launch_cluster(k_kv8_move<I4D_CODE_E4M3, 2>, grid, kMoveThreads, 0, movers, s, d, movers));
-        else
-            OP_CK(int8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8, 4>, grid, kMoveThreads, 0, movers, s, d, movers)
-                       : launch_cluster(k_kv8_move<I4D_CODE_E4M3, 4>, grid, kMoveThreads, 0, movers, s, d, movers));
+        OP_CK(a->cache.code == I4D_CODE_INT8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8>, grid, kMoveThreads, 0, movers, s, d, movers)
+                                             : launch_cluster(k_kv8_move<I4D_CODE_E4M3>, grid, kMoveThreads, 0, movers, s, d, movers));
     }
     return I4D_OK;
 }
@@ -753,13 +817,26 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     OP_ARG(a->stride >= 0 && (a->rows == 1 || a->out_stride >= a->vocab), "stride %lld, out_stride %lld for %d entries",
            static_cast<long long>(a->stride), static_cast<long long>(a->out_stride), a->vocab);
     OP_ARG((a->logits == a->out && a->stride == a->out_stride) ||
-               !overlap(span_of(a->logits, a->rows, a->stride, 1, 0, a->vocab, bytes), span_of(a->out, a->rows, a->out_stride, 1, 0, a->vocab, bytes)),
+               !overlap(View{"logits", a->logits, a->rows, a->stride, 1, 0, a->vocab, bytes}, View{"out", a->out, a->rows, a->out_stride, 1, 0, a->vocab, bytes}),
            "out overlaps logits");
     OP_ARG(!a->history || (a->history_len && a->history_stride >= 0 && a->history_max >= 0 && a->history_max <= kMaxTokens), "history without history_len, or bad history_stride or history_max");
     OP_ARG(a->history || !(a->repetition || a->frequency || a->presence || a->prompt_len), "penalties without a history");
     OP_ARG(!a->bias_ids == !a->bias_values && !a->bias_ids == !a->bias_len, "bias_ids, bias_values and bias_len go together");
     OP_ARG(!a->bias_ids || (a->bias_stride >= 0 && a->bias_max >= 0 && a->bias_max <= kMaxTokens), "bad bias_stride or bias_max");
     OP_ARG(!a->mask || a->mask_stride >= 0, "negative mask_stride");
+    const Span out = span_of("out", a->out, a->rows, a->out_stride, 1, 0, a->vocab, bytes), best = span_of("best", a->best, a->rows, 4);
+    i4d_status st = check_apart(
+        ctx, {out, best},
+        {span_of("history", a->history, a->rows, a->history_stride, 1, 0, a->history_max, 4), span_of("history_len", a->history_len, a->rows, 4),
+         span_of("prompt_len", a->prompt_len, a->rows, 4), span_of("repetition", a->repetition, a->rows, 4), span_of("frequency", a->frequency, a->rows, 4),
+         span_of("presence", a->presence, a->rows, 4), span_of("bias_ids", a->bias_ids, a->rows, a->bias_stride, 1, 0, a->bias_max, 4),
+         span_of("bias_values", a->bias_values, a->rows, a->bias_stride, 1, 0, a->bias_max, 4), span_of("bias_len", a->bias_len, a->rows, 4),
+         span_of("mask", a->mask, a->rows, a->mask_stride, 1, 0, (a->vocab + 31) / 32, 4)});
+    if (st == I4D_OK) st = check_apart(ctx, {best}, {span_of("logits", a->logits, a->rows, a->stride, 1, 0, a->vocab, bytes)});
+    if (st != I4D_OK) return st;
+    OP_ARG(aligned(a->best, 4) && aligned(a->history, 4) && aligned(a->history_len, 4) && aligned(a->prompt_len, 4) && aligned(a->repetition, 4) &&
+               aligned(a->frequency, 4) && aligned(a->presence, 4) && aligned(a->bias_ids, 4) && aligned(a->bias_values, 4) && aligned(a->bias_len, 4) &&
+               aligned(a->mask, 4), "arrays need 4-byte alignment");
     LogitsDev d = {};
     d.in = a->logits;
     d.out = a->out;

@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include "i4d.h"
+#include "i4d_seq.h"
 
 namespace i4d_ops {
 
@@ -19,8 +20,6 @@ namespace i4d_ops {
 constexpr unsigned kBadSequence = 1u;  // q_start or lengths outside what the call's arguments allow
 constexpr unsigned kBadBlock = 2u;     // a block id outside the pool
 constexpr unsigned kTimeout = 4u;      // a bounded wait gave up
-
-constexpr int kMaxTokens = 1 << 30;  // of one sequence, so that a block's end is an int
 
 template <int DT>
 struct ElemOf;
@@ -92,8 +91,7 @@ struct Seq {
 // A sequence whose arrays contradict the call's bounds is skipped (n = 0).
 __device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) {
     const int q0 = __ldg(a.q_start + b), q1 = __ldg(a.q_start + b + 1), len = __ldg(a.lengths + b);
-    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.tokens && q1 - q0 <= a.max_q && len >= q1 - q0 &&
-                    len <= static_cast<int64_t>(a.table_blocks) * a.block_tokens && len <= kMaxTokens;
+    const bool ok = seq_ok(q0, q1, len, a.tokens, a.max_q, a.table_blocks, a.block_tokens);
     if (!ok && report) atomicOr(a.err, kBadSequence);
     return {q0, ok ? q1 - q0 : 0, ok ? len : 0};
 }
@@ -101,7 +99,7 @@ __device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) 
 // Block id of a table entry, or -1 for one outside the pool.
 __device__ __forceinline__ int load_block(const SeqArrays& a, int b, int j, bool report) {
     const int id = __ldg(a.table + static_cast<int64_t>(b) * a.table_stride + j);
-    if (static_cast<unsigned>(id) < static_cast<unsigned>(a.blocks)) return id;
+    if (block_ok(id, a.blocks)) return id;
     if (report) atomicOr(a.err, kBadBlock);
     return -1;
 }

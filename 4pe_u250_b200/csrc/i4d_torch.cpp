@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <Python.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -97,6 +98,7 @@ class Args {
         if (o == Py_None && none_ok) return nullptr;
         if (!THPVariable_Check(o)) refuse("%s is not a tensor", what);
         const at::Tensor& t = THPVariable_Unpack(o);
+        if (t.requires_grad() && c10::GradMode::is_enabled()) refuse("%s requires a gradient, which the operators do not give: call them under torch.no_grad()", what);
         if (!t.is_cuda() || t.get_device() != device_) refuse("%s is not on GPU %d", what, device_);
         if (t.dim() != dims) refuse("%s has %lld dimensions, not %d", what, static_cast<long long>(t.dim()), dims);
         if (dims && t.size(-1) > 1 && t.stride(-1) != 1) refuse("%s is not contiguous in its last dimension", what);
@@ -311,8 +313,8 @@ at::Tensor workspace(Args& a, size_t need) {
 
 void weights_shape(const at::Tensor& w, const char* what, int64_t batch, int64_t heads, int64_t length) {
     if (w.size(0) != batch || w.size(1) != heads || w.size(2) < length) refuse("%s is [batch, cache heads, >= max_length]", what);
-    if (batch > 1 && w.stride(0) != heads * w.stride(1)) refuse("%s has gaps between its sequences", what);
-    if (heads > 1 && w.stride(1) < w.size(2)) refuse("rows of %s overlap", what);
+    if (batch > 1 && heads > 1 && w.stride(0) != heads * w.stride(1)) refuse("%s has gaps between its sequences", what);
+    if ((heads > 1 && w.stride(1) < w.size(2)) || (batch > 1 && w.stride(0) < w.size(2))) refuse("rows of %s overlap", what);
 }
 
 PyObject* kv8_attention(Args& a) {
