@@ -522,7 +522,7 @@ __device__ __forceinline__ void store_lse(const AttnDev& a, const Seq& s, int h,
     const int64_t at = (s.first + row / a.group) * static_cast<int64_t>(a.heads) + h * a.group + row % a.group;
     const float l2 = stats.y == 0.f ? -INFINITY : stats.x + log2f(stats.y);
     if (a.lse) a.lse[at] = l2 * kLn2;
-    if (a.weights) a.lse2[at] = l2;
+    if (a.weights) a.lse2[at] = l2 == -INFINITY ? INFINITY : l2;  // a row that saw nothing weighs nothing: 2^(x - inf)
 }
 
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
@@ -555,7 +555,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
             for (int j = 0; j < 4; ++j) acc[i][nt][j] = 0.f;
 
     if (begin < end) {
-        const int bs = a.cache.block_tokens, dim = a.cache.dim, shift = 31 - __clz(bs);
+        const int bs = a.cache.block_tokens, shift = 31 - __clz(bs);
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(attn_ring)) + warp * kSlots * 32 * DT;
         const uint32_t bars = static_cast<uint32_t>(__cvta_generic_to_shared(s_bar)) + warp * kSlots * 8;
         QTile<DT, NT, HLQ> q;

@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
             if (piece.whole) {
                 const float l2 = l == 0.f ? -INFINITY : M + log2f(l);
                 if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-                if (a.weights) a.lse2[tok * a.heads + head] = l2;
+                if (a.weights) a.lse2[tok * a.heads + head] = l2 == -INFINITY ? INFINITY : l2;
             } else {
                 a.stats[part] = make_float4(M, l, R, 0.f);
             }
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(256) k_kv8_prompt_join(AttnDev a) {
         if (lane == 0) {
             const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
             if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-            if (a.weights) a.lse2[tok * a.heads + head] = l2;
+            if (a.weights) a.lse2[tok * a.heads + head] = l2 == -INFINITY ? INFINITY : l2;
         }
     }
 }
