@@ -26,6 +26,8 @@ __device__ __forceinline__ int64_t code_offset(const Kv8Dev& c, int block, int h
 
 // ---------------------------------------------------------------- append
 
+constexpr int kAppendHeld = 4;  // groups of eight values that a thread holds
+
 struct AppendDev {
     Kv8Dev cache;
     SeqArrays seq;
@@ -34,23 +36,23 @@ struct AppendDev {
     int touched;  // blocks that a sequence of max_q new tokens can touch
 };
 
+// Eight values as they lie in memory.
 template <typename T, int V>
-__device__ __forceinline__ void load8(const T* p, float out[8]) {
-    if constexpr (V == 8) {
-        const Vec<T, 8> x = load_vec<T, 8>(p);
+__device__ __forceinline__ Vec<T, 8> load8(const T* p) {
+    if constexpr (V == 8) return load_vec<T, 8>(p);
+    Vec<T, 8> x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = to_f32(x.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = to_f32(p[i]);
-    }
+    for (int i = 0; i < 8; ++i) x.v[i] = p[i];
+    return x;
 }
 
 // One unit (sequence, touched block, head, K or V) for each group of
 // THREADS threads.  Two passes over the new values: the largest, then the
-// codes (the second pass reads L1/L2).  Bound: the values in, the codes out.
+// codes.  The first four groups of eight of each thread stay in registers between them, in
+// their own type, which covers blocks of 8192 values (64 tokens of 128); the
+// rest is read again from L1/L2.  Bound: the values in, the codes out.
 template <typename T, int V, int CODE, int THREADS>
-__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_kv8_append(AppendDev a, int units) {
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append(AppendDev a, int units) {
     constexpr int kPerCta = THREADS < 128 ? 128 / THREADS : 1;
     constexpr int kWarps = THREADS / 32;
     const int tid = threadIdx.x % THREADS;
@@ -65,24 +67,31 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_kv8_append(Ap
     const int bs = a.cache.block_tokens, dim = a.cache.dim;
     const int first = s.len - s.n, blk = first / bs + j;
     if (blk * bs >= s.len) return;
-    const int id = load_block(a.seq, b, blk, report);
-    if (id < 0) return;
     const int lo = max(first, blk * bs), hi = min(s.len, (blk + 1) * bs), old = lo - blk * bs;
     const T* in = static_cast<const T*>(a.in[which]) + static_cast<int64_t>(s.first + lo - first) * a.tok[which] +
                   h * a.head[which];
+    const int per_tok = dim / 8, items = (hi - lo) * per_tok;
+    auto load = [&](int i) { return load8<T, V>(in + static_cast<int64_t>(i / per_tok) * a.tok[which] + i % per_tok * 8); };
+    Vec<T, 8> held[kAppendHeld];  // on their way before the block's id is known
+#pragma unroll
+    for (int k = 0; k < kAppendHeld; ++k)
+        if (k * THREADS + tid < items) held[k] = load(k * THREADS + tid);
+    const int id = load_block(a.seq, b, blk, report);
+    if (id < 0) return;
     float* scale = a.cache.scale[which] + static_cast<int64_t>(id) * a.cache.heads + h;
     const float had = old ? *scale : 0.f;
-    const int per_tok = dim / 8, items = (hi - lo) * per_tok;
     float amax = 0.f;
-    for (int i = tid; i < items; i += THREADS) {
-        float x[8];
-        load8<T, V>(in + static_cast<int64_t>(i / per_tok) * a.tok[which] + i % per_tok * 8, x);
+    auto measure = [&](const Vec<T, 8>& x) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float m = fabsf(x[k]);
+            const float m = fabsf(to_f32(x.v[k]));
             amax = m < INFINITY ? fmaxf(amax, m) : amax;
         }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kAppendHeld; ++k)
+        if (k * THREADS + tid < items) measure(held[k]);
+    for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS) measure(load(i));
     amax = warp_max(amax);
     if constexpr (kWarps > 1) {
         __shared__ float part[kWarps];
@@ -107,13 +116,16 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_kv8_append(Ap
     const bool power = (__float_as_int(now) & 0x7fffff) == 0;
     const float inv = power ? __fdiv_rn(1.f, now) : 0.f;
     uint2* p = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(old) * dim);
-    for (int i = tid; i < items; i += THREADS) {
+    auto put = [&](int i, const Vec<T, 8>& v) {
         float x[8];
-        load8<T, V>(in + static_cast<int64_t>(i / per_tok) * a.tok[which] + i % per_tok * 8, x);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = power ? __fmul_rn(x[k], inv) : __fdiv_rn(x[k], now);
+        for (int k = 0; k < 8; ++k) x[k] = power ? __fmul_rn(to_f32(v.v[k]), inv) : __fdiv_rn(to_f32(v.v[k]), now);
         p[i] = make_uint2(encode4<CODE>(x[0], x[1], x[2], x[3]), encode4<CODE>(x[4], x[5], x[6], x[7]));
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kAppendHeld; ++k)
+        if (k * THREADS + tid < items) put(k * THREADS + tid, held[k]);
+    for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS) put(i, load(i));
 }
 
 // ------------------------------------------------------------------ read
