@@ -173,6 +173,32 @@ __device__ __forceinline__ void store_out(const AttnDev& a, int64_t i, float v) 
     else static_cast<__half*>(a.out)[i] = __float2half_rn(v);
 }
 
+// Four neighbouring values from a multiple of four on.
+__device__ __forceinline__ void store_out4(const AttnDev& a, int64_t i, float4 v) {
+    if (!a.wide_out) {
+        store_out(a, i, v.x);
+        store_out(a, i + 1, v.y);
+        store_out(a, i + 2, v.z);
+        store_out(a, i + 3, v.w);
+    } else if (a.dtype == I4D_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + i) = v;
+    } else {
+        union {
+            __nv_bfloat162 b[2];
+            __half2 h[2];
+            uint2 w;
+        } u;
+        if (a.dtype == I4D_BF16) {
+            u.b[0] = __floats2bfloat162_rn(v.x, v.y);
+            u.b[1] = __floats2bfloat162_rn(v.z, v.w);
+        } else {
+            u.h[0] = __floats2half2_rn(v.x, v.y);
+            u.h[1] = __floats2half2_rn(v.z, v.w);
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + i) = u.w;
+    }
+}
+
 // First of the 16 dims of lane t's piece c of a token's codes: neighbouring
 // pieces, so that two rows of an access phase take the even and the odd pieces
 // of a swizzled row and hit all banks.
@@ -511,10 +537,7 @@ struct Piece {
 // Four values of a finished row from dim d on.
 __device__ __forceinline__ void store_row(const AttnDev& a, const Seq& s, int h, int row, int d, float4 o) {
     const int64_t at = (s.first + row / a.group) * a.out_tok + (h * a.group + row % a.group) * a.out_head + d;
-    store_out(a, at, o.x);
-    store_out(a, at + 1, o.y);
-    store_out(a, at + 2, o.z);
-    store_out(a, at + 3, o.w);
+    store_out4(a, at, o);
 }
 
 // stats: M, l of a finished row.

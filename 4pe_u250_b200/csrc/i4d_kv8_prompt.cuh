@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 
 // Joins the pieces of a segment that several CTAs of k_kv8_prompt shared:
 // blockIdx.x / 8 + 1 is the first CTA whose share begins inside the segment,
-// blockIdx.x % 8 the 32 rows; a warp for a row at a time.
+// blockIdx.x % 8 the 32 rows.
 __global__ void __launch_bounds__(256) k_kv8_prompt_join(AttnDev a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ int64_t s_sums[8], s_before;
@@ -740,46 +740,55 @@ __global__ void __launch_bounds__(256) k_kv8_prompt_join(AttnDev a) {
     const int64_t seg0 = s_before + static_cast<int64_t>(h) * span.tiles, seg1 = seg0 + span.tiles;
     if (u == seg0 || u - share > seg0) return;  // no CTA's share begins inside, or an earlier one's does
     const int c0 = c - 1, c1 = static_cast<int>((seg1 - 1) / share);
-    for (int r = (blockIdx.x & 7) * 32 + (threadIdx.x >> 5); r < min(span.live, (static_cast<int>(blockIdx.x) & 7) * 32 + 32); r += 8) {
-        // the first CTA's last piece (or its only one), the others' first
-        auto index = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 && share * c0 < seg0 ? 1 : 0)) * kPrRows + r; };
-        float m = -INFINITY, rr = -INFINITY, sum = 0.f;
-        for (int k = c0 + lane; k <= c1; k += 32) {
-            const float4 x = a.stats[index(k)];
-            m = fmaxf(m, x.x);
-            rr = fmaxf(rr, x.z);
+    // Four rows a warp, eight lanes each, so that all their loads are on their way at once.
+    const int sub = lane & 7, r = (blockIdx.x & 7) * 32 + (threadIdx.x >> 3);
+    const bool live = r < span.live;
+    // the first CTA's last piece (or its only one), the others' first
+    auto index = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 && share * c0 < seg0 ? 1 : 0)) * kPrRows + (live ? r : 0); };
+    float m = -INFINITY, rr = -INFINITY, sum = 0.f;
+    for (int k = c0 + sub; k <= c1; k += 8) {
+        const float4 x = a.stats[index(k)];
+        m = fmaxf(m, x.x);
+        rr = fmaxf(rr, x.z);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        rr = fmaxf(rr, __shfl_xor_sync(~0u, rr, o));
+    }
+    float4 acc[4] = {};
+#pragma unroll 2
+    for (int k = c0; k <= c1; ++k) {
+        const float4 x = a.stats[index(k)];
+        const float4* part = reinterpret_cast<const float4*>(a.part + index(k) * dim);
+        float4 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = 4 * (8 * j + sub) < dim ? part[8 * j + sub] : make_float4(0.f, 0.f, 0.f, 0.f);
+        sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
+        const float f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[j].x += y[j].x * f;
+            acc[j].y += y[j].y * f;
+            acc[j].z += y[j].z * f;
+            acc[j].w += y[j].w * f;
         }
-        m = warp_max(m);
-        rr = warp_max(rr);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = c0; k <= c1; ++k) {
-            const float4 x = a.stats[index(k)];
-            sum += x.y * (x.x == -INFINITY ? 1.f : ex2(x.x - m));
-            const float f = x.z == -INFINITY ? 1.f : ex2(x.z - rr);
-            if (4 * lane < dim) {
-                const float4 y = *reinterpret_cast<const float4*>(a.part + index(k) * dim + 4 * lane);
-                o.x += y.x * f;
-                o.y += y.y * f;
-                o.z += y.z * f;
-                o.w += y.w * f;
-            }
-        }
-        const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
-        const int row = rt * kPrRows + r;
-        const int64_t tok = s.first + row / a.group;
-        const int head = h * a.group + row % a.group;
-        if (4 * lane < dim) {
-            const int64_t to = tok * a.out_tok + head * a.out_head + 4 * lane;
-            store_out(a, to, o.x * back);
-            store_out(a, to + 1, o.y * back);
-            store_out(a, to + 2, o.z * back);
-            store_out(a, to + 3, o.w * back);
-        }
-        if (lane == 0) {
-            const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-            if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
-            if (a.weights) a.lse2[tok * a.heads + head] = l2 == -INFINITY ? INFINITY : l2;
-        }
+    }
+    if (!live) return;
+    const float back = sum == 0.f || rr == -INFINITY ? 0.f : ex2(rr - m) / sum;
+    const int row = rt * kPrRows + r;
+    const int64_t tok = s.first + row / a.group;
+    const int head = h * a.group + row % a.group;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (4 * (8 * j + sub) >= dim) continue;
+        store_out4(a, tok * a.out_tok + head * a.out_head + 4 * (8 * j + sub),
+                   make_float4(acc[j].x * back, acc[j].y * back, acc[j].z * back, acc[j].w * back));
+    }
+    if (sub == 0) {
+        const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
+        if (a.lse) a.lse[tok * a.heads + head] = l2 * kLn2;
+        if (a.weights) a.lse2[tok * a.heads + head] = l2 == -INFINITY ? INFINITY : l2;
     }
 }
 
