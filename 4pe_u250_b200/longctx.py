@@ -114,7 +114,10 @@ class KV8Cache:
     def empty(cls, blocks, heads, block_tokens, dim, code="int8", device="cuda"):
         """A cache with zeroed codes and scales."""
         import torch
-        kind = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[code]
+        kinds = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+        if code not in kinds:
+            raise _error(f"code {code!r} is none of {sorted(kinds)}")
+        kind = kinds[code]
         k, v = (torch.zeros(blocks, heads, block_tokens, dim, dtype=torch.int8, device=device).view(kind) for _ in range(2))
         return cls(k, v, *(torch.zeros(blocks, heads, device=device) for _ in range(2)))
 

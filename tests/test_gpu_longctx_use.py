@@ -315,6 +315,7 @@ def test_binding_refuses(pkg, ctx):
         lambda: ctx.logits_process(torch.zeros(2, 9, device="cuda"), best=torch.zeros(3, dtype=torch.int32, device="cuda")),
         lambda: pkg.KV8Cache(s.cache.k, s.cache.v, s.cache.k_scale.half(), s.cache.v_scale),
         lambda: pkg.KV8Cache(s.cache.k.cpu(), s.cache.v.cpu(), s.cache.k_scale.cpu(), s.cache.v_scale.cpu()),
+        lambda: pkg.KV8Cache.empty(4, 2, 16, 64, "int4"),
         lambda: pkg.RopeTable(65),
         lambda: pkg.RopeTable(64, scaling="other"),
     ]
@@ -393,6 +394,35 @@ def test_evict_long_rows(pkg, ctx, length, budget, recent):
         for j in range(-(-n // 128)):
             part, blk = min(128, n - j * 128), s.table[0, j]
             assert np.array_equal(got[blk, :, :part], want.codes[0][blk, :, :part]) and np.array_equal(sc[blk], want.scale[0][blk])
+
+
+def test_cache_beyond_32_bit_offsets(pkg, ctx):
+    """Blocks 4.4 GB into the codes give what the same blocks of a small cache give."""
+    torch = _torch()
+    dim, bs, heads, far = 128, 128, 2, 136000  # 32 KB a block
+    lens, q_lens = [300, 90], [3, 90]
+    near = Setup(pkg, lens, heads, dim, bs, "int8", 109)
+    low = -(-near.cache.blocks // 8) * 8
+    big = pkg.KV8Cache.empty(far + low, heads, bs, dim, "int8")
+    for a, b in ((big.k, near.cache.k), (big.v, near.cache.v), (big.k_scale, near.cache.k_scale), (big.v_scale, near.cache.v_scale)):
+        a[far:far + near.cache.blocks] = b
+    start, n = near.dev(_starts(q_lens)), near.dev(lens)
+    tables = near.dev(near.table), near.dev(near.table + far)
+    g = torch.Generator().manual_seed(5)
+    rows = (torch.randn(93, 8, dim, generator=g)).bfloat16().cuda()
+    results = []
+    for cache, table in zip((near.cache, big), tables):
+        ctx.kv8_append(cache, rows[:, :2], rows[:, 2:4], start, n, table, 90)
+        weights = torch.zeros(2, heads, 300, device="cuda")
+        out = [ctx.kv8_attention(cache, rows[:, :h], start, n, table, 90, 300, weights=weights) for h in (2, 8)]
+        one = ctx.kv8_attention(cache, rows[:2], near.dev([0, 1, 2]), n, table, 1, 300, weights=weights)
+        back = ctx.kv8_read(cache, start, n, table, 90, 93)
+        lo, keep, _ = ctx.kv8_evict(cache, n, table, weights, 70, 10, 300)
+        after = ctx.kv8_read(cache, near.dev([0, 70, 140]), lo, table, 70, 140)
+        results.append([*out, one, *back, lo, keep, weights, *after])
+    ctx.ops_check()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert torch.all(big.k[:far].view(torch.int64) == 0)  # nothing below them was written
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
