@@ -71,35 +71,60 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append
     const T* in = static_cast<const T*>(a.in[which]) + static_cast<int64_t>(s.first + lo - first) * a.tok[which] +
                   h * a.head[which];
     const int per_tok = dim / 8, items = (hi - lo) * per_tok;
-    auto load = [&](int i) { return load8<T, V>(in + static_cast<int64_t>(i / per_tok) * a.tok[which] + i % per_tok * 8); };
+    // item i of eight values: token i / per_tok, values from 8 * (i % per_tok); this thread's lie THREADS apart
+    const int step_tok = THREADS / per_tok, step_part = THREADS % per_tok;
+    struct Place {
+        int tok, part;
+    };
+    auto start = [&]() -> Place { return {tid / per_tok, tid % per_tok}; };
+    auto advance = [&](Place& x) {
+        x.tok += step_tok;
+        x.part += step_part;
+        if (x.part >= per_tok) {
+            x.part -= per_tok;
+            ++x.tok;
+        }
+    };
+    auto load = [&](const Place& x) { return load8<T, V>(in + static_cast<int64_t>(x.tok) * a.tok[which] + x.part * 8); };
     Vec<T, 8> held[kAppendHeld];  // on their way before the block's id is known
+    Place behind = start();
 #pragma unroll
-    for (int k = 0; k < kAppendHeld; ++k)
-        if (k * THREADS + tid < items) held[k] = load(k * THREADS + tid);
+    for (int k = 0; k < kAppendHeld; ++k) {
+        if (k * THREADS + tid < items) held[k] = load(behind);
+        advance(behind);
+    }
     const int id = load_block(a.seq, b, blk, report);
     if (id < 0) return;
     float* scale = a.cache.scale[which] + static_cast<int64_t>(id) * a.cache.heads + h;
     const float had = old ? *scale : 0.f;
-    float amax = 0.f;
-    auto measure = [&](const Vec<T, 8>& x) {
+    // The greatest magnitude (a maximum passes NaN over); only if that is an
+    // infinity, again without those.
+    auto greatest = [&](auto&& magnitude) {
+        float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float m = fabsf(to_f32(x.v[k]));
-            amax = m < INFINITY ? fmaxf(amax, m) : amax;
+        for (int k = 0; k < kAppendHeld; ++k)
+            if (k * THREADS + tid < items)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, magnitude(to_f32(held[k].v[j])));
+        Place at = behind;
+        for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS, advance(at)) {
+            const Vec<T, 8> x = load(at);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, magnitude(to_f32(x.v[j])));
         }
+        amax = warp_max(amax);
+        if constexpr (kWarps > 1) {
+            __shared__ float part[kWarps];
+            __syncthreads();
+            if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, part[w]);
+        }
+        return amax;
     };
-#pragma unroll
-    for (int k = 0; k < kAppendHeld; ++k)
-        if (k * THREADS + tid < items) measure(held[k]);
-    for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS) measure(load(i));
-    amax = warp_max(amax);
-    if constexpr (kWarps > 1) {
-        __shared__ float part[kWarps];
-        if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = amax;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, part[w]);
-    }
+    float amax = greatest([](float x) { return fabsf(x); });
+    if (amax == INFINITY) amax = greatest([](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; });
     const float now = fmaxf(power_scale(amax, CODE), had);
     if (tid == 0) *scale = now;  // every thread has read `had` (the barrier above, or the shuffles)
     uint8_t* codes = a.cache.codes[which] + code_offset(a.cache, id, h);
@@ -125,7 +150,7 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append
 #pragma unroll
     for (int k = 0; k < kAppendHeld; ++k)
         if (k * THREADS + tid < items) put(k * THREADS + tid, held[k]);
-    for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS) put(i, load(i));
+    for (int i = kAppendHeld * THREADS + tid; i < items; i += THREADS, advance(behind)) put(i, load(behind));
 }
 
 // ------------------------------------------------------------------ read

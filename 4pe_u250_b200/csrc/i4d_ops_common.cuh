@@ -120,19 +120,19 @@ __device__ __forceinline__ float power_scale(float amax, int code) {
 // largest code, else the nearest with ties to even.
 template <int CODE>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-    a = a == a ? a : 0.f;
-    b = b == b ? b : 0.f;
-    c = c == c ? c : 0.f;
-    d = d == d ? d : 0.f;
     if constexpr (CODE == I4D_CODE_INT8) {
-        const int ia = __float2int_rn(fminf(fmaxf(a, -127.f), 127.f)), ib = __float2int_rn(fminf(fmaxf(b, -127.f), 127.f));
-        const int ic = __float2int_rn(fminf(fmaxf(c, -127.f), 127.f)), id = __float2int_rn(fminf(fmaxf(d, -127.f), 127.f));
+        // (a conversion to an integer saturates and makes 0 of NaN)
+        const int ia = max(min(__float2int_rn(a), 127), -127), ib = max(min(__float2int_rn(b), 127), -127);
+        const int ic = max(min(__float2int_rn(c), 127), -127), id = max(min(__float2int_rn(d), 127), -127);
         return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
     } else {
         uint16_t lo, hi;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-        return lo | static_cast<uint32_t>(hi) << 16;
+        const uint32_t w = lo | static_cast<uint32_t>(hi) << 16;
+        // NaN alone becomes 0x7f or 0xff
+        const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u;
+        return nan ? w & ~((nan >> 7) * 255u) : w;
     }
 }
 
