@@ -229,24 +229,25 @@ __device__ __forceinline__ int evict_length(const EvictDev& a, int b, bool repor
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 
-// Inclusive sum over the CTA of one value a thread; *total receives the sum.
-__device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// Inclusive sum over the warp.
+__device__ __forceinline__ int warp_scan(int x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(~0u, x, o);
-        if (lane >= o) x += y;
+        if ((threadIdx.x & 31) >= o) x += y;
     }
+    return x;
+}
+
+// Inclusive sum over the CTA of one value a thread; *total receives the sum.
+__device__ __forceinline__ int cta_scan(int x, int* warp_sums, int* total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    x = warp_scan(x);
     __syncthreads();
     if (lane == 31) warp_sums[w] = x;
     __syncthreads();
     if (w == 0) {
-        int y = lane < kSelectWarps ? warp_sums[lane] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(~0u, y, o);
-            if (lane >= o) y += z;
-        }
+        const int y = warp_scan(lane < kSelectWarps ? warp_sums[lane] : 0);
         if (lane < kSelectWarps) warp_sums[lane] = y;
     }
     __syncthreads();
@@ -267,12 +268,13 @@ constexpr int kSelectHeld = 16;  // weights that a thread holds in registers
 // read once into registers.  Bound: the chain of cluster barriers.
 __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, int ctas) {
     __shared__ __align__(16) int hist[kSelectBins];
+    __shared__ __align__(8) int groups[kSelectBins / 32];
     __shared__ int sums[32];
     __shared__ int chosen, above;
-    __shared__ int counts[2];
+    __shared__ __align__(8) int counts[2];
     cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
     const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
-    const int b = row / a.cache.heads, h = row % a.cache.heads, tid = threadIdx.x;
+    const int b = row / a.cache.heads, h = row % a.cache.heads, tid = threadIdx.x, lane = tid & 31;
     const int len = evict_length(a, b, tid == 0 && h == 0 && rank == 0);
     const float* w = a.weights + row * a.weights_stride;
     float* wo = a.weights_out + row * a.weights_out_stride;
@@ -308,33 +310,43 @@ __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, in
             const uint32_t k = weight_key(x);
             if (i < free_len && (k & high) == key) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
         });
-        cl.sync();
-        // the cluster's sums of the four bins from the greatest that are this thread's
-        const int bin = kSelectBins - 4 - 4 * tid;  // bin + 3 is the greatest
-        int4 n4 = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        // Sums of 32 bins each, so that the search reads these of all CTAs and
+        // then one group of their bins, not every bin (5 us a pass with all).
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (c >= ctas) break;
-            const int4 x = *reinterpret_cast<const int4*>(cl.map_shared_rank(hist, c) + bin);
-            n4.x += x.x;
-            n4.y += x.y;
-            n4.z += x.z;
-            n4.w += x.w;
+        for (int k = 0; k < kSelectBins / 32 / kSelectWarps; ++k) {
+            const int g = (tid >> 5) * (kSelectBins / 32 / kSelectWarps) + k;
+            const int sum = __reduce_add_sync(~0u, hist[g * 32 + lane]);
+            if (lane == 0) groups[g] = sum;
         }
-        const int sum = n4.x + n4.y + n4.z + n4.w;
-        int total;
-        const int upto = cta_scan(sum, sums, &total), before = upto - sum;
-        if (upto >= want && before < want) {
-            int at = before, k = 3;
-            const int size[4] = {n4.x, n4.y, n4.z, n4.w};
+        cl.sync();
+        if (tid < 32) {
+            // groups 63 - 2 lane and 62 - 2 lane, from the greatest on
+            int2 n = make_int2(0, 0);
 #pragma unroll
-            for (int i = 3; i > 0; --i)
-                if (k == i && at + size[i] < want) {
-                    at += size[i];
-                    --k;
-                }
-            chosen = bin + k;
-            above = at;
+            for (int c = 0; c < 8; ++c) {
+                if (c >= ctas) break;
+                const int2 x = reinterpret_cast<const int2*>(cl.map_shared_rank(groups, c))[31 - lane];
+                n.x += x.x;
+                n.y += x.y;
+            }
+            const int before = warp_scan(n.x + n.y) - n.x - n.y;
+            const bool upper = before + n.y >= want;
+            const unsigned here = __ballot_sync(~0u, before < want && before + n.x + n.y >= want);
+            const int at = __shfl_sync(~0u, upper ? before : before + n.y, __ffs(here) - 1);
+            const int group = __shfl_sync(~0u, 63 - 2 * lane - !upper, __ffs(here) - 1);
+            const int bin = group * 32 + 31 - lane;
+            int m = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c >= ctas) break;
+                m += cl.map_shared_rank(hist, c)[bin];
+            }
+            const int upto = at + warp_scan(m);
+            if (upto >= want && upto - m < want) {
+                chosen = bin;
+                above = upto - m;
+            }
         }
         cl.sync();  // hist is read, chosen is written
         key |= static_cast<uint32_t>(chosen) << shift;
@@ -359,10 +371,12 @@ __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, in
     }
     cl.sync();
     int equal = same_upto - same, larger = more_upto - more;
-    for (int c = 0; c < rank; ++c) {
-        const int* other = cl.map_shared_rank(counts, c);
-        equal += other[0];
-        larger += other[1];
+#pragma unroll
+    for (int c = 0; c < 7; ++c) {
+        if (c >= rank) break;
+        const int2 other = *reinterpret_cast<const int2*>(cl.map_shared_rank(counts, c));
+        equal += other.x;
+        larger += other.y;
     }
     int place = larger + min(equal, want);
     // In place and more than the registers hold: the weights move after the

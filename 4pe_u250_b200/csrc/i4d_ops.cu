@@ -788,10 +788,11 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     d.max_length = a->max_length;
     const int64_t rows = static_cast<int64_t>(a->batch) * heads;
     // CTAs of a row of weights: two thousand or more each; of a moved row: a
-    // round's tokens each; eight at most (the portable cluster size).
+    // round's tokens each, no more than fit the GPU at once; eight at most (the
+    // portable cluster size).
     int ctas = 1, movers = 1;
     while (ctas < 8 && a->max_length / (2 * ctas) >= 2048) ctas *= 2;
-    while (movers < 8 && a->budget > movers * move_tokens(a->cache.dim)) movers *= 2;
+    while (movers < 8 && a->budget > movers * move_tokens(a->cache.dim) && rows * 4 * movers <= 2 * o.num_sms) movers *= 2;
     OP_ARG(rows * 2 * 8 <= kMaxGrid, "too many sequences in one call");
     DeviceScope scope(o.device);
     OP_CK(scope.error());
