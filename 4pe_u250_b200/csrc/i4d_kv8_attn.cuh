@@ -615,6 +615,10 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
                 if (!bar_wait(bars + slot * 8, phases >> slot & 1)) {
                     if (lane == 0) atomicOr(a.seq.err, kTimeout);
+                    for (int k = 1, ahead = slot; k < kSlots && i + k * kAttnWarps < tiles; ++k) {  // the copies behind it
+                        ahead = ahead == kSlots - 1 ? 0 : ahead + 1;
+                        bar_wait(bars + ahead * 8, phases >> ahead & 1);
+                    }
                     break;
                 }
                 phases ^= 1u << slot;

@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
     if (warp == 12) {  // ------------------------------------------- producer
         constexpr int kBoxBytes = 16 * DT;
         int n = 0;  // tiles so far, over all pieces
+        int sent[2] = {0, 0};  // of K, of V
         each_piece(a, u, u_end, before, pair, [&](const PrPiece& p) {
             bool ok = true;
             for (int j = p.j0; ok && j < p.j1; ++j, ++n) {
@@ -390,15 +391,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                                          base + L::raw + (st * 2 + which) * L::kRaw + lane * kBoxBytes),
                                      "l"(&a.maps[which]), "r"(0), "r"(row), "r"(bar)
                                      : "memory");
+                    ++sent[which];
                 }
             }
             return ok;
         });
         if (sh.abort)  // copies in flight land before the CTA leaves
-            for (int j = max(0, n - 2); j < n; ++j) {
-                bar_wait(bar_at(sh, kRawKFull + (j & 1)), j >> 1 & 1);
-                bar_wait(bar_at(sh, kRawVFull + (j & 1)), j >> 1 & 1);
-            }
+#pragma unroll
+            for (int which = 0; which < 2; ++which)
+                for (int j = max(0, sent[which] - 2); j < sent[which]; ++j)
+                    bar_wait(bar_at(sh, (which ? kRawVFull : kRawKFull) + (j & 1)), j >> 1 & 1);
     } else if (warp >= 13) {  // ------------------------------------- products
         const int t = warp - 13;  // the row tile
         if (lane == 0) {
