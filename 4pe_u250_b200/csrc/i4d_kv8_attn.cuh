@@ -818,6 +818,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
 
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(const __grid_constant__ AttnDev a) {
+    op_begin();
     constexpr int kRows = 8 * NT;
     extern __shared__ unsigned char attn_smem_base[];
     // the copies' swizzle counts from 1024-byte boundaries
@@ -881,8 +882,8 @@ constexpr int kJoinThreads = 512;
 // segment, whose warps take rows and, if there are fewer rows than warps,
 // every so-manieth piece of one, so that the pieces are read at once.
 __global__ void __launch_bounds__(kJoinThreads) k_kv8_join(AttnDev a, int rows_per_tile) {
+    op_begin();
     constexpr int kWarps = kJoinThreads / 32;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ float4 s_o[kWarps][64];
     __shared__ float s_sum[kWarps];
     const int4 segment = a.segments[blockIdx.x];
@@ -953,7 +954,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv8_join(AttnDev a, int rows_p
 // Probabilities summed over a head's few rows for each token, from the scores
 // that k_kv8_attn kept: four tokens a thread, rows in order.
 __global__ void __launch_bounds__(128) k_kv8_weights_kept(AttnDev a, int rows_per_tile, int chunks) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    op_begin();
     const int64_t bh = blockIdx.x / chunks;
     const int n = ((blockIdx.x % chunks) * 128 + threadIdx.x) * 4, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const Seq s = load_seq(a.seq, b, false);
@@ -983,6 +984,7 @@ __global__ void __launch_bounds__(128) k_kv8_weights_kept(AttnDev a, int rows_pe
 // 2^(x - lse2), a warp for 16 tokens, rows in order.
 template <int DT, int CODE, bool HL>
 __global__ void __launch_bounds__(kAttnThreads) k_kv8_weights(AttnDev a, int tiles) {
+    op_begin();
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const Seq s = load_seq(a.seq, b, false);

@@ -53,6 +53,7 @@ __device__ __forceinline__ Vec<T, 8> load8(const T* p) {
 // rest is read again from L1/L2.  Bound: the values in, the codes out.
 template <typename T, int V, int CODE, int THREADS>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append(AppendDev a, int units) {
+    op_begin();
     constexpr int kPerCta = THREADS < 128 ? 128 / THREADS : 1;
     constexpr int kWarps = THREADS / 32;
     const int tid = threadIdx.x % THREADS;
@@ -168,6 +169,7 @@ constexpr int kReadItems = 512;  // of a CTA of 256 threads
 // took 30 us for 1024 tokens of 32 heads).
 template <int CODE>
 __global__ void __launch_bounds__(256) k_kv8_read(ReadDev a, int chunks) {
+    op_begin();
     const int b = blockIdx.x / chunks, i0 = blockIdx.x % chunks * kReadItems;
     const Seq s = load_seq(a.seq, b, threadIdx.x == 0 && i0 == 0);
     const int bs = a.cache.block_tokens, shift = 31 - __clz(bs), per_head = a.cache.dim / 16, per_tok = a.cache.heads * per_head;
@@ -267,6 +269,7 @@ constexpr int kSelectHeld = 16;  // weights that a thread holds in registers
 // of the scales, which the move overwrites.  Rows of up to 65536 weights are
 // read once into registers.  Bound: the chain of cluster barriers.
 __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, int ctas) {
+    op_begin();
     __shared__ __align__(16) int hist[kSelectBins];
     __shared__ __align__(8) int groups[kSelectBins / 32];
     __shared__ int sums[32];
@@ -440,6 +443,7 @@ __host__ __device__ constexpr int move_tokens(int dim) { return kMovePieces * (k
 // Bound: kept codes read and written in whole rows.
 template <int CODE>
 __global__ void __launch_bounds__(kMoveThreads, 2) k_kv8_move(EvictDev a, int ctas) {
+    op_begin();
     constexpr int VECS = kMovePieces;
     __shared__ float token_scale[2][kMoveThreads * VECS];
     __shared__ float block_scale[2][kMoveThreads * VECS / 16];

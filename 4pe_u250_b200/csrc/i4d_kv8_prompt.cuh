@@ -312,6 +312,7 @@ __device__ __forceinline__ void each_piece(const AttnDev& a, int64_t u, int64_t 
 
 template <int DT, int CODE>
 __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_constant__ AttnDev a) {
+    op_begin();
     using L = PromptSmem<DT>;
     extern __shared__ unsigned char pr_base[];
     __shared__ PrShared sh;
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 // blockIdx.x / 8 + 1 is the first CTA whose share begins inside the segment,
 // blockIdx.x % 8 the 32 rows.
 __global__ void __launch_bounds__(256) k_kv8_prompt_join(AttnDev a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    op_begin();
     __shared__ int64_t s_sums[8], s_before;
     __shared__ int s_pair;
     const int c = blockIdx.x / 8 + 1, lane = threadIdx.x & 31, dim = a.cache.dim;

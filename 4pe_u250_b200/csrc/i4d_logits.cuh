@@ -116,6 +116,7 @@ struct Touched {
 
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int ctas) {
+    op_begin();
     extern __shared__ __align__(16) unsigned char logits_smem[];
     constexpr int V = 16 / sizeof(T);
     Touched t;

@@ -176,36 +176,24 @@ SeqArrays seq_arrays(const OpContext& o, const i4d_kv8& c, const int32_t* q_star
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
 
-// A kernel in clusters of `ctas` CTAs.
+// A kernel of the operators, in clusters of `ctas` CTAs.  Each begins with
+// op_begin(), which waits for what the stream holds before it, so its launch
+// may overlap that one's end.
 template <typename... Params, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, int ctas, cudaStream_t st, Args... args) {
+cudaError_t launch(void (*kernel)(Params...), int64_t grid, unsigned block, size_t smem, int ctas, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-// A kernel that waits for the one before it by itself (griddepcontrol.wait
-// first of all), so that its launch overlaps that one's end.
-template <typename... Params, typename... Args>
-cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -217,13 +205,11 @@ cudaError_t launch_rope(const RopeDev& d, int num_sms, cudaStream_t st) {
     const int items = (d.heads[0] + d.heads[1]) * (rot_items + (d.copy_tail ? (d.dim - d.rot) / V : 0));
     // Few tokens: their heads are spread over CTAs, up to two waves of them.
     if (d.tokens >= 16 * num_sms) {
-        k_rope_many<T, V, IL><<<(d.tokens + kRopeWarps - 1) / kRopeWarps, 32 * kRopeWarps, 0, st>>>(d);
-        return cudaGetLastError();
+        return launch(k_rope_many<T, V, IL>, (d.tokens + kRopeWarps - 1) / kRopeWarps, 32 * kRopeWarps, 0, 1, st, d);
     }
     const int most = (items + kRopeThreads - 1) / kRopeThreads;
     const int groups = std::max(1, std::min(most, 2 * num_sms / d.tokens));
-    k_rope<T, V, IL><<<d.tokens * groups, kRopeThreads, 0, st>>>(d, groups);
-    return cudaGetLastError();
+    return launch(k_rope<T, V, IL>, d.tokens * groups, kRopeThreads, 0, 1, st, d, groups);
 }
 
 template <typename T>
@@ -238,12 +224,8 @@ cudaError_t launch_rope_t(const RopeDev& d, bool interleaved, bool wide, int num
 template <typename T, int V, int CODE>
 cudaError_t launch_append(const AppendDev& d, int64_t units, int64_t unit_items, cudaStream_t st) {
     // A warp for the few values of a decode step, a CTA for a block of a prompt.
-    if (unit_items <= 64) {
-        k_kv8_append<T, V, CODE, 32><<<static_cast<unsigned>((units + 3) / 4), 128, 0, st>>>(d, static_cast<int>(units));
-    } else {
-        k_kv8_append<T, V, CODE, 256><<<static_cast<unsigned>(units), 256, 0, st>>>(d, static_cast<int>(units));
-    }
-    return cudaGetLastError();
+    if (unit_items <= 64) return launch(k_kv8_append<T, V, CODE, 32>, (units + 3) / 4, 128, 0, 1, st, d, static_cast<int>(units));
+    return launch(k_kv8_append<T, V, CODE, 256>, units, 256, 0, 1, st, d, static_cast<int>(units));
 }
 
 template <typename T>
@@ -360,7 +342,7 @@ i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 cudaError_t launch_attn(const AttnDev& d, int64_t grid, cudaStream_t st) {
     static_assert(attn_smem<DT, NT>() <= 114688, "two CTAs an SM");
-    return launch_cluster(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, static_cast<unsigned>(grid), kAttnThreads, attn_smem<DT, NT>(), d.cluster, st, d);
+    return launch(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, grid, kAttnThreads, attn_smem<DT, NT>(), d.cluster, st, d);
 }
 
 template <int DT, int CODE>
@@ -394,8 +376,7 @@ constexpr int kPromptSmem = PromptSmem<DT>::total + 1024;
 
 template <int DT, int CODE>
 cudaError_t launch_prompt(const AttnDev& d, int64_t grid, cudaStream_t st) {
-    k_kv8_prompt<DT, CODE><<<static_cast<unsigned>(grid), kPrThreads, kPromptSmem<DT>, st>>>(d);
-    return cudaGetLastError();
+    return launch(k_kv8_prompt<DT, CODE>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
 }
 
 template <int DT, int CODE>
@@ -411,9 +392,8 @@ cudaError_t launch_attn_c(const AttnDev& d, const AttnPlan& p, int64_t grid, cud
 
 template <int DT, int CODE>
 cudaError_t launch_weights(const AttnDev& d, int tiles, int64_t grid, cudaStream_t st) {
-    if (d.dtype == I4D_F32) k_kv8_weights<DT, CODE, true><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d, tiles);
-    else k_kv8_weights<DT, CODE, false><<<static_cast<unsigned>(grid), kAttnThreads, 0, st>>>(d, tiles);
-    return cudaGetLastError();
+    if (d.dtype == I4D_F32) return launch(k_kv8_weights<DT, CODE, true>, grid, kAttnThreads, 0, 1, st, d, tiles);
+    return launch(k_kv8_weights<DT, CODE, false>, grid, kAttnThreads, 0, 1, st, d, tiles);
 }
 
 template <int CODE>
@@ -644,9 +624,8 @@ i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* a) {
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
-    if (a->cache.code == I4D_CODE_INT8) k_kv8_read<I4D_CODE_INT8><<<static_cast<unsigned>(grid), 256, 0, s>>>(d, chunks);
-    else k_kv8_read<I4D_CODE_E4M3><<<static_cast<unsigned>(grid), 256, 0, s>>>(d, chunks);
-    OP_CK(cudaGetLastError());
+    OP_CK(a->cache.code == I4D_CODE_INT8 ? launch(k_kv8_read<I4D_CODE_INT8>, grid, 256, 0, 1, s, d, chunks)
+                                         : launch(k_kv8_read<I4D_CODE_E4M3>, grid, 256, 0, 1, s, d, chunks));
     return I4D_OK;
 }
 
@@ -728,12 +707,12 @@ i4d_status i4d_kv8_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
     if (enc != I4D_OK) return enc;
     OP_CK(int8 ? launch_attn_c<I4D_CODE_INT8>(d, p, grid, s) : launch_attn_c<I4D_CODE_E4M3>(d, p, grid, s));
     if (p.prompt) {
-        if (p.even > 1) OP_CK(launch_after(k_kv8_prompt_join, static_cast<unsigned>(8 * (p.even - 1)), 256, s, d));
-    } else if (p.even > 1) OP_CK(launch_after(k_kv8_join, static_cast<unsigned>(p.segments), kJoinThreads, s, d, 8 * p.nt));
+        if (p.even > 1) OP_CK(launch(k_kv8_prompt_join, 8 * (p.even - 1), 256, 0, 1, s, d));
+    } else if (p.even > 1) OP_CK(launch(k_kv8_join, p.segments, kJoinThreads, 0, 1, s, d, 8 * p.nt));
     if (d.scores) {
         const int chunks = (a->max_length + 511) / 512;
         if (chunks > 0) {
-            OP_CK(launch_after(k_kv8_weights_kept, static_cast<unsigned>(static_cast<int64_t>(a->batch) * a->cache.heads * chunks), 128, s, d, 8 * p.nt, chunks));
+            OP_CK(launch(k_kv8_weights_kept, static_cast<int64_t>(a->batch) * a->cache.heads * chunks, 128, 0, 1, s, d, 8 * p.nt, chunks));
         }
     } else if (a->weights && wgrid > 0)
         OP_CK(int8 ? launch_weights_c<I4D_CODE_INT8>(d, p, wtiles, wgrid, s) : launch_weights_c<I4D_CODE_E4M3>(d, p, wtiles, wgrid, s));
@@ -797,11 +776,11 @@ i4d_status i4d_kv8_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     DeviceScope scope(o.device);
     OP_CK(scope.error());
     const cudaStream_t s = stream_of(o, a->stream);
-    OP_CK(launch_cluster(k_kv8_select, static_cast<unsigned>(rows * ctas), kSelectThreads, 0, ctas, s, d, ctas));
+    OP_CK(launch(k_kv8_select, static_cast<unsigned>(rows * ctas), kSelectThreads, 0, ctas, s, d, ctas));
     if (a->max_length > a->budget) {
         const unsigned grid = static_cast<unsigned>(rows * 2 * movers);
-        OP_CK(a->cache.code == I4D_CODE_INT8 ? launch_cluster(k_kv8_move<I4D_CODE_INT8>, grid, kMoveThreads, 0, movers, s, d, movers)
-                                             : launch_cluster(k_kv8_move<I4D_CODE_E4M3>, grid, kMoveThreads, 0, movers, s, d, movers));
+        OP_CK(a->cache.code == I4D_CODE_INT8 ? launch(k_kv8_move<I4D_CODE_INT8>, grid, kMoveThreads, 0, movers, s, d, movers)
+                                             : launch(k_kv8_move<I4D_CODE_E4M3>, grid, kMoveThreads, 0, movers, s, d, movers));
     }
     return I4D_OK;
 }
@@ -878,9 +857,9 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     d.words = std::min(kLogitsPart / 32, ((a->vocab + ctas - 1) / ctas + 32 + 127) / 128 * 4);
     const int smem = logits_smem_bytes(d.places, d.words);
     switch (a->dtype) {
-        case I4D_F32: OP_CK(launch_cluster(k_logits<float>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
-        case I4D_BF16: OP_CK(launch_cluster(k_logits<__nv_bfloat16>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
-        default: OP_CK(launch_cluster(k_logits<__half>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        case I4D_F32: OP_CK(launch(k_logits<float>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        case I4D_BF16: OP_CK(launch(k_logits<__nv_bfloat16>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        default: OP_CK(launch(k_logits<__half>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
     }
     return I4D_OK;
 }

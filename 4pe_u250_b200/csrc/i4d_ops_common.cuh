@@ -74,6 +74,14 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& r) {
     }
 }
 
+// First of all in every kernel of the operators: waits for what the stream
+// holds before it, whose end its launch may overlap, then lets the next one's
+// launch overlap its own.
+__device__ __forceinline__ void op_begin() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // The arrays that say where the tokens of a batch are.
 struct SeqArrays {
     const int32_t* q_start;

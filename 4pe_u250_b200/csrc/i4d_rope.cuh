@@ -100,6 +100,7 @@ struct RopeItem {
 // Few tokens: `groups` CTAs for each.
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeThreads) k_rope(RopeDev a, int groups) {
+    op_begin();
     __shared__ float2 cs[128];
     const int t = blockIdx.x / groups, part = blockIdx.x % groups;
     const int rot_items = (INTERLEAVED ? a.rot : a.rot / 2) / V;
@@ -123,6 +124,7 @@ constexpr int kRopeWarps = 4;
 // 195 instructions an item: 8191 tokens of 40 heads, half rotated, 41 us.)
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(32 * kRopeWarps) k_rope_many(RopeDev a) {
+    op_begin();
     constexpr int kPairs = INTERLEAVED ? V / 2 : V;
     constexpr int kAhead = 4;
     __shared__ float2 angles[kRopeWarps][128];
