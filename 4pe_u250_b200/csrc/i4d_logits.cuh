@@ -11,7 +11,7 @@
 // Bound: the logits in and out; but a list of thousands of ids costs a CTA's
 // phases, each with its barriers, as much again (192 rows of 128001 in bf16:
 // 32 us without lists, 60 with histories and biases, 15 at the copy's rate),
-// and one row the chain of those phases (10 us).
+// and one row the chain of those phases (7 us for 32000 in FP32).
 #pragma once
 
 #include <cooperative_groups.h>

@@ -293,7 +293,7 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     p.segments = static_cast<int64_t>(a.batch) * c.heads * p.row_tiles;
     // Few segments of moderate length: as many CTAs of a cluster for each as
     // fit the GPU at once, which need no second kernel (one stream of 2047
-    // tokens, 32 heads: 20.5 us through partial sums in memory, 13 so).  Long
+    // tokens, 32 heads: 20.5 us through partial sums in memory, 13.3 so).  Long
     // ones: the CTAs that fit the GPU share all tokens evenly, whatever the
     // lengths are (which the device alone knows), but no more of them than have
     // two tiles a warp.  Many rows are work enough by themselves.
