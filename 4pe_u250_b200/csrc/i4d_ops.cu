@@ -261,9 +261,15 @@ i4d_status encode_codes(i4d_ctx* ctx, const i4d_kv8& c, const void* codes, int r
     const cuuint64_t size[2] = {static_cast<cuuint64_t>(c.dim), static_cast<cuuint64_t>(c.blocks) * c.heads * c.block_tokens};
     const cuuint64_t stride[1] = {static_cast<cuuint64_t>(c.dim)};
     const cuuint32_t box[2] = {narrow ? 64u : 128u, static_cast<cuuint32_t>(rows)}, step[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), size, stride, box, step,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto encode = [&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread's first CUDA call: the runtime has bound no context to it yet
+        OP_CK(cudaSetDevice(op_context(ctx).device));
+        r = encode();
+    }
     if (r != CUDA_SUCCESS) return op_fail(ctx, I4D_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return I4D_OK;
 }

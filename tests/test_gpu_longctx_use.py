@@ -129,6 +129,40 @@ def test_sequences_out_of_range_are_skipped(pkg, ctx, q_start, lens):
     assert torch.all(back[~rows.cuda()] == 7)
 
 
+def test_sync_reports_what_was_skipped_once(pkg):
+    torch = _torch()
+    with pkg.Context(num_layers=1, kv_capacity=8) as c:
+        s = Setup(pkg, [20], 1, 64, 16, "int8", 44)
+        k = torch.randn(1, 1, 64, device="cuda").bfloat16()
+        c.kv8_append(s.cache, k, k, s.dev([0, 1]), s.dev([999]), s.dev(s.table), 1)
+        torch.cuda.synchronize()
+        with pytest.raises(pkg.I4DError, match="q_start or lengths"):
+            c.sync()
+        c.sync()
+
+
+def test_another_thread_and_the_default_stream(pkg, ctx):
+    import threading
+    torch = _torch()
+    s = Setup(pkg, [700], 2, 64, 16, "int8", 45)
+    q = torch.randn(1, 8, 64, device="cuda").bfloat16()
+    args = (s.dev([0, 1]), s.dev([700]), s.dev(s.table), 1, 700)
+    want = ctx.kv8_attention(s.cache, q, *args)
+    got = []
+
+    def work():
+        for _ in range(20):
+            got.append(ctx.kv8_attention(s.cache, q, *args))
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 60 and all(torch.equal(x, want) for x in got)
+
+
 def test_evict_skips_lengths_out_of_range(pkg, ctx):
     torch = _torch()
     s = Setup(pkg, [60, 60, 60], 1, 64, 16, "int8", 47)

@@ -299,3 +299,30 @@ def test_blocks_and_lengths_that_pass_stay_in_bounds(lib):
     for x in (-top - 1, -1, 0, 1, 7, 8, 9, top):
         assert bool(lib.stub_block_ok(x, 8)) == (0 <= x < 8)
         assert bool(lib.stub_length_ok(x, 8)) == (0 <= x <= 8)
+
+
+def test_binding_refuses_before_it_calls(pkg):
+    """Tensors that are not on the context's GPU, wrong types and counts of arguments: the library is not reached."""
+    torch = pytest.importorskip("torch")
+    longctx = importlib.import_module("4pe_u250_b200.longctx")
+    ops = longctx.ops()
+    q, pos, turns = torch.zeros(2, 3, 8), torch.zeros(2, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(pkg.I4DError, match="q is not on GPU 0"):
+        ops.rope(1, 0, q, None, pos, turns, 8, 1.0, True, False, None, None)
+    with pytest.raises(pkg.I4DError, match="not a tensor"):
+        ops.rope(1, 0, 7, None, pos, turns, 8, 1.0, True, False, None, None)
+    with pytest.raises(pkg.I4DError, match="arguments"):
+        ops.rope(1, 0, q)
+    with pytest.raises(TypeError):
+        ops.rope("x", 0, q, None, pos, turns, 8, 1.0, True, False, None, None)
+    with pytest.raises(pkg.I4DError, match="KV8Cache"):
+        ops.kv8_append(1, 0, None, q, q, pos, pos, pos, 1)
+    with pytest.raises(pkg.I4DError, match="gradient"):
+        ops.logits_process(1, 0, torch.zeros(1, 9, requires_grad=True), *[None] * 12)
+    with pytest.raises(pkg.I4DError):
+        pkg.KV8Cache(*(torch.zeros(2, 1, 16, 16, dtype=torch.int8) for _ in range(2)), *(torch.zeros(2, 1) for _ in range(2)))
+    for bad in (dict(rot_dim=3), dict(rot_dim=0), dict(rot_dim=258), dict(rot_dim=8, base=1.0), dict(rot_dim=8, base=float("nan")),
+                dict(rot_dim=8, scaling="linear", factor=0.5), dict(rot_dim=2, scaling="base", factor=2.0),
+                dict(rot_dim=8, scaling="parts", factor=2.0, low=4.0, high=4.0), dict(rot_dim=8, scaling="cubic")):
+        with pytest.raises(pkg.I4DError):
+            pkg.rope_frequencies(**bad)
