@@ -390,6 +390,60 @@ def test_single_tokens_of_many_and_few_sequences(pkg, ctx, batch, length, group)
     _run_attention(pkg, ctx, s, [1] * batch, lens, group, "bf16", 0)
 
 
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("max_q,max_length", [(1, 300), (40, 400), (900, 4000), (5000, 20000)])
+def test_bounds_far_above_what_the_sequences_have(pkg, ctx, name, max_q, max_length):
+    """max_q and max_length only bound: with any of them the results are within the same bounds, whichever kernel they choose."""
+    from test_gpu_longctx import _attention_bounds
+    torch = _torch()
+    lens, t = [300, 17, 64], _type(name)
+    s = Setup(pkg, lens, 2, 128, 16, "int8", 113)
+    table = np.zeros((3, max(s.table.shape[1], -(-max_length // 16))), np.int32)
+    table[:, :s.table.shape[1]] = s.table
+    start = _starts([1, 1, 1])
+    g = torch.Generator().manual_seed(3)
+    q, k = torch.randn(3, 4, 128, generator=g).to(t).cuda(), torch.randn(3, 2, 128, generator=g).to(t).cuda()
+    want = s.ref()
+    want.append((_np(k), _np(k)), start, lens, table)
+    args = (s.dev(start), s.dev(lens), s.dev(table), max_q)
+    ctx.kv8_append(s.cache, k, k, *args)
+    _same_cache(s.cache, want)
+    weights = torch.zeros(3, 2, max_length, device="cuda")
+    lse = torch.empty(3, 4, device="cuda")
+    out = ctx.kv8_attention(s.cache, q, *args, max_length, weights=weights, lse=lse)
+    w_out, w_lse, sums, mag, size = ref.attention(want, _np(q), start, lens, table, 128 ** -0.5)
+    b_out, b_lse, b_p = _attention_bounds(t, 128, w_out, mag, size, w_lse, 300)
+    assert np.all(np.abs(_np(out) - w_out) <= b_out) and np.all(np.abs(_np(lse) - w_lse) <= b_lse)
+    for b, n in enumerate(lens):  # two rows a head: their probabilities and two sums
+        assert np.all(np.abs(_np(weights)[b, :, :n] - sums[b]) <= sums[b] * (b_p.max() + 2.0 ** -21))
+        assert torch.all(weights[b, :, n:] == 0)
+    back = ctx.kv8_read(s.cache, *args, 3)
+    for b, n in enumerate(lens):
+        for h in range(2):
+            assert np.array_equal(_np(back[1])[b, h], want.tokens(1, table[b], h, np.array([n - 1]))[0])
+    lo, keep, _ = ctx.kv8_evict(s.cache, args[1], args[2], weights, 50, 10, max_length)
+    assert lo.tolist() == [50, 17, 50]
+    ctx.ops_check()
+
+
+@pytest.mark.parametrize("batch", [3000, 70000])
+def test_thousands_of_sequences(pkg, ctx, batch):
+    """Many sequences that share one block (read only), some without rows."""
+    torch = _torch()
+    s = Setup(pkg, [16], 1, 64, 16, "int8", 127)
+    n = torch.ones(batch, dtype=torch.int32)
+    n[::3] = 0
+    start = torch.cat([torch.zeros(1, dtype=torch.int32), n.cumsum(0).int()]).cuda()
+    total = int(start[-1])
+    q = torch.randn(1, 2, 64, device="cuda").half()
+    table = torch.full((1, 1), int(s.table[0, 0]), dtype=torch.int32, device="cuda").expand(batch, 1)
+    lens = torch.full((batch,), 13, dtype=torch.int32, device="cuda")
+    one = ctx.kv8_attention(s.cache, q, s.dev([0, 1]), s.dev([13]), s.dev(s.table), 1, 16)
+    out = ctx.kv8_attention(s.cache, q.expand(total, -1, -1), start, lens, table, 1, 16)
+    assert torch.equal(out, one.expand(total, -1, -1))
+    ctx.ops_check()
+
+
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 64, 10 ** 9])
 def test_windows(pkg, ctx, window):
     s = Setup(pkg, [3000, 64, 1], 1, 64, 32, "int8", 89)
