@@ -44,7 +44,9 @@ struct PromptSmem {
 // Barriers.
 enum {
     kRawKFull = 0, kRawVFull = 2, kRawKEmpty = 4, kRawVEmpty = 6, kKFull = 8, kKEmpty = 10,
-    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 4, kPvDone = kPFull + 4, kQFull = kPvDone + 4, kODone = kQFull + 2, kPrBars = kODone + 2
+    kVFull = 12, kVEmpty, kSFull, kPFull = kSFull + 4, kPvDone = kPFull + 4, kQFull = kPvDone + 4, kODone = kQFull + 2,
+    kFirstP = kODone + 2,  // completes once: tile 0's first probabilities of the CTA
+    kPrBars
 };
 
 constexpr int kPrWarps = kPrThreads / 32;
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPrBars; ++i) {
-            const bool warps = (i >= kRawKEmpty && i < kKEmpty) || i == kVFull || (i >= kPFull && i < kPvDone) || i == kQFull || i == kQFull + 1;
+            const bool warps = (i >= kRawKEmpty && i < kKEmpty) || i == kVFull || (i >= kPFull && i < kPvDone) || i == kQFull || i == kQFull + 1 || i == kFirstP;
             const int count = warps ? 4 : (i >= kKEmpty && i < kVFull) || i == kVEmpty ? 2 : 1;
             bar_init(bar_at(sh, i), count);
         }
@@ -428,8 +430,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                 }
                 ok = pr_wait(sh, kQFull + t, pieces++ & 1);
                 // Tile 1 begins when tile 0 has its first probabilities: the
-                // one's products then run under the other's softmax.
-                if (t == 1 && n == 0) ok = ok && pr_wait(sh, kPFull, 0);
+                // one's products then run under the other's softmax.  (Not by
+                // kPFull, whose phases tile 0 goes on through: tile 1, with rows
+                // that come late, would find it two on and wait for good.)
+                if (t == 1 && n == 0) ok = ok && pr_wait(sh, kFirstP, 0);
                 for (int j = 0; ok && j <= count; ++j) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -652,7 +656,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                 tmem_wait_store();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) pr_arrive(sh, kPFull + 2 * tile + half);
+                if (lane == 0) {
+                    pr_arrive(sh, kPFull + 2 * tile + half);
+                    if (tile + half + n + j == 0) pr_arrive(sh, kFirstP);
+                }
             }
         }
         const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
