@@ -34,6 +34,7 @@
 #include <cuda.h>
 
 #include "i4d_kv8_cache.cuh"
+#include "i4d_ring.h"
 
 namespace i4d_ops {
 
@@ -553,7 +554,7 @@ __device__ __forceinline__ void store_lse(const AttnDev& a, const Seq& s, int h,
 
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block, uint64_t* s_bar, uint32_t& phases) {
+__device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block, uint64_t* s_bar, Ring& copies) {
     constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
     float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -609,29 +610,22 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 if (id >= 0) copy_tile<DT>(a, ring + slot * 32 * DT, bars + slot * 8, (id * a.cache.heads + h) * bs + (at & (bs - 1)));
                 else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + slot * 8) : "memory");
             };
-            // the slots are used in turn; `phases` holds the parity of each one's next phase
-            for (int i = 0; i < kSlots - 1; ++i) issue(warp + i * kAttnWarps, i);
+            ring_fill<kSlots>(copies, warp, kAttnWarps, issue);
             if (from_tok == begin) load_qtile<DT, CODE, NT, HLQ>(a, s, h, row0, q);
-            int slot = 0;
-            for (int i = warp; i < tiles; i += kAttnWarps) {
-                __syncwarp();  // all lanes are done with the slot to fill
-                issue(i + (kSlots - 1) * kAttnWarps, slot == 0 ? kSlots - 1 : slot - 1);
-                if (!bar_wait(bars + slot * 8, phases >> slot & 1)) {
-                    if (lane == 0) atomicOr(a.seq.err, kTimeout);
-                    for (int k = 1, ahead = slot; k < kSlots && i + k * kAttnWarps < tiles; ++k) {  // the copies behind it
-                        ahead = ahead == kSlots - 1 ? 0 : ahead + 1;
-                        bar_wait(bars + ahead * 8, phases >> ahead & 1);
-                    }
-                    break;
-                }
-                phases ^= 1u << slot;
+            const auto wait = [&](int slot, uint32_t parity) { return bar_wait(bars + slot * 8, parity); };
+            const auto any_late = [&](bool landed) {  // (the whole warp)
+                if (__all_sync(~0u, landed)) return false;
+                if (lane == 0) atomicOr(a.seq.err, kTimeout);
+                return true;
+            };
+            // (free: all lanes are done with the slot to fill)
+            ring_walk<kSlots>(copies, warp, kAttnWarps, tiles, issue, wait, [] { __syncwarp(); }, [&](int i, int slot, bool landed) {
                 const uint32_t at_slot = ring + slot * 32 * DT;
-                slot = slot == kSlots - 1 ? 0 : slot + 1;
                 const int at = from_tok + 16 * i;
                 const float4 block = s_block[(at >> shift) - blk0];
                 const float lvs = block.w;
                 const int live = __float_as_int(block.x) < 0 ? 0 : min(16, to_tok - at);
-                if (live == 0 && !a.scores) continue;  // (the kept scores of a bad block are -inf)
+                if (live == 0 && !a.scores) return !any_late(landed);  // (the kept scores of a bad block are -inf)
                 float x[NT][4];
                 {
                     KTile<DT> kt;
@@ -643,7 +637,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 if (live < 16) clear_vtile<DT>(live, vt);
                 float top[NT][2];
                 const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
-                bool raise = false;
+                bool raise = !landed;  // one vote a tile answers both
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -661,6 +655,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                         raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + kSlack;
                     }
                 if (__any_sync(~0u, raise)) {
+                    if (any_late(landed)) return false;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -716,7 +711,8 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                     }
                 }
                 value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
-            }
+                return true;
+            });
             from_tok = to_tok;
         }
         __syncthreads();  // the ring is free for the join
@@ -827,7 +823,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
     // the copies' swizzle counts from 1024-byte boundaries
     unsigned char* attn_ring = attn_smem_base + (-static_cast<uint32_t>(__cvta_generic_to_shared(attn_smem_base)) & 1023u);
     __shared__ uint64_t s_bar[kAttnWarps * kAttnSlots<DT>];
-    uint32_t phases = 0;
+    Ring copies;
     if (threadIdx.x < kAttnWarps * kAttnSlots<DT>) bar_init(static_cast<uint32_t>(__cvta_generic_to_shared(s_bar + threadIdx.x)), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
@@ -841,7 +837,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
         if (s.len > a.max_length || rt * kRows >= s.n * a.group) return;  // the whole cluster
         const int first = s.len - s.n, lo = row_span(a, first + rt * kRows / a.group).x & ~15;
         const int share = ((s.len - lo + 15) / 16 + a.cluster - 1) / a.cluster * 16;
-        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, lo + rank * share, min(s.len, lo + (rank + 1) * share), true, 0}, attn_ring, s_block, s_bar, phases);
+        attend<DT, CODE, NT, HLQ, HLP>(a, s, {b, h, rt, lo + rank * share, min(s.len, lo + (rank + 1) * share), true, 0}, attn_ring, s_block, s_bar, copies);
         return;
     }
     Place at;
@@ -874,7 +870,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(
             __syncthreads();
         }
         attend<DT, CODE, NT, HLQ, HLP>(a, s, {at.seq, seg / row_tiles, seg % row_tiles, lo + 16 * t0, min(s.len, lo + 16 * t1), t0 == 0 && t1 == n.tiles, u == u0 ? 0 : 1},
-                                       attn_ring, s_block, s_bar, phases);
+                                       attn_ring, s_block, s_bar, copies);
         u = seg0 + t1;
     }
 }
