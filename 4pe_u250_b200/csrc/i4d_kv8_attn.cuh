@@ -43,6 +43,10 @@ constexpr int kAttnWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 6.f;
+// R stays above M - 126, so 2^(M - R) and 2^(R - M) are normal numbers.  Less
+// would be needed only where a row has seen nothing but value scales under
+// 2^-126, or of 0.
+constexpr float kFarScales = 126.f;
 
 struct AttnDev {
     CUtensorMap maps[2];  // K, V codes as rows of dim bytes; boxes of 16 rows x 128 (dim <= 64: 64) bytes
@@ -445,6 +449,11 @@ __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (
     }
 }
 
+// 2^(M - R) v_scale.  It passes FP32's range only for a block that the row sees
+// nothing of (0 times it must be 0), or nothing but tokens 2^-113 of the
+// greatest.
+__device__ __forceinline__ float weight_unit(float to_r, float v_scale) { return fminf(to_r * v_scale, 0x1.fffffep127f); }
+
 // First and one past the last token that a row at cache index pos sees.
 __device__ __forceinline__ int2 row_span(const AttnDev& a, int pos) {
     return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, pos + 1);
@@ -663,8 +672,9 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                             float m = top[nt][j];
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                            const float r = fmaxf(m + lvs, R[nt][j]);
+                            const float mr = fmaxf(m + lvs, R[nt][j]);
                             m = fmaxf(m, M[nt][j]);
+                            const float r = fmaxf(mr, m - kFarScales);
                             const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
                             l[nt][j] *= fm;
 #pragma unroll
@@ -697,7 +707,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                         const int j = k & 1;
                         const float e = ex2(x[nt][k] - from[nt][j]);
                         l[nt][j] += e;
-                        w[k] = e * (to_r[nt][j] * block.z);
+                        w[k] = e * weight_unit(to_r[nt][j], block.z);
                     }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {

@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         const float2 f = g ? make_float2(f1, f1) : make_float2(f0, f0), o = make_float2(-off, -off);
-                        const float wv = to_r * (g ? b1.y : b0.y);
+                        const float wv = weight_unit(to_r, g ? b1.y : b0.y);
                         const float2 w = make_float2(wv, wv);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                     }
                     const bool raise = top > M + kSlack || rtop > R + kSlack;
                     if (!__any_sync(~0u, raise)) break;
-                    const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(rtop, R) : R;
+                    const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(fmaxf(rtop, R), m - kFarScales) : R;
                     const float fm = M == m ? 1.f : ex2(M - m), f = R == rr ? 1.f : ex2(R - rr);
                     sum[0].x *= fm;
                     sum[0].y *= fm;

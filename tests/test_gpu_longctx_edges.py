@@ -3,8 +3,7 @@ bounds lie far apart."""
 import numpy as np
 import pytest
 
-import longctx_ref as ref
-from test_gpu_longctx import Setup, _half_step, _np, _starts, _torch, _type
+from test_gpu_longctx import Setup, _np, _run_attention, _torch
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +36,38 @@ def test_prompt_rows_that_arrive_late(pkg, ctx, first):
         ctx.kv8_attention(s.cache, q, *args, out=got)
         assert torch.equal(got, want)
     ctx.ops_check()
+
+
+# ------------------------------------------------------------------ scales
+
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("group", [1, 4])
+def test_zero_values_before_large_ones(pkg, ctx, name, kind, group):
+    """The first rows see only a block of zeros, whose scale is 2^-126, in tiles whose later blocks have scales of 8 and more."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(7)
+    s = Setup(pkg, [40], 2, 64, 16, kind, 73)
+    k, v = torch.randn(40, 2, 64, generator=g), torch.randn(40, 2, 64, generator=g) * 1000
+    v[:16] = 0
+    ctx.kv8_append(s.cache, k.cuda(), v.cuda(), s.dev([0, 40]), s.dev([40]), s.dev(s.table), 40)
+    assert s.cache.v_scale[s.table[0, 0]].max() == 2.0 ** -126 and s.cache.v_scale[s.table[0, 1]].min() >= 4
+    for n in (40, 35):  # (row tiles that end at the block's border, and that do not)
+        _, out = _run_attention(pkg, ctx, s, [n], [40], 2 * group, name, 0)
+        assert torch.all(out[:16 - 40 + n] == 0)
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("up", [1, 2 ** 7])
+def test_value_scales_of_exactly_zero(pkg, ctx, name, group, up):
+    """A scale of 0 makes zeros of its block's codes, however far its scores lie above or below the others'."""
+    s = Setup(pkg, [60], 2, 64, 16, "int8", 79)
+    for block in s.table[0, [0, 2]]:
+        s.cache.v_scale[int(block)] = 0
+        s.cache.k_scale[int(block)] *= up
+    for n, window in ((60, 0), (55, 0), (55, 9)):
+        _run_attention(pkg, ctx, s, [n], [60], 2 * group, name, window)
+    s.cache.v_scale.zero_()
+    _, out = _run_attention(pkg, ctx, s, [60], [60], 2 * group, name, 0)
+    assert np.all(_np(out) == 0)
