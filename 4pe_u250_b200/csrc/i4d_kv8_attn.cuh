@@ -16,16 +16,22 @@
 //   output   O^T [16 dims x 8 rows]  += V^T [16 x 16 tokens] P^T
 // Every code is exact in FP16.  A query row is scaled by a power of two into
 // FP16's range, which is exact for BF16 and FP16 rows up to 2^-39 of the row's
-// largest value; FP32 rows are split in two FP16 parts (2^-22).  Probabilities
-// go to FP16 in one part (2^-11, an eighth of a BF16 output's rounding) or,
-// for FP16 and FP32 outputs, in two.
+// largest value; FP32 rows are split in two FP16 parts (2^-22).  A weight goes to
+// FP16 in one part (2^-11 of it at most, an eighth of a BF16 output's rounding);
+// for FP16 outputs in two (2^-22, but not less than 2^-34 of the row's greatest
+// weight), for FP32 outputs in two of which the second is scaled (2^-22).
+// Weights under 2^-23 of the greatest go in again, 2^24 times, so that they are
+// right where the greatest ones meet codes of 0; under 2^-95 they are 0.
 //
 // One pass over the tokens: M is a bound of the scores so far (in powers of
 // two), l the sum of 2^(x - M), R a bound of x + log2(v_scale): the values
 // that enter the second product are 2^(x - R) v_scale, so a block whose scale
 // is far above the others' costs the others no bits unless it outweighs them.
-// M and R are raised only when a score passes them by more than 2^6 (FP16
-// holds 2^15), so most tiles do without the reduction over lanes.
+// M and R are raised only when a score passes them by more than 2^6 (R lies 2^9
+// under the greatest, FP16 holds 2^15), so most tiles do without the reduction
+// over lanes; the vote that asks for it asks for small weights too (which
+// costs 24 ragged contexts 3 %, three rows a sequence 6 %, FP32 rows of 256
+// 10 %).
 // Bound: the codes of K and V, read once (24 contexts of 301 to 32749 tokens,
 // 8 heads of 128, 812 MB of INT8 codes: 151 to 166 us, 5.4 to 4.9 TB/s; the same
 // copies without arithmetic 133 us).
@@ -43,6 +49,11 @@ constexpr int kAttnWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 6.f;
+// R lies this far under the greatest x + log2(v_scale): a weight is at most
+// 2^(kHead + kSlack) in FP16, which keeps its precision down to 2^-14.
+constexpr float kHead = 9.f;
+constexpr float kSmallWeight = 0x1p-14f;
+constexpr float kSmallStep = 0x1p24f, kSmallMost = 0x1p72f;  // (sums reach 2^54: 2^28 tokens a warp, weights under 2^16, codes under 2^9)
 // R stays above M - 126, so 2^(M - R) and 2^(R - M) are normal numbers.  Less
 // would be needed only where a row has seen nothing but value scales under
 // 2^-126, or of 0.
@@ -422,9 +433,77 @@ __device__ __forceinline__ void clear_vtile(int live, VTile<DT>& vt) {
         }
 }
 
+// How a weight goes to FP16: in one part, in two, or in two of which the second
+// is 2^11 times what the first leaves (it meets codes times 2^-11, which are
+// exact too), so that it has its eleven bits wherever the first has.
+enum { kOnePart, kTwoParts, kTwoPartsFar };
+
+template <int PARTS>
+__device__ __forceinline__ uint32_t second_part(float lo, float hi, uint32_t first) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
+    constexpr float up = PARTS == kTwoPartsFar ? 2048.f : 1.f;
+    return pack_h2((lo - f.x) * up, (hi - f.y) * up);
+}
+
+// The weights of a tile as operands: w[nt][k] of row 2t + k % 2 and token
+// g + k / 2 * 8.
+template <int NT, int PARTS>
+__device__ __forceinline__ void pack_weights(const float (&w)[NT][4], uint32_t (&p)[NT][2], uint32_t (&pl)[NT][2]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t hi = pack_h2(w[nt][2 * r], w[nt][2 * r + 1]);
+            p[nt][r] = transpose8(hi);
+            pl[nt][r] = 0;
+            if constexpr (PARTS != kOnePart) pl[nt][r] = transpose8(second_part<PARTS>(w[nt][2 * r], w[nt][2 * r + 1], hi));
+        }
+}
+
+// The codes as if they had just been read: what is made of them is made here, not
+// ahead of a loop, where it would take the registers of twice the codes.
+template <int DT>
+__device__ __forceinline__ void fresh_vtile(VTile<DT>& vt) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < DT / 32; ++w) asm volatile("" : "+r"(vt.w[r][w]));
+}
+
+// Takes the weights that are too small for FP16 out of w, kSmallStep times into
+// `kept`; whether any lane has one.
+template <int NT>
+__device__ __forceinline__ bool split_small(float (&w)[NT][4], volatile float (&kept)[NT][4]) {
+    bool any = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= w[nt][k] > 0.f && w[nt][k] < kSmallWeight;
+    if (!__any_sync(~0u, any)) return false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool small = w[nt][k] < kSmallWeight;
+            kept[nt][k] = small ? w[nt][k] * kSmallStep : 0.f;
+            if (small) w[nt][k] = 0.f;
+        }
+    return true;
+}
+
+template <int DT, int NT>
+__device__ __forceinline__ void scale_sums(float acc[DT / 16][NT][4], float by) {
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][nt][k] *= by;
+}
+
 // acc[i]: dims v_dim(lane / 4, i / 2) + 2 (i % 2) and the next, rows 2t and
 // 2t + 1 of each tile.
-template <int DT, int CODE, int NT, bool HL>
+template <int DT, int CODE, int NT, int PARTS>
 __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (&p)[NT][2], const uint32_t (&pl)[NT][2], float acc[DT / 16][NT][4]) {
 #pragma unroll
     for (int w = 0; w < DT / 32; ++w) {
@@ -439,11 +518,17 @@ __device__ __forceinline__ void value_tile(const VTile<DT>& vt, const uint32_t (
                 halves2<CODE, 0>(w0, w1, x);
                 halves2<CODE, 0>(w2, w3, y);
             }
-            const uint32_t f[4] = {x[0], x[1], y[0], y[1]};
+            uint32_t f[4] = {x[0], x[1], y[0], y[1]};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma(acc[2 * w + half][nt], f, p[nt][0], p[nt][1]);
-                if constexpr (HL) mma(acc[2 * w + half][nt], f, pl[nt][0], pl[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma(acc[2 * w + half][nt], f, p[nt][0], p[nt][1]);
+            if constexpr (PARTS == kTwoPartsFar) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)  // times 2^-11
+                    asm volatile("mul.rn.f16x2 %0, %0, %1;" : "+r"(f[i]) : "r"(0x10001000u));
+            }
+            if constexpr (PARTS != kOnePart) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(acc[2 * w + half][nt], f, pl[nt][0], pl[nt][1]);
             }
         }
     }
@@ -470,9 +555,9 @@ constexpr size_t attn_smem() {
     return (ring > merge ? ring : merge) + 1024;
 }
 
-// CTAs an SM: by shared memory and by registers (8 rows of up to 128 values in 128 registers).
-template <int DT, int NT>
-constexpr int kAttnPlaces = DT == 256 || NT == 2 ? 2 : 4;
+// CTAs an SM: by shared memory and by registers (8 rows of up to 128 values in
+// 128 registers, FP32 ones in two parts in 168).
+constexpr int attn_places(int dt, int nt, bool hlq) { return dt == 256 || nt == 2 ? 2 : dt == 128 && hlq ? 3 : 4; }
 
 // The work of a call in units of 16 tokens: sequence by sequence, its row
 // tiles of each head, the tokens that any row of the sequence sees.
@@ -564,7 +649,7 @@ __device__ __forceinline__ void store_lse(const AttnDev& a, const Seq& s, int h,
 // HLQ: FP32 query rows in two parts; HLP: probabilities in two parts.
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Piece& pc, unsigned char* attn_ring, float4* s_block, uint64_t* s_bar, Ring& copies) {
-    constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>;
+    constexpr int kRows = 8 * NT, kSlots = kAttnSlots<DT>, kParts = !HLP ? kOnePart : HLQ ? kTwoPartsFar : kTwoParts;
     float (*merge)[kRows][DT + 4] = reinterpret_cast<float (*)[kRows][DT + 4]>(attn_ring);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int b = pc.b, h = pc.h, row0 = pc.rt * kRows;
@@ -642,8 +727,13 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                     score_tile<DT, CODE, NT, HLQ>(kt, q, x);
                 }
                 VTile<DT> vt;
-                read_vtile<DT>(at_slot, vt);
-                if (live < 16) clear_vtile<DT>(live, vt);
+                // FP32 rows read V's codes late, for their registers (24 contexts, dim
+                // 256: 214 us, 276 with the codes read here).
+                constexpr bool kLate = HLQ;
+                if constexpr (!kLate) {
+                    read_vtile<DT>(at_slot, vt);
+                    if (live < 16) clear_vtile<DT>(live, vt);
+                }
                 float top[NT][2];
                 const bool whole = live == 16 && at >= all_from && at + 16 <= all_to;
                 bool raise = !landed;  // one vote a tile answers both
@@ -661,9 +751,11 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                         x[nt][j] = y0;
                         x[nt][j + 2] = y1;
                         top[nt][j] = fmaxf(y0, y1);
-                        raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + kSlack;
+                        raise |= top[nt][j] > M[nt][j] + kSlack || top[nt][j] + lvs > R[nt][j] + (kSlack + kHead);
+                        raise |= fminf(y0, y1) + lvs < R[nt][j] - 14.f;  // small weights, and tokens that are not seen
                     }
-                if (__any_sync(~0u, raise)) {
+                const bool voted = __any_sync(~0u, raise);
+                if (voted) {
                     if (any_late(landed)) return false;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -672,7 +764,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                             float m = top[nt][j];
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                            const float mr = fmaxf(m + lvs, R[nt][j]);
+                            const float mr = fmaxf(m + lvs - kHead, R[nt][j]);
                             m = fmaxf(m, M[nt][j]);
                             const float r = fmaxf(mr, m - kFarScales);
                             const float fm = M[nt][j] == m ? 1.f : ex2(M[nt][j] - m), fr = R[nt][j] == r ? 1.f : ex2(R[nt][j] - r);
@@ -698,29 +790,42 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                             if (at + n < to_tok && row0 + r <= last_row) a.scores[(tile * kRows + r) * a.score_stride + at + n] = x[nt][k];
                         }
                 }
-                uint32_t p[NT][2], pl[NT][2];
+                float w[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float w[4];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int j = k & 1;
                         const float e = ex2(x[nt][k] - from[nt][j]);
                         l[nt][j] += e;
-                        w[k] = e * weight_unit(to_r[nt][j], block.z);
+                        w[nt][k] = e * weight_unit(to_r[nt][j], block.z);
                     }
+                // Weights under FP16's range count where the greatest ones' codes
+                // are 0: they go in 2^24 times, to 2^24 times the sums, and so on.
+                volatile float kept[NT][4];  // (in memory: most tiles have none)
+                bool more = voted && split_small<NT>(w, kept);
+                float down = 1.f;
+#pragma unroll 1
+                for (;;) {
+                    uint32_t p[NT][2], pl[NT][2];
+                    pack_weights<NT, kParts>(w, p, pl);
+                    if constexpr (kLate) {
+                        read_vtile<DT>(at_slot, vt);
+                        if (live < 16) clear_vtile<DT>(live, vt);
+                    } else {
+                        fresh_vtile<DT>(vt);
+                    }
+                    value_tile<DT, CODE, NT, kParts>(vt, p, pl, acc);
+                    if (!more) break;
+                    down *= 1.f / kSmallStep;
+                    scale_sums<DT, NT>(acc, kSmallStep);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint32_t hi = pack_h2(w[2 * r], w[2 * r + 1]);
-                        p[nt][r] = transpose8(hi);
-                        pl[nt][r] = 0;
-                        if constexpr (HLP) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            pl[nt][r] = transpose8(pack_h2(w[2 * r] - f.x, w[2 * r + 1] - f.y));
-                        }
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[nt][k] = kept[nt][k];
+                    more = split_small<NT>(w, kept) && down > 1.f / kSmallMost;
                 }
-                value_tile<DT, CODE, NT, HLP>(vt, p, pl, acc);
+                if (down != 1.f) scale_sums<DT, NT>(acc, down);
                 return true;
             });
             from_tok = to_tok;
@@ -826,7 +931,7 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
 }
 
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-__global__ void __launch_bounds__(kAttnThreads, kAttnPlaces<DT, NT>) k_kv8_attn(const __grid_constant__ AttnDev a) {
+__global__ void __launch_bounds__(kAttnThreads, attn_places(DT, NT, HLQ)) k_kv8_attn(const __grid_constant__ AttnDev a) {
     op_begin();
     constexpr int kRows = 8 * NT;
     extern __shared__ unsigned char attn_smem_base[];

@@ -303,7 +303,7 @@ AttnPlan attn_plan(const OpContext& o, const i4d_kv8_attention_args& a) {
     // ones: the CTAs that fit the GPU share all tokens evenly, whatever the
     // lengths are (which the device alone knows), but no more of them than have
     // two tiles a warp.  Many rows are work enough by themselves.
-    const int64_t places = (p.dt == 256 || p.nt == 2 ? 2 : 4) * static_cast<int64_t>(o.num_sms);
+    const int64_t places = attn_places(p.dt, p.nt, a.dtype == I4D_F32) * static_cast<int64_t>(o.num_sms);
     p.cluster = 1;
     if (!p.prompt && p.row_tiles <= 4) {
         while (p.cluster < 8 && p.segments * p.cluster * 2 <= places && a.max_length > 128 * p.cluster) p.cluster *= 2;
