@@ -623,14 +623,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                         for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
                         tmem_store16(o_at + 16 * k, y);
                     }
-                    if (c & 1) {
-                        const __half2 fh = __float2half2_rn(f);
+                    if (c & 1) {  // (in FP32: FP16 may not hold the factor where it holds the product)
                         tmem_load16(p_at(c - 1), y);
                         tmem_wait_load16(y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y[i]), fh);
-                            y[i] = *reinterpret_cast<const uint32_t*>(&z);
+                            const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&y[i]));
+                            y[i] = pack_h2(z.x * f, z.y * f);
                         }
                         tmem_store16(p_at(c - 1), y);
                     }

@@ -78,8 +78,7 @@ def test_value_scales_of_exactly_zero(pkg, ctx, name, group, up):
 
 def _attend(pkg, ctx, s, q, n, length, scale, floor=0.0, one_part=2.0 ** -11):
     """Output within the bounds of tests/test_gpu_longctx.py (`one_part`: the probabilities' rounding for 16-bit outputs), and
-    `floor` of a row's greatest weight for each token that it sees.  The greatest weight is at most 1 times the
-    greatest value scale, and a token's code at most its |v| over its own scale."""
+    `floor` of a row's greatest weight (a probability times a value scale) for each token that it sees."""
     torch = _torch()
     lse = torch.empty(n, q.shape[1], device="cuda")
     out = ctx.kv8_attention(s.cache, q, s.dev([0, n]), s.dev([length]), s.dev(s.table), n, length, scale=scale, lse=lse)
@@ -89,10 +88,12 @@ def _attend(pkg, ctx, s, q, n, length, scale, floor=0.0, one_part=2.0 ** -11):
     p = 2 * dx + (2.0 ** -21 if q.dtype == torch.float32 else one_part) + length / 16 * 2.0 ** -23
     err = mag * p[..., None]
     if floor:
-        c = s.ref()
-        blocks = s.table[0, :-(-length // s.bs)]
-        codes = np.abs(c.codes[1][blocks]).transpose(1, 0, 2, 3).reshape(s.heads, -1, s.dim)[:, :length].sum(1)
-        err = err + floor * np.repeat(codes * c.scale[1][blocks].max(0)[:, None], q.shape[1] // s.heads, 0)
+        c, blocks = s.ref(), s.table[0, np.arange(length) // s.bs]
+        for row, a in np.ndindex(n, q.shape[1]):
+            h, see = a // (q.shape[1] // s.heads), length - n + row + 1
+            x = c.tokens(0, s.table[0], h, np.arange(see)) @ _np(q)[row, a] * scale
+            greatest = (np.exp(x - w_lse[row, a]) * c.scale[1][blocks[:see], h]).max()
+            err[row, a] += floor * greatest * np.abs(c.codes[1][blocks[:see], h, np.arange(see) % s.bs]).sum(0)
     # (FP16 values under 2^-14 lie 2^-24 apart)
     assert np.all(np.abs(_np(out) - w_out) <= err + _half(q.dtype) * (np.abs(w_out) + err) + (2.0 ** -25 if q.dtype == torch.float16 else 1e-30))
     assert np.all(np.abs(_np(lse) - w_lse) <= dx + length / 16 * 2.0 ** -23 + 2.0 ** -22 * (np.abs(w_lse) + 1))
@@ -103,8 +104,9 @@ def _half(t):
     return _torch().finfo(t).eps / 2
 
 
-def _sink(pkg, kind, length, at, seed):
-    """Equal scores, but for one token at `at` of value 0; positive values, so that errors of equal probabilities add up."""
+def _sinks(pkg, kind, length, at, seed):
+    """Equal scores, but for the tokens of value 0 at `at` and every 100 behind it, so that all CTAs and warps have some;
+    positive values, so that errors of equal probabilities add up."""
     torch = _torch()
     s = Setup(pkg, [length], 1, 64, 64, kind, seed)
     top = 12 if kind == "int8" else 10
@@ -113,20 +115,21 @@ def _sink(pkg, kind, length, at, seed):
     s.cache.v.copy_(v.to(s.cache.v.dtype))
     for x in (s.cache.k_scale, s.cache.v_scale):
         x.fill_(1.0)
-    block, slot = int(s.table[0, at // 64]), at % 64
-    s.cache.k[block, 0, slot, 0] = 64
-    s.cache.v[block, 0, slot] = 0
+    where = np.arange(at, length, 100)
+    block, slot = torch.from_numpy(s.table[0, where // 64].astype(np.int64)).cuda(), torch.from_numpy(where % 64).cuda()
+    s.cache.k.view(torch.int8)[block, 0, slot, 0] = 64 if kind == "int8" else 0x68  # 64 as a code of either kind
+    s.cache.v.view(torch.int8)[block, 0, slot] = 0
     return s
 
 
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("kind,at", [("int8", 0), ("e4m3", 0), ("int8", 20001), ("e4m3", 32768)])
+@pytest.mark.parametrize("kind,at", [("int8", 0), ("e4m3", 0), ("int8", 17), ("e4m3", 99)])
 @pytest.mark.parametrize("down", [22.3, 26.7, 60.2])
 def test_small_probabilities_of_a_long_tail(pkg, ctx, name, kind, at, down):
-    """32768 tokens of 2^-down of the greatest weight, whose own value is 0: their relative precision is the output's.  Ones
+    """32441 tokens of 2^-down of the greatest weights, whose own values are 0: their relative precision is the output's.  Ones
     under FP16's range for 16-bit outputs too, though those of FP16 are then 0."""
     torch = _torch()
-    s = _sink(pkg, kind, 32769, at, 83)
+    s = _sinks(pkg, kind, 32769, at, 83)
     q = torch.zeros(1, 3, 64, device="cuda", dtype=_type(name))
     q[:, :, 0] = 1
     _attend(pkg, ctx, s, q, 1, 32769, down * np.log(2) / 64)
@@ -141,3 +144,25 @@ def test_far_scores_of_many_draws(pkg, ctx, name, kind):
         s = Setup(pkg, [300], 2, 128, 32, kind, 100 + seed)
         q = torch.randn(1, 8, 128, generator=torch.Generator().manual_seed(seed)).to(_type(name)).cuda()
         _attend(pkg, ctx, s, q, 1, 300, 0.2 * (1 + seed % 5))
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("down", [15.0, 25.9, 31.0])
+@pytest.mark.parametrize("at", [5, 40, 70, 100])
+def test_probabilities_before_a_far_greater_one_in_prompts(pkg, ctx, name, kind, down, at):
+    """One score of 2^down times the others', of value 0, anywhere among the first 128 tokens, and 32 of 2^(down / 4.8) before
+    it, which do not raise their row's bound: the weights before it are scaled down with the sums, by less than FP16 holds."""
+    torch = _torch()
+    s = Setup(pkg, [128], 1, 64, 64, kind, 97)
+    s.cache.k.zero_()
+    s.cache.v.fill_(64)
+    for x in (s.cache.k_scale, s.cache.v_scale):
+        x.fill_(1.0)
+    block, slot = int(s.table[0, at // 64]), at % 64
+    s.cache.k[block, 0, slot - slot % 64:slot - slot % 64 + 32, 0] = 20  # the 32 tokens of a half's first part
+    s.cache.k[block, 0, slot, 0] = 96
+    s.cache.v.view(torch.int8)[block, 0, slot] = 0
+    q = torch.zeros(1, 80, 64, device="cuda", dtype=_type(name))
+    q[:, :, 0] = 1
+    _attend(pkg, ctx, s, q, 1, 128, down * np.log(2) / 96, floor=2.0 ** -24)
