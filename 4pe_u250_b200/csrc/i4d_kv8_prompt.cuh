@@ -12,7 +12,9 @@
 // dims contiguous too (the transposed form), so both convert alike; P is the
 // first operand straight from tensor memory.  The arithmetic is
 // i4d_kv8_attn.cuh's: exact codes and query rows, FP32 sums, probabilities in
-// one FP16 part.  A row's statistics stay in its thread, and O is rescaled
+// one FP16 part (2^-11 of it, but not less than 2^-32 of the row's greatest:
+// the few-row kernel's second look at small weights has no tensor memory left
+// for its sums here).  A row's statistics stay in its thread, and O is rescaled
 // only where a score passes the bound by more than 2^6.
 // Bound: 4 dim products a visible (row, token) at the tensor rate, and one
 // exponential for each at the rate of the special-function units, which for
@@ -148,6 +150,8 @@ __device__ __forceinline__ void tmem_wait_load16(uint32_t x[16]) {
                  : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]),
                    "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15])::"memory");
 }
+// 2^x for a whole x <= 0; -inf and NaN (of two -inf) 0.
+__device__ __forceinline__ float whole_ex2(float x) { return x >= -126.f ? __int_as_float((static_cast<int>(x) + 127) << 23) : 0.f; }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -595,10 +599,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                             p[8 * g + i] = pack_h2(z.x, z.y);
                         }
                     }
-                    const bool raise = top > M + kSlack || rtop > R + kSlack;
+                    const bool raise = top > M + kSlack || rtop > R + (kSlack + kHead);
                     if (!__any_sync(~0u, raise)) break;
-                    const float m = raise ? fmaxf(top, M) : M, rr = raise ? fmaxf(fmaxf(rtop, R), m - kFarScales) : R;
-                    const float fm = M == m ? 1.f : ex2(M - m), f = R == rr ? 1.f : ex2(R - rr);
+                    // (whole powers of two: the sums and the halves so far are scaled exactly)
+                    const float m = raise ? fmaxf(top, M) : M, rr = raise ? ceilf(fmaxf(fmaxf(rtop - kHead, R), m - kFarScales)) : R;
+                    const float fm = M == m ? 1.f : ex2(M - m), f = whole_ex2(R - rr);
                     sum[0].x *= fm;
                     sum[0].y *= fm;
                     sum[1].x *= fm;

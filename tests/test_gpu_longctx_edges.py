@@ -166,3 +166,30 @@ def test_probabilities_before_a_far_greater_one_in_prompts(pkg, ctx, name, kind,
     q = torch.zeros(1, 80, 64, device="cuda", dtype=_type(name))
     q[:, :, 0] = 1
     _attend(pkg, ctx, s, q, 1, 128, down * np.log(2) / 96, floor=2.0 ** -24)
+
+
+# Above 64 rows a weight in FP16 is off by half a step of 2^-24 when it is made
+# and once more when its row's bound is raised, 2^-24 in all, where the greatest
+# is at least 2^8 (2^9, and the bound goes up to a whole power of two).
+PROMPT_FLOOR = 2.0 ** -32
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("kind,at", [("int8", 0), ("e4m3", 0), ("int8", 17), ("e4m3", 99)])
+def test_small_probabilities_of_a_long_tail_in_prompts(pkg, ctx, name, kind, at):
+    """As above for many rows, whose weights are right to 2^-32 of the greatest: 2^-9.7 of each here, 2^-2.7 if they lay at 1."""
+    torch = _torch()
+    s = _sinks(pkg, kind, 32769, at, 89)
+    q = torch.zeros(1, 80, 64, device="cuda", dtype=_type(name))
+    q[:, :, 0] = 1
+    _attend(pkg, ctx, s, q, 1, 32769, 22.3 * np.log(2) / 64, floor=PROMPT_FLOOR)
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_far_scores_of_many_draws_in_prompts(pkg, ctx, name, kind):
+    torch = _torch()
+    for seed in range(8):
+        s = Setup(pkg, [300], 2, 128, 32, kind, 200 + seed)
+        q = torch.randn(2, 80, 128, generator=torch.Generator().manual_seed(seed)).to(_type(name)).cuda()
+        _attend(pkg, ctx, s, q, 2, 300, 0.2 * (1 + seed % 5), floor=PROMPT_FLOOR)
