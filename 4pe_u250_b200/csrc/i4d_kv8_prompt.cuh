@@ -12,9 +12,10 @@
 // dims contiguous too (the transposed form), so both convert alike; P is the
 // first operand straight from tensor memory.  The arithmetic is
 // i4d_kv8_attn.cuh's: exact codes and query rows, FP32 sums, probabilities in
-// one FP16 part (2^-11 of it, but not less than 2^-32 of the row's greatest:
-// the few-row kernel's second look at small weights has no tensor memory left
-// for its sums here).  A row's statistics stay in its thread, and O is rescaled
+// one FP16 part for BF16 outputs (2^-11), in two for FP16 ones (2^-22, twice the
+// second products), but not less than 2^-31 of the row's greatest: the few-row
+// kernel's second look at small weights has no tensor memory left for its sums
+// here.  A row's statistics stay in its thread, and O is rescaled
 // only where a score passes the bound by more than 2^6.
 // Bound: 4 dim products a visible (row, token) at the tensor rate, and one
 // exponential for each at the rate of the special-function units, which for
@@ -318,7 +319,8 @@ __device__ __forceinline__ void each_piece(const AttnDev& a, int64_t u, int64_t 
     }
 }
 
-template <int DT, int CODE>
+// HLP: probabilities in two parts, which both lie in place of their own scores.
+template <int DT, int CODE, bool HLP>
 __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_constant__ AttnDev a) {
     op_begin();
     using L = PromptSmem<DT>;
@@ -449,8 +451,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                             if (!ok) break;
                             fence_after();
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                product_ts(o_at, s_at + half * 64 + i * 8, v_desc + ((4 * half + i) * 2048 >> 4), kValues, j > 1 || half > 0 || i > 0);
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t p = s_at + half * 64 + (HLP ? (i >> 1) * 32 + (i & 1) * 8 : i * 8);
+                                const uint64_t vd = v_desc + ((4 * half + i) * 2048 >> 4);
+                                product_ts(o_at, p, vd, kValues, j > 1 || half > 0 || i > 0);
+                                if constexpr (HLP) product_ts(o_at, p + 16, vd, kValues, true);
+                            }
                             pr_commit(sh, kPvDone + at);
                             if (half) pr_commit(sh, kVEmpty);
                             if (j == count) continue;
@@ -565,7 +571,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
             bool whole = false;
             const float4* table = sh.table[(n + j) & 3];
             // 32 scores to probabilities, which overlay those of their half of the tile.
-            auto p_at = [&](int c) { return s_at + (c >> 1) * 64 + (c & 1) * 16; };
+            // (HLP: of their own chunk, the second parts 16 columns behind the first)
+            auto p_at = [&](int c) { return s_at + (c >> 1) * 64 + (c & 1) * (HLP ? 32 : 16); };
             auto chunk = [&](uint32_t (&x)[32], int c) {
                 if (!whole) {  // scores that the row does not see
                     const int lo = min(32, max(0, span.x - at - 32 * c)), hi = min(32, max(lo, min(span.y, s.len) - at - 32 * c));
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                 const float f0 = fmaxf(down * b0.x, 1e-37f), f1 = fmaxf(down * b1.x, 1e-37f);
                 const float m0 = max16(x) * f0, m1 = max16(x + 16) * f1;
                 const float top = fmaxf(m0, m1), rtop = fmaxf(m0 + b0.z, m1 + b1.z);
-                uint32_t p[16];
+                uint32_t p[16], pl[HLP ? 16 : 1];
                 float2 part[2];
                 for (;;) {
                     // With the bounds as they are; if a score passes them, again with raised ones.
@@ -597,6 +604,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                             part[g] = i ? add2(part[g], e) : e;
                             const float2 z = mul2(e, w);
                             p[8 * g + i] = pack_h2(z.x, z.y);
+                            if constexpr (HLP) pl[8 * g + i] = second_part<kTwoParts>(z.x, z.y, p[8 * g + i]);
                         }
                     }
                     const bool raise = top > M + kSlack || rtop > R + (kSlack + kHead);
@@ -628,20 +636,22 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                         for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
                         tmem_store16(o_at + 16 * k, y);
                     }
-                    if (c & 1) {  // (in FP32: FP16 may not hold the factor where it holds the product)
-                        tmem_load16(p_at(c - 1), y);
+#pragma unroll 1
+                    for (int k = 0; k < (c & 1) * (HLP ? 2 : 1); ++k) {  // (in FP32: FP16 may not hold the factor where it holds the product)
+                        tmem_load16(p_at(c - 1) + 16 * k, y);
                         tmem_wait_load16(y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&y[i]));
                             y[i] = pack_h2(z.x * f, z.y * f);
                         }
-                        tmem_store16(p_at(c - 1), y);
+                        tmem_store16(p_at(c - 1) + 16 * k, y);
                     }
                 }
                 sum[0] = add2(sum[0], part[0]);
                 sum[1] = add2(sum[1], part[1]);
                 tmem_store16(p_at(c), p);
+                if constexpr (HLP) tmem_store16(p_at(c) + 16, pl);
             };
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {

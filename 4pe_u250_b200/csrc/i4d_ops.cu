@@ -382,12 +382,14 @@ constexpr int kPromptSmem = PromptSmem<DT>::total + 1024;
 
 template <int DT, int CODE>
 cudaError_t launch_prompt(const AttnDev& d, int64_t grid, cudaStream_t st) {
-    return launch(k_kv8_prompt<DT, CODE>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
+    if (d.dtype == I4D_F16) return launch(k_kv8_prompt<DT, CODE, true>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
+    return launch(k_kv8_prompt<DT, CODE, false>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
 }
 
 template <int DT, int CODE>
 cudaError_t prompt_attr() {
-    return cudaFuncSetAttribute(k_kv8_prompt<DT, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
+    const cudaError_t e = cudaFuncSetAttribute(k_kv8_prompt<DT, CODE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_kv8_prompt<DT, CODE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
 }
 
 template <int CODE>
