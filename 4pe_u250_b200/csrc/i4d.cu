@@ -126,6 +126,8 @@ struct i4d_ctx {
     unsigned* d_counters = nullptr;
     unsigned* d_err = nullptr;
     unsigned* d_op_err = nullptr;  // error word of the long-context operators
+    unsigned* h_op_err = nullptr;  // where it is read from, by a stream of its own
+    cudaStream_t op_err_stream = nullptr;
     int* d_pos = nullptr;
     int* d_tok = nullptr;                    // greedy: input token id
     unsigned long long* d_argmax = nullptr;  // greedy: argmax key of the step's logits
@@ -574,7 +576,7 @@ bool all_loaded(const i4d_ctx* c) {
 
 namespace i4d_ops {
 
-OpContext op_context(const i4d_ctx* c) { return {c->device, c->num_sms, c->stream, c->d_op_err}; }
+OpContext op_context(const i4d_ctx* c) { return {c->device, c->num_sms, c->stream, c->d_op_err, c->h_op_err, c->op_err_stream}; }
 
 i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) {
     char buf[512];
@@ -614,9 +616,10 @@ void i4d_destroy(i4d_ctx* c) {
     for (void* p : dev)
         if (p) cudaFree(p);
     void* host[] = {c->h_resid_in, c->h_resid_out, c->h_logits, c->h_pos, c->h_err, c->h_tok, c->h_argmax,
-                    c->h_sample_state, c->h_sample_out, c->h_pf_resid, c->h_pf_pos, c->h_pf_ids, c->h_pf_terms};
+                    c->h_sample_state, c->h_sample_out, c->h_pf_resid, c->h_pf_pos, c->h_pf_ids, c->h_pf_terms, c->h_op_err};
     for (void* p : host)
         if (p) cudaFreeHost(p);
+    if (c->op_err_stream) cudaStreamDestroy(c->op_err_stream);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
 }
@@ -709,6 +712,8 @@ static i4d_status create_impl(const i4d_config* cfg, int rank, int world, i4d_ct
     CKC(cudaMemset(c->d_err, 0, sizeof(unsigned)));
     CKC(cudaMalloc(&c->d_op_err, sizeof(unsigned)));
     CKC(cudaMemset(c->d_op_err, 0, sizeof(unsigned)));
+    CKC(cudaMallocHost(&c->h_op_err, sizeof(unsigned)));
+    CKC(cudaStreamCreateWithFlags(&c->op_err_stream, cudaStreamNonBlocking));
     CKC(i4d_ops::ops_init());
     CKC(cudaMalloc(&c->d_pos, sizeof(int)));
     CKC(cudaMalloc(&c->d_tok, sizeof(int)));

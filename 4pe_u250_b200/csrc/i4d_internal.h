@@ -12,6 +12,8 @@ struct OpContext {
     int num_sms;
     cudaStream_t stream;
     unsigned* err;  // device error word of the operators
+    unsigned* err_taken;       // host memory that the device can write: what ops_report took out of it
+    cudaStream_t err_stream;   // which nothing else uses
 };
 
 // i4d.cu
@@ -20,7 +22,8 @@ i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) __attribute_
 
 // i4d_ops.cu: shared-memory sizes of the operators' kernels, with the context's device current.
 cudaError_t ops_init();
-// The operators' error word since the last call, and zero in its place; the caller has waited for their stream.
+// The operators' error word since the last call, with zero put in its place in
+// the same step; the caller has waited for the operators that it asks about.
 i4d_status ops_report(i4d_ctx* c);
 
 }  // namespace i4d_ops

@@ -19,6 +19,10 @@ using namespace i4d_ops;
 
 namespace {
 
+// Takes the error word and leaves zero in one step: what an operator on another
+// stream reports meanwhile is either taken or still there for the next call.
+__global__ void k_take_errors(unsigned* err, unsigned* taken) { *taken = atomicExch(err, 0u); }
+
 // The context's device for the length of a call; the caller's is put back.
 class DeviceScope {
   public:
@@ -453,12 +457,11 @@ cudaError_t ops_init() {
 
 i4d_status ops_report(i4d_ctx* ctx) {
     const OpContext o = op_context(ctx);
-    unsigned e = 0;
-    OP_CK(cudaMemcpyAsync(&e, o.err, sizeof(e), cudaMemcpyDeviceToHost, o.stream));
-    OP_CK(cudaStreamSynchronize(o.stream));
+    k_take_errors<<<1, 1, 0, o.err_stream>>>(o.err, o.err_taken);
+    OP_CK(cudaGetLastError());
+    OP_CK(cudaStreamSynchronize(o.err_stream));
+    const unsigned e = *static_cast<volatile unsigned*>(o.err_taken);
     if (!e) return I4D_OK;
-    OP_CK(cudaMemsetAsync(o.err, 0, sizeof(e), o.stream));
-    OP_CK(cudaStreamSynchronize(o.stream));
     if (e & kTimeout) return op_fail(ctx, I4D_ERR_TIMEOUT, "a bounded device wait of an operator gave up (error word 0x%x)", e);
     return op_fail(ctx, I4D_ERR_ARG, "an operator skipped tokens:%s%s", e & kBadSequence ? " q_start or lengths out of range;" : "",
                    e & kBadBlock ? " block id outside the pool;" : "");

@@ -607,7 +607,10 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* args);
 
 /* Waits for `stream` (as above) and reports the device error bits of the
  * operators above since the last check: I4D_ERR_ARG and a message naming what
- * was out of range.  i4d_sync reports them too, for the context's stream. */
+ * was out of range.  The bits belong to the context: a check reports, once,
+ * what its operators have found by then on any stream, and what they find
+ * later is left for the next.  i4d_sync reports them too, behind the context's
+ * stream. */
 i4d_status i4d_ops_check(i4d_ctx* ctx, void* stream);
 
 #ifdef __cplusplus

@@ -213,3 +213,30 @@ def test_probabilities_go_in_two_parts(pkg, ctx, name, kind, heads):
     q[:, :, 0] = 1
     out = _attend(pkg, ctx, s, q, 1, 128, 0.3 * np.log(2), floor=PROMPT_FLOOR, one_part=2.0 ** -21)
     assert torch.all(out.abs() < 0.1)
+
+
+# ------------------------------------------------------------------ errors
+
+def test_no_report_is_lost_between_streams(pkg, ctx):
+    """A wrong block id found on one stream while a check on another one takes what was found before: a check reports it."""
+    torch = _torch()
+    s = Setup(pkg, [20], 1, 64, 16, "int8", 103)
+    k = torch.randn(1, 1, 64, device="cuda").bfloat16()
+    start, long, fits, table = s.dev([0, 1]), s.dev([999]), s.dev([20]), s.dev(s.table)
+    bad = torch.full_like(table, -1)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.ops_check()
+    for i in range(600):
+        ctx.kv8_append(s.cache, k, k, start, long, table, 1)
+        torch.cuda.current_stream().synchronize()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(200 * i)  # up to 60 us: before, in and behind the check
+            ctx.kv8_append(s.cache, k, k, start, fits, bad, 1)
+        with pytest.raises(pkg.I4DError, match="lengths") as first:
+            ctx.ops_check()
+        other.synchronize()
+        if "block id" not in str(first.value):
+            with pytest.raises(pkg.I4DError, match="block id"):
+                ctx.ops_check()
+    ctx.ops_check()
