@@ -128,6 +128,7 @@ struct i4d_ctx {
     unsigned* d_op_err = nullptr;  // error word of the long-context operators
     unsigned* h_op_err = nullptr;  // where it is read from, by a stream of its own
     cudaStream_t op_err_stream = nullptr;
+    mutable bool ops_used = false;           // since then i4d_sync looks at it
     int* d_pos = nullptr;
     int* d_tok = nullptr;                    // greedy: input token id
     unsigned long long* d_argmax = nullptr;  // greedy: argmax key of the step's logits
@@ -576,7 +577,7 @@ bool all_loaded(const i4d_ctx* c) {
 
 namespace i4d_ops {
 
-OpContext op_context(const i4d_ctx* c) { return {c->device, c->num_sms, c->stream, c->d_op_err, c->h_op_err, c->op_err_stream}; }
+OpContext op_context(const i4d_ctx* c) { return {c->device, c->num_sms, c->stream, c->d_op_err, c->h_op_err, c->op_err_stream, &c->ops_used}; }
 
 i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) {
     char buf[512];
@@ -1355,7 +1356,7 @@ i4d_status i4d_sync(i4d_ctx* c) {
     if (!c) return I4D_ERR_ARG;
     CK(cudaSetDevice(c->device));
     const i4d_status st = finish(c);
-    return st == I4D_OK ? i4d_ops::ops_report(c) : st;
+    return st == I4D_OK && c->ops_used ? i4d_ops::ops_report(c) : st;
 }
 
 void* i4d_stream(i4d_ctx* c) { return c ? static_cast<void*>(c->stream) : nullptr; }

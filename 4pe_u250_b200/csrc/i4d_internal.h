@@ -14,6 +14,7 @@ struct OpContext {
     unsigned* err;  // device error word of the operators
     unsigned* err_taken;       // host memory that the device can write: what ops_report took out of it
     cudaStream_t err_stream;   // which nothing else uses
+    bool* used;                // host: an operator has been enqueued (null: nobody asks)
 };
 
 // i4d.cu

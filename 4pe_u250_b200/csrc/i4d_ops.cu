@@ -59,7 +59,9 @@ int dtype_bytes(int t) { return t == I4D_F32 ? 4 : 2; }
 bool is_dtype(int t) { return t == I4D_F32 || t == I4D_BF16 || t == I4D_F16; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// The stream of an operator that is about to be enqueued.
 cudaStream_t stream_of(const OpContext& o, void* stream) {
+    if (o.used) *o.used = true;
     return stream ? static_cast<cudaStream_t>(stream) : o.stream;
 }
 
@@ -880,7 +882,7 @@ i4d_status i4d_ops_check(i4d_ctx* ctx, void* stream) {
     const OpContext o = op_context(ctx);
     DeviceScope scope(o.device);
     OP_CK(scope.error());
-    OP_CK(cudaStreamSynchronize(stream_of(o, stream)));
+    OP_CK(cudaStreamSynchronize(stream ? static_cast<cudaStream_t>(stream) : o.stream));
     return ops_report(ctx);
 }
 

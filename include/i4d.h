@@ -610,7 +610,7 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* args);
  * was out of range.  The bits belong to the context: a check reports, once,
  * what its operators have found by then on any stream, and what they find
  * later is left for the next.  i4d_sync reports them too, behind the context's
- * stream. */
+ * stream, once the context has enqueued an operator. */
 i4d_status i4d_ops_check(i4d_ctx* ctx, void* stream);
 
 #ifdef __cplusplus

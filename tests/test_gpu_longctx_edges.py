@@ -240,3 +240,37 @@ def test_no_report_is_lost_between_streams(pkg, ctx):
             with pytest.raises(pkg.I4DError, match="block id"):
                 ctx.ops_check()
     ctx.ops_check()
+
+
+def test_sync_asks_for_reports_only_where_operators_ran(pkg):
+    """A context of the decoder alone does not wait for the operators' error word; one whose operators are in a graph does."""
+    import time
+    torch = _torch()
+
+    def micros(c):
+        best = 1e9
+        for _ in range(20):
+            t = time.perf_counter()
+            for _ in range(50):
+                c.sync()
+            best = min(best, (time.perf_counter() - t) / 50 * 1e6)
+        return best
+
+    with pkg.Context(num_layers=1, kv_capacity=8) as c:
+        alone = micros(c)
+        s = Setup(pkg, [20], 1, 64, 16, "int8", 107)
+        k = torch.randn(1, 1, 64, device="cuda").bfloat16()
+        lens = s.dev([20])
+        args = (s.cache, k, k, s.dev([0, 1]), lens, s.dev(s.table), 1)
+        c.kv8_append(*args)
+        c.sync()
+        assert alone < 0.8 * micros(c)  # one wait and one copy of three of each
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.kv8_append(*args)
+        lens.fill_(999)
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(pkg.I4DError, match="lengths"):
+            c.sync()
