@@ -9,6 +9,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <Python.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -504,7 +505,17 @@ PyObject* logits_process(Args& a) {
     return give(out);
 }
 
+// Waits for the stream without Python's lock, which what the stream waits for
+// may need; what follows then waits for nothing of it, and the context and its
+// message are touched with the lock held.
 PyObject* ops_check(Args& a) {
+    const cudaStream_t s = a.stream();
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(a.device()));
+    cudaError_t e;
+    Py_BEGIN_ALLOW_THREADS;
+    e = cudaStreamSynchronize(s);
+    Py_END_ALLOW_THREADS;
+    if (e != cudaSuccess) throw OpError{I4D_ERR_CUDA, cudaGetErrorString(e)};
     check(a.ctx(), i4d_ops_check(a.ctx(), a.stream()));
     Py_RETURN_NONE;
 }

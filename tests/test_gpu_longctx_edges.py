@@ -274,3 +274,30 @@ def test_sync_asks_for_reports_only_where_operators_ran(pkg):
         torch.cuda.synchronize()
         with pytest.raises(pkg.I4DError, match="lengths"):
             c.sync()
+
+
+def test_a_check_lets_other_threads_run(pkg, ctx):
+    """What the stream of a check waits for may need Python: the check waits without holding it."""
+    import threading
+    import time
+    torch = _torch()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    began = threading.Event()
+
+    def check():
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(10 ** 9)  # about half a second
+            began.set()
+            ctx.ops_check()
+
+    t = threading.Thread(target=check)
+    t.start()
+    began.wait()
+    ran = 0
+    for _ in range(10):
+        time.sleep(0.01)
+        ran += t.is_alive()
+    t.join()
+    assert ran == 10
+    ctx.ops_check()
