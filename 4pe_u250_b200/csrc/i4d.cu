@@ -715,7 +715,6 @@ static i4d_status create_impl(const i4d_config* cfg, int rank, int world, i4d_ct
     CKC(cudaMemset(c->d_op_err, 0, sizeof(unsigned)));
     CKC(cudaMallocHost(&c->h_op_err, sizeof(unsigned)));
     CKC(cudaStreamCreateWithFlags(&c->op_err_stream, cudaStreamNonBlocking));
-    CKC(i4d_ops::ops_init());
     CKC(cudaMalloc(&c->d_pos, sizeof(int)));
     CKC(cudaMalloc(&c->d_tok, sizeof(int)));
     CKC(cudaMalloc(&c->d_argmax, sizeof(unsigned long long)));

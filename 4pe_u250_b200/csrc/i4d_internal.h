@@ -21,9 +21,7 @@ struct OpContext {
 OpContext op_context(const i4d_ctx* c);
 i4d_status op_fail(i4d_ctx* c, i4d_status st, const char* fmt, ...) __attribute__((format(printf, 3, 4)));
 
-// i4d_ops.cu: shared-memory sizes of the operators' kernels, with the context's device current.
-cudaError_t ops_init();
-// The operators' error word since the last call, with zero put in its place in
+// i4d_ops.cu.  The operators' error word since the last call, with zero put in its place in
 // the same step; the caller has waited for the operators that it asks about.
 i4d_status ops_report(i4d_ctx* c);
 

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
@@ -203,6 +204,31 @@ cudaError_t launch(void (*kernel)(Params...), int64_t grid, unsigned block, size
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// A kernel with more shared memory than every kernel has.  `allowed`, of that
+// kernel alone: the devices where it has been said how much; that is said at
+// its first launch, which loads it, and not for the contexts that never call it
+// (27 ms of i4d_create).  Saying it is no work for a stream and may happen
+// while one is captured.
+template <typename... Params, typename... Args>
+cudaError_t launch_large(std::atomic<uint64_t>& allowed, int most, void (*kernel)(Params...), int64_t grid, unsigned block, size_t smem, int ctas,
+                         cudaStream_t st, Args... args) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(allowed.load(std::memory_order_acquire) & bit)) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        e = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return e;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e == cudaSuccess) e = back;
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_release);
+    }
+    return launch(kernel, grid, block, smem, ctas, st, args...);
+}
+
 // ------------------------------------------------------------------ rope
 
 template <typename T, int V, bool IL>
@@ -354,7 +380,8 @@ i4d_status check_attention(i4d_ctx* ctx, const i4d_kv8_attention_args* a) {
 template <int DT, int CODE, int NT, bool HLQ, bool HLP>
 cudaError_t launch_attn(const AttnDev& d, int64_t grid, cudaStream_t st) {
     static_assert(attn_smem<DT, NT>() <= 114688, "two CTAs an SM");
-    return launch(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, grid, kAttnThreads, attn_smem<DT, NT>(), d.cluster, st, d);
+    static std::atomic<uint64_t> allowed{0};
+    return launch_large(allowed, attn_smem<DT, NT>(), k_kv8_attn<DT, CODE, NT, HLQ, HLP>, grid, kAttnThreads, attn_smem<DT, NT>(), d.cluster, st, d);
 }
 
 template <int DT, int CODE>
@@ -366,41 +393,23 @@ cudaError_t launch_attn_d(const AttnDev& d, const AttnPlan& p, int64_t grid, cud
     return d.dtype == I4D_F16 ? launch_attn<DT, CODE, 1, false, true>(d, grid, st) : launch_attn<DT, CODE, 1, false, false>(d, grid, st);
 }
 
-template <int DT, int CODE, int NT, bool HLQ, bool HLP>
-cudaError_t attn_attr() {
-    return cudaFuncSetAttribute(k_kv8_attn<DT, CODE, NT, HLQ, HLP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(attn_smem<DT, NT>()));
-}
-
-template <int DT, int CODE>
-cudaError_t attn_attrs() {
-    cudaError_t e = attn_attr<DT, CODE, 1, true, true>();
-    if (e == cudaSuccess) e = attn_attr<DT, CODE, 1, false, true>();
-    if (e == cudaSuccess) e = attn_attr<DT, CODE, 1, false, false>();
-    if constexpr (DT <= 128) {
-        if (e == cudaSuccess) e = attn_attr<DT, CODE, 2, false, true>();
-        if (e == cudaSuccess) e = attn_attr<DT, CODE, 2, false, false>();
-    }
-    return e;
-}
-
 template <int DT>
 constexpr int kPromptSmem = PromptSmem<DT>::total + 1024;
 
-template <int DT, int CODE>
+template <int DT, int CODE, bool HLP>
 cudaError_t launch_prompt(const AttnDev& d, int64_t grid, cudaStream_t st) {
-    if (d.dtype == I4D_F16) return launch(k_kv8_prompt<DT, CODE, true>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
-    return launch(k_kv8_prompt<DT, CODE, false>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
+    static std::atomic<uint64_t> allowed{0};
+    return launch_large(allowed, kPromptSmem<DT>, k_kv8_prompt<DT, CODE, HLP>, grid, kPrThreads, kPromptSmem<DT>, 1, st, d);
 }
 
 template <int DT, int CODE>
-cudaError_t prompt_attr() {
-    const cudaError_t e = cudaFuncSetAttribute(k_kv8_prompt<DT, CODE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_kv8_prompt<DT, CODE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem<DT>);
+cudaError_t launch_prompt_t(const AttnDev& d, int64_t grid, cudaStream_t st) {
+    return d.dtype == I4D_F16 ? launch_prompt<DT, CODE, true>(d, grid, st) : launch_prompt<DT, CODE, false>(d, grid, st);
 }
 
 template <int CODE>
 cudaError_t launch_attn_c(const AttnDev& d, const AttnPlan& p, int64_t grid, cudaStream_t st) {
-    if (p.prompt) return p.dt == 64 ? launch_prompt<64, CODE>(d, grid, st) : launch_prompt<128, CODE>(d, grid, st);
+    if (p.prompt) return p.dt == 64 ? launch_prompt_t<64, CODE>(d, grid, st) : launch_prompt_t<128, CODE>(d, grid, st);
     return p.dt == 64 ? launch_attn_d<64, CODE>(d, p, grid, st) : p.dt == 128 ? launch_attn_d<128, CODE>(d, p, grid, st) : launch_attn_d<256, CODE>(d, p, grid, st);
 }
 
@@ -413,6 +422,15 @@ cudaError_t launch_weights(const AttnDev& d, int tiles, int64_t grid, cudaStream
 template <int CODE>
 cudaError_t launch_weights_c(const AttnDev& d, const AttnPlan& p, int tiles, int64_t grid, cudaStream_t st) {
     return p.dt == 64 ? launch_weights<64, CODE>(d, tiles, grid, st) : p.dt == 128 ? launch_weights<128, CODE>(d, tiles, grid, st) : launch_weights<256, CODE>(d, tiles, grid, st);
+}
+
+// ---------------------------------------------------------------- logits
+
+template <typename T>
+cudaError_t launch_logits(const LogitsDev& d, unsigned grid, int ctas, cudaStream_t st) {
+    static std::atomic<uint64_t> allowed{0};
+    return launch_large(allowed, logits_smem_bytes(kLogitsTouched, kLogitsPart / 32), k_logits<T>, grid, kLogitsThreads, logits_smem_bytes(d.places, d.words),
+                        ctas, st, d, ctas);
 }
 
 // ----------------------------------------------------------------- evict
@@ -438,24 +456,6 @@ i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
 }  // namespace
 
 namespace i4d_ops {
-
-cudaError_t ops_init() {
-    const int logits_smem = logits_smem_bytes(kLogitsTouched, kLogitsPart / 32);
-    cudaError_t e = cudaFuncSetAttribute(k_logits<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logits<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, logits_smem);
-    if (e == cudaSuccess) e = attn_attrs<64, I4D_CODE_INT8>();
-    if (e == cudaSuccess) e = attn_attrs<64, I4D_CODE_E4M3>();
-    if (e == cudaSuccess) e = attn_attrs<128, I4D_CODE_INT8>();
-    if (e == cudaSuccess) e = attn_attrs<128, I4D_CODE_E4M3>();
-    if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_INT8>();
-    if (e == cudaSuccess) e = attn_attrs<256, I4D_CODE_E4M3>();
-    if (e == cudaSuccess) e = prompt_attr<64, I4D_CODE_INT8>();
-    if (e == cudaSuccess) e = prompt_attr<64, I4D_CODE_E4M3>();
-    if (e == cudaSuccess) e = prompt_attr<128, I4D_CODE_INT8>();
-    if (e == cudaSuccess) e = prompt_attr<128, I4D_CODE_E4M3>();
-    return e;
-}
 
 i4d_status ops_report(i4d_ctx* ctx) {
     const OpContext o = op_context(ctx);
@@ -868,11 +868,10 @@ i4d_status i4d_logits_process(i4d_ctx* ctx, const i4d_logits_args* a) {
     const int64_t ids = static_cast<int64_t>(a->history ? a->history_max : 0) + (a->bias_ids ? a->bias_max : 0);
     d.places = static_cast<int>(std::min<int64_t>(kLogitsTouched, (ids + 255) / 256 * 256));
     d.words = std::min(kLogitsPart / 32, ((a->vocab + ctas - 1) / ctas + 32 + 127) / 128 * 4);
-    const int smem = logits_smem_bytes(d.places, d.words);
     switch (a->dtype) {
-        case I4D_F32: OP_CK(launch(k_logits<float>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
-        case I4D_BF16: OP_CK(launch(k_logits<__nv_bfloat16>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
-        default: OP_CK(launch(k_logits<__half>, grid, kLogitsThreads, smem, ctas, s, d, ctas)); break;
+        case I4D_F32: OP_CK(launch_logits<float>(d, grid, ctas, s)); break;
+        case I4D_BF16: OP_CK(launch_logits<__nv_bfloat16>(d, grid, ctas, s)); break;
+        default: OP_CK(launch_logits<__half>(d, grid, ctas, s)); break;
     }
     return I4D_OK;
 }
