@@ -67,8 +67,8 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append
     const Seq s = load_seq(a.seq, b, report && j == 0);
     if (s.n == 0) return;
     const int bs = a.cache.block_tokens, dim = a.cache.dim;
-    const int first = s.len - s.n, blk = first / bs + j;
-    if (blk * bs >= s.len) return;
+    const int first = s.len - s.n, blk = touched_block(first, s.len, bs, j);
+    if (blk < 0) return;
     const int lo = max(first, blk * bs), hi = min(s.len, (blk + 1) * bs), old = lo - blk * bs;
     const T* in = static_cast<const T*>(a.in[which]) + static_cast<int64_t>(s.first + lo - first) * a.tok[which] +
                   h * a.head[which];

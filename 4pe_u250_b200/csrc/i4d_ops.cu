@@ -593,7 +593,7 @@ i4d_status i4d_kv8_append(i4d_ctx* ctx, const i4d_kv8_append_args* a) {
     d.head[0] = a->k_head_stride;
     d.head[1] = a->v_head_stride;
     const int bs = a->cache.block_tokens;
-    d.touched = (a->max_q + bs - 2) / bs + 1;
+    d.touched = touched_blocks(a->max_q, a->tokens, bs);
     const int64_t units = static_cast<int64_t>(a->batch) * d.touched * a->cache.heads * 2;
     OP_ARG(units <= kMaxGrid, "too many blocks in one call");
     // 8 elements an access: two of 16 bytes for FP32, one for the others

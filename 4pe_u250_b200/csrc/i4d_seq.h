@@ -23,6 +23,20 @@ I4D_HD bool seq_ok(int q0, int q1, int len, int tokens, int max_q, int table_blo
 
 I4D_HD bool block_ok(int id, int blocks) { return static_cast<unsigned>(id) < static_cast<unsigned>(blocks); }
 
+// Blocks that the new tokens of one sequence can touch: it has no more of them
+// than its call allows, has rows, or can have.
+I4D_HD int touched_blocks(int max_q, int tokens, int block_tokens) {
+    const int most = max_q < tokens ? max_q : tokens, n = most < kMaxTokens ? most : kMaxTokens;
+    return n <= 0 ? 0 : (n - 1 + block_tokens - 1) / block_tokens + 1;
+}
+
+// Block j of those that the tokens [first, len) of a sequence lie in, or -1.
+// (Blocks are compared, not tokens: the last one's end may pass 32 bits.)
+I4D_HD int touched_block(int first, int len, int block_tokens, int j) {
+    const int at = first / block_tokens + j;
+    return first < len && at <= (len - 1) / block_tokens ? at : -1;
+}
+
 // Length of a sequence that eviction reads.
 I4D_HD bool length_ok(int len, int max_length) { return len >= 0 && len <= max_length; }
 

@@ -386,3 +386,20 @@ print(*times)
         best.append(first / second)
     # the first context of a process also loads the decoder's few kernels (7.6 ms after 3.6); with the operators' forty it took 35
     assert min(best) < 5
+
+
+# ------------------------------------------------------------------ bounds
+
+@pytest.mark.parametrize("max_q", [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 30 + 1])
+@pytest.mark.parametrize("bs", [16, 128])
+def test_append_with_a_bound_of_new_tokens_near_32_bits(pkg, ctx, max_q, bs):
+    """The bound says nothing that the rows do not: the same cache as with the greatest count."""
+    torch = _torch()
+    new = torch.randn(45, 2, 64, generator=torch.Generator().manual_seed(9)).cuda().bfloat16()
+    found = []
+    for most in (40, max_q):
+        s = Setup(pkg, [300, 5], 2, 64, bs, "int8", 109)
+        ctx.kv8_append(s.cache, new, new, s.dev([0, 40, 45]), s.dev([300, 5]), s.dev(s.table), most)
+        found.append([x.clone() for x in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale)])
+    ctx.ops_check()
+    assert all(torch.equal(x, y) for x, y in zip(*found))
