@@ -447,6 +447,7 @@ i4d_status check_evict(i4d_ctx* ctx, const i4d_kv8_evict_args* a) {
     OP_ARG(a->batch >= 0, "negative batch");
     OP_ARG(a->max_length >= 0 && a->max_length <= kMaxTokens, "max_length %d", a->max_length);
     OP_ARG(a->budget > 0 && a->recent >= 0 && a->recent <= a->budget, "budget %d, recent %d (0 <= recent <= budget, 0 < budget)", a->budget, a->recent);
+    OP_ARG(a->budget <= kMaxTokens, "budget %d (2^30 at most: no sequence is longer)", a->budget);  // (an index and a step are an int)
     OP_ARG(a->table_stride >= 0 && a->table_blocks >= 0 && static_cast<int64_t>(a->table_blocks) * a->cache.block_tokens >= a->max_length,
            "block_table rows of %d blocks hold fewer than max_length %d tokens", a->table_blocks, a->max_length);
     OP_ARG(a->weights_stride >= a->max_length && a->weights_out_stride >= a->max_length, "weights' rows are shorter than max_length");

@@ -548,7 +548,7 @@ i4d_status i4d_kv8_attention_workspace(i4d_ctx* ctx, const i4d_kv8_attention_arg
 /* Brings every sequence that is longer than `budget` back to budget tokens,
  * for each cache head on its own: its last `recent` tokens stay, and of the
  * others the budget - recent of greatest weight (ties: the lower index; NaN
- * counts as the least).  The kept tokens move up in their order within the
+ * counts as the least); budget is at most 2^30.  The kept tokens move up in their order within the
  * sequence's own blocks, so the blocks behind the new length are free.  A
  * block's scale becomes the greatest of the scales its tokens had, codes
  * round(code * had / greatest).  keep [batch][cache heads][budget] receives

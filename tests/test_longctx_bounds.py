@@ -51,3 +51,14 @@ def test_a_block_lies_in_the_sequence_or_nowhere(seq, bs):
                 at = first // bs + j
                 want = at if first < length and at * bs < length else -1
                 assert seq.touched_block(first, length, bs, j) == want, (first, length, j)
+
+
+from test_longctx_refusals import ERR_ARG, ERR_CUDA, _call, _evict, lib  # noqa: E402,F401
+
+
+@pytest.mark.parametrize("budget,accepted", [(MOST, True), (MOST + 1, False), (TOP - 4095, False), (TOP, False)])
+def test_budgets_beyond_any_sequence_are_refused(lib, budget, accepted):  # noqa: F811
+    """An index that steps through keep's entries of one row stays in 32 bits."""
+    args = _evict(budget=budget, recent=0, keep=0x70000000000)
+    assert _call(lib, "i4d_kv8_evict", args) == (ERR_CUDA if accepted else ERR_ARG)
+    assert accepted or b"budget" in lib.stub_message()
