@@ -162,10 +162,10 @@ __device__ __forceinline__ void load_q16(const AttnDev& a, int64_t i, float out[
         const float* p = static_cast<const float*>(a.q) + i;
         if (a.wide_q) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(out + 4 * k) = __ldg(reinterpret_cast<const float4*>(p) + k);
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(out + 4 * k) = fetch(reinterpret_cast<const float4*>(p) + k);
         } else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) out[k] = __ldg(p + k);
+            for (int k = 0; k < 16; ++k) out[k] = fetch(p + k);
         }
         return;
     }
@@ -175,11 +175,11 @@ __device__ __forceinline__ void load_q16(const AttnDev& a, int64_t i, float out[
         unsigned short h[16];
     } x;
     if (a.wide_q) {
-        x.v[0] = __ldg(reinterpret_cast<const uint4*>(p));
-        x.v[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        x.v[0] = fetch(reinterpret_cast<const uint4*>(p));
+        x.v[1] = fetch(reinterpret_cast<const uint4*>(p) + 1);
     } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) x.h[k] = __ldg(p + k);
+        for (int k = 0; k < 16; ++k) x.h[k] = fetch(p + k);
     }
 #pragma unroll
     for (int k = 0; k < 16; ++k)
@@ -302,7 +302,7 @@ __device__ __forceinline__ void load_ktile(const uint8_t* k, int dim, int n, KTi
 #pragma unroll
         for (int c = 0; c < DT / 64; ++c) {
             const int d0 = k_dim<DT>(t, c);
-            kt.w[r][c] = (g + 8 * r < n && d0 < dim) ? __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * r) * dim + d0)) : make_uint4(0, 0, 0, 0);
+            kt.w[r][c] = (g + 8 * r < n && d0 < dim) ? fetch(reinterpret_cast<const uint4*>(k + (g + 8 * r) * dim + d0)) : make_uint4(0, 0, 0, 0);
         }
 }
 
@@ -690,8 +690,8 @@ __device__ __forceinline__ void attend(const AttnDev& a, const Seq& s, const Pie
                 float4 x = make_float4(__int_as_float(id), 0.f, 0.f, 0.f);
                 if (id >= 0) {
                     const int64_t at = static_cast<int64_t>(id) * a.cache.heads + h;
-                    x.y = __ldg(a.cache.scale[0] + at);
-                    x.z = __ldg(a.cache.scale[1] + at);
+                    x.y = fetch(a.cache.scale[0] + at);
+                    x.z = fetch(a.cache.scale[1] + at);
                     x.w = __log2f(x.z);  // only a bound: its rounding cancels
                 }
                 s_block[i] = x;
@@ -1110,7 +1110,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv8_weights(AttnDev a, int til
     const int live = min(16, s.len - at);
     KTile<DT> kt;
     load_ktile<DT>(a.cache.codes[0] + code_offset(a.cache, id, h) + static_cast<int64_t>(at % bs) * dim, dim, live, kt);
-    const float ks = __ldg(a.cache.scale[0] + static_cast<int64_t>(id) * a.cache.heads + h);
+    const float ks = fetch(a.cache.scale[0] + static_cast<int64_t>(id) * a.cache.heads + h);
     float sum[2] = {0.f, 0.f};
     // rows whose query stands at or behind the first token and, with a window, not past the last one's
     const int rows = s.n * a.group;

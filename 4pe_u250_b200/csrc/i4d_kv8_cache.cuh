@@ -174,28 +174,42 @@ __global__ void __launch_bounds__(256) k_kv8_read(ReadDev a, int chunks) {
     const int b = blockIdx.x / chunks, i0 = blockIdx.x % chunks * kReadItems;
     const Seq s = load_seq(a.seq, b, threadIdx.x == 0 && i0 == 0);
     const int bs = a.cache.block_tokens, shift = 31 - __clz(bs), per_head = a.cache.dim / 16, per_tok = a.cache.heads * per_head;
+    // (all loads before the first store)
+    constexpr int kItems = kReadItems / 256;
+    uint4 codes[kItems][2];
+    float scale[kItems][2];
+    int64_t to[kItems];
 #pragma unroll
-    for (int u = 0; u < kReadItems / 256; ++u) {
+    for (int u = 0; u < kItems; ++u) {
         const int i = i0 + u * 256 + threadIdx.x;
         const int r = i / per_tok, e = i - r * per_tok, h = e / per_head, c = e - h * per_head;
+        to[u] = -1;
         if (r >= s.n) continue;
         const int p = s.len - s.n + r, id = load_block(a.seq, b, p >> shift, true);
         if (id < 0) continue;
+        to[u] = (static_cast<int64_t>(s.first + r) * a.cache.heads + h) * a.cache.dim + c * 16;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-            const float scale = __ldg(a.cache.scale[which] + static_cast<int64_t>(id) * a.cache.heads + h);
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.cache.codes[which] + code_offset(a.cache, id, h) +
-                                                                 static_cast<int64_t>(p & (bs - 1)) * a.cache.dim) + c);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+            scale[u][which] = fetch(a.cache.scale[which] + static_cast<int64_t>(id) * a.cache.heads + h);
+            codes[u][which] = fetch(reinterpret_cast<const uint4*>(a.cache.codes[which] + code_offset(a.cache, id, h) +
+                                                                   static_cast<int64_t>(p & (bs - 1)) * a.cache.dim) + c);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        if (to[u] < 0) continue;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const uint32_t ws[4] = {codes[u][which].x, codes[u][which].y, codes[u][which].z, codes[u][which].w};
             Vec<__nv_bfloat16, 16> o;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float f[4];
                 decode4<CODE>(ws[k], f);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) o.v[4 * k + m] = __float2bfloat16_rn(f[m] * scale);
+                for (int m = 0; m < 4; ++m) o.v[4 * k + m] = __float2bfloat16_rn(f[m] * scale[u][which]);
             }
-            store_vec<__nv_bfloat16, 16>(a.out[which] + (static_cast<int64_t>(s.first + r) * a.cache.heads + h) * a.cache.dim + c * 16, o);
+            store_vec<__nv_bfloat16, 16>(a.out[which] + to[u], o);
         }
     }
 }
@@ -223,7 +237,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 __device__ __forceinline__ int evict_length(const EvictDev& a, int b, bool report) {
-    const int len = __ldg(a.seq.lengths + b);
+    const int len = fetch(a.seq.lengths + b);
     const bool ok = length_ok(len, a.max_length);
     if (!ok && report) atomicOr(a.seq.err, kBadSequence);
     return ok ? len : 0;
@@ -412,7 +426,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, in
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int i = base + u * stride + first;
-                x[u] = i < a.budget ? __ldcg(w + keep[i]) : 0.f;
+                x[u] = i < a.budget ? fetch_l2(w + keep[i]) : 0.f;
             }
             cl.sync();  // the sources of this round are read; those of later rounds lie behind its destinations
 #pragma unroll
@@ -462,14 +476,14 @@ __global__ void __launch_bounds__(kMoveThreads, 2) k_kv8_move(EvictDev a, int ct
     const int tok = tid < per * pieces ? tid / pieces : tokens, col = tid % pieces * 16;
     auto live = [&](int base, int u) { return tok + u * per < tokens && base + rank * tokens + tok + u * per < a.budget; };
     // kept index of a piece's token (-1: none), its codes, its scale
-    auto kept = [&](int base, int u) { return live(base, u) ? __ldg(keep + base + tok + u * per) : -1; };
+    auto kept = [&](int base, int u) { return live(base, u) ? fetch(keep + base + tok + u * per) : -1; };
     auto piece = [&](int from, float& scale) {
         uint4 x = make_uint4(0, 0, 0, 0);
         scale = 0.f;
         if (from >= 0) {
             const int id = load_block(a.seq, b, from >> shift, false);
-            scale = __ldg(old + (from >> shift));
-            if (id >= 0) x = __ldcg(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) + static_cast<int64_t>(from & (bs - 1)) * dim + col));
+            scale = fetch(old + (from >> shift));
+            if (id >= 0) x = fetch_l2(reinterpret_cast<const uint4*>(codes + code_offset(a.cache, id, h) + static_cast<int64_t>(from & (bs - 1)) * dim + col));
         }
         return x;
     };

@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv8_prompt(const __grid_const
                     id = load_block(a.seq, p.b, at >> shift, true);
                     if (id >= 0) {
                         const int64_t sc = static_cast<int64_t>(id) * a.cache.heads + p.h;
-                        entry.x = __ldg(a.cache.scale[0] + sc);
-                        entry.y = __ldg(a.cache.scale[1] + sc);
+                        entry.x = fetch(a.cache.scale[0] + sc);
+                        entry.y = fetch(a.cache.scale[1] + sc);
                         entry.z = __log2f(entry.y);  // only a bound: its rounding cancels
                     }
                 }

@@ -135,13 +135,13 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
     const int32_t* hist = a.history ? a.history + row * a.history_stride : nullptr;
-    const int n_hist = hist ? min(max(__ldg(a.history_len + row), 0), a.history_max) : 0;
-    const int n_prompt = hist && a.prompt_len ? __ldg(a.prompt_len + row) : 0;
+    const int n_hist = hist ? min(max(fetch(a.history_len + row), 0), a.history_max) : 0;
+    const int n_prompt = hist && a.prompt_len ? fetch(a.prompt_len + row) : 0;
     const int32_t* bias_ids = a.bias_ids ? a.bias_ids + row * a.bias_stride : nullptr;
-    const int n_bias = bias_ids ? min(max(__ldg(a.bias_len + row), 0), a.bias_max) : 0;
-    const float rep = a.repetition ? __ldg(a.repetition + row) : 1.f;
-    const float freq = a.frequency ? __ldg(a.frequency + row) : 0.f;
-    const float pres = a.presence ? __ldg(a.presence + row) : 0.f;
+    const int n_bias = bias_ids ? min(max(fetch(a.bias_len + row), 0), a.bias_max) : 0;
+    const float rep = a.repetition ? fetch(a.repetition + row) : 1.f;
+    const float freq = a.frequency ? fetch(a.frequency + row) : 0.f;
+    const float pres = a.presence ? fetch(a.presence + row) : 0.f;
     const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
     // Vector j holds entries [V j - skew, V j - skew + V): 16-byte aligned in
     // the input, and in the output if its rows have the same alignment.
@@ -160,15 +160,15 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
     int held[kHeld], held_bias = -1;
     float held_value = 0.f;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) held[k] = k * kLogitsThreads + tid < n_hist ? __ldg(hist + k * kLogitsThreads + tid) : -1;
+    for (int k = 0; k < kHeld; ++k) held[k] = k * kLogitsThreads + tid < n_hist ? fetch(hist + k * kLogitsThreads + tid) : -1;
     if (tid < n_bias) {
-        held_bias = __ldg(bias_ids + tid);
-        held_value = __ldg(a.bias_values + row * a.bias_stride + tid);
+        held_bias = fetch(bias_ids + tid);
+        held_value = fetch(a.bias_values + row * a.bias_stride + tid);
     }
     auto each_id = [&](auto&& f) {
 #pragma unroll
         for (int k = 0; k < kHeld; ++k) f(k * kLogitsThreads + tid, held[k]);
-        for (int i = kHeld * kLogitsThreads + tid; i < n_hist; i += kLogitsThreads) f(i, __ldg(hist + i));
+        for (int i = kHeld * kLogitsThreads + tid; i < n_hist; i += kLogitsThreads) f(i, fetch(hist + i));
     };
     unsigned long long key = 0;
     float best = -INFINITY;  // of this thread's streamed logits, whose ids only grow
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
             });
             if (t.holds(held_bias)) t.mark(held_bias);
             for (int i = kLogitsThreads + tid; i < n_bias; i += kLogitsThreads) {
-                const int id = __ldg(bias_ids + i);
+                const int id = fetch(bias_ids + i);
                 if (t.holds(id)) t.mark(id);
             }
             __syncthreads();
@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
             // place adds alone; else the part's entries of the round are listed in
             // their order, and the first of each id adds up the values of that id.
             for (int i = 0; i < n_bias; i += kLogitsThreads) {
-                const int id = i == 0 ? held_bias : i + tid < n_bias ? __ldg(bias_ids + i + tid) : -1;
-                const float value = i == 0 ? held_value : i + tid < n_bias ? __ldg(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
+                const int id = i == 0 ? held_bias : i + tid < n_bias ? fetch(bias_ids + i + tid) : -1;
+                const float value = i == 0 ? held_value : i + tid < n_bias ? fetch(a.bias_values + row * a.bias_stride + i + tid) : 0.f;
                 const bool in_part = t.holds(id);
                 float* sum_of = &t.bias[in_part ? t.place(id) : 0];
                 float prior = 0.f;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
             words_ahead[u] = make_uint2(~0u, ~0u);
             if (v < v1 && e >= 0 && e + V <= a.vocab) {
                 ahead[u] = *reinterpret_cast<const Vec<T, V>*>(in + e);
-                if (mask) words_ahead[u] = make_uint2(__ldg(mask + (e >> 5)), __ldg(mask + ((e + V - 1) >> 5)));
+                if (mask) words_ahead[u] = make_uint2(fetch(mask + (e >> 5)), fetch(mask + ((e + V - 1) >> 5)));
             }
         }
 #pragma unroll
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
                     const T x = in[id];
                     const int at = id - t.first;
                     const bool raw = touched && (t.bits[at >> 5] >> (at & 31) & 1);
-                    const bool gone = mask && !(__ldg(mask + (id >> 5)) >> (id & 31) & 1);
+                    const bool gone = mask && !(fetch(mask + (id >> 5)) >> (id & 31) & 1);
                     out[id] = gone && !raw ? from_f32<T>(-INFINITY) : x;
                     if (to_f32(x) > best && !gone && !raw) {
                         best = to_f32(x);
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(LogitsDev a, int c
                     const int k = kb + u * kLogitsThreads;
                     ids[u] = k < touched ? t.first + t.ids[k] : t.first;
                     ys[u] = k < touched ? to_f32(out[ids[u]]) : 0.f;
-                    seen[u] = mask ? __ldg(mask + (ids[u] >> 5)) >> (ids[u] & 31) & 1 : 1;
+                    seen[u] = mask ? fetch(mask + (ids[u] >> 5)) >> (ids[u] & 31) & 1 : 1;
                 }
 #pragma unroll
                 for (int u = 0; u < kLate; ++u) {

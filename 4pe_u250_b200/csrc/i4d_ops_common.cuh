@@ -42,6 +42,28 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+// A load of what a kernel before this one may have written, or this one writes in
+// place.  A plain one, not of the read-only path (__ldg): the launches overlap,
+// so that memory is not constant while the kernel lives, and nothing would keep
+// such a load behind op_begin()'s wait.
+template <typename T>
+__device__ __forceinline__ T fetch(const T* p) {
+    return *p;
+}
+
+// Loads from the L2 of what other CTAs of the cluster write between barriers.
+// (volatile: they stay between the barriers where they stand)
+__device__ __forceinline__ float fetch_l2(const float* p) {
+    float x;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p));
+    return x;
+}
+__device__ __forceinline__ uint4 fetch_l2(const uint4* p) {
+    uint4 x;
+    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+    return x;
+}
+
 // N elements by 16-byte accesses (N * sizeof(T) a multiple of 16, aligned).
 template <typename T, int N>
 struct alignas(16) Vec {
@@ -54,7 +76,7 @@ __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
     if constexpr (N * sizeof(T) % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(N * sizeof(T) / 16); ++i)
-            reinterpret_cast<uint4*>(&r)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            reinterpret_cast<uint4*>(&r)[i] = fetch(reinterpret_cast<const uint4*>(p) + i);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) r.v[i] = p[i];
@@ -98,7 +120,7 @@ struct Seq {
 
 // A sequence whose arrays contradict the call's bounds is skipped (n = 0).
 __device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) {
-    const int q0 = __ldg(a.q_start + b), q1 = __ldg(a.q_start + b + 1), len = __ldg(a.lengths + b);
+    const int q0 = fetch(a.q_start + b), q1 = fetch(a.q_start + b + 1), len = fetch(a.lengths + b);
     const bool ok = seq_ok(q0, q1, len, a.tokens, a.max_q, a.table_blocks, a.block_tokens);
     if (!ok && report) atomicOr(a.err, kBadSequence);
     return {q0, ok ? q1 - q0 : 0, ok ? len : 0};
@@ -106,7 +128,7 @@ __device__ __forceinline__ Seq load_seq(const SeqArrays& a, int b, bool report) 
 
 // Block id of a table entry, or -1 for one outside the pool.
 __device__ __forceinline__ int load_block(const SeqArrays& a, int b, int j, bool report) {
-    const int id = __ldg(a.table + static_cast<int64_t>(b) * a.table_stride + j);
+    const int id = fetch(a.table + static_cast<int64_t>(b) * a.table_stride + j);
     if (block_ok(id, a.blocks)) return id;
     if (report) atomicOr(a.err, kBadBlock);
     return -1;

@@ -42,7 +42,7 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t turn, float magnitude) {
 
 // (cos, sin) * magnitude of pair i's angle at token t.
 __device__ __forceinline__ float2 rope_angle(const RopeDev& a, int t, int i) {
-    const uint64_t turn = static_cast<uint64_t>(static_cast<int64_t>(__ldg(a.positions + t))) * __ldg(a.turns + i);
+    const uint64_t turn = static_cast<uint64_t>(static_cast<int64_t>(fetch(a.positions + t))) * fetch(a.turns + i);
     return turn_cos_sin(a.inverse ? 0 - turn : turn, a.magnitude);
 }
 
