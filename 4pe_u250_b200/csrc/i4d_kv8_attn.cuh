@@ -33,8 +33,8 @@
 // costs 24 ragged contexts 3 %, three rows a sequence 6 %, FP32 rows of 256
 // 10 %).
 // Bound: the codes of K and V, read once (24 contexts of 301 to 32749 tokens,
-// 8 heads of 128, 812 MB of INT8 codes: 151 to 166 us, 5.4 to 4.9 TB/s; the same
-// copies without arithmetic 133 us).
+// 8 heads of 128, 812 MB of INT8 codes: 173 to 178 us, 4.7 TB/s; the same copies
+// without arithmetic 133 us).
 #pragma once
 
 #include <cuda.h>

@@ -51,7 +51,7 @@ __device__ __forceinline__ Vec<T, 8> load8(const T* p) {
 // codes.  The first four groups of eight of each thread stay in registers between them, in
 // their own type, which covers blocks of 8192 values (64 tokens of 128); the
 // rest is read again from L1/L2.  Bound: the values in, the codes out (6 x 501
-// to 1531 FP32 rows of 8 heads of 128: 15 us, 60 MB; 48 rows in BF16: 4 us).
+// to 1531 FP32 rows of 8 heads of 128: 16 us, 60 MB; 48 rows in BF16: 4 us).
 template <typename T, int V, int CODE, int THREADS>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, 4) k_kv8_append(AppendDev a, int units) {
     op_begin();
@@ -283,7 +283,7 @@ constexpr int kSelectHeld = 16;  // weights that a thread holds in registers
 // indices in order (of equal keys the first ones), their weights, and a copy
 // of the scales, which the move overwrites.  Rows of up to 65536 weights are
 // read once into registers.  Bound: the chain of cluster barriers (8 heads of 4
-// rows of up to 40009 weights: 23 us; one row of 2047, 32 heads: 13 us).
+// rows of up to 40009 weights: 23 us; one row of 2047, 32 heads: 12 us).
 __global__ void __launch_bounds__(kSelectThreads, 2) k_kv8_select(EvictDev a, int ctas) {
     op_begin();
     __shared__ __align__(16) int hist[kSelectBins];

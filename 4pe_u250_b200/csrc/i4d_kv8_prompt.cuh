@@ -20,8 +20,9 @@
 // Bound: 4 dim products a visible (row, token) at the tensor rate, and one
 // exponential for each at the rate of the special-function units, which for
 // dim 128 takes as long (16 a cycle and SM against 8192 products).  Two chunks
-// of 1537 to 2048 rows over 6151 to 8192 tokens, 32 heads of 128: 542 us with the
-// join, 693 TFLOP/s; tensor pipe 52 %, exponentials 37 %, issue slots 44 % busy.
+// of 1537 to 2048 rows over 6151 to 8192 tokens, 32 heads of 128: 569 us with the
+// join, 661 TFLOP/s (FP16 outputs 15 % more); tensor pipe 50 %, exponentials 36 %,
+// issue slots 43 % busy: the softmax threads wait for tensor memory.
 #pragma once
 
 #include "i4d_kv8_attn.cuh"

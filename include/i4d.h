@@ -519,7 +519,13 @@ i4d_status i4d_kv8_read(i4d_ctx* ctx, const i4d_kv8_read_args* args);
  * A row at cache index p sees the tokens j <= p and, with window > 0,
  * j > p - window.  out (q's type) = softmax(scale q.k) v; lse [tokens][heads]
  * FP32 (may be NULL) the logarithm of the softmax sum.  A row that sees
- * nothing gives zeros and -inf.  weights (may be NULL): FP32
+ * nothing gives zeros and -inf.  Codes are exact, 16-bit queries too, FP32 ones
+ * to 2^-22; sums are FP32.  A weight (a probability times its block's value
+ * scale) is right to 2^-22 of it for FP32 outputs; for FP16 ones to 2^-22, but
+ * not less than 2^-31 of the row's greatest weight; for BF16 ones to 2^-11,
+ * where a call has more than 64 rows a cache head (max_q * heads / cache heads)
+ * and dim <= 128 also not less than 2^-31 of the greatest.  Weights under 2^-95
+ * of the greatest may count as 0.  weights (may be NULL): FP32
  * [batch][cache heads][weights_stride], to whose first max_length entries of
  * a head the probabilities are added that the call's rows of that head gave
  * each token (what i4d_kv8_evict reads); the order of the sum is fixed.
